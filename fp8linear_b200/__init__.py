@@ -8,12 +8,16 @@ from . import layers
 from ._ops import ops
 from .layers import (
     Fp8Linear,
+    fp8_grouped_gemm,
+    fp8_grouped_linear,
     fp8_linear,
+    fp8_linear_lora,
     fp8_linear_modulated,
     layernorm_modulate_quantize_fp8,
     mxfp8_linear,
     nvfp4_linear,
     quantize_,
+    quantize_expert_weights,
     quantize_weight,
     quantize_weight_mxfp8,
     quantize_weight_nvfp4,
@@ -45,4 +49,8 @@ __all__ = [
     "nvfp4_gemm",
     "layernorm_modulate_quantize_fp8",
     "fp8_linear_modulated",
+    "quantize_expert_weights",
+    "fp8_grouped_gemm",
+    "fp8_grouped_linear",
+    "fp8_linear_lora",
 ]

@@ -43,6 +43,12 @@ SIGNATURES = {
     "fp8lin_nvfp4_linear": (_I, [_P, _I, _P, _P, _P, _I, _P, _I, _I64, _I64, _I64, _P, _SZ, _P]),
     "fp8lin_fp8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _P, _I, _I64, _I64, _I64, _P]),
     "fp8lin_linear_workspace_size": (_SZ, [_I64, _I64]),
+    "fp8lin_fp8_grouped_gemm": (_I, [_P, _P, _P, _P, _P, _P, _I, _P, _I, _I64, _I64, _I64, _I64, _P]),
+    "fp8lin_fp8_grouped_linear": (_I, [_P, _I, _P, _P, _P, _P, _I, _P, _I, _I64, _I64, _I64, _I64,
+                                       _P, _SZ, _P]),
+    "fp8lin_fp8_linear_lora_workspace_size": (_SZ, [_I64, _I64, _I64]),
+    "fp8lin_fp8_linear_lora": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I64, _I64, _I64,
+                                    _I64, _I64, _P, _SZ, _P]),
     "fp8lin_fp8_linear": (_I, [_P, _I, _P, _P, _P, _I, _P, _I, _I64, _I64, _I64, _P, _SZ, _P]),
     "fp8lin_device_status": (_I, [ctypes.POINTER(ctypes.c_uint), _I]),
     "fp8lin_fp8_linear_noalloc": (_I, [_P, _I, _P, _P, _P, _I, _P, _I, _I64, _I64, _I64, _P]),
@@ -273,6 +279,56 @@ class CApi:
             out.data_ptr(), DTYPE[out.dtype], M, N, K, workspace.data_ptr(),
             workspace.numel(), self._stream(x))
         self._check(rc, "fp8lin_fp8_linear")
+        return out
+
+    def fp8_grouped_gemm(self, xq, x_scale, wq, w_scale, offsets, bias=None,
+                         out_dtype=torch.bfloat16, out=None):
+        """Rows of xq [M, K] sorted by expert (offsets int32 [E + 1] on the device) against
+        wq [E, N, K]; rows of no expert become zeros."""
+        M, K = xq.shape
+        E, N = wq.shape[:2]
+        out = torch.empty((M, N), dtype=out_dtype, device=xq.device) if out is None else out
+        rc = self.lib.fp8lin_fp8_grouped_gemm(
+            xq.data_ptr(), x_scale.data_ptr(), wq.data_ptr(), w_scale.data_ptr(),
+            offsets.data_ptr(), self._bias_ptr(bias), self._bias_dtype(bias), out.data_ptr(),
+            DTYPE[out.dtype], M, N, K, E, self._stream(xq))
+        self._check(rc, "fp8lin_fp8_grouped_gemm")
+        return out
+
+    def fp8_grouped_linear(self, x, wq, w_scale, offsets, bias=None, out=None, workspace=None):
+        M, K = x.shape
+        E, N = wq.shape[:2]
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device) if out is None else out
+        if workspace is None:
+            workspace = torch.empty((max(self.workspace_size(M, K), 1),), dtype=torch.uint8,
+                                    device=x.device)
+        rc = self.lib.fp8lin_fp8_grouped_linear(
+            x.data_ptr(), DTYPE[x.dtype], wq.data_ptr(), w_scale.data_ptr(), offsets.data_ptr(),
+            self._bias_ptr(bias), self._bias_dtype(bias), out.data_ptr(), DTYPE[out.dtype], M, N,
+            K, E, workspace.data_ptr(), workspace.numel(), self._stream(x))
+        self._check(rc, "fp8lin_fp8_grouped_linear")
+        return out
+
+    def lora_workspace_size(self, M: int, K: int, R: int) -> int:
+        return int(self.lib.fp8lin_fp8_linear_lora_workspace_size(M, K, R))
+
+    def fp8_linear_lora(self, x, wq, w_scale, lora_a, lora_b, adapters, scaling, bias=None,
+                        out=None, workspace=None):
+        """fp8_linear plus the low-rank adapter of each row: lora_a [L, R, K], lora_b
+        [L, N, R] in x's dtype, adapters int32 [M] (none outside [0, L)), scaling fp32 [L]."""
+        M, K = x.shape
+        N = wq.shape[0]
+        L, R = lora_a.shape[:2]
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device) if out is None else out
+        if workspace is None:
+            workspace = torch.empty((max(self.lora_workspace_size(M, K, R), 1),),
+                                    dtype=torch.uint8, device=x.device)
+        rc = self.lib.fp8lin_fp8_linear_lora(
+            x.data_ptr(), DTYPE[x.dtype], wq.data_ptr(), w_scale.data_ptr(), lora_a.data_ptr(),
+            lora_b.data_ptr(), adapters.data_ptr(), scaling.data_ptr(), self._bias_ptr(bias),
+            self._bias_dtype(bias), out.data_ptr(), DTYPE[out.dtype], M, N, K, L, R,
+            workspace.data_ptr(), workspace.numel(), self._stream(x))
+        self._check(rc, "fp8lin_fp8_linear_lora")
         return out
 
     def fp8_linear_noalloc(self, x, wq, w_scale, bias=None, out=None):

@@ -87,6 +87,22 @@ int check_gemm_args(const void *xq, const float *xs, const void *wq, const float
   return FP8LIN_OK;
 }
 
+// The further arguments of the grouped forms, after check_gemm_args.
+int check_group_args(const int32_t *offsets, int64_t M, int64_t N, int64_t K, int64_t E,
+                     const char *op) {
+  const std::string o(op);
+  if (E < 1 || E > kMaxExperts)
+    return fail(FP8LIN_ERR_UNSUPPORTED, o + ": the number of experts must be 1 to " +
+                                            std::to_string(kMaxExperts) + ", got " +
+                                            std::to_string(E));
+  if (M > 0x7fffffffLL || N > 0x7fffffffLL || K > 0x7fffffffLL)
+    return fail(FP8LIN_ERR_UNSUPPORTED, o + ": dimensions must fit in int32");
+  if (M == 0 || N == 0) return FP8LIN_OK;
+  if (!offsets) return fail(FP8LIN_ERR_INVALID_ARGUMENT, o + ": null offsets");
+  if (!aligned(offsets, 4)) return fail(FP8LIN_ERR_UNSUPPORTED, o + ": offsets must be 4-byte aligned");
+  return FP8LIN_OK;
+}
+
 }  // namespace
 }  // namespace fp8lin
 
@@ -674,6 +690,130 @@ int fp8lin_fp8_linear_allgather(const void *x, int x_dtype, const void *wq, cons
   return launch_gemm(a, s, true);
 }
 
+int fp8lin_fp8_grouped_gemm(const void *xq, const float *x_scale, const void *wq,
+                            const float *w_scale, const int32_t *offsets, const void *bias,
+                            int bias_dtype, void *out, int out_dtype, int64_t M, int64_t N,
+                            int64_t K, int64_t E, void *stream) {
+  clear_error();
+  int rc = check_gemm_args(xq, x_scale, wq, w_scale, bias, bias_dtype, out, out_dtype, M, N, K,
+                           "fp8_grouped_gemm");
+  if (rc == FP8LIN_OK) rc = check_group_args(offsets, M, N, K, E, "fp8_grouped_gemm");
+  if (rc != FP8LIN_OK || M == 0 || N == 0) return rc;
+  GroupedArgs a{static_cast<const uint8_t *>(xq), x_scale, static_cast<const uint8_t *>(wq),
+                w_scale, bias, bias ? bias_dtype : kNone, out, out_dtype, offsets, M, N, K, E};
+  return launch_grouped(a, static_cast<cudaStream_t>(stream), true);
+}
+
+int fp8lin_fp8_grouped_linear(const void *x, int x_dtype, const void *wq, const float *w_scale,
+                              const int32_t *offsets, const void *bias, int bias_dtype, void *out,
+                              int out_dtype, int64_t M, int64_t N, int64_t K, int64_t E,
+                              void *workspace, size_t workspace_bytes, void *stream) {
+  clear_error();
+  if (x_dtype != kBF16 && x_dtype != kF16)
+    return fail(FP8LIN_ERR_INVALID_ARGUMENT, "fp8_grouped_linear: x must be fp16 or bf16");
+  int rc = check_gemm_args(reinterpret_cast<const void *>(16), w_scale, wq, w_scale, bias,
+                           bias_dtype, out, out_dtype, M, N, K, "fp8_grouped_linear");
+  if (rc == FP8LIN_OK) rc = check_group_args(offsets, M, N, K, E, "fp8_grouped_linear");
+  if (rc != FP8LIN_OK || M == 0 || N == 0) return rc;
+  if (!x) return fail(FP8LIN_ERR_INVALID_ARGUMENT, "fp8_grouped_linear: null x");
+  const size_t need = fp8lin_linear_workspace_size(M, K);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, kWsAlign))
+    return fail(FP8LIN_ERR_WORKSPACE, "fp8_grouped_linear: workspace of " + std::to_string(need) +
+                                          " bytes (256-byte aligned) required, got " +
+                                          std::to_string(workspace_bytes));
+  uint8_t *xq = static_cast<uint8_t *>(workspace);
+  float *xs = reinterpret_cast<float *>(
+      xq + round_up(static_cast<size_t>(M) * static_cast<size_t>(K), kWsAlign));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_quantize_rows(x, x_dtype, M, K, xq, xs, s, true);
+  if (e != cudaSuccess)
+    return fail(FP8LIN_ERR_CUDA, std::string("fp8_grouped_linear: quantize launch: ") +
+                                     cudaGetErrorString(e));
+  GroupedArgs a{xq, xs, static_cast<const uint8_t *>(wq), w_scale, bias,
+                bias ? bias_dtype : kNone, out, out_dtype, offsets, M, N, K, E};
+  a.weights_before_wait = true;  // the previous kernel is this call's quantizer
+  return launch_grouped(a, s, true);
+}
+
+size_t fp8lin_fp8_linear_lora_workspace_size(int64_t M, int64_t K, int64_t R) {
+  if (M <= 0 || K <= 0) return 0;
+  return fp8lin_linear_workspace_size(M, K) +
+         (R > 0 ? lora_workspace(nullptr, M, R).bytes : 0);
+}
+
+int fp8lin_fp8_linear_lora(const void *x, int x_dtype, const void *wq, const float *w_scale,
+                           const void *lora_a, const void *lora_b, const int32_t *adapters,
+                           const float *scaling, const void *bias, int bias_dtype, void *out,
+                           int out_dtype, int64_t M, int64_t N, int64_t K, int64_t L, int64_t R,
+                           void *workspace, size_t workspace_bytes, void *stream) {
+  clear_error();
+  const char *op = "fp8_linear_lora";
+  const std::string o(op);
+  if (x_dtype != kBF16 && x_dtype != kF16)
+    return fail(FP8LIN_ERR_INVALID_ARGUMENT, o + ": x must be fp16 or bf16");
+  int rc = check_gemm_args(reinterpret_cast<const void *>(16), w_scale, wq, w_scale, bias,
+                           bias_dtype, out, out_dtype, M, N, K, op);
+  if (rc != FP8LIN_OK) return rc;
+  if (L < 0 || R < 0) return fail(FP8LIN_ERR_INVALID_ARGUMENT, o + ": negative size");
+  if (L == 0)  // no adapters: the linear alone
+    return fp8lin_fp8_linear(x, x_dtype, wq, w_scale, bias, bias_dtype, out, out_dtype, M, N, K,
+                             workspace, workspace_bytes, stream);
+  if (R == 0 || R % 8 != 0 || R > kLoraMaxRank)
+    return fail(FP8LIN_ERR_UNSUPPORTED, o + ": the rank must be a multiple of 8 from 8 to " +
+                                            std::to_string(kLoraMaxRank) + " (pad with zeros), got " +
+                                            std::to_string(R));
+  if (M > 0x7fffffffLL || N > 0x7fffffffLL || K > 0x7fffffffLL || L > 0x7fffffffLL)
+    return fail(FP8LIN_ERR_UNSUPPORTED, o + ": dimensions must fit in int32");
+  if (M == 0 || N == 0) return FP8LIN_OK;
+  if (!x || !lora_a || !lora_b || !adapters || !scaling)
+    return fail(FP8LIN_ERR_INVALID_ARGUMENT, o + ": null pointer");
+  if (!aligned(x, 16) || !aligned(lora_a, 16) || !aligned(lora_b, 16))
+    return fail(FP8LIN_ERR_UNSUPPORTED, o + ": x, lora_a and lora_b must be 16-byte aligned");
+  const size_t need = fp8lin_fp8_linear_lora_workspace_size(M, K, R);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, kWsAlign))
+    return fail(FP8LIN_ERR_WORKSPACE, o + ": workspace of " + std::to_string(need) +
+                                          " bytes (256-byte aligned) required, got " +
+                                          std::to_string(workspace_bytes));
+  uint8_t *xq = static_cast<uint8_t *>(workspace);
+  float *xs = reinterpret_cast<float *>(
+      xq + round_up(static_cast<size_t>(M) * static_cast<size_t>(K), kWsAlign));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  L2Prefetch pf;
+  if (M <= kLoraRowsMaxM) {  // as fp8_linear: the weights come into L2 on the way
+    pf.ptr = wq;
+    pf.bytes = N * K;
+  }
+  cudaError_t e = launch_quantize_rows(x, x_dtype, M, K, xq, xs, s, true, pf);
+  if (e != cudaSuccess)
+    return fail(FP8LIN_ERR_CUDA, o + ": quantize launch: " + cudaGetErrorString(e));
+  LoraArgs a{};
+  a.x = x;
+  a.dtype = x_dtype;
+  a.lora_a = lora_a;
+  a.lora_b = lora_b;
+  a.ids = adapters;
+  a.scaling = scaling;
+  a.L = L;
+  a.R = R;
+  a.xq = xq;
+  a.xs = xs;
+  a.wq = static_cast<const uint8_t *>(wq);
+  a.ws = w_scale;
+  a.bias = bias;
+  a.bias_dtype = bias ? bias_dtype : kNone;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.workspace = xq + fp8lin_linear_workspace_size(M, K);
+  // the kernels before are this call's quantizer and down projection
+  a.weights_before_wait = true;
+  rc = launch_lora_down(a, s);
+  if (rc != FP8LIN_OK) return rc;
+  return launch_lora_gemm(a, s, true);
+}
+
 static_assert(sizeof(cudaIpcMemHandle_t) == FP8LIN_PEER_HANDLE_BYTES,
               "CUDA IPC handle size differs from FP8LIN_PEER_HANDLE_BYTES");
 
@@ -746,13 +886,15 @@ int fp8lin_selftest_watchdog(unsigned int limit_us, unsigned int *status, void *
 int fp8lin_device_status(unsigned int *status, int clear) {
   clear_error();
   if (!status) return fail(FP8LIN_ERR_INVALID_ARGUMENT, "device_status: null pointer");
-  unsigned int q = 0, sm = 0;
+  unsigned int q = 0, sm = 0, rs = 0, lo = 0;
   cudaError_t e = read_gemm_status(status, clear != 0);
   if (e == cudaSuccess) e = read_quant_status(&q, clear != 0);
   if (e == cudaSuccess) e = read_small_status(&sm, clear != 0);
+  if (e == cudaSuccess) e = read_rowsel_status(&rs, clear != 0);
+  if (e == cudaSuccess) e = read_lora_status(&lo, clear != 0);
   if (e != cudaSuccess)
     return fail(FP8LIN_ERR_CUDA, std::string("device_status: ") + cudaGetErrorString(e));
-  *status |= q | sm;
+  *status |= q | sm | rs | lo;
   return FP8LIN_OK;
 }
 

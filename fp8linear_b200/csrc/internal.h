@@ -136,6 +136,94 @@ cudaError_t launch_watchdog_selftest(unsigned int limit_us, unsigned int *status
 constexpr int kSmallDeclined = -1;
 int launch_gemm_small(const GemmArgs &a, cudaStream_t stream, bool pdl);
 cudaError_t read_small_status(unsigned int *bits, bool clear);
+
+// ---- rowsel_sm100.cu (weights chosen per row)
+// Rows sorted by expert: row i uses expert e with offsets[e] <= i < offsets[e + 1]. The
+// offsets are device data; the kernels clamp them to [0, M] and to their running maximum,
+// and write zeros to rows of no expert.
+constexpr int kMaxExperts = 1024;
+struct GroupedArgs {
+  const uint8_t *xq;     // [M, K] e4m3
+  const float *xs;       // [M]
+  const uint8_t *wq;     // [E, N, K] e4m3
+  const float *ws;       // [E, N]
+  const void *bias;      // [E, N] or null
+  int bias_dtype;
+  void *out;             // [M, N]
+  int out_dtype;
+  const int *offsets;    // [E + 1]
+  int64_t M, N, K, E;
+  // As GemmArgs::weights_before_wait; covers the offsets too.
+  bool weights_before_wait = false;
+};
+int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl);
+
+// One shared projection plus the low-rank adapter of each row (ids[i], none outside [0, L)):
+// out = acc * xs * ws + bias + sum_r h[i, r] * lora_b[ids[i], n, r], h from launch_lora_down.
+constexpr int kLoraMaxRank = 128;
+constexpr int64_t kLoraRowsMaxM = 128;  // up to here h is fp32 and CUDA cores add the adapters
+struct LoraArgs {
+  const void *x;         // [M, K] bf16 or fp16
+  int dtype;             // of x, lora_a, lora_b
+  const void *lora_a;    // [L, R, K]
+  const void *lora_b;    // [L, N, R]
+  const int *ids;        // [M]
+  const float *scaling;  // [L]
+  int64_t L, R;
+  const uint8_t *xq;     // [M, K] e4m3, and the rest as in GroupedArgs (one expert)
+  const float *xs;
+  const uint8_t *wq;
+  const float *ws;
+  const void *bias;
+  int bias_dtype;
+  void *out;
+  int out_dtype;
+  int64_t M, N, K;
+  void *workspace;       // lora_workspace_bytes(M, R), 256-byte aligned
+  bool weights_before_wait = false;
+};
+int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl);
+cudaError_t read_rowsel_status(unsigned int *bits, bool clear);
+
+// ---- lora_sm100.cu
+// Layout of the adapters' intermediate h in the workspace.
+//   M <= kLoraRowsMaxM: h fp32 [M][R].
+//   otherwise: hl [M][2 * rank_pad] of x's type, h / hscale as a high and a low part
+//   (h = hscale * (hi + lo), to fp32's last bits), hscale fp32 [M] (a power of two), and
+//   the adapter of each token tile of the GEMM (int: >= 0 all rows' adapter, -1 none, -2
+//   more than one).
+inline int64_t lora_rank_pad(int64_t R) { return (R + 15) / 16 * 16; }
+constexpr int kLoraTileTokens = 160;  // tokens per tile of the GEMM with adapters, at most
+inline int64_t lora_tiles(int64_t M) { return (M + kLoraTileTokens - 1) / kLoraTileTokens; }
+inline int64_t lora_tile_tokens(int64_t M) {
+  const int64_t nt = lora_tiles(M);
+  return ((M + nt - 1) / nt + 31) / 32 * 32;
+}
+struct LoraWorkspace {
+  float *h = nullptr;
+  void *hl = nullptr;
+  float *hscale = nullptr;
+  int *tile_adapter = nullptr;
+  size_t bytes = 0;
+};
+LoraWorkspace lora_workspace(void *base, int64_t M, int64_t R);
+// h = scaling[a] * x . lora_a[a]^T for every row with an adapter. Launched as a programmatic
+// dependent; reads x, ids and the adapters before its dependency wait (the kernel before
+// must be this call's quantizer, see GemmArgs::weights_before_wait) and writes after it.
+int launch_lora_down(const LoraArgs &a, cudaStream_t stream);
+cudaError_t read_lora_status(unsigned int *bits, bool clear);
+
+// ---- tensor maps
+// 3-D map over a dense or strided array of `dtype` (inner, mid, outer) with byte strides
+// mid_bytes / outer_bytes, box box_inner x box_mid x 1, 128-byte swizzle.
+bool make_tmap_3d_sw128(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
+                        uint64_t inner, uint64_t mid, uint64_t outer, uint64_t mid_bytes,
+                        uint64_t outer_bytes, uint32_t box_inner, uint32_t box_mid,
+                        std::string *err);
+// 2-D form with any element type and row pitch.
+bool make_tmap_2d_sw128(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
+                        uint64_t inner, uint64_t outer, uint64_t row_bytes, uint32_t box_inner,
+                        uint32_t box_outer, std::string *err);
 // 2-D uint8 tensor map with 128-byte swizzle (shared by both GEMM shapes).
 bool make_tmap_2d_u8(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
                      uint32_t box_inner, uint32_t box_outer, std::string *err);

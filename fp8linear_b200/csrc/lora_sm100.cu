@@ -1,0 +1,569 @@
+// lora_sm100.cu -- the down projection of the per-row low-rank adapters:
+//   h[i,r] = scaling[a_i] * sum_k x[i,k] A[a_i][r,k]     (x unquantized; sums in fp32)
+// for the rows i whose adapter a_i is in [0, L). The up projection is part of the linear's
+// GEMM (rowsel_sm100.cu), which adds h . B^T before its one rounding.
+//
+//   down_rows_kernel  few rows: CUDA cores, x and A read as they lie, K split over the warps
+//       of a CTA; h stays fp32.
+//   down_tile_kernel  many rows: tcgen05 (kind::f16) on tiles of 128 rows. All of a tile's
+//       adapters stand side by side on the MMA's N side (rank_pad columns each, 128 columns
+//       a pass), and each row keeps the columns of its own; rows never mix, so an adapter's
+//       infinities and NaN stay with its rows. A cluster splits K when the tiles are few.
+//
+// The GEMM's tensor cores take h in x's 16-bit type. h is a sum, so it keeps fp32's accuracy:
+// it goes as a high and a low part, h / hscale = hi + lo (bf16: 2^-17 relative; f16: hscale,
+// a power of two, puts the row's largest value in [1, 2), the error is 2^-22 of it), at the
+// price of twice the rank in a product that is a few per cent of the whole.
+//
+// Both kernels read x, ids and A before the dependency wait (the kernel before is the call's
+// quantizer, which lets them launch only after its own wait) and write after it.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <mutex>
+#include <string>
+
+#include "internal.h"
+#include "ptx.cuh"
+
+namespace fp8lin {
+
+__device__ unsigned int g_lora_status;  // watchdog bits (128 = a wait ran out)
+
+namespace lora {
+
+constexpr uint64_t kWaitLimitNs = 4000000000ull;
+constexpr uint64_t kDrainLimitNs = 1000000000ull;
+
+struct Params {
+  const void *x;
+  const void *a;
+  const int *ids;
+  const float *scaling;
+  int dtype;
+  int M, K, L, R, rank_pad;
+  float *h;
+  void *hl;
+  float *hscale;
+  int *tile_adapter;
+  int gemm_tiles, gemm_tile_tokens;
+  int split, kps, k_blocks;
+};
+
+__device__ __forceinline__ bool has_adapter(const Params &p, int id) {
+  return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L);
+}
+
+// Eight 16-bit values as floats.
+__device__ __forceinline__ void unpack8(const uint4 &v, bool f16, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (f16) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    } else {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+
+constexpr int FEW_ROWS = 8;   // rows per CTA
+constexpr int FEW_RANK = 4;   // values of h per row and CTA
+constexpr int FEW_WARPS = 8;  // K in chunks of 8 values over all lanes of all warps
+
+__global__ void __launch_bounds__(32 * FEW_WARPS) down_rows_kernel(const Params p) {
+  __shared__ float s_sum[FEW_WARPS][FEW_ROWS * FEW_RANK];
+  ptx::grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int m0 = blockIdx.x * FEW_ROWS;
+  const int r0 = blockIdx.y * FEW_RANK;
+  const bool f16 = p.dtype == kF16;
+  int id[FEW_ROWS];
+#pragma unroll
+  for (int i = 0; i < FEW_ROWS; ++i) {
+    id[i] = m0 + i < p.M ? __ldg(p.ids + m0 + i) : -1;
+    if (!has_adapter(p, id[i])) id[i] = -1;
+  }
+  float acc[FEW_ROWS][FEW_RANK];
+#pragma unroll
+  for (int i = 0; i < FEW_ROWS; ++i)
+#pragma unroll
+    for (int r = 0; r < FEW_RANK; ++r) acc[i][r] = 0.0f;
+  const uint4 *x4 = reinterpret_cast<const uint4 *>(p.x);
+  const uint4 *a4 = reinterpret_cast<const uint4 *>(p.a);
+  const int chunks = p.K / 8;  // K % 16 == 0
+  for (int c = threadIdx.x; c < chunks; c += 32 * FEW_WARPS) {
+    int cur = -1;
+    uint4 aw[FEW_RANK];
+#pragma unroll
+    for (int r = 0; r < FEW_RANK; ++r) aw[r] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < FEW_ROWS; ++i) {
+      if (id[i] < 0) continue;  // uniform in the CTA
+      if (id[i] != cur) {
+        cur = id[i];
+#pragma unroll
+        for (int r = 0; r < FEW_RANK; ++r)  // (R % 8 == 0: r0 + r < R)
+          aw[r] = __ldg(a4 + (static_cast<int64_t>(cur) * p.R + r0 + r) * chunks + c);
+      }
+      float xv[8];
+      unpack8(__ldg(x4 + static_cast<int64_t>(m0 + i) * chunks + c), f16, xv);
+#pragma unroll
+      for (int r = 0; r < FEW_RANK; ++r) {
+        float av[8];
+        unpack8(aw[r], f16, av);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][r] = fmaf(xv[j], av[j], acc[i][r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FEW_ROWS; ++i)
+#pragma unroll
+    for (int r = 0; r < FEW_RANK; ++r) {
+      float v = acc[i][r];
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+      if (lane == 0) s_sum[warp][i * FEW_RANK + r] = v;
+    }
+  __syncthreads();
+  ptx::grid_dependency_wait();  // (every thread: the GEMM's wait covers the quantizer too)
+  if (threadIdx.x < FEW_ROWS * FEW_RANK) {
+    const int i = threadIdx.x / FEW_RANK, r = threadIdx.x % FEW_RANK;
+    const int m = m0 + i;
+    const int a = m < p.M ? __ldg(p.ids + m) : -1;
+    if (has_adapter(p, a)) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < FEW_WARPS; ++w) v += s_sum[w][threadIdx.x];
+      p.h[static_cast<int64_t>(m) * p.R + r0 + r] = v * __ldg(p.scaling + a);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- many rows
+
+constexpr int ROWS = 128;
+constexpr int KB = 64;     // 16-bit elements per K-block: one 128-byte swizzle row
+constexpr int COLS = 128;  // columns (adapters x rank_pad) per pass
+constexpr int STAGES = 4;
+constexpr int NUM_THREADS = 192;
+constexpr uint32_t X_STAGE = ROWS * 128;
+constexpr uint32_t A_STAGE = COLS * 128;
+constexpr uint32_t STAGE = X_STAGE + A_STAGE;
+constexpr uint32_t OFF_PART = STAGES * STAGE;  // fp32 [ROWS][rank_pad + 1]
+constexpr uint32_t SMEM_BYTES = OFF_PART + ROWS * (kLoraMaxRank + 1) * 4 + 1024;
+constexpr int MAX_SPLIT = 8;
+static_assert(SMEM_BYTES <= 231424, "shared memory budget (the static part is below 2 KB)");
+
+__device__ __forceinline__ void record_timeout(volatile int *abort) {
+  if (!*abort) {
+    atomicOr(&g_lora_status, 128u);
+    *abort = 1;
+  }
+}
+
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    down_tile_kernel(const __grid_constant__ CUtensorMap tmap_x,
+                     const __grid_constant__ CUtensorMap tmap_a,
+                     const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t sbase = ptx::smem_u32(smem);
+  __shared__ alignas(8) uint64_t s_bar[2 * STAGES + 3];
+  __shared__ uint32_t s_slot;
+  __shared__ int s_abort;
+  __shared__ int s_id[ROWS];     // adapter of each row, -1: none
+  __shared__ int s_first[ROWS];  // the row's adapter appears first at this row of the tile
+  __shared__ int s_rank[ROWS];   // .. and is this one of the tile's adapters
+  __shared__ int s_list[ROWS];   // the tile's adapters
+  __shared__ int s_count[5];
+  const uint32_t bar_full = ptx::smem_u32(s_bar);
+  const uint32_t bar_empty = bar_full + 8 * STAGES;
+  const uint32_t bar_acc = bar_empty + 8 * STAGES;
+  const uint32_t bar_free = bar_acc + 8;
+  const uint32_t bar_drain = bar_free + 8;
+  volatile int *abort = &s_abort;
+  float *part = reinterpret_cast<float *>(smem + OFF_PART);
+  const int pitch = p.rank_pad + 1;  // odd: a column of it hits all banks
+
+  ptx::grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const int m0 = static_cast<int>(blockIdx.x / p.split) * ROWS;
+
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tmap(&tmap_x);
+    ptx::prefetch_tmap(&tmap_a);
+    for (int s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(bar_full + 8 * s, 1);
+      ptx::mbar_init(bar_empty + 8 * s, 1);
+    }
+    ptx::mbar_init(bar_acc, 1);
+    ptx::mbar_init(bar_free, 4);
+    ptx::mbar_init(bar_drain, 1);
+    s_abort = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(&s_slot), COLS);
+    ptx::tmem_relinquish<1>();
+  }
+  // The tile's adapters, in the order of their first rows.
+  const int me = threadIdx.x;
+  if (me < ROWS) {
+    const int id = m0 + me < p.M ? __ldg(p.ids + m0 + me) : -1;
+    s_id[me] = has_adapter(p, id) ? id : -1;
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *const_cast<volatile uint32_t *>(&s_slot);
+  bool first = false;
+  if (me < ROWS) {
+    int f = me;
+    if (s_id[me] >= 0)
+      for (f = 0; s_id[f] != s_id[me]; ++f) {
+      }
+    first = s_id[me] >= 0 && f == me;
+    s_first[me] = f;
+    const uint32_t votes = __ballot_sync(0xFFFFFFFFu, first);
+    s_rank[me] = __popc(votes & ((1u << lane) - 1u));
+    if (lane == 0) s_count[warp] = __popc(votes);
+  }
+  __syncthreads();
+  int before = 0, distinct = 0;
+  for (int w = 0; w < ROWS / 32; ++w) {
+    if (w < warp) before += s_count[w];
+    distinct += s_count[w];
+  }
+  if (me < ROWS) {
+    s_rank[me] += before;
+    if (first) s_list[s_rank[me]] = s_id[me];
+  }
+  __syncthreads();
+
+  const int per_pass = COLS / p.rank_pad;
+  const int passes = (distinct + per_pass - 1) / per_pass;
+  const int kb0 = rank * p.kps;
+  const int nkb = min(p.k_blocks, kb0 + p.kps) - kb0;  // >= 1 (the host's split)
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t issued = 0;
+      bool ok = true;
+      for (int ps = 0; ps < passes && ok; ++ps) {
+        const int d0 = ps * per_pass, nd = min(per_pass, distinct - d0);
+        for (int i = 0; i < nkb; ++i) {
+          if (!ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort, kWaitLimitNs)) {
+            record_timeout(abort);
+            ok = false;
+            break;
+          }
+          const uint32_t fb = bar_full + 8 * stage;
+          const uint32_t dst = sbase + static_cast<uint32_t>(stage) * STAGE;
+          ptx::mbar_arrive_expect_tx(fb, X_STAGE + static_cast<uint32_t>(nd * p.rank_pad) * 128u);
+          ptx::tma_load_2d(dst, &tmap_x, (kb0 + i) * KB, m0, fb);
+          for (int d = 0; d < nd; ++d)  // ranks past R read as zero
+            ptx::tma_load_3d(dst + X_STAGE + static_cast<uint32_t>(d * p.rank_pad) * 128u, &tmap_a,
+                             (kb0 + i) * KB, 0, s_list[d0 + d], fb);
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      const uint32_t n_drain = issued < STAGES ? issued : STAGES;
+      for (uint32_t i = 0; i < n_drain; ++i) {
+        if (stage == 0) {
+          stage = STAGES - 1;
+          phase ^= 1u;
+        } else {
+          --stage;
+        }
+        ptx::mbar_wait_timeout(bar_empty + 8 * stage, phase, kDrainLimitNs);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int ps = 0; ps < passes && ok; ++ps) {
+        const int nd = min(per_pass, distinct - ps * per_pass);
+        const uint32_t idesc = ptx::idesc_f16_f32(ROWS, nd * p.rank_pad, p.dtype == kBF16);
+        if (ps > 0 && !ptx::mbar_wait_bounded(bar_free, static_cast<uint32_t>(ps - 1) & 1u, abort,
+                                              kWaitLimitNs)) {
+          record_timeout(abort);
+          break;
+        }
+        ptx::tc_fence_after();
+        for (int i = 0; i < nkb; ++i) {
+          if (!ptx::mbar_wait_bounded(bar_full + 8 * stage, phase, abort, kWaitLimitNs)) {
+            record_timeout(abort);
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t st = sbase + static_cast<uint32_t>(stage) * STAGE;
+          const uint64_t adesc = ptx::sw128_kmajor_desc(st);
+          const uint64_t bdesc = ptx::sw128_kmajor_desc(st + X_STAGE);
+#pragma unroll
+          for (int kk = 0; kk < KB / 16; ++kk)
+            ptx::mma_f16<1>(tmem, adesc + 2 * kk, bdesc + 2 * kk, idesc, (i | kk) != 0 ? 1u : 0u);
+          ptx::mma_commit(bar_empty + 8 * stage);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) ptx::mma_commit(bar_acc);
+      }
+      ptx::mma_commit(bar_drain);
+      ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
+    }
+  } else {
+    // TMEM lane = row: keep the columns of the row's own adapter
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const int mine = s_id[row] >= 0 ? s_rank[s_first[row]] : -1;
+    for (int ps = 0; ps < passes; ++ps) {
+      const int d0 = ps * per_pass, nd = min(per_pass, distinct - d0);
+      if (!ptx::mbar_wait_bounded(bar_acc, static_cast<uint32_t>(ps) & 1u, abort, kWaitLimitNs)) {
+        if (lane == 0) record_timeout(abort);
+        break;
+      }
+      ptx::tc_fence_after();
+      for (int d = 0; d < nd; ++d) {
+        const bool keep = mine == d0 + d;
+        if (!__any_sync(0xFFFFFFFFu, keep)) continue;
+        for (int c = 0; c < p.rank_pad; c += 16) {
+          uint32_t r[16];
+          ptx::tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                      static_cast<uint32_t>(d * p.rank_pad + c),
+                                  r);
+          ptx::tmem_wait_ld();
+          if (keep) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) part[row * pitch + c + j] = __uint_as_float(r[j]);
+          }
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar_free);
+    }
+  }
+
+  __syncwarp();
+  __syncthreads();
+  ptx::cluster_sync();  // every CTA's partial sums are in its shared memory
+  ptx::grid_dependency_wait();
+
+  // Row by row: add the K-splits in rank order, scale, split into the two parts. CTA `rank`
+  // of the cluster has rows rank, rank + split, ..; a warp has a row, a lane four values.
+  const uint32_t part_base = ptx::smem_u32(part);
+  const bool f16 = p.dtype == kF16;
+  const bool fine = *abort == 0;
+  for (int row = rank + warp * p.split; row < ROWS && fine; row += NUM_THREADS / 32 * p.split) {
+    const int id = s_id[row];
+    if (id < 0) continue;
+    const float sc = __ldg(p.scaling + id);
+    float v[kLoraMaxRank / 32];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kLoraMaxRank / 32; ++i) {
+      const int c = i * 32 + lane;
+      v[i] = 0.0f;
+      if (c < p.R) {
+        const uint32_t at = part_base + static_cast<uint32_t>(row * pitch + c) * 4u;
+        for (int s = 0; s < p.split; ++s)
+          v[i] += ptx::ld_shared_cluster_f32(ptx::map_shared_rank(at, s));
+        v[i] *= sc;
+        const float a = fabsf(v[i]);
+        if (a <= 3.402823466e38f) top = fmaxf(top, a);  // finite values only
+      }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    // f16: the row divided by 2^ex, its largest finite value's exponent (exact)
+    int ex = 0;
+    if (f16 && top > 0.0f)
+      ex = min(126, max(-126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+    const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+    const int64_t base = static_cast<int64_t>(m0 + row) * (2 * p.rank_pad);
+#pragma unroll
+    for (int i = 0; i < kLoraMaxRank / 32; ++i) {
+      const int c = i * 32 + lane;
+      if (c >= p.rank_pad) break;
+      const float t = v[i] * inv;
+      // an infinity or NaN is the high part's alone
+      if (f16) {
+        const __half hi = __float2half_rn(t);
+        const float back = __half2float(hi);
+        __half *dst = reinterpret_cast<__half *>(p.hl) + base;
+        dst[c] = hi;
+        dst[p.rank_pad + c] = __float2half_rn(fabsf(back) <= 65504.0f ? t - back : 0.0f);
+      } else {
+        const __nv_bfloat16 hi = __float2bfloat16_rn(t);
+        const float back = __bfloat162float(hi);
+        __nv_bfloat16 *dst = reinterpret_cast<__nv_bfloat16 *>(p.hl) + base;
+        dst[c] = hi;
+        dst[p.rank_pad + c] =
+            __float2bfloat16_rn(fabsf(back) <= 3.402823466e38f ? t - back : 0.0f);
+      }
+    }
+    if (lane == 0)
+      p.hscale[m0 + row] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+  }
+  // The adapter of each token tile of the GEMM: one for all rows, none, or several (-2).
+  for (int t = static_cast<int>(blockIdx.x) * (NUM_THREADS / 32) + warp; t < p.gemm_tiles;
+       t += static_cast<int>(gridDim.x) * (NUM_THREADS / 32)) {
+    const int t0 = t * p.gemm_tile_tokens, t1 = min(p.M, t0 + p.gemm_tile_tokens);
+    int lead = __ldg(p.ids + t0);
+    if (!has_adapter(p, lead)) lead = -1;
+    bool same = true;
+    for (int m = t0 + lane; m < t1; m += 32) {
+      int id = __ldg(p.ids + m);
+      if (!has_adapter(p, id)) id = -1;
+      same = same && id == lead;
+    }
+    same = __all_sync(0xFFFFFFFFu, same);
+    if (lane == 0) p.tile_adapter[t] = same ? lead : -2;
+  }
+
+  ptx::cluster_sync();  // peers may still be reading this CTA's partial sums
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<1>(tmem, COLS);
+  }
+}
+
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+}  // namespace lora
+
+LoraWorkspace lora_workspace(void *base, int64_t M, int64_t R) {
+  LoraWorkspace w;
+  uint8_t *b = static_cast<uint8_t *>(base);
+  if (M <= kLoraRowsMaxM) {
+    w.h = reinterpret_cast<float *>(b);
+    w.bytes = lora::align256(static_cast<size_t>(M) * R * 4);
+    return w;
+  }
+  const size_t hl = lora::align256(static_cast<size_t>(M) * 2 * lora_rank_pad(R) * 2);
+  const size_t sc = lora::align256(static_cast<size_t>(M) * 4);
+  w.hl = b;
+  w.hscale = reinterpret_cast<float *>(b + hl);
+  w.tile_adapter = reinterpret_cast<int *>(b + hl + sc);
+  w.bytes = hl + sc + lora::align256(static_cast<size_t>(lora_tiles(M)) * 4);
+  return w;
+}
+
+int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
+  using namespace lora;
+  DeviceInfo dev;
+  if (!current_device_info(&dev)) return 5;
+  const LoraWorkspace w = lora_workspace(a.workspace, a.M, a.R);
+  Params p = {};
+  p.x = a.x;
+  p.a = a.lora_a;
+  p.ids = a.ids;
+  p.scaling = a.scaling;
+  p.dtype = a.dtype;
+  p.M = static_cast<int>(a.M);
+  p.K = static_cast<int>(a.K);
+  p.L = static_cast<int>(a.L);
+  p.R = static_cast<int>(a.R);
+  p.rank_pad = static_cast<int>(lora_rank_pad(a.R));
+  p.h = w.h;
+  p.hl = w.hl;
+  p.hscale = w.hscale;
+  p.tile_adapter = w.tile_adapter;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e;
+  if (a.M <= kLoraRowsMaxM) {
+    cfg.gridDim = dim3(static_cast<unsigned>((a.M + FEW_ROWS - 1) / FEW_ROWS),
+                       static_cast<unsigned>(a.R / FEW_RANK));
+    cfg.blockDim = dim3(32 * FEW_WARPS);
+    e = cudaLaunchKernelEx(&cfg, down_rows_kernel, p);
+  } else {
+    p.gemm_tiles = static_cast<int>(lora_tiles(a.M));
+    p.gemm_tile_tokens = static_cast<int>(lora_tile_tokens(a.M));
+    p.k_blocks = static_cast<int>((a.K + KB - 1) / KB);
+    const int64_t tiles = (a.M + ROWS - 1) / ROWS;
+    // K-splits while CTAs are left over, four K-blocks at least for each
+    const int split = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>({dev.sm_count / tiles, MAX_SPLIT, (p.k_blocks + 3) / 4})));
+    p.kps = (p.k_blocks + split - 1) / split;
+    p.split = (p.k_blocks + p.kps - 1) / p.kps;
+    const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    std::string err;
+    CUtensorMap tx, ta;
+    if (!make_tmap_2d_sw128(&tx, t16, a.x, a.K, a.M, a.K * 2, KB, ROWS, &err) ||
+        !make_tmap_3d_sw128(&ta, t16, a.lora_a, a.K, a.R, a.L, a.K * 2, a.R * a.K * 2, KB,
+                            static_cast<uint32_t>(p.rank_pad), &err)) {
+      set_error("fp8_linear_lora: " + err);
+      return 4;
+    }
+    static bool set[64];
+    static std::mutex mu;
+    {
+      std::lock_guard<std::mutex> lock(mu);
+      if (!set[dev.device & 63]) {
+        e = cudaFuncSetAttribute(down_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(SMEM_BYTES));
+        if (e != cudaSuccess) {
+          set_error(std::string("fp8_linear_lora: kernel setup: ") + cudaGetErrorString(e));
+          return 4;
+        }
+        set[dev.device & 63] = true;
+      }
+    }
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(p.split);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.split));
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    e = cudaLaunchKernelEx(&cfg, down_tile_kernel, tx, ta, p);
+  }
+  if (e != cudaSuccess) {
+    set_error(std::string("fp8_linear_lora: launch failed: ") + cudaGetErrorString(e));
+    return 4;
+  }
+  return 0;
+}
+
+cudaError_t read_lora_status(unsigned int *bits, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(bits, g_lora_status, sizeof(unsigned int));
+  if (e != cudaSuccess) return e;
+  if (clear) {
+    const unsigned int zero = 0;
+    e = cudaMemcpyToSymbol(g_lora_status, &zero, sizeof(unsigned int));
+  }
+  return e;
+}
+
+}  // namespace fp8lin

@@ -1,0 +1,1142 @@
+// rowsel_sm100.cu -- e4m3 linears whose weights depend on the row: rows grouped by expert,
+// and one shared projection with a low-rank adapter per row.
+//
+//   grouped:  out[i,n] = fma(acc[i,n] * xs[i], ws[e,n], bias[e,n]),  e the expert of row i
+//   adapters: out[i,n] = fma(acc[i,n] * xs[i], ws[n], bias[n]) + sum_r h[i,r] B[a_i][n,r]
+//   acc[i,n] = sum_k e4m3(xq[i,k]) * e4m3(wq[.,n,k])      (fp32, tensor cores)
+//
+// Both kernels here put the weights on the MMA's M side (D^T = W . X^T): 128 weight rows per
+// CTA fill the tensor core's 128 rows whatever the group's size, and a group of few tokens
+// only narrows N (a multiple of 16, 32 for a CTA pair), which the instruction descriptor
+// gives per tile. A tile is (expert, block of weight rows, block of tokens); token blocks
+// never cross an expert's border, and the tokens of a group are split evenly. The table of
+// tiles is made by every CTA from the offsets, which are device data.
+//
+//   persist_kernel<CG, LORA>  persistent CTAs (CG = 2: pairs, 256 weight rows x up to 256
+//       tokens; CG = 1: 128 x up to 128, for groups of few rows), TMA ring, two TMEM
+//       accumulators, epilogue of one tile under the main loop of the next.
+//   split_kernel<LORA>  when all tiles together do not fill the GPU: a cluster of CTAs per
+//       tile splits K and adds its partial tiles through distributed shared memory, in rank
+//       order (the result does not depend on timing).
+//
+// Rows outside the experts' ranges are written as zeros. Offsets are clamped to [0, M] and to
+// their running maximum, so that no value of them leads outside a tensor.
+// Every mbarrier wait is bounded; a wait that runs out sets bit 64 of the device status.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <mutex>
+#include <string>
+
+#include "internal.h"
+#include "ptx.cuh"
+
+namespace fp8lin {
+
+__device__ unsigned int g_rowsel_status;  // watchdog bits (64 = a wait ran out)
+
+namespace rowsel {
+
+constexpr int WROWS = 128;  // weight rows per CTA = MMA M (per CTA)
+constexpr int BK = 128;     // bytes (= e4m3 elements) per K-block: one 128-byte swizzle row
+constexpr int UMMA_K = 32;  // bytes of K per MMA
+constexpr int NUM_THREADS = 192;
+constexpr int EPI_WARPS = 4;
+constexpr uint32_t W_STAGE = WROWS * BK;  // 16 KB
+constexpr int X_MAPS = 8;                 // token boxes of 16, 32, .. 128 rows
+constexpr int H_MAPS = kLoraTileTokens / 32;  // boxes of the adapters' h: 16, 32, .. 80 rows
+constexpr uint64_t kWaitLimitNs = 4000000000ull;
+constexpr uint64_t kDrainLimitNs = 1000000000ull;
+
+struct Maps {
+  CUtensorMap x[X_MAPS];  // xq [M][K], box 128 B x 16 (i + 1) rows
+  CUtensorMap w;          // wq [E][N][K], box 128 B x 128 rows x 1
+  CUtensorMap lb;         // lora_b [L][N][R], box 64 x 128 rows x 1
+  CUtensorMap h[H_MAPS];  // hl [M][2 rank_pad], box 64 x 16 (i + 1) rows
+};
+
+struct Params {
+  const float *xs;
+  const float *ws;
+  const void *bias;
+  int bias_dtype;
+  void *out;
+  int out_dtype;
+  const int *offsets;  // null: one group of all rows
+  int M, N, E;
+  int k_blocks;
+  int n_wb;        // blocks of weight rows
+  int pdl, pre_w;  // pre_w: weights and offsets may be read before the dependency wait
+  // split_kernel
+  int split, kps, stages;
+  int tok_cap;        // tokens per tile at most
+  uint32_t off_part;  // shared-memory offsets
+  uint32_t off_lora;
+  uint32_t off_tab;
+  // adapters
+  const int *ids;
+  const void *lora_b;
+  int lora_dtype;
+  int L, R, rank_pad;
+  const int *tile_adapter;  // persist_kernel
+  const void *hl;
+  const float *hscale;
+  const float *h;           // split_kernel
+};
+
+__device__ __forceinline__ float load_bias(const void *bias, int dtype, int64_t n) {
+  switch (dtype) {
+    case kBF16: {
+      const uint16_t b = __ldg(reinterpret_cast<const unsigned short *>(bias) + n);
+      return __uint_as_float(static_cast<uint32_t>(b) << 16);
+    }
+    case kF16: return __half2float(__ldg(reinterpret_cast<const __half *>(bias) + n));
+    case kF32: return __ldg(reinterpret_cast<const float *>(bias) + n);
+    default: return 0.0f;
+  }
+}
+
+__device__ __forceinline__ void store_out(void *out, int dtype, int64_t i, float v) {
+  if (dtype == kF16)
+    reinterpret_cast<__half *>(out)[i] = __float2half_rn(v);
+  else
+    reinterpret_cast<__nv_bfloat16 *>(out)[i] = __float2bfloat16_rn(v);
+}
+
+// Eight 16-bit values as floats.
+__device__ __forceinline__ void unpack8(const uint4 &v, bool f16, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (f16) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    } else {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+
+__device__ __forceinline__ void record_timeout(volatile int *abort) {
+  if (!*abort) {
+    atomicOr(&g_rowsel_status, 64u);
+    *abort = 1;
+  }
+}
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// The groups' rows and tiles, in shared memory: row[e] .. row[e + 1] are the rows of group e,
+// tile[e] its first tile. Called by the whole CTA; ends with a CTA barrier.
+__device__ __forceinline__ void build_groups(const Params &p, int tok_max, int *row, int *tile) {
+  const int E = p.E;
+  if (p.offsets == nullptr) {
+    if (threadIdx.x == 0) {
+      row[0] = 0;
+      row[1] = p.M;
+      tile[0] = 0;
+      tile[1] = ceil_div(p.M, tok_max) * p.n_wb;
+    }
+    __syncthreads();
+    return;
+  }
+  for (int i = threadIdx.x; i <= E; i += NUM_THREADS)
+    row[i] = min(max(__ldg(p.offsets + i), 0), p.M);
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int carry = 0;  // running maximum of the offsets before this chunk
+    for (int b = 0; b <= E; b += 32) {
+      const int i = b + lane;
+      int v = i <= E ? row[i] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        if (lane >= d) v = max(v, u);
+      }
+      v = max(v, carry);
+      if (i <= E) row[i] = v;
+      carry = __shfl_sync(0xFFFFFFFFu, v, 31);
+    }
+    __syncwarp();
+    int first = 0;
+    for (int b = 0; b <= E; b += 32) {
+      const int i = b + lane;
+      const int n = i < E ? ceil_div(row[i + 1] - row[i], tok_max) * p.n_wb : 0;
+      int v = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        if (lane >= d) v += u;
+      }
+      if (i <= E) tile[i] = first + v - n;
+      first += __shfl_sync(0xFFFFFFFFu, v, 31);
+    }
+  }
+  __syncthreads();
+}
+
+struct Tile {
+  int e;       // group
+  int wb;      // block of weight rows
+  int t0, t1;  // tokens
+  int nn;      // MMA N: tokens padded to a multiple of 16 x CG
+  int tb;      // token block within the group
+};
+
+// Tile t of the table; `e` is a group at or before the tile's (advanced to it).
+template <int CG>
+__device__ __forceinline__ Tile find_tile(const Params &p, int tok_max, const int *row,
+                                          const int *tile, int t, int &e) {
+  while (tile[e + 1] <= t) ++e;
+  Tile q;
+  q.e = e;
+  const int r0 = row[e], rows = row[e + 1] - r0;
+  const int n_tb = ceil_div(rows, tok_max);
+  const int per = (ceil_div(rows, n_tb) + 16 * CG - 1) / (16 * CG) * (16 * CG);
+  const int l = t - tile[e];
+  // The larger operand of the group streams once, the tiles that run side by side share the
+  // smaller one through L2.
+  if (rows >= p.N) {
+    q.tb = l / p.n_wb;
+    q.wb = l - q.tb * p.n_wb;
+  } else {
+    q.wb = l / n_tb;
+    q.tb = l - q.wb * n_tb;
+  }
+  q.t0 = r0 + q.tb * per;
+  q.t1 = min(r0 + rows, q.t0 + per);
+  q.nn = (q.t1 - q.t0 + 16 * CG - 1) / (16 * CG) * (16 * CG);
+  return q;
+}
+
+// Zeros to the rows that no group holds; the `n` threads from `first` of every CTA.
+__device__ __forceinline__ void zero_rows(const Params &p, const int *row, int first, int n) {
+  const int lo = row[0], hi = row[p.E];
+  const int todo = lo + p.M - hi;
+  uint16_t *out = reinterpret_cast<uint16_t *>(p.out);
+  for (int i = blockIdx.x; i < todo; i += gridDim.x) {
+    uint16_t *dst = out + static_cast<int64_t>(i < lo ? i : i - lo + hi) * p.N;
+    for (int c = static_cast<int>(threadIdx.x) - first; c < p.N; c += n) dst[c] = 0;
+  }
+}
+
+// ---------------------------------------------------------------- persistent kernel
+
+template <int CG, bool LORA>
+struct Cfg {
+  static constexpr int TOK_MAX = LORA ? kLoraTileTokens : CG == 2 ? 256 : 128;
+  static constexpr int X_ROWS = TOK_MAX / CG;  // tokens this CTA loads, at most
+  static constexpr uint32_t X_STAGE = X_ROWS * BK;
+  static constexpr uint32_t STAGE = W_STAGE + X_STAGE;
+  static constexpr int STAGES = LORA ? 7 : 6;
+  // TMEM: two accumulators; the adapters' products have a third, which only the epilogue of
+  // one tile holds at a time
+  static constexpr uint32_t ACC1 = TOK_MAX;
+  static constexpr uint32_t ACC_L = 2 * TOK_MAX;
+  static constexpr uint32_t TMEM_COLS = CG == 1 && !LORA ? 256 : 512;
+  static constexpr uint32_t OFF_PAR = STAGES * STAGE;
+  static constexpr uint32_t PAR_WARP = TOK_MAX * 4u * (LORA ? 3u : 1u);  // xs (hscale, ids)
+  static constexpr uint32_t OFF_TAB = OFF_PAR + EPI_WARPS * PAR_WARP;
+  static constexpr int TAB = LORA ? 2 : kMaxExperts + 1;
+  static constexpr uint32_t OFF_BAR = (OFF_TAB + 2 * TAB * 4 + 7u) & ~7u;
+  static constexpr uint32_t NUM_BARS = 2 * STAGES + 5;  // full, empty, tfull, tempty, drain
+  static constexpr uint32_t OFF_SLOT = OFF_BAR + NUM_BARS * 8;
+  static constexpr uint32_t SMEM_BYTES = OFF_SLOT + 8 + 1024;
+  static_assert(STAGE % 1024 == 0, "swizzle atoms need 1024 B alignment");
+  static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+  static_assert(!LORA || 3 * TOK_MAX <= 512, "TMEM budget");
+};
+
+template <int CG, bool LORA>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    persist_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  using C = Cfg<CG, LORA>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t sbase = ptx::smem_u32(smem);
+  const uint32_t bar_full = sbase + C::OFF_BAR;
+  const uint32_t bar_empty = bar_full + C::STAGES * 8;
+  const uint32_t bar_tfull = bar_empty + C::STAGES * 8;
+  const uint32_t bar_tempty = bar_tfull + 2 * 8;
+  const uint32_t bar_drain = bar_tempty + 2 * 8;
+  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + C::OFF_SLOT);
+  volatile int *abort = reinterpret_cast<volatile int *>(smem + C::OFF_SLOT + 4);
+  int *g_row = reinterpret_cast<int *>(smem + C::OFF_TAB);
+  int *g_tile = g_row + C::TAB;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? ptx::cluster_ctarank() : 0u;  // 0 = leader (issues MMAs)
+  const bool leader = rank == 0;
+  const int group = blockIdx.x / CG;
+  const int n_groups = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tmap(&maps.w);
+    for (int s = 0; s < C::STAGES; ++s) {
+      ptx::mbar_init(bar_full + 8 * s, 1);
+      ptx::mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(bar_tfull + 8 * a, 1);
+      ptx::mbar_init(bar_tempty + 8 * a, EPI_WARPS * CG);
+    }
+    ptx::mbar_init(bar_drain, 1);
+    *abort = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<CG>(sbase + C::OFF_SLOT, C::TMEM_COLS);
+    ptx::tmem_relinquish<CG>();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) ptx::cluster_sync();  // peer barriers initialised before any signal
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
+  if (p.pdl) ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  if (!p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
+
+  const int num_tiles = g_tile[p.E];
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t issued = 0;
+      int e = 0;
+      // One stage: the weight box and the token box at the given coordinates.
+      auto load = [&](const CUtensorMap *mw, int wx, int wy, int wz, const CUtensorMap *mx, int xx,
+                      int xy, int nn) -> bool {
+        if (!ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort, kWaitLimitNs)) {
+          record_timeout(abort);
+          return false;
+        }
+        const uint32_t fb = bar_full + 8 * stage;
+        const uint32_t dst = sbase + static_cast<uint32_t>(stage) * C::STAGE;
+        const uint32_t tx = CG * W_STAGE + static_cast<uint32_t>(nn) * BK;
+        if constexpr (CG == 1) {
+          ptx::mbar_arrive_expect_tx(fb, tx);
+          ptx::tma_load_3d(dst, mw, wx, wy, wz, fb);
+          ptx::tma_load_2d(dst + W_STAGE, mx, xx, xy, fb);
+        } else {
+          // both CTAs' bytes complete the leader's barrier; only the leader arms it
+          if (leader) ptx::mbar_arrive_expect_tx(fb, tx);
+          const uint32_t fl = ptx::map_shared_rank(fb, 0);
+          ptx::tma_load_3d_pair(dst, mw, wx, wy, wz, fl);
+          ptx::tma_load_2d_pair(dst + W_STAGE, mx, xx, xy, fl);
+        }
+        ++issued;
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+        return true;
+      };
+      bool ok = true;
+      for (int t = group; t < num_tiles && ok; t += n_groups) {
+        const Tile q = find_tile<CG>(p, C::TOK_MAX, g_row, g_tile, t, e);
+        const int wrow = (q.wb * CG + static_cast<int>(rank)) * WROWS;
+        const int xrows = q.nn / CG;
+        const int xrow = q.t0 + static_cast<int>(rank) * xrows;
+        const int mi = xrows / 16 - 1;
+        for (int kb = 0; kb < p.k_blocks && ok; ++kb)
+          ok = load(&maps.w, kb * BK, wrow, q.e, &maps.x[mi], kb * BK, xrow, q.nn);
+        if constexpr (LORA) {
+          const int a = __ldg(p.tile_adapter + q.tb);
+          if (a >= 0) {
+            // the adapter's B rows and the tokens' h as further stages (64 16-bit elements
+            // are 128 bytes): up to rank 32 the high and low parts of h share a stage
+            const int parts = p.rank_pad <= 32 ? 1 : 2;
+            for (int part = 0; part < parts; ++part)
+              for (int c = 0; c < p.rank_pad && ok; c += 64)
+                ok = load(&maps.lb, c, wrow, a, &maps.h[mi], part * p.rank_pad + c, xrow, q.nn);
+          }
+        }
+      }
+      // Drain: every load issued here has landed and been consumed.
+      const uint32_t n_drain = issued < C::STAGES ? issued : C::STAGES;
+      for (uint32_t i = 0; i < n_drain; ++i) {
+        if (stage == 0) {
+          stage = C::STAGES - 1;
+          phase ^= 1u;
+        } else {
+          --stage;
+        }
+        ptx::mbar_wait_timeout(bar_empty + 8 * stage, phase, kDrainLimitNs);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && leader) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;
+      int e = 0;
+      bool ok = true;
+      auto next_stage = [&]() {
+        // the stage is reusable (in both CTAs) once its MMAs have read it
+        if constexpr (CG == 1)
+          ptx::mma_commit(bar_empty + 8 * stage);
+        else
+          ptx::mma_commit_pair_mc(bar_empty + 8 * stage, 0x3);
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      };
+      auto wait_full = [&]() -> bool {
+        if (!ptx::mbar_wait_bounded(bar_full + 8 * stage, phase, abort, kWaitLimitNs)) {
+          record_timeout(abort);
+          return false;
+        }
+        ptx::tc_fence_after();
+        return true;
+      };
+      for (int t = group; t < num_tiles && ok; t += n_groups, ++it) {
+        const Tile q = find_tile<CG>(p, C::TOK_MAX, g_row, g_tile, t, e);
+        const int acc = it & 1;
+        const uint32_t acc_phase = (it >> 1) & 1;
+        if (!ptx::mbar_wait_bounded(bar_tempty + 8 * acc, acc_phase ^ 1u, abort, kWaitLimitNs)) {
+          record_timeout(abort);
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t d = tmem_base + (acc ? C::ACC1 : 0u);
+        const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS * CG, q.nn);
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!(ok = wait_full())) break;
+          const uint32_t st = sbase + static_cast<uint32_t>(stage) * C::STAGE;
+          const uint64_t adesc = ptx::sw128_kmajor_desc(st);
+          const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+            const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
+            const uint32_t accumulate = (kb | kk) != 0 ? 1u : 0u;
+            if constexpr (CG == 1)
+              ptx::mma_f8f6f4(d, adesc + koff, bdesc + koff, idesc, accumulate);
+            else
+              ptx::mma_f8f6f4_pair(d, adesc + koff, bdesc + koff, idesc, accumulate);
+          }
+          next_stage();
+        }
+        if constexpr (LORA) {
+          const int a = ok ? __ldg(p.tile_adapter + q.tb) : -1;
+          if (a >= 0) {
+            // the third accumulator is free once the epilogue of the tile before has let
+            // its own go (the same arrival that this loop waits for one tile later)
+            if (it > 0 && !ptx::mbar_wait_bounded(bar_tempty + 8 * (acc ^ 1),
+                                                  static_cast<uint32_t>((it - 1) >> 1) & 1u, abort,
+                                                  kWaitLimitNs)) {
+              record_timeout(abort);
+              break;
+            }
+            ptx::tc_fence_after();
+            const uint32_t dl = tmem_base + C::ACC_L;
+            const uint32_t id16 =
+                ptx::idesc_f16_f32(WROWS * CG, q.nn, p.lora_dtype == kBF16);
+            uint32_t accumulate = 0;
+            const int parts = p.rank_pad <= 32 ? 1 : 2;
+            for (int part = 0; part < parts && ok; ++part)
+              for (int c = 0; c < p.rank_pad; c += 64) {
+                if (!(ok = wait_full())) break;
+                const uint32_t st = sbase + static_cast<uint32_t>(stage) * C::STAGE;
+                const uint64_t adesc = ptx::sw128_kmajor_desc(st);
+                const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
+                const int steps = min(64, p.rank_pad - c) / 16;  // 16 elements = 32 bytes
+                for (int kk = 0; kk < steps; ++kk) {
+                  ptx::mma_f16<CG>(dl, adesc + 2 * kk, bdesc + 2 * kk, id16, accumulate);
+                  accumulate = 1;
+                }
+                if (parts == 1)  // low part: next to the high part in the same box
+                  for (int kk = 0; kk < steps; ++kk)
+                    ptx::mma_f16<CG>(dl, adesc + 2 * kk, bdesc + 2 * (kk + steps), id16, 1);
+                next_stage();
+              }
+          }
+        }
+        if (!ok) break;
+        if constexpr (CG == 1)
+          ptx::mma_commit(bar_tfull + 8 * acc);
+        else
+          ptx::mma_commit_pair_mc(bar_tfull + 8 * acc, 0x3);
+      }
+      // No MMA may still be running when the CTAs free TMEM.
+      if constexpr (CG == 1)
+        ptx::mma_commit(bar_drain);
+      else
+        ptx::mma_commit_pair(bar_drain);
+      ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    // TMEM lane = weight row, column = token: a thread holds one output column, a warp
+    // stores 32 adjacent columns (64 bytes) of a token at a time.
+    const int quarter = warp & 3;
+    float *e_xs = reinterpret_cast<float *>(smem + C::OFF_PAR + (warp - 2) * C::PAR_WARP);
+    float *e_hs = e_xs + C::TOK_MAX;
+    int *e_id = reinterpret_cast<int *>(e_hs + C::TOK_MAX);
+    const bool f16 = LORA && p.lora_dtype == kF16;
+    int it = 0;
+    int e = 0;
+    for (int t = group; t < num_tiles; t += n_groups, ++it) {
+      const Tile q = find_tile<CG>(p, C::TOK_MAX, g_row, g_tile, t, e);
+      const int acc = it & 1;
+      const uint32_t acc_phase = (it >> 1) & 1;
+      const int cnt = q.t1 - q.t0;
+      const int n = (q.wb * CG + static_cast<int>(rank)) * WROWS + quarter * 32 + lane;
+      const bool live = n < p.N;
+      const int64_t wn = static_cast<int64_t>(q.e) * p.N + min(n, p.N - 1);
+      int adapter = -1;
+      if constexpr (LORA) adapter = __ldg(p.tile_adapter + q.tb);
+      __syncwarp();
+      for (int i = lane; i < cnt; i += 32) {
+        e_xs[i] = __ldg(p.xs + q.t0 + i);
+        if constexpr (LORA) {
+          e_hs[i] = adapter != -1 ? __ldg(p.hscale + q.t0 + i) : 0.0f;
+          e_id[i] = __ldg(p.ids + q.t0 + i);
+        }
+      }
+      const float w = __ldg(p.ws + wn);
+      const float b = load_bias(p.bias, p.bias_dtype, wn);
+      __syncwarp();
+      if (!ptx::mbar_wait_bounded(bar_tfull + 8 * acc, acc_phase, abort, kWaitLimitNs)) {
+        if (lane == 0) record_timeout(abort);
+        break;
+      }
+      ptx::tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+      for (int c = 0; c < cnt; c += 32) {
+        uint32_t r[32];
+        ptx::tmem_ld_32x32b_x32(t_row + (acc ? C::ACC1 : 0u) + static_cast<uint32_t>(c), r);
+        ptx::tmem_wait_ld();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[j]) * e_xs[min(c + j, cnt - 1)], w, b);
+        if constexpr (LORA) {
+          if (adapter >= 0) {
+            ptx::tmem_ld_32x32b_x32(t_row + C::ACC_L + static_cast<uint32_t>(c), r);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              v[j] = fmaf(__uint_as_float(r[j]), e_hs[min(c + j, cnt - 1)], v[j]);
+          } else if (adapter == -2) {
+            // A tile of several adapters: the sums over the rank on CUDA cores, each row
+            // with its own adapter's values only. The B rows of a run of equal ids are
+            // loaded once per 8 values of the rank.
+            float s[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[j] = 0.0f;
+            const uint16_t *hl = reinterpret_cast<const uint16_t *>(p.hl);
+            const uint16_t *lb = reinterpret_cast<const uint16_t *>(p.lora_b);
+            for (int rc = 0; rc < p.R; rc += 8) {
+              int cur = -1;
+              float bw[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) bw[i] = 0.0f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const int id = c + j < cnt ? e_id[c + j] : -1;
+                if (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L)) {
+                  if (id != cur) {
+                    cur = id;
+                    unpack8(__ldg(reinterpret_cast<const uint4 *>(
+                                lb + (static_cast<int64_t>(id) * p.N + min(n, p.N - 1)) * p.R +
+                                rc)),
+                            f16, bw);
+                  }
+                  const uint16_t *hr =
+                      hl + static_cast<int64_t>(q.t0 + c + j) * (2 * p.rank_pad) + rc;
+                  float hi[8], lo[8];
+                  unpack8(__ldg(reinterpret_cast<const uint4 *>(hr)), f16, hi);
+                  unpack8(__ldg(reinterpret_cast<const uint4 *>(hr + p.rank_pad)), f16, lo);
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) s[j] = fmaf(hi[i] + lo[i], bw[i], s[j]);
+                }
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const int id = c + j < cnt ? e_id[c + j] : -1;
+              if (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L))
+                v[j] = fmaf(s[j], e_hs[c + j], v[j]);
+            }
+          }
+        }
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < cnt)
+              store_out(p.out, p.out_dtype, static_cast<int64_t>(q.t0 + c + j) * p.N + n, v[j]);
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 1)
+          ptx::mbar_arrive(bar_tempty + 8 * acc);
+        else
+          ptx::mbar_arrive_cluster(ptx::map_shared_rank(bar_tempty + 8 * acc, 0));
+      }
+    }
+    zero_rows(p, g_row, 64, NUM_THREADS - 64);
+  }
+
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) ptx::cluster_sync();  // the leader's MMAs read the peer's memory
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<CG>(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- split-K kernel
+
+constexpr int SPLIT_TOK = 128;   // tokens per tile, at most
+constexpr int SPLIT_STAGES = 8;  // ring slots, at most
+constexpr int SPLIT_MAX = 8;     // CTAs per cluster, at most (portable)
+constexpr uint32_t SPLIT_EPI = (SPLIT_TOK + 2 * WROWS) * 4;  // xs, ws, bias of the reduction
+constexpr uint32_t SPLIT_SMEM = 232448;
+
+template <bool LORA>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t sbase = ptx::smem_u32(smem);
+  __shared__ alignas(8) uint64_t s_bar[2 * SPLIT_STAGES + 2];
+  __shared__ uint32_t s_slot;
+  __shared__ int s_abort;
+  const uint32_t bar_full = ptx::smem_u32(s_bar);
+  const uint32_t bar_empty = bar_full + 8 * SPLIT_STAGES;
+  const uint32_t bar_acc = bar_empty + 8 * SPLIT_STAGES;
+  const uint32_t bar_drain = bar_acc + 8;
+  volatile uint32_t *tmem_slot = &s_slot;
+  volatile int *abort = &s_abort;
+  float *part = reinterpret_cast<float *>(smem + p.off_part);  // [tokens][WROWS]
+  float *lora = reinterpret_cast<float *>(smem + p.off_lora);  // [tokens][rows reduced here]
+  int *g_row = reinterpret_cast<int *>(smem + p.off_tab);
+  int *g_tile = g_row + p.E + 1;
+  float *e_xs = reinterpret_cast<float *>(g_tile + p.E + 1);  // [SPLIT_TOK]
+  float *e_ws = e_xs + SPLIT_TOK;                              // [WROWS]
+  float *e_b = e_ws + WROWS;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const int stages = p.stages;
+  const uint32_t stage_bytes = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
+  uint32_t tmem_cols = 32;
+  while (tmem_cols < static_cast<uint32_t>(p.tok_cap)) tmem_cols <<= 1;
+
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tmap(&maps.w);
+    for (int s = 0; s < stages; ++s) {
+      ptx::mbar_init(bar_full + 8 * s, 1);
+      ptx::mbar_init(bar_empty + 8 * s, 1);
+    }
+    ptx::mbar_init(bar_acc, 1);
+    ptx::mbar_init(bar_drain, 1);
+    s_abort = 0;
+    ptx::fence_mbar_init();
+  }
+  if (!p.pre_w && p.pdl) ptx::grid_dependency_wait();
+  build_groups(p, p.tok_cap, g_row, g_tile);
+  const int t = blockIdx.x / p.split;
+  if (t >= g_tile[p.E]) {  // the whole cluster: fewer tiles than clusters
+    if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    zero_rows(p, g_row, 0, NUM_THREADS);
+    return;
+  }
+  int ge = 0;
+  const Tile q = find_tile<1>(p, p.tok_cap, g_row, g_tile, t, ge);
+  const int kb0 = rank * p.kps;
+  const int nkb = min(p.k_blocks, kb0 + p.kps) - kb0;  // >= 1 (the host's split)
+  const int cnt = q.t1 - q.t0;
+  const CUtensorMap *mx = &maps.x[q.nn / 16 - 1];
+  const uint32_t tx = W_STAGE + static_cast<uint32_t>(q.nn) * BK;
+
+  // The first stages' weight boxes go out at once: before the dependency wait where the
+  // weights cannot depend on the kernel before (pre_w).
+  auto weights_first = [&]() {
+    const int n = min(stages, nkb);
+    for (int i = 0; i < n; ++i) {
+      const uint32_t fb = bar_full + 8 * i;
+      ptx::mbar_arrive_expect_tx(fb, tx);
+      ptx::tma_load_3d(sbase + static_cast<uint32_t>(i) * stage_bytes, &maps.w, (kb0 + i) * BK,
+                       q.wb * WROWS, q.e, fb);
+    }
+  };
+  if (threadIdx.x == 0) weights_first();
+  if (warp == 1) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(&s_slot), tmem_cols);
+    ptx::tmem_relinquish<1>();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+
+  // rows of the tile that this CTA reduces
+  const int R = ((WROWS + p.split - 1) / p.split + 3) & ~3;
+  const int r0 = rank * R;
+  const int r1 = min(WROWS, r0 + R);
+  const int quads = r1 > r0 ? (r1 - r0) >> 2 : 0;
+  const int n0 = q.wb * WROWS;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const int first = min(stages, nkb);
+      for (int i = 0; i < first; ++i)
+        ptx::tma_load_2d(sbase + static_cast<uint32_t>(i) * stage_bytes + W_STAGE, mx,
+                         (kb0 + i) * BK, q.t0, bar_full + 8 * i);
+      int issued = first;
+      int s = first == stages ? 0 : first;
+      uint32_t ph = 1;
+      for (int i = first; i < nkb; ++i) {
+        if (!ptx::mbar_wait_bounded(bar_empty + 8 * s, ph ^ 1u, abort, kWaitLimitNs)) {
+          record_timeout(abort);
+          break;
+        }
+        const uint32_t fb = bar_full + 8 * s;
+        const uint32_t dst = sbase + static_cast<uint32_t>(s) * stage_bytes;
+        ptx::mbar_arrive_expect_tx(fb, tx);
+        ptx::tma_load_3d(dst, &maps.w, (kb0 + i) * BK, n0, q.e, fb);
+        ptx::tma_load_2d(dst + W_STAGE, mx, (kb0 + i) * BK, q.t0, fb);
+        ++issued;
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      for (int i = issued - 1; i >= 0 && i >= issued - stages; --i)
+        ptx::mbar_wait_timeout(bar_empty + 8 * (i % stages),
+                               static_cast<uint32_t>(i / stages) & 1u, kDrainLimitNs);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS, q.nn);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int i = 0; i < nkb; ++i) {
+        if (!ptx::mbar_wait_bounded(bar_full + 8 * s, ph, abort, kWaitLimitNs)) {
+          record_timeout(abort);
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t st = sbase + static_cast<uint32_t>(s) * stage_bytes;
+        const uint64_t adesc = ptx::sw128_kmajor_desc(st);
+        const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
+#pragma unroll
+        for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+          const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
+          ptx::mma_f8f6f4(tmem, adesc + koff, bdesc + koff, idesc, (i | kk) != 0 ? 1u : 0u);
+        }
+        ptx::mma_commit(bar_empty + 8 * s);
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      if (ok) ptx::mma_commit(bar_acc);
+      ptx::mma_commit(bar_drain);
+      ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
+    }
+  } else {
+    const int et = threadIdx.x - 64;
+    for (int i = et; i < cnt; i += NUM_THREADS - 64) e_xs[i] = __ldg(p.xs + q.t0 + i);
+    for (int i = et; i < r1 - r0; i += NUM_THREADS - 64) {
+      const int n = n0 + r0 + i;
+      const int64_t wn = static_cast<int64_t>(q.e) * p.N + n;
+      e_ws[i] = n < p.N ? __ldg(p.ws + wn) : 0.0f;
+      e_b[i] = n < p.N ? load_bias(p.bias, p.bias_dtype, wn) : 0.0f;
+    }
+    if constexpr (LORA) {
+      // The adapters' part of the rows reduced here, while the weights stream: one task is 4
+      // rows of one token, with that token's adapter only.
+      const uint16_t *lb = reinterpret_cast<const uint16_t *>(p.lora_b);
+      const bool f16 = p.lora_dtype == kF16;
+      for (int idx = et; idx < cnt * quads; idx += NUM_THREADS - 64) {
+        const int m = idx / quads, qd = idx - m * quads;
+        const int id = __ldg(p.ids + q.t0 + m);
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L)) {
+          const float *hr = p.h + static_cast<int64_t>(q.t0 + m) * p.R;
+          const int nb = n0 + r0 + 4 * qd;
+          for (int rc = 0; rc < p.R; rc += 8) {
+            const float4 h0 = *reinterpret_cast<const float4 *>(hr + rc);
+            const float4 h1 = *reinterpret_cast<const float4 *>(hr + rc + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float bw[8];
+              unpack8(__ldg(reinterpret_cast<const uint4 *>(
+                          lb + (static_cast<int64_t>(id) * p.N + min(nb + i, p.N - 1)) * p.R + rc)),
+                      f16, bw);
+              s[i] = fmaf(h0.x, bw[0], s[i]);
+              s[i] = fmaf(h0.y, bw[1], s[i]);
+              s[i] = fmaf(h0.z, bw[2], s[i]);
+              s[i] = fmaf(h0.w, bw[3], s[i]);
+              s[i] = fmaf(h1.x, bw[4], s[i]);
+              s[i] = fmaf(h1.y, bw[5], s[i]);
+              s[i] = fmaf(h1.z, bw[6], s[i]);
+              s[i] = fmaf(h1.w, bw[7], s[i]);
+            }
+          }
+        }
+        *reinterpret_cast<float4 *>(lora + m * R + 4 * qd) = make_float4(s[0], s[1], s[2], s[3]);
+      }
+    }
+    // TMEM (lane = weight row, column = token) -> part[token][row], fp32
+    const int quarter = warp & 3;
+    const bool ok = ptx::mbar_wait_bounded(bar_acc, 0, abort, kWaitLimitNs);
+    if (!ok && lane == 0) record_timeout(abort);
+    ptx::tc_fence_after();
+    const int row = quarter * 32 + lane;
+    for (int c = 0; c < q.nn; c += 16) {
+      uint32_t r[16];
+      if (ok) {
+        ptx::tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                    static_cast<uint32_t>(c),
+                                r);
+        ptx::tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) part[(c + j) * WROWS + row] = __uint_as_float(r[j]);
+    }
+    ptx::tc_fence_before();
+  }
+
+  __syncwarp();
+  __syncthreads();
+  ptx::cluster_sync();  // every CTA's partial tile is in its shared memory
+
+  const uint32_t part_base = ptx::smem_u32(part);
+  for (int idx = threadIdx.x; idx < cnt * quads; idx += NUM_THREADS) {
+    const int m = idx / quads;
+    const int qd = idx - m * quads;
+    const uint32_t off = static_cast<uint32_t>(m * WROWS + r0 + 4 * qd) * 4u;
+    float4 v[SPLIT_MAX];
+#pragma unroll
+    for (int s = 0; s < SPLIT_MAX; ++s)
+      if (s < p.split) v[s] = ptx::ld_shared_cluster_v4(ptx::map_shared_rank(part_base + off, s));
+    float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < SPLIT_MAX; ++s)
+      if (s < p.split) {
+        a[0] += v[s].x;
+        a[1] += v[s].y;
+        a[2] += v[s].z;
+        a[3] += v[s].w;
+      }
+    const float xs = e_xs[m];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int nl = 4 * qd + i;
+      const int n = n0 + r0 + nl;
+      if (n >= p.N) break;
+      float val = fmaf(a[i] * xs, e_ws[nl], e_b[nl]);
+      if constexpr (LORA) val += lora[m * R + nl];
+      store_out(p.out, p.out_dtype, static_cast<int64_t>(q.t0 + m) * p.N + n, val);
+    }
+  }
+  zero_rows(p, g_row, 0, NUM_THREADS);
+
+  ptx::cluster_sync();  // peers may still be reading this CTA's partial tile
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<1>(tmem, tmem_cols);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+
+struct LaunchInfo {
+  bool ready = false;
+  cudaError_t err = cudaSuccess;
+  int max_groups = 0;
+};
+
+template <int CG, bool LORA>
+LaunchInfo &persist_info(const DeviceInfo &dev) {
+  static LaunchInfo info[64];
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  LaunchInfo &li = info[dev.device & 63];
+  if (!li.ready) {
+    li.ready = true;
+    li.err = cudaFuncSetAttribute(persist_kernel<CG, LORA>,
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(Cfg<CG, LORA>::SMEM_BYTES));
+    li.max_groups = dev.sm_count / CG;
+    if (li.err == cudaSuccess && CG == 2) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(dev.sm_count / CG * CG);
+      cfg.blockDim = dim3(NUM_THREADS);
+      cfg.dynamicSmemBytes = Cfg<CG, LORA>::SMEM_BYTES;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = CG;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      li.err = cudaOccupancyMaxActiveClusters(&clusters, persist_kernel<CG, LORA>, &cfg);
+      if (li.err == cudaSuccess) li.max_groups = std::min(li.max_groups, clusters);
+      if (li.err == cudaSuccess && li.max_groups < 1) li.err = cudaErrorInvalidConfiguration;
+    }
+  }
+  return li;
+}
+
+int launch_failed(const char *op, cudaError_t e) {
+  set_error(std::string(op) + ": launch failed: " + cudaGetErrorString(e));
+  return 4;
+}
+
+cudaError_t launch(const void *kernel, const Maps &maps, const Params &p, int ctas, int cluster,
+                   size_t smem, cudaStream_t stream, bool pdl) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster > 0) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = static_cast<unsigned>(n);
+  void *args[] = {const_cast<Maps *>(&maps), const_cast<Params *>(&p)};
+  return cudaLaunchKernelExC(&cfg, kernel, args);
+}
+
+template <int CG, bool LORA>
+int launch_persist(const char *op, const Maps &maps, Params &p, int64_t tiles,
+                   const DeviceInfo &dev, cudaStream_t stream, bool pdl) {
+  LaunchInfo &li = persist_info<CG, LORA>(dev);
+  if (li.err != cudaSuccess) return launch_failed(op, li.err);
+  const int groups = static_cast<int>(std::min<int64_t>(tiles, li.max_groups));
+  const cudaError_t e =
+      launch(reinterpret_cast<const void *>(&persist_kernel<CG, LORA>), maps, p, groups * CG,
+             CG == 2 ? 2 : 0, Cfg<CG, LORA>::SMEM_BYTES, stream, pdl);
+  return e == cudaSuccess ? 0 : launch_failed(op, e);
+}
+
+template <bool LORA>
+int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const DeviceInfo &dev,
+                 cudaStream_t stream, bool pdl) {
+  static bool set[64];
+  static std::mutex mu;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!set[dev.device & 63]) {
+      // (the static barriers take a little of the 227 KB)
+      const cudaError_t e = cudaFuncSetAttribute(
+          split_kernel<LORA>, cudaFuncAttributeMaxDynamicSharedMemorySize, SPLIT_SMEM - 1024);
+      if (e != cudaSuccess) return launch_failed(op, e);
+      set[dev.device & 63] = true;
+    }
+  }
+  // K-splits: as many CTAs as the GPU holds, at least two K-blocks for each
+  int split = std::max(1, std::min({dev.sm_count / tiles, SPLIT_MAX, (p.k_blocks + 1) / 2}));
+  p.kps = (p.k_blocks + split - 1) / split;
+  p.split = (p.k_blocks + p.kps - 1) / p.kps;
+  const uint32_t stage = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
+  const uint32_t part = static_cast<uint32_t>(p.tok_cap) * WROWS * 4;
+  const uint32_t rows = static_cast<uint32_t>(((WROWS + p.split - 1) / p.split + 3) & ~3);
+  const uint32_t lora = LORA ? static_cast<uint32_t>(p.tok_cap) * rows * 4 : 0;
+  const uint32_t tab = static_cast<uint32_t>(p.E + 1) * 8 + SPLIT_EPI;
+  const uint32_t room = SPLIT_SMEM - 2048 - part - lora - tab;
+  p.stages = std::max(1, std::min({static_cast<int>(room / stage), SPLIT_STAGES, p.kps}));
+  p.off_part = static_cast<uint32_t>(p.stages) * stage;
+  p.off_lora = p.off_part + part;
+  p.off_tab = p.off_lora + lora;
+  const size_t smem = p.off_tab + tab + 1024;
+  const cudaError_t e = launch(reinterpret_cast<const void *>(&split_kernel<LORA>), maps, p,
+                               tiles * p.split, p.split, smem, stream, pdl);
+  return e == cudaSuccess ? 0 : launch_failed(op, e);
+}
+
+bool make_common_maps(Maps *m, const uint8_t *xq, const uint8_t *wq, int64_t M, int64_t N,
+                      int64_t K, int64_t E, std::string *err) {
+  for (int i = 0; i < X_MAPS; ++i)
+    if (!make_tmap_2d_sw128(&m->x[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, K, M, K, BK, 16 * (i + 1),
+                            err))
+      return false;
+  return make_tmap_3d_sw128(&m->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, K, N, E, K, N * K, BK, WROWS,
+                            err);
+}
+
+}  // namespace rowsel
+
+namespace {
+
+bool check_device(const char *op, DeviceInfo *dev) {
+  if (!current_device_info(dev)) return false;
+  if (dev->cc_major == 10) return true;
+  set_error(std::string(op) + " needs an sm_100 (B200-class) device; current device is sm_" +
+            std::to_string(dev->cc_major) + std::to_string(dev->cc_minor));
+  return false;
+}
+
+}  // namespace
+
+int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl) {
+  using namespace rowsel;
+  const char *op = "fp8_grouped_gemm";
+  DeviceInfo dev;
+  if (!check_device(op, &dev)) return 5;
+  std::string err;
+  Maps maps;
+  if (!make_common_maps(&maps, a.xq, a.wq, a.M, a.N, a.K, a.E, &err)) {
+    set_error(std::string(op) + ": " + err);
+    return 4;
+  }
+  maps.lb = maps.w;
+  for (auto &h : maps.h) h = maps.x[0];
+  Params p = {};
+  p.xs = a.xs;
+  p.ws = a.ws;
+  p.bias = a.bias;
+  p.bias_dtype = a.bias ? a.bias_dtype : kNone;
+  p.out = a.out;
+  p.out_dtype = a.out_dtype;
+  p.offsets = a.offsets;
+  p.M = static_cast<int>(a.M);
+  p.N = static_cast<int>(a.N);
+  p.E = static_cast<int>(a.E);
+  p.k_blocks = static_cast<int>((a.K + BK - 1) / BK);
+  p.pdl = pdl ? 1 : 0;
+  p.pre_w = a.weights_before_wait ? 1 : 0;
+  // Tiles at most, whatever the offsets: every group with rows starts a token block of its own.
+  const int64_t live = std::min(a.E, a.M);
+  const int64_t wb1 = (a.N + WROWS - 1) / WROWS;
+  const int64_t ub1 = wb1 * (live + a.M / SPLIT_TOK);
+  if (ub1 > 0x3fffffffLL) {
+    set_error(std::string(op) + ": too many output tiles");
+    return 2;
+  }
+  p.n_wb = static_cast<int>(wb1);
+  if (ub1 <= dev.sm_count) {
+    p.tok_cap = static_cast<int>(std::min<int64_t>((a.M + 15) / 16 * 16, SPLIT_TOK));
+    return launch_split<false>(op, maps, p, static_cast<int>(ub1), dev, stream, pdl);
+  }
+  if (a.M / live < 48) return launch_persist<1, false>(op, maps, p, ub1, dev, stream, pdl);
+  const int64_t wb2 = (a.N + 2 * WROWS - 1) / (2 * WROWS);
+  p.n_wb = static_cast<int>(wb2);
+  return launch_persist<2, false>(op, maps, p, wb2 * (live + a.M / 256), dev, stream, pdl);
+}
+
+int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
+  using namespace rowsel;
+  const char *op = "fp8_linear_lora";
+  DeviceInfo dev;
+  if (!check_device(op, &dev)) return 5;
+  std::string err;
+  Maps maps;
+  const LoraWorkspace w = lora_workspace(a.workspace, a.M, a.R);
+  const int64_t rp = lora_rank_pad(a.R);
+  const bool few = a.M <= kLoraRowsMaxM;
+  const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  bool ok = make_common_maps(&maps, a.xq, a.wq, a.M, a.N, a.K, 1, &err);
+  if (few) {
+    maps.lb = maps.w;
+    for (auto &h : maps.h) h = maps.x[0];
+  } else {
+    ok = ok && make_tmap_3d_sw128(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2,
+                                  64, WROWS, &err);
+    for (int i = 0; ok && i < H_MAPS; ++i)
+      ok = make_tmap_2d_sw128(&maps.h[i], t16, w.hl, 2 * rp, a.M, 4 * rp, 64, 16 * (i + 1), &err);
+  }
+  if (!ok) {
+    set_error(std::string(op) + ": " + err);
+    return 4;
+  }
+  Params p = {};
+  p.xs = a.xs;
+  p.ws = a.ws;
+  p.bias = a.bias;
+  p.bias_dtype = a.bias ? a.bias_dtype : kNone;
+  p.out = a.out;
+  p.out_dtype = a.out_dtype;
+  p.M = static_cast<int>(a.M);
+  p.N = static_cast<int>(a.N);
+  p.E = 1;
+  p.k_blocks = static_cast<int>((a.K + BK - 1) / BK);
+  p.pdl = pdl ? 1 : 0;
+  p.pre_w = a.weights_before_wait ? 1 : 0;
+  p.ids = a.ids;
+  p.lora_b = a.lora_b;
+  p.lora_dtype = a.dtype;
+  p.L = static_cast<int>(a.L);
+  p.R = static_cast<int>(a.R);
+  p.rank_pad = static_cast<int>(rp);
+  p.tile_adapter = w.tile_adapter;
+  p.hl = w.hl;
+  p.hscale = w.hscale;
+  p.h = w.h;
+  if (few) {
+    const int64_t wb = (a.N + WROWS - 1) / WROWS;
+    if (wb > 0x3fffffLL) {
+      set_error(std::string(op) + ": too many output tiles");
+      return 2;
+    }
+    p.n_wb = static_cast<int>(wb);
+    p.tok_cap = static_cast<int>((a.M + 15) / 16 * 16);
+    return launch_split<true>(op, maps, p, static_cast<int>(wb), dev, stream, pdl);
+  }
+  const int64_t wb = (a.N + 2 * WROWS - 1) / (2 * WROWS);
+  const int64_t tiles = wb * lora_tiles(a.M);
+  if (tiles > 0x3fffffffLL) {
+    set_error(std::string(op) + ": too many output tiles");
+    return 2;
+  }
+  p.n_wb = static_cast<int>(wb);
+  return launch_persist<2, true>(op, maps, p, tiles, dev, stream, pdl);
+}
+
+cudaError_t read_rowsel_status(unsigned int *bits, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(bits, g_rowsel_status, sizeof(unsigned int));
+  if (e != cudaSuccess) return e;
+  if (clear) {
+    const unsigned int zero = 0;
+    e = cudaMemcpyToSymbol(g_rowsel_status, &zero, sizeof(unsigned int));
+  }
+  return e;
+}
+
+}  // namespace fp8lin

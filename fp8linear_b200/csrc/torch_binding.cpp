@@ -476,6 +476,177 @@ at::Tensor fp8_linear_modulated(at::Tensor x, at::Tensor shift, at::Tensor scale
   return out.reshape(out_shape);
 }
 
+// Linears whose weights depend on the row (no reference ops).
+void check_on(const at::Tensor &t, const at::Tensor &x, const char *op, const char *name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == x.device(), op, ": ", name,
+              " must be on x's CUDA device");
+}
+
+// Experts' weights [E, N, K]: every row of every expert as quantize_weight's per-channel form.
+std::tuple<at::Tensor, at::Tensor> quantize_expert_weights(at::Tensor weight) {
+  TORCH_CHECK(weight.is_cuda() && weight.dim() == 3,
+              "quantize_expert_weights: weight must be a 3D CUDA tensor [E, N, K]");
+  const int code = dtype_code(weight.scalar_type());
+  TORCH_CHECK(code >= 0, "quantize_expert_weights: weight must be bf16, fp16 or fp32");
+  c10::cuda::CUDAGuard guard(weight.device());
+  auto w = weight.detach().contiguous();
+  const int64_t E = w.size(0), N = w.size(1), K = w.size(2);
+  auto wq = at::empty({E, N, K}, w.options().dtype(at::kFloat8_e4m3fn));
+  auto scale = at::empty({E, N}, w.options().dtype(at::kFloat));
+  if (E * N == 0) return {wq, scale};
+  if (K == 0) {
+    scale.fill_(1e-12f);
+    return {wq, scale};
+  }
+  check_rc(fp8lin_quantize_weight(w.data_ptr(), code, E * N, K, wq.data_ptr(),
+                                  scale.data_ptr<float>(), stream_of(w)),
+           "quantize_expert_weights");
+  return {wq, scale};
+}
+
+// The experts' side of both grouped ops, checked against x [M, K].
+struct ExpertArgs {
+  at::Tensor wq, ws, offsets;
+  BiasArg bias;
+  int64_t E = 0, N = 0;
+};
+
+ExpertArgs prep_experts(const at::Tensor &x, const at::Tensor &wq, const at::Tensor &w_scale,
+                        const at::Tensor &offsets, const std::optional<at::Tensor> &bias,
+                        const char *op) {
+  TORCH_CHECK(x.dim() == 2, op, ": x must be 2D [M, K], its rows sorted by expert");
+  TORCH_CHECK(wq.scalar_type() == at::kFloat8_e4m3fn && wq.dim() == 3, op,
+              ": wq must be a 3D float8_e4m3fn tensor [E, N, K]");
+  TORCH_CHECK(wq.size(2) == x.size(1), op, ": K mismatch: x[M, K], wq[E, N, K]");
+  const int64_t K = x.size(1);
+  TORCH_CHECK(K > 0 && K % 16 == 0, op, ": K must be a positive multiple of 16, got ", K);
+  ExpertArgs a;
+  a.E = wq.size(0);
+  a.N = wq.size(1);
+  TORCH_CHECK(a.E >= 1 && a.E <= 1024, op, ": 1 to 1024 experts, got ", a.E);
+  TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.numel() == a.E * a.N, op,
+              ": w_scale must be fp32 [E, N]");
+  TORCH_CHECK(offsets.scalar_type() == at::kInt && offsets.dim() == 1 &&
+                  offsets.size(0) == a.E + 1,
+              op, ": offsets must be int32 [E + 1]");
+  check_on(wq, x, op, "wq");
+  check_on(w_scale, x, op, "w_scale");
+  check_on(offsets, x, op, "offsets");
+  a.wq = aligned16(wq);
+  a.ws = w_scale.contiguous();
+  a.offsets = offsets.contiguous();
+  if (bias.has_value() && bias->defined()) {
+    check_on(*bias, x, op, "bias");
+    TORCH_CHECK(bias->dim() == 2 && bias->size(0) == a.E && bias->size(1) == a.N, op,
+                ": bias must be [E, N]");
+    a.bias = prep_bias(bias, a.E * a.N);
+  }
+  return a;
+}
+
+at::Tensor fp8_grouped_gemm(at::Tensor xq, at::Tensor x_scale, at::Tensor wq, at::Tensor w_scale,
+                            at::Tensor offsets, std::optional<at::Tensor> bias) {
+  const char *op = "fp8_grouped_gemm";
+  TORCH_CHECK(xq.is_cuda(), op, ": xq must be on CUDA");
+  TORCH_CHECK(xq.scalar_type() == at::kFloat8_e4m3fn, op, ": xq must be float8_e4m3fn");
+  c10::cuda::CUDAGuard guard(xq.device());
+  ExpertArgs a = prep_experts(xq, wq, w_scale, offsets, bias, op);
+  const int64_t M = xq.size(0), K = xq.size(1);
+  TORCH_CHECK(x_scale.scalar_type() == at::kFloat && x_scale.numel() == M, op,
+              ": x_scale must be fp32 with M entries (per-token)");
+  check_on(x_scale, xq, op, "x_scale");
+  auto xqc = aligned16(xq);
+  auto xs = x_scale.contiguous();
+  auto out = at::empty({M, a.N}, xqc.options().dtype(at::kBFloat16));
+  if (M == 0 || a.N == 0) return out;
+  check_rc(fp8lin_fp8_grouped_gemm(xqc.data_ptr(), xs.data_ptr<float>(), a.wq.data_ptr(),
+                                   a.ws.data_ptr<float>(), a.offsets.data_ptr<int>(), a.bias.ptr,
+                                   a.bias.dtype, out.data_ptr(), FP8LIN_DTYPE_BF16, M, a.N, K,
+                                   a.E, stream_of(xqc)),
+           op);
+  return out;
+}
+
+at::Tensor fp8_grouped_linear(at::Tensor x, at::Tensor wq, at::Tensor w_scale, at::Tensor offsets,
+                              std::optional<at::Tensor> bias) {
+  const char *op = "fp8_grouped_linear";
+  TORCH_CHECK(x.is_cuda(), op, ": x must be on CUDA");
+  TORCH_CHECK(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, op,
+              ": x must be fp16 or bf16");
+  c10::cuda::CUDAGuard guard(x.device());
+  ExpertArgs a = prep_experts(x, wq, w_scale, offsets, bias, op);
+  auto xc = aligned16(x);
+  const int64_t M = xc.size(0), K = xc.size(1);
+  auto out = at::empty({M, a.N}, xc.options());
+  if (M == 0 || a.N == 0) return out;
+  const size_t ws_bytes = fp8lin_linear_workspace_size(M, K);
+  auto workspace = at::empty({static_cast<int64_t>(ws_bytes)}, xc.options().dtype(at::kByte));
+  check_rc(fp8lin_fp8_grouped_linear(xc.data_ptr(), dtype_code(xc.scalar_type()),
+                                     a.wq.data_ptr(), a.ws.data_ptr<float>(),
+                                     a.offsets.data_ptr<int>(), a.bias.ptr, a.bias.dtype,
+                                     out.data_ptr(), dtype_code(xc.scalar_type()), M, a.N, K, a.E,
+                                     workspace.data_ptr(), ws_bytes, stream_of(xc)),
+           op);
+  return out;
+}
+
+at::Tensor fp8_linear_lora(at::Tensor x, at::Tensor wq, at::Tensor w_scale, at::Tensor lora_a,
+                           at::Tensor lora_b, at::Tensor adapters, at::Tensor scaling,
+                           std::optional<at::Tensor> bias) {
+  const char *op = "fp8_linear_lora";
+  TORCH_CHECK(x.is_cuda(), op, ": x must be on CUDA");
+  TORCH_CHECK(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, op,
+              ": x must be fp16 or bf16");
+  TORCH_CHECK(x.dim() >= 1, op, ": x must have at least one dimension");
+  TORCH_CHECK(wq.scalar_type() == at::kFloat8_e4m3fn && wq.dim() == 2, op,
+              ": wq must be a 2D float8_e4m3fn tensor [N, K]");
+  const int64_t K = x.size(-1), N = wq.size(0);
+  TORCH_CHECK(wq.size(1) == K, op, ": K mismatch: x[..., K], wq[N, K]");
+  TORCH_CHECK(K > 0 && K % 16 == 0, op, ": K must be a positive multiple of 16, got ", K);
+  TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.numel() == N, op,
+              ": w_scale must be fp32 with N entries (per-channel)");
+  TORCH_CHECK(lora_a.dim() == 3 && lora_b.dim() == 3 && lora_a.size(0) == lora_b.size(0) &&
+                  lora_a.size(1) == lora_b.size(2) && lora_a.size(2) == K && lora_b.size(1) == N,
+              op, ": lora_a must be [L, R, K] and lora_b [L, N, R]");
+  TORCH_CHECK(lora_a.scalar_type() == x.scalar_type() && lora_b.scalar_type() == x.scalar_type(),
+              op, ": lora_a and lora_b must have x's dtype");
+  const int64_t L = lora_a.size(0), R = lora_a.size(1);
+  TORCH_CHECK(L == 0 || (R > 0 && R % 8 == 0 && R <= 128), op,
+              ": the rank must be a multiple of 8 from 8 to 128 (pad with zeros), got ", R);
+  const int64_t M = x.numel() / K;
+  TORCH_CHECK(adapters.scalar_type() == at::kInt && adapters.numel() == M, op,
+              ": adapters must be int32 with one entry per row of x");
+  TORCH_CHECK(scaling.scalar_type() == at::kFloat && scaling.numel() == L, op,
+              ": scaling must be fp32 [L]");
+  check_on(wq, x, op, "wq");
+  check_on(w_scale, x, op, "w_scale");
+  check_on(lora_a, x, op, "lora_a");
+  check_on(lora_b, x, op, "lora_b");
+  check_on(adapters, x, op, "adapters");
+  check_on(scaling, x, op, "scaling");
+  if (bias.has_value() && bias->defined()) check_on(*bias, x, op, "bias");
+  c10::cuda::CUDAGuard guard(x.device());
+  auto x2d = aligned16(x.reshape({M, K}));
+  auto wqc = aligned16(wq), ac = aligned16(lora_a), bc = aligned16(lora_b);
+  auto ws = w_scale.contiguous(), ids = adapters.contiguous(), sc = scaling.contiguous();
+  auto out_shape = x.sizes().vec();
+  out_shape.back() = N;
+  auto out = at::empty({M, N}, x2d.options());
+  if (M > 0 && N > 0) {
+    BiasArg b = prep_bias(bias, N);
+    const size_t ws_bytes = fp8lin_fp8_linear_lora_workspace_size(M, K, R);
+    auto workspace = at::empty({static_cast<int64_t>(ws_bytes)}, x2d.options().dtype(at::kByte));
+    check_rc(fp8lin_fp8_linear_lora(
+                 x2d.data_ptr(), dtype_code(x2d.scalar_type()), wqc.data_ptr(),
+                 ws.data_ptr<float>(), ac.data_ptr(), bc.data_ptr(), ids.data_ptr<int>(),
+                 sc.data_ptr<float>(), b.ptr, b.dtype, out.data_ptr(),
+                 dtype_code(x2d.scalar_type()), M, N, K, L, R, workspace.data_ptr(), ws_bytes,
+                 stream_of(x2d)),
+             op);
+  }
+  return out.reshape(out_shape);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(fp8linear_b200, m) {
@@ -493,6 +664,13 @@ TORCH_LIBRARY(fp8linear_b200, m) {
         "-> (Tensor, Tensor)");
   m.def("fp8_linear_modulated(Tensor x, Tensor shift, Tensor scale, Tensor wq, Tensor w_scale, "
         "Tensor? bias, float eps=1e-06) -> Tensor");
+  m.def("quantize_expert_weights(Tensor weight) -> (Tensor, Tensor)");
+  m.def("fp8_grouped_gemm(Tensor xq, Tensor x_scale, Tensor wq, Tensor w_scale, Tensor offsets, "
+        "Tensor? bias) -> Tensor");
+  m.def("fp8_grouped_linear(Tensor x, Tensor wq, Tensor w_scale, Tensor offsets, Tensor? bias) "
+        "-> Tensor");
+  m.def("fp8_linear_lora(Tensor x, Tensor wq, Tensor w_scale, Tensor lora_a, Tensor lora_b, "
+        "Tensor adapters, Tensor scaling, Tensor? bias) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(fp8linear_b200, CUDA, m) {
@@ -508,4 +686,8 @@ TORCH_LIBRARY_IMPL(fp8linear_b200, CUDA, m) {
   m.impl("nvfp4_linear", &nvfp4_linear);
   m.impl("layernorm_modulate_quantize_fp8", &layernorm_modulate_quantize_fp8);
   m.impl("fp8_linear_modulated", &fp8_linear_modulated);
+  m.impl("quantize_expert_weights", &quantize_expert_weights);
+  m.impl("fp8_grouped_gemm", &fp8_grouped_gemm);
+  m.impl("fp8_grouped_linear", &fp8_grouped_linear);
+  m.impl("fp8_linear_lora", &fp8_linear_lora);
 }

@@ -171,6 +171,66 @@ def fp8_linear_modulated(x, shift, scale, wq, w_scale, bias=None, eps: float = 1
     return ops.fp8_linear_modulated(x, shift, scale, wq, w_scale, bias, eps)
 
 
+@torch.library.register_fake(add_op_namespace_prefix("quantize_expert_weights"))
+def _quantize_expert_weights_fake(weight):
+    wq = weight.new_empty(weight.shape, dtype=torch.float8_e4m3fn)
+    return wq, weight.new_empty(weight.shape[:2], dtype=torch.float32)
+
+
+@torch.library.register_fake(add_op_namespace_prefix("fp8_grouped_gemm"))
+def _fp8_grouped_gemm_fake(xq, x_scale, wq, w_scale, offsets, bias=None):
+    return xq.new_empty((xq.shape[0], wq.shape[1]), dtype=torch.bfloat16)
+
+
+@torch.library.register_fake(add_op_namespace_prefix("fp8_grouped_linear"))
+def _fp8_grouped_linear_fake(x, wq, w_scale, offsets, bias=None):
+    return x.new_empty((x.shape[0], wq.shape[1]), dtype=x.dtype)
+
+
+@torch.library.register_fake(add_op_namespace_prefix("fp8_linear_lora"))
+def _fp8_linear_lora_fake(x, wq, w_scale, lora_a, lora_b, adapters, scaling, bias=None):
+    return x.new_empty((*x.shape[:-1], wq.shape[0]), dtype=x.dtype)
+
+
+def quantize_expert_weights(weight: torch.Tensor):
+    """Per-output-channel e4m3 quantization of the experts' weights ``[E, N, K]`` (offline):
+    ``(wq e4m3 [E, N, K], w_scale fp32 [E, N])``, each expert as ``quantize_weight`` does it.
+    Always per channel: the block-scaled formats have no grouped linear."""
+    return ops.quantize_expert_weights(weight)
+
+
+def fp8_grouped_gemm(xq, x_scale, wq, w_scale, offsets, bias=None):
+    """``fp8_gemm`` with weights of the row's expert. The rows of ``xq [M, K]`` (e4m3, with
+    ``x_scale [M]``) are sorted by expert: expert e has rows ``offsets[e]`` to
+    ``offsets[e + 1] - 1`` (int32 ``[E + 1]`` on the device; empty experts are fine), weights
+    ``wq [E, N, K]``, ``w_scale [E, N]`` and, if given, ``bias [E, N]``. Rows outside
+    ``offsets[0] .. offsets[E]`` come out as zeros. The offsets are read on the device only (no
+    synchronization); they are clamped to ``[0, M]`` and never run backwards. At most 1024
+    experts, K a multiple of 16. Returns bf16 ``[M, N]``; no reference counterpart."""
+    return ops.fp8_grouped_gemm(xq, x_scale, wq, w_scale, offsets, bias)
+
+
+def fp8_grouped_linear(x, wq, w_scale, offsets, bias=None):
+    """``fp8_linear`` with weights of the row's expert: ``x [M, K]`` bf16/fp16, its rows sorted
+    by expert, is quantized per token and multiplied as ``fp8_grouped_gemm`` does. Returns
+    ``[M, N]`` in x's dtype."""
+    return ops.fp8_grouped_linear(x, wq, w_scale, offsets, bias)
+
+
+def fp8_linear_lora(x, wq, w_scale, lora_a, lora_b, adapters, scaling, bias=None):
+    """``fp8_linear(x, wq, w_scale, bias)`` plus the low-rank adapter of each row, added before
+    the one rounding to x's dtype:
+
+    ``out[i] = fp8_linear(x)[i] + scaling[a] * (x[i] @ lora_a[a].T) @ lora_b[a].T``
+
+    with ``a = adapters[i]`` (int32, one per row of ``x [..., K]``, on the device); a row whose
+    entry lies outside ``[0, L)`` (-1, say) has no adapter. ``lora_a [L, R, K]`` and
+    ``lora_b [L, N, R]`` in x's dtype, ``scaling`` fp32 ``[L]``, R a multiple of 8 up to 128
+    (smaller adapters are padded with zeros). x goes into the adapters unquantized. Rows of one
+    request next to each other are fastest; any order is right. No reference counterpart."""
+    return ops.fp8_linear_lora(x, wq, w_scale, lora_a, lora_b, adapters, scaling, bias)
+
+
 def quantize_weight(weight: torch.Tensor):
     """Per-output-channel e4m3 quantization of a ``[N, K]`` CUDA weight (offline).
 

@@ -367,10 +367,59 @@ FP8LIN_API int fp8lin_fp8_linear_noalloc(const void *x, int x_dtype, const void 
                                          int64_t N, int64_t K, void *stream);
 
 /*
+ * FP8 GEMM whose weights depend on the row: rows sorted by expert, ragged group sizes.
+ * No reference counterpart; beside fp8lin_fp8_gemm for mixture-of-experts layers.
+ *   out[i,n] = (sum_k xq[i,k]*wq[e,n,k]) * x_scale[i] * w_scale[e,n] + bias[e,n]
+ *   for the expert e with offsets[e] <= i < offsets[e+1]; rows of no expert get zeros
+ *   xq [M,K] e4m3, x_scale [M] fp32; wq [E,N,K] e4m3, w_scale [E,N] fp32
+ *   offsets [E+1] int32 in device memory, never read on the host: clamped to [0, M] and to
+ *   their running maximum (offsets that run backwards leave the later group empty)
+ *   bias [E,N] BF16/F16/F32 or NULL; out [M,N] BF16 or F16
+ * Requirements (checked): 1 <= E <= 1024, K % 16 == 0, K > 0, xq/wq 16-byte aligned, M, N and
+ * K below 2^31. M == 0 or N == 0 is a no-op.
+ */
+FP8LIN_API int fp8lin_fp8_grouped_gemm(const void *xq, const float *x_scale, const void *wq,
+                                       const float *w_scale, const int32_t *offsets,
+                                       const void *bias, int bias_dtype, void *out, int out_dtype,
+                                       int64_t M, int64_t N, int64_t K, int64_t E, void *stream);
+
+/*
+ * fp8lin_quantize_fp8 of x [M,K] (BF16 or F16) into the workspace
+ * (fp8lin_linear_workspace_size(M, K) bytes, 256-byte aligned), then fp8lin_fp8_grouped_gemm
+ * as its programmatic dependent.
+ */
+FP8LIN_API int fp8lin_fp8_grouped_linear(const void *x, int x_dtype, const void *wq,
+                                         const float *w_scale, const int32_t *offsets,
+                                         const void *bias, int bias_dtype, void *out,
+                                         int out_dtype, int64_t M, int64_t N, int64_t K, int64_t E,
+                                         void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Fused FP8 linear with a low-rank adapter per row (many requests' adapters beside one
+ * shared projection). No reference counterpart; beside fp8lin_fp8_linear.
+ *   out[i,n] = fp8_linear(x)[i,n] + sum_r h[i,r] * lora_b[a,n,r],  a = adapters[i]
+ *   h[i,r]   = scaling[a] * sum_k x[i,k] * lora_a[a,r,k]    (x unquantized, fp32 sums)
+ * rounded once to out_dtype; rows whose adapters entry is outside [0, L) have no adapter.
+ *   lora_a [L,R,K], lora_b [L,N,R] of x_dtype, scaling [L] fp32, adapters [M] int32, all in
+ *   device memory; the others as fp8lin_fp8_linear
+ *   workspace fp8lin_fp8_linear_lora_workspace_size(M, K, R) bytes, 256-byte aligned
+ * Requirements (checked): R % 8 == 0, 8 <= R <= 128; x, wq, lora_a and lora_b 16-byte aligned;
+ * K % 16 == 0; sizes below 2^31. L == 0 is fp8lin_fp8_linear. M == 0 or N == 0 is a no-op.
+ */
+FP8LIN_API size_t fp8lin_fp8_linear_lora_workspace_size(int64_t M, int64_t K, int64_t R);
+FP8LIN_API int fp8lin_fp8_linear_lora(const void *x, int x_dtype, const void *wq,
+                                      const float *w_scale, const void *lora_a,
+                                      const void *lora_b, const int32_t *adapters,
+                                      const float *scaling, const void *bias, int bias_dtype,
+                                      void *out, int out_dtype, int64_t M, int64_t N, int64_t K,
+                                      int64_t L, int64_t R, void *workspace,
+                                      size_t workspace_bytes, void *stream);
+
+/*
  * Watchdog status of the kernels on the current device: every wait in them is
  * bounded; a wait that runs out sets a bit here and the kernel returns early instead
  * of hanging (GEMM: 1 = TMA producer, 2 = MMA issuer, 4 = epilogue; 8 = quantizer;
- * 16 = few-token GEMM).
+ * 16 = few-token GEMM; 64 = grouped and adapter GEMM; 128 = adapters' down projection).
  * *status receives the bits; clear != 0 resets them. Synchronous on the device.
  * No counterpart in the reference (cuBLASLt has no such report).
  */

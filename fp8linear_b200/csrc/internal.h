@@ -161,7 +161,7 @@ int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl);
 // One shared projection plus the low-rank adapter of each row (ids[i], none outside [0, L)):
 // out = acc * xs * ws + bias + sum_r h[i, r] * lora_b[ids[i], n, r], h from launch_lora_down.
 constexpr int kLoraMaxRank = 128;
-constexpr int64_t kLoraRowsMaxM = 128;  // up to here h is fp32 and CUDA cores add the adapters
+constexpr int64_t kLoraRowsMaxM = 128;  // up to here all tokens are one tile, K is split
 struct LoraArgs {
   const void *x;         // [M, K] bf16 or fp16
   int dtype;             // of x, lora_a, lora_b
@@ -186,24 +186,27 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl);
 cudaError_t read_rowsel_status(unsigned int *bits, bool clear);
 
 // ---- lora_sm100.cu
-// Layout of the adapters' intermediate h in the workspace.
-//   M <= kLoraRowsMaxM: h fp32 [M][R].
-//   otherwise: hl [M][2 * rank_pad] of x's type, h / hscale as a high and a low part
-//   (h = hscale * (hi + lo), to fp32's last bits), hscale fp32 [M] (a power of two), and
-//   the adapter of each token tile of the GEMM (int: >= 0 all rows' adapter, -1 none, -2
-//   more than one).
+// The adapters' intermediate h and the adapters of each token tile of the GEMM, in the
+// workspace:
+//   hl [M + 1][2 * rank_pad] of x's type: h / hscale as a high and a low part, h = hscale *
+//   (hi + lo) to fp32's last bits; row M is zeros, the row that the GEMM's gathers take for
+//   tokens of another adapter; hscale fp32 [M], powers of two;
+//   count int [tiles]: how many adapters the tile's tokens have, tokens without any aside;
+//   list int [tiles][kLoraTileTokens]: which.
 inline int64_t lora_rank_pad(int64_t R) { return (R + 15) / 16 * 16; }
 constexpr int kLoraTileTokens = 160;  // tokens per tile of the GEMM with adapters, at most
-inline int64_t lora_tiles(int64_t M) { return (M + kLoraTileTokens - 1) / kLoraTileTokens; }
+inline int64_t lora_tiles(int64_t M) {
+  return M <= kLoraRowsMaxM ? 1 : (M + kLoraTileTokens - 1) / kLoraTileTokens;
+}
 inline int64_t lora_tile_tokens(int64_t M) {
   const int64_t nt = lora_tiles(M);
   return ((M + nt - 1) / nt + 31) / 32 * 32;
 }
 struct LoraWorkspace {
-  float *h = nullptr;
   void *hl = nullptr;
   float *hscale = nullptr;
-  int *tile_adapter = nullptr;
+  int *count = nullptr;
+  int *list = nullptr;
   size_t bytes = 0;
 };
 LoraWorkspace lora_workspace(void *base, int64_t M, int64_t R);

@@ -3,20 +3,18 @@
 // for the rows i whose adapter a_i is in [0, L). The up projection is part of the linear's
 // GEMM (rowsel_sm100.cu), which adds h . B^T before its one rounding.
 //
-//   down_rows_kernel  few rows: CUDA cores, x and A read as they lie, K split over the warps
-//       of a CTA; h stays fp32.
-//   down_tile_kernel  many rows: tcgen05 (kind::f16) on tiles of 128 rows. All of a tile's
-//       adapters stand side by side on the MMA's N side (rank_pad columns each, 128 columns
-//       a pass), and each row keeps the columns of its own; rows never mix, so an adapter's
-//       infinities and NaN stay with its rows. A cluster splits K when the tiles are few.
+// tcgen05 (kind::f16) on tiles of 128 rows. All of a tile's adapters stand side by side on the
+// MMA's N side (rank_pad columns each, 128 columns a pass), and each row keeps the columns of
+// its own; rows never mix, so an adapter's infinities and NaN stay with its rows. When the
+// tiles are few, a cluster splits K and the passes go to clusters of their own.
 //
 // The GEMM's tensor cores take h in x's 16-bit type. h is a sum, so it keeps fp32's accuracy:
 // it goes as a high and a low part, h / hscale = hi + lo (bf16: 2^-17 relative; f16: hscale,
 // a power of two, puts the row's largest value in [1, 2), the error is 2^-22 of it), at the
 // price of twice the rank in a product that is a few per cent of the whole.
 //
-// Both kernels read x, ids and A before the dependency wait (the kernel before is the call's
-// quantizer, which lets them launch only after its own wait) and write after it.
+// The kernel reads x, ids and A before the dependency wait (the kernel before is the call's
+// quantizer, which lets it launch only after its own wait) and writes after it.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -45,111 +43,17 @@ struct Params {
   const float *scaling;
   int dtype;
   int M, K, L, R, rank_pad;
-  float *h;
   void *hl;
   float *hscale;
-  int *tile_adapter;
+  int *count, *list;
   int gemm_tiles, gemm_tile_tokens;
   int split, kps, k_blocks;
+  int par;  // clusters per tile, each with every par-th pass
 };
 
 __device__ __forceinline__ bool has_adapter(const Params &p, int id) {
   return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L);
 }
-
-// Eight 16-bit values as floats.
-__device__ __forceinline__ void unpack8(const uint4 &v, bool f16, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (f16) {
-      const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    } else {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    }
-  }
-}
-
-// ---------------------------------------------------------------- few rows
-
-constexpr int FEW_ROWS = 8;   // rows per CTA
-constexpr int FEW_RANK = 4;   // values of h per row and CTA
-constexpr int FEW_WARPS = 8;  // K in chunks of 8 values over all lanes of all warps
-
-__global__ void __launch_bounds__(32 * FEW_WARPS) down_rows_kernel(const Params p) {
-  __shared__ float s_sum[FEW_WARPS][FEW_ROWS * FEW_RANK];
-  ptx::grid_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = blockIdx.x * FEW_ROWS;
-  const int r0 = blockIdx.y * FEW_RANK;
-  const bool f16 = p.dtype == kF16;
-  int id[FEW_ROWS];
-#pragma unroll
-  for (int i = 0; i < FEW_ROWS; ++i) {
-    id[i] = m0 + i < p.M ? __ldg(p.ids + m0 + i) : -1;
-    if (!has_adapter(p, id[i])) id[i] = -1;
-  }
-  float acc[FEW_ROWS][FEW_RANK];
-#pragma unroll
-  for (int i = 0; i < FEW_ROWS; ++i)
-#pragma unroll
-    for (int r = 0; r < FEW_RANK; ++r) acc[i][r] = 0.0f;
-  const uint4 *x4 = reinterpret_cast<const uint4 *>(p.x);
-  const uint4 *a4 = reinterpret_cast<const uint4 *>(p.a);
-  const int chunks = p.K / 8;  // K % 16 == 0
-  for (int c = threadIdx.x; c < chunks; c += 32 * FEW_WARPS) {
-    int cur = -1;
-    uint4 aw[FEW_RANK];
-#pragma unroll
-    for (int r = 0; r < FEW_RANK; ++r) aw[r] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < FEW_ROWS; ++i) {
-      if (id[i] < 0) continue;  // uniform in the CTA
-      if (id[i] != cur) {
-        cur = id[i];
-#pragma unroll
-        for (int r = 0; r < FEW_RANK; ++r)  // (R % 8 == 0: r0 + r < R)
-          aw[r] = __ldg(a4 + (static_cast<int64_t>(cur) * p.R + r0 + r) * chunks + c);
-      }
-      float xv[8];
-      unpack8(__ldg(x4 + static_cast<int64_t>(m0 + i) * chunks + c), f16, xv);
-#pragma unroll
-      for (int r = 0; r < FEW_RANK; ++r) {
-        float av[8];
-        unpack8(aw[r], f16, av);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][r] = fmaf(xv[j], av[j], acc[i][r]);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < FEW_ROWS; ++i)
-#pragma unroll
-    for (int r = 0; r < FEW_RANK; ++r) {
-      float v = acc[i][r];
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
-      if (lane == 0) s_sum[warp][i * FEW_RANK + r] = v;
-    }
-  __syncthreads();
-  ptx::grid_dependency_wait();  // (every thread: the GEMM's wait covers the quantizer too)
-  if (threadIdx.x < FEW_ROWS * FEW_RANK) {
-    const int i = threadIdx.x / FEW_RANK, r = threadIdx.x % FEW_RANK;
-    const int m = m0 + i;
-    const int a = m < p.M ? __ldg(p.ids + m) : -1;
-    if (has_adapter(p, a)) {
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < FEW_WARPS; ++w) v += s_sum[w][threadIdx.x];
-      p.h[static_cast<int64_t>(m) * p.R + r0 + r] = v * __ldg(p.scaling + a);
-    }
-  }
-}
-
-// ---------------------------------------------------------------- many rows
 
 constexpr int ROWS = 128;
 constexpr int KB = 64;     // 16-bit elements per K-block: one 128-byte swizzle row
@@ -199,7 +103,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   ptx::grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
-  const int m0 = static_cast<int>(blockIdx.x / p.split) * ROWS;
+  const int cluster = static_cast<int>(blockIdx.x) / p.split;
+  const int m0 = cluster / p.par * ROWS;
+  const int ps0 = cluster % p.par;
 
   if (threadIdx.x == 0) {
     ptx::prefetch_tmap(&tmap_x);
@@ -263,7 +169,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       uint32_t phase = 0;
       uint32_t issued = 0;
       bool ok = true;
-      for (int ps = 0; ps < passes && ok; ++ps) {
+      for (int ps = ps0; ps < passes && ok; ps += p.par) {
         const int d0 = ps * per_pass, nd = min(per_pass, distinct - d0);
         for (int i = 0; i < nkb; ++i) {
           if (!ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort, kWaitLimitNs)) {
@@ -301,11 +207,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int ps = 0; ps < passes && ok; ++ps) {
+      for (int ps = ps0; ps < passes && ok; ps += p.par) {
         const int nd = min(per_pass, distinct - ps * per_pass);
         const uint32_t idesc = ptx::idesc_f16_f32(ROWS, nd * p.rank_pad, p.dtype == kBF16);
-        if (ps > 0 && !ptx::mbar_wait_bounded(bar_free, static_cast<uint32_t>(ps - 1) & 1u, abort,
-                                              kWaitLimitNs)) {
+        if (ps > ps0 && !ptx::mbar_wait_bounded(
+                            bar_free, static_cast<uint32_t>((ps - ps0) / p.par - 1) & 1u, abort,
+                            kWaitLimitNs)) {
           record_timeout(abort);
           break;
         }
@@ -339,9 +246,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int mine = s_id[row] >= 0 ? s_rank[s_first[row]] : -1;
-    for (int ps = 0; ps < passes; ++ps) {
+    for (int ps = ps0; ps < passes; ps += p.par) {
       const int d0 = ps * per_pass, nd = min(per_pass, distinct - d0);
-      if (!ptx::mbar_wait_bounded(bar_acc, static_cast<uint32_t>(ps) & 1u, abort, kWaitLimitNs)) {
+      if (!ptx::mbar_wait_bounded(bar_acc, static_cast<uint32_t>((ps - ps0) / p.par) & 1u, abort,
+                                  kWaitLimitNs)) {
         if (lane == 0) record_timeout(abort);
         break;
       }
@@ -379,7 +287,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const bool fine = *abort == 0;
   for (int row = rank + warp * p.split; row < ROWS && fine; row += NUM_THREADS / 32 * p.split) {
     const int id = s_id[row];
-    if (id < 0) continue;
+    if (id < 0 || s_rank[s_first[row]] / per_pass % p.par != ps0) continue;
     const float sc = __ldg(p.scaling + id);
     float v[kLoraMaxRank / 32];
     float top = 0.0f;
@@ -428,20 +336,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     if (lane == 0)
       p.hscale[m0 + row] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
   }
-  // The adapter of each token tile of the GEMM: one for all rows, none, or several (-2).
+  // Row M of hl: zeros.
+  if (blockIdx.x == 0)
+    for (int c = threadIdx.x; c < 2 * p.rank_pad; c += NUM_THREADS)
+      reinterpret_cast<uint16_t *>(p.hl)[static_cast<int64_t>(p.M) * (2 * p.rank_pad) + c] = 0;
+  // The adapters of each token tile of the GEMM, a warp to a tile: 32 tokens at a time, the
+  // first of each id among them looks the id up in the list and appends it.
   for (int t = static_cast<int>(blockIdx.x) * (NUM_THREADS / 32) + warp; t < p.gemm_tiles;
        t += static_cast<int>(gridDim.x) * (NUM_THREADS / 32)) {
     const int t0 = t * p.gemm_tile_tokens, t1 = min(p.M, t0 + p.gemm_tile_tokens);
-    int lead = __ldg(p.ids + t0);
-    if (!has_adapter(p, lead)) lead = -1;
-    bool same = true;
-    for (int m = t0 + lane; m < t1; m += 32) {
-      int id = __ldg(p.ids + m);
-      if (!has_adapter(p, id)) id = -1;
-      same = same && id == lead;
+    int *list = p.list + static_cast<int64_t>(t) * kLoraTileTokens;
+    int n = 0;
+    for (int b = t0; b < t1; b += 32) {
+      const int id = b + lane < t1 ? __ldg(p.ids + b + lane) : -1;
+      const uint32_t same = __match_any_sync(0xFFFFFFFFu, id);
+      bool add = has_adapter(p, id) && (same & ((1u << lane) - 1u)) == 0;
+      for (int i = 0; i < n && add; ++i) add = *const_cast<volatile int *>(list + i) != id;
+      const uint32_t votes = __ballot_sync(0xFFFFFFFFu, add);
+      if (add) list[n + __popc(votes & ((1u << lane) - 1u))] = id;
+      n += __popc(votes);
+      __syncwarp();
     }
-    same = __all_sync(0xFFFFFFFFu, same);
-    if (lane == 0) p.tile_adapter[t] = same ? lead : -2;
+    if (lane == 0) p.count[t] = n;
   }
 
   ptx::cluster_sync();  // peers may still be reading this CTA's partial sums
@@ -458,17 +374,14 @@ size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 LoraWorkspace lora_workspace(void *base, int64_t M, int64_t R) {
   LoraWorkspace w;
   uint8_t *b = static_cast<uint8_t *>(base);
-  if (M <= kLoraRowsMaxM) {
-    w.h = reinterpret_cast<float *>(b);
-    w.bytes = lora::align256(static_cast<size_t>(M) * R * 4);
-    return w;
-  }
-  const size_t hl = lora::align256(static_cast<size_t>(M) * 2 * lora_rank_pad(R) * 2);
+  const size_t hl = lora::align256(static_cast<size_t>(M + 1) * 2 * lora_rank_pad(R) * 2);
   const size_t sc = lora::align256(static_cast<size_t>(M) * 4);
+  const size_t ct = lora::align256(static_cast<size_t>(lora_tiles(M)) * 4);
   w.hl = b;
   w.hscale = reinterpret_cast<float *>(b + hl);
-  w.tile_adapter = reinterpret_cast<int *>(b + hl + sc);
-  w.bytes = hl + sc + lora::align256(static_cast<size_t>(lora_tiles(M)) * 4);
+  w.count = reinterpret_cast<int *>(b + hl + sc);
+  w.list = reinterpret_cast<int *>(b + hl + sc + ct);
+  w.bytes = hl + sc + ct + lora::align256(static_cast<size_t>(lora_tiles(M)) * kLoraTileTokens * 4);
   return w;
 }
 
@@ -488,67 +401,63 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   p.L = static_cast<int>(a.L);
   p.R = static_cast<int>(a.R);
   p.rank_pad = static_cast<int>(lora_rank_pad(a.R));
-  p.h = w.h;
   p.hl = w.hl;
   p.hscale = w.hscale;
-  p.tile_adapter = w.tile_adapter;
+  p.count = w.count;
+  p.list = w.list;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
+  cudaError_t e;
+  p.gemm_tiles = static_cast<int>(lora_tiles(a.M));
+  p.gemm_tile_tokens = static_cast<int>(lora_tile_tokens(a.M));
+  p.k_blocks = static_cast<int>((a.K + KB - 1) / KB);
+  const int64_t tiles = (a.M + ROWS - 1) / ROWS;
+  // K-splits while CTAs are left over, four K-blocks at least for each
+  const int split = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>({dev.sm_count / tiles, MAX_SPLIT, (p.k_blocks + 3) / 4})));
+  p.kps = (p.k_blocks + split - 1) / split;
+  p.split = (p.k_blocks + p.kps - 1) / p.kps;
+  // passes side by side while CTAs are left over still
+  const int64_t most = (std::min<int64_t>(a.L, ROWS) + COLS / p.rank_pad - 1) / (COLS / p.rank_pad);
+  p.par = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(dev.sm_count / (tiles * p.split), most)));
+  const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  std::string err;
+  CUtensorMap tx, ta;
+  if (!make_tmap_2d_sw128(&tx, t16, a.x, a.K, a.M, a.K * 2, KB, ROWS, &err) ||
+      !make_tmap_3d_sw128(&ta, t16, a.lora_a, a.K, a.R, a.L, a.K * 2, a.R * a.K * 2, KB,
+                          static_cast<uint32_t>(p.rank_pad), &err)) {
+    set_error("fp8_linear_lora: " + err);
+    return 4;
+  }
+  static bool set[64];
+  static std::mutex mu;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!set[dev.device & 63]) {
+      e = cudaFuncSetAttribute(down_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(SMEM_BYTES));
+      if (e != cudaSuccess) {
+        set_error(std::string("fp8_linear_lora: kernel setup: ") + cudaGetErrorString(e));
+        return 4;
+      }
+      set[dev.device & 63] = true;
+    }
+  }
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(p.split);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e;
-  if (a.M <= kLoraRowsMaxM) {
-    cfg.gridDim = dim3(static_cast<unsigned>((a.M + FEW_ROWS - 1) / FEW_ROWS),
-                       static_cast<unsigned>(a.R / FEW_RANK));
-    cfg.blockDim = dim3(32 * FEW_WARPS);
-    e = cudaLaunchKernelEx(&cfg, down_rows_kernel, p);
-  } else {
-    p.gemm_tiles = static_cast<int>(lora_tiles(a.M));
-    p.gemm_tile_tokens = static_cast<int>(lora_tile_tokens(a.M));
-    p.k_blocks = static_cast<int>((a.K + KB - 1) / KB);
-    const int64_t tiles = (a.M + ROWS - 1) / ROWS;
-    // K-splits while CTAs are left over, four K-blocks at least for each
-    const int split = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>({dev.sm_count / tiles, MAX_SPLIT, (p.k_blocks + 3) / 4})));
-    p.kps = (p.k_blocks + split - 1) / split;
-    p.split = (p.k_blocks + p.kps - 1) / p.kps;
-    const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    std::string err;
-    CUtensorMap tx, ta;
-    if (!make_tmap_2d_sw128(&tx, t16, a.x, a.K, a.M, a.K * 2, KB, ROWS, &err) ||
-        !make_tmap_3d_sw128(&ta, t16, a.lora_a, a.K, a.R, a.L, a.K * 2, a.R * a.K * 2, KB,
-                            static_cast<uint32_t>(p.rank_pad), &err)) {
-      set_error("fp8_linear_lora: " + err);
-      return 4;
-    }
-    static bool set[64];
-    static std::mutex mu;
-    {
-      std::lock_guard<std::mutex> lock(mu);
-      if (!set[dev.device & 63]) {
-        e = cudaFuncSetAttribute(down_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(SMEM_BYTES));
-        if (e != cudaSuccess) {
-          set_error(std::string("fp8_linear_lora: kernel setup: ") + cudaGetErrorString(e));
-          return 4;
-        }
-        set[dev.device & 63] = true;
-      }
-    }
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(p.split);
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.numAttrs = 2;
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.split));
-    cfg.blockDim = dim3(NUM_THREADS);
-    cfg.dynamicSmemBytes = SMEM_BYTES;
-    e = cudaLaunchKernelEx(&cfg, down_tile_kernel, tx, ta, p);
-  }
+  cfg.numAttrs = 2;
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.par * p.split));
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  e = cudaLaunchKernelEx(&cfg, down_tile_kernel, tx, ta, p);
   if (e != cudaSuccess) {
     set_error(std::string("fp8_linear_lora: launch failed: ") + cudaGetErrorString(e));
     return 4;

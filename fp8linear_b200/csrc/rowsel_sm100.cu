@@ -47,7 +47,6 @@ constexpr int NUM_THREADS = 192;
 constexpr int EPI_WARPS = 4;
 constexpr uint32_t W_STAGE = WROWS * BK;  // 16 KB
 constexpr int X_MAPS = 8;                 // token boxes of 16, 32, .. 128 rows
-constexpr int H_MAPS = kLoraTileTokens / 32;  // boxes of the adapters' h: 16, 32, .. 80 rows
 constexpr uint64_t kWaitLimitNs = 4000000000ull;
 constexpr uint64_t kDrainLimitNs = 1000000000ull;
 
@@ -55,7 +54,7 @@ struct Maps {
   CUtensorMap x[X_MAPS];  // xq [M][K], box 128 B x 16 (i + 1) rows
   CUtensorMap w;          // wq [E][N][K], box 128 B x 128 rows x 1
   CUtensorMap lb;         // lora_b [L][N][R], box 64 x 128 rows x 1
-  CUtensorMap h[H_MAPS];  // hl [M][2 rank_pad], box 64 x 16 (i + 1) rows
+  CUtensorMap h;          // hl [M + 1][2 rank_pad], box 64 x 1 (gathered)
 };
 
 struct Params {
@@ -74,17 +73,15 @@ struct Params {
   int split, kps, stages;
   int tok_cap;        // tokens per tile at most
   uint32_t off_part;  // shared-memory offsets
-  uint32_t off_lora;
   uint32_t off_tab;
   // adapters
   const int *ids;
   const void *lora_b;
   int lora_dtype;
   int L, R, rank_pad;
-  const int *tile_adapter;  // persist_kernel
+  const int *count, *list;  // adapters of each token tile
   const void *hl;
   const float *hscale;
-  const float *h;           // split_kernel
 };
 
 __device__ __forceinline__ float load_bias(const void *bias, int dtype, int64_t n) {
@@ -104,22 +101,6 @@ __device__ __forceinline__ void store_out(void *out, int dtype, int64_t i, float
     reinterpret_cast<__half *>(out)[i] = __float2half_rn(v);
   else
     reinterpret_cast<__nv_bfloat16 *>(out)[i] = __float2bfloat16_rn(v);
-}
-
-// Eight 16-bit values as floats.
-__device__ __forceinline__ void unpack8(const uint4 &v, bool f16, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (f16) {
-      const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    } else {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    }
-  }
 }
 
 __device__ __forceinline__ void record_timeout(volatile int *abort) {
@@ -226,6 +207,94 @@ __device__ __forceinline__ void zero_rows(const Params &p, const int *row, int f
   }
 }
 
+// ---------------------------------------------------------------- adapters
+//
+// A token tile's adapters are taken one after the other, as further stages of the ring: the
+// adapter's B rows beside the tile's h, in which tokens of other adapters are rows of zeros
+// (gathered from the zero row of hl). Their products add up in one accumulator. 64 16-bit
+// elements are the 128 bytes of a stage's row: up to rank 32 the high and the low part of h
+// share a stage, above it each 64 values of the rank take one for either part.
+//
+// 0 * B is zero only for finite B: an infinity or NaN in an adapter also makes NaN of the
+// tokens that are not its own. So in a tile of several adapters the epilogue computes every
+// sum that is not finite once more (exact_sum), with the token's own adapter alone.
+
+__device__ __forceinline__ int lora_stages(const Params &p) {
+  return p.rank_pad <= 32 ? 1 : 2 * ((p.rank_pad + 63) / 64);
+}
+
+// Rows 4 * lane .. + 3 of a token tile half (lanes up to rows / 4), with their adapters.
+struct GatherRows {
+  int row[4];
+  int id[4];
+};
+
+__device__ __forceinline__ GatherRows gather_rows(const Params &p, int first, int end, int lane) {
+  GatherRows g;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    g.row[i] = first + 4 * lane + i;
+    g.id[i] = g.row[i] < end ? __ldg(p.ids + g.row[i]) : -1;
+  }
+  return g;
+}
+
+// Stage `j` (of lora_stages) of adapter `a`: columns of B and of hl.
+__device__ __forceinline__ void lora_columns(const Params &p, int j, int &bx, int &hx) {
+  const int chunks = (p.rank_pad + 63) / 64;
+  bx = (j % chunks) * 64;
+  hx = (j / chunks) * p.rank_pad + bx;
+}
+
+template <int CG>
+__device__ __forceinline__ void gather_h(const Params &p, const CUtensorMap *map,
+                                         const GatherRows &g, int rows, int a, int x,
+                                         uint32_t dst, uint32_t bar, int lane) {
+  if (4 * lane < rows) {
+    int r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = g.id[i] == a ? g.row[i] : p.M;
+    ptx::tma_gather4<CG>(dst + static_cast<uint32_t>(lane) * 4 * BK, map, x, r[0], r[1], r[2],
+                         r[3], bar);
+  }
+}
+
+// The MMAs of stage `j` of an adapter; `first`: nothing in the accumulator counts yet.
+template <int CG>
+__device__ __forceinline__ void lora_mma(const Params &p, uint32_t d, uint32_t stage, uint32_t idesc,
+                                         int j, bool first) {
+  const uint64_t adesc = ptx::sw128_kmajor_desc(stage);
+  const uint64_t bdesc = ptx::sw128_kmajor_desc(stage + W_STAGE);
+  int bx, hx;
+  lora_columns(p, j, bx, hx);
+  const int steps = min(64, p.rank_pad - bx) / 16;  // 16 elements: 32 bytes
+  for (int kk = 0; kk < steps; ++kk)
+    ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + 2 * kk, idesc, first && kk == 0 ? 0u : 1u);
+  if (p.rank_pad <= 32)  // the low part, next to the high part
+    for (int kk = 0; kk < steps; ++kk)
+      ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + 2 * (kk + steps), idesc, 1u);
+}
+
+__device__ __forceinline__ float load16(const uint16_t *v, bool f16) {
+  const uint16_t b = __ldg(v);
+  return f16 ? __half2float(__ushort_as_half(b)) : __uint_as_float(static_cast<uint32_t>(b) << 16);
+}
+
+// sum_r (hi + lo)[token][r] * B[id][n][r], on CUDA cores.
+__device__ __noinline__ float exact_sum(const Params &p, int token, int id, int n) {
+  const bool f16 = p.lora_dtype == kF16;
+  const uint16_t *h = reinterpret_cast<const uint16_t *>(p.hl) +
+                      static_cast<int64_t>(token) * (2 * p.rank_pad);
+  const uint16_t *b = reinterpret_cast<const uint16_t *>(p.lora_b) +
+                      (static_cast<int64_t>(id) * p.N + n) * p.R;
+  float s = 0.0f;
+  for (int r = 0; r < p.R; ++r)
+    s = fmaf(load16(h + r, f16) + load16(h + p.rank_pad + r, f16), load16(b + r, f16), s);
+  return s;
+}
+
+__device__ __forceinline__ bool is_finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+
 // ---------------------------------------------------------------- persistent kernel
 
 template <int CG, bool LORA>
@@ -311,60 +380,81 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
+    // (the whole warp: the rows of h are gathered by all lanes)
+    {
       int stage = 0;
       uint32_t phase = 0;
       uint32_t issued = 0;
       int e = 0;
-      // One stage: the weight box and the token box at the given coordinates.
-      auto load = [&](const CUtensorMap *mw, int wx, int wy, int wz, const CUtensorMap *mx, int xx,
-                      int xy, int nn) -> bool {
-        if (!ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort, kWaitLimitNs)) {
-          record_timeout(abort);
-          return false;
+      // A free stage: false when the wait ran out.
+      auto take = [&]() -> bool {
+        bool got = true;
+        if (lane == 0) {
+          got = ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort, kWaitLimitNs);
+          if (!got) record_timeout(abort);
         }
-        const uint32_t fb = bar_full + 8 * stage;
-        const uint32_t dst = sbase + static_cast<uint32_t>(stage) * C::STAGE;
-        const uint32_t tx = CG * W_STAGE + static_cast<uint32_t>(nn) * BK;
-        if constexpr (CG == 1) {
-          ptx::mbar_arrive_expect_tx(fb, tx);
-          ptx::tma_load_3d(dst, mw, wx, wy, wz, fb);
-          ptx::tma_load_2d(dst + W_STAGE, mx, xx, xy, fb);
-        } else {
-          // both CTAs' bytes complete the leader's barrier; only the leader arms it
-          if (leader) ptx::mbar_arrive_expect_tx(fb, tx);
-          const uint32_t fl = ptx::map_shared_rank(fb, 0);
-          ptx::tma_load_3d_pair(dst, mw, wx, wy, wz, fl);
-          ptx::tma_load_2d_pair(dst + W_STAGE, mx, xx, xy, fl);
-        }
+        return LORA ? __shfl_sync(0xFFFFFFFFu, got ? 1 : 0, 0) != 0 : got;
+      };
+      auto next = [&]() {
         ++issued;
         if (++stage == C::STAGES) {
           stage = 0;
           phase ^= 1u;
         }
-        return true;
       };
       bool ok = true;
-      for (int t = group; t < num_tiles && ok; t += n_groups) {
+      for (int t = group; t < num_tiles && ok && (LORA || lane == 0); t += n_groups) {
         const Tile q = find_tile<CG>(p, C::TOK_MAX, g_row, g_tile, t, e);
         const int wrow = (q.wb * CG + static_cast<int>(rank)) * WROWS;
         const int xrows = q.nn / CG;
         const int xrow = q.t0 + static_cast<int>(rank) * xrows;
-        const int mi = xrows / 16 - 1;
-        for (int kb = 0; kb < p.k_blocks && ok; ++kb)
-          ok = load(&maps.w, kb * BK, wrow, q.e, &maps.x[mi], kb * BK, xrow, q.nn);
+        const uint32_t tx = CG * W_STAGE + static_cast<uint32_t>(q.nn) * BK;
+        // both CTAs' bytes complete the leader's barrier; only the leader arms it
+        auto arm = [&](const CUtensorMap *m, int x, int z) {
+          const uint32_t fb = bar_full + 8 * stage;
+          const uint32_t dst = sbase + static_cast<uint32_t>(stage) * C::STAGE;
+          if (leader) ptx::mbar_arrive_expect_tx(fb, tx);
+          if constexpr (CG == 1)
+            ptx::tma_load_3d(dst, m, x, wrow, z, fb);
+          else
+            ptx::tma_load_3d_pair(dst, m, x, wrow, z, ptx::map_shared_rank(fb, 0));
+        };
+        auto dst_x = [&]() { return sbase + static_cast<uint32_t>(stage) * C::STAGE + W_STAGE; };
+        auto bar_x = [&]() {
+          const uint32_t fb = bar_full + 8 * stage;
+          return CG == 1 ? fb : ptx::map_shared_rank(fb, 0);
+        };
+        const CUtensorMap *mx = &maps.x[xrows / 16 - 1];
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!(ok = take())) break;
+          if (lane == 0) {
+            arm(&maps.w, kb * BK, q.e);
+            if constexpr (CG == 1)
+              ptx::tma_load_2d(dst_x(), mx, kb * BK, xrow, bar_x());
+            else
+              ptx::tma_load_2d_pair(dst_x(), mx, kb * BK, xrow, bar_x());
+          }
+          next();
+        }
         if constexpr (LORA) {
-          const int a = __ldg(p.tile_adapter + q.tb);
-          if (a >= 0) {
-            // the adapter's B rows and the tokens' h as further stages (64 16-bit elements
-            // are 128 bytes): up to rank 32 the high and low parts of h share a stage
-            const int parts = p.rank_pad <= 32 ? 1 : 2;
-            for (int part = 0; part < parts; ++part)
-              for (int c = 0; c < p.rank_pad && ok; c += 64)
-                ok = load(&maps.lb, c, wrow, a, &maps.h[mi], part * p.rank_pad + c, xrow, q.nn);
+          const int count = __ldg(p.count + q.tb), per = lora_stages(p);
+          GatherRows g;
+          if (count > 0) g = gather_rows(p, xrow, q.t1, lane);
+          for (int d = 0; d < count && ok; ++d) {
+            const int a = __ldg(p.list + static_cast<int64_t>(q.tb) * kLoraTileTokens + d);
+            for (int j = 0; j < per; ++j) {
+              if (!(ok = take())) break;
+              int bx, hx;
+              lora_columns(p, j, bx, hx);
+              if (lane == 0) arm(&maps.lb, bx, a);
+              __syncwarp();
+              gather_h<CG>(p, &maps.h, g, xrows, a, hx, dst_x(), bar_x(), lane);
+              next();
+            }
           }
         }
       }
+      if (lane == 0) {
       // Drain: every load issued here has landed and been consumed.
       const uint32_t n_drain = issued < C::STAGES ? issued : C::STAGES;
       for (uint32_t i = 0; i < n_drain; ++i) {
@@ -375,6 +465,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           --stage;
         }
         ptx::mbar_wait_timeout(bar_empty + 8 * stage, phase, kDrainLimitNs);
+      }
       }
     }
   } else if (warp == 1) {
@@ -432,8 +523,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           next_stage();
         }
         if constexpr (LORA) {
-          const int a = ok ? __ldg(p.tile_adapter + q.tb) : -1;
-          if (a >= 0) {
+          const int count = ok ? __ldg(p.count + q.tb) : 0;
+          if (count > 0) {
             // the third accumulator is free once the epilogue of the tile before has let
             // its own go (the same arrival that this loop waits for one tile later)
             if (it > 0 && !ptx::mbar_wait_bounded(bar_tempty + 8 * (acc ^ 1),
@@ -443,27 +534,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               break;
             }
             ptx::tc_fence_after();
-            const uint32_t dl = tmem_base + C::ACC_L;
-            const uint32_t id16 =
-                ptx::idesc_f16_f32(WROWS * CG, q.nn, p.lora_dtype == kBF16);
-            uint32_t accumulate = 0;
-            const int parts = p.rank_pad <= 32 ? 1 : 2;
-            for (int part = 0; part < parts && ok; ++part)
-              for (int c = 0; c < p.rank_pad; c += 64) {
-                if (!(ok = wait_full())) break;
-                const uint32_t st = sbase + static_cast<uint32_t>(stage) * C::STAGE;
-                const uint64_t adesc = ptx::sw128_kmajor_desc(st);
-                const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
-                const int steps = min(64, p.rank_pad - c) / 16;  // 16 elements = 32 bytes
-                for (int kk = 0; kk < steps; ++kk) {
-                  ptx::mma_f16<CG>(dl, adesc + 2 * kk, bdesc + 2 * kk, id16, accumulate);
-                  accumulate = 1;
-                }
-                if (parts == 1)  // low part: next to the high part in the same box
-                  for (int kk = 0; kk < steps; ++kk)
-                    ptx::mma_f16<CG>(dl, adesc + 2 * kk, bdesc + 2 * (kk + steps), id16, 1);
-                next_stage();
-              }
+            const uint32_t id16 = ptx::idesc_f16_f32(WROWS * CG, q.nn, p.lora_dtype == kBF16);
+            const int per = lora_stages(p);
+            for (int i = 0; i < count * per; ++i) {
+              if (!(ok = wait_full())) break;
+              lora_mma<CG>(p, tmem_base + C::ACC_L, sbase + static_cast<uint32_t>(stage) * C::STAGE,
+                           id16, i % per, i == 0);
+              next_stage();
+            }
           }
         }
         if (!ok) break;
@@ -487,7 +565,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     float *e_xs = reinterpret_cast<float *>(smem + C::OFF_PAR + (warp - 2) * C::PAR_WARP);
     float *e_hs = e_xs + C::TOK_MAX;
     int *e_id = reinterpret_cast<int *>(e_hs + C::TOK_MAX);
-    const bool f16 = LORA && p.lora_dtype == kF16;
     int it = 0;
     int e = 0;
     for (int t = group; t < num_tiles; t += n_groups, ++it) {
@@ -498,14 +575,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int n = (q.wb * CG + static_cast<int>(rank)) * WROWS + quarter * 32 + lane;
       const bool live = n < p.N;
       const int64_t wn = static_cast<int64_t>(q.e) * p.N + min(n, p.N - 1);
-      int adapter = -1;
-      if constexpr (LORA) adapter = __ldg(p.tile_adapter + q.tb);
+      int adapters = 0;
+      if constexpr (LORA) adapters = __ldg(p.count + q.tb);
       __syncwarp();
       for (int i = lane; i < cnt; i += 32) {
         e_xs[i] = __ldg(p.xs + q.t0 + i);
         if constexpr (LORA) {
-          e_hs[i] = adapter != -1 ? __ldg(p.hscale + q.t0 + i) : 0.0f;
-          e_id[i] = __ldg(p.ids + q.t0 + i);
+          const int id = __ldg(p.ids + q.t0 + i);
+          const bool has = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L);
+          e_id[i] = has ? id : -1;
+          e_hs[i] = has ? __ldg(p.hscale + q.t0 + i) : 0.0f;
         }
       }
       const float w = __ldg(p.ws + wn);
@@ -526,52 +605,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[j]) * e_xs[min(c + j, cnt - 1)], w, b);
         if constexpr (LORA) {
-          if (adapter >= 0) {
+          if (adapters > 0) {
             ptx::tmem_ld_32x32b_x32(t_row + C::ACC_L + static_cast<uint32_t>(c), r);
             ptx::tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              v[j] = fmaf(__uint_as_float(r[j]), e_hs[min(c + j, cnt - 1)], v[j]);
-          } else if (adapter == -2) {
-            // A tile of several adapters: the sums over the rank on CUDA cores, each row
-            // with its own adapter's values only. The B rows of a run of equal ids are
-            // loaded once per 8 values of the rank.
-            float s[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) s[j] = 0.0f;
-            const uint16_t *hl = reinterpret_cast<const uint16_t *>(p.hl);
-            const uint16_t *lb = reinterpret_cast<const uint16_t *>(p.lora_b);
-            for (int rc = 0; rc < p.R; rc += 8) {
-              int cur = -1;
-              float bw[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) bw[i] = 0.0f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int id = c + j < cnt ? e_id[c + j] : -1;
-                if (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L)) {
-                  if (id != cur) {
-                    cur = id;
-                    unpack8(__ldg(reinterpret_cast<const uint4 *>(
-                                lb + (static_cast<int64_t>(id) * p.N + min(n, p.N - 1)) * p.R +
-                                rc)),
-                            f16, bw);
-                  }
-                  const uint16_t *hr =
-                      hl + static_cast<int64_t>(q.t0 + c + j) * (2 * p.rank_pad) + rc;
-                  float hi[8], lo[8];
-                  unpack8(__ldg(reinterpret_cast<const uint4 *>(hr)), f16, hi);
-                  unpack8(__ldg(reinterpret_cast<const uint4 *>(hr + p.rank_pad)), f16, lo);
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) s[j] = fmaf(hi[i] + lo[i], bw[i], s[j]);
-                }
-              }
-            }
-#pragma unroll
             for (int j = 0; j < 32; ++j) {
-              const int id = c + j < cnt ? e_id[c + j] : -1;
-              if (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L))
-                v[j] = fmaf(s[j], e_hs[c + j], v[j]);
+              const int i = min(c + j, cnt - 1);
+              float s = __uint_as_float(r[j]);
+              const int id = e_id[i];
+              if (adapters > 1 && !is_finite(s) && id >= 0 && live)
+                s = exact_sum(p, q.t0 + i, id, n);
+              v[j] = id >= 0 ? fmaf(s, e_hs[i], v[j]) : v[j];
             }
           }
         }
@@ -609,7 +653,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 constexpr int SPLIT_TOK = 128;   // tokens per tile, at most
 constexpr int SPLIT_STAGES = 8;  // ring slots, at most
 constexpr int SPLIT_MAX = 8;     // CTAs per cluster, at most (portable)
-constexpr uint32_t SPLIT_EPI = (SPLIT_TOK + 2 * WROWS) * 4;  // xs, ws, bias of the reduction
+constexpr uint32_t SPLIT_EPI = (3 * SPLIT_TOK + 2 * WROWS) * 4;  // xs, ws, bias, hscale, ids
 constexpr uint32_t SPLIT_SMEM = 232448;
 
 template <bool LORA>
@@ -629,19 +673,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   volatile uint32_t *tmem_slot = &s_slot;
   volatile int *abort = &s_abort;
   float *part = reinterpret_cast<float *>(smem + p.off_part);  // [tokens][WROWS]
-  float *lora = reinterpret_cast<float *>(smem + p.off_lora);  // [tokens][rows reduced here]
   int *g_row = reinterpret_cast<int *>(smem + p.off_tab);
   int *g_tile = g_row + p.E + 1;
   float *e_xs = reinterpret_cast<float *>(g_tile + p.E + 1);  // [SPLIT_TOK]
   float *e_ws = e_xs + SPLIT_TOK;                              // [WROWS]
   float *e_b = e_ws + WROWS;
+  float *e_hs = e_b + WROWS;                              // [SPLIT_TOK]
+  int *e_id = reinterpret_cast<int *>(e_hs + SPLIT_TOK);  // [SPLIT_TOK]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
   const int stages = p.stages;
   const uint32_t stage_bytes = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
+  // TMEM: the accumulator, and behind it the adapters'
+  const uint32_t acc_l = static_cast<uint32_t>(p.tok_cap);
   uint32_t tmem_cols = 32;
-  while (tmem_cols < static_cast<uint32_t>(p.tok_cap)) tmem_cols <<= 1;
+  while (tmem_cols < (LORA ? 2 : 1) * static_cast<uint32_t>(p.tok_cap)) tmem_cols <<= 1;
 
   if (threadIdx.x == 0) {
     ptx::prefetch_tmap(&maps.w);
@@ -701,42 +748,59 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int quads = r1 > r0 ? (r1 - r0) >> 2 : 0;
   const int n0 = q.wb * WROWS;
 
+  // This CTA's adapters: every split-th of the tile's, as stages behind its K-blocks.
+  const int adapters = LORA ? __ldg(p.count) : 0;
+  const int mine = LORA && adapters > rank ? (adapters - rank + p.split - 1) / p.split : 0;
+  const int per = LORA ? lora_stages(p) : 0;
+  const int nst = nkb + mine * per;
+
   if (warp == 0) {
-    if (lane == 0) {
-      const int first = min(stages, nkb);
-      for (int i = 0; i < first; ++i)
-        ptx::tma_load_2d(sbase + static_cast<uint32_t>(i) * stage_bytes + W_STAGE, mx,
-                         (kb0 + i) * BK, q.t0, bar_full + 8 * i);
-      int issued = first;
-      int s = first == stages ? 0 : first;
-      uint32_t ph = 1;
-      for (int i = first; i < nkb; ++i) {
-        if (!ptx::mbar_wait_bounded(bar_empty + 8 * s, ph ^ 1u, abort, kWaitLimitNs)) {
-          record_timeout(abort);
-          break;
-        }
-        const uint32_t fb = bar_full + 8 * s;
-        const uint32_t dst = sbase + static_cast<uint32_t>(s) * stage_bytes;
-        ptx::mbar_arrive_expect_tx(fb, tx);
-        ptx::tma_load_3d(dst, &maps.w, (kb0 + i) * BK, n0, q.e, fb);
-        ptx::tma_load_2d(dst + W_STAGE, mx, (kb0 + i) * BK, q.t0, fb);
-        ++issued;
-        if (++s == stages) {
-          s = 0;
-          ph ^= 1u;
-        }
+    GatherRows g;
+    if (LORA && mine > 0) g = gather_rows(p, q.t0, q.t1, lane);
+    int issued = 0;
+    for (int i = 0; i < nst; ++i) {
+      const int s = i % stages;
+      const uint32_t fb = bar_full + 8 * s;
+      const uint32_t dst = sbase + static_cast<uint32_t>(s) * stage_bytes;
+      // (the first K-blocks' stages are armed, their weight boxes under way)
+      const bool armed = i < nkb && i < stages;
+      bool got = true;
+      if (lane == 0 && i >= stages) {
+        got = ptx::mbar_wait_bounded(bar_empty + 8 * s,
+                                     static_cast<uint32_t>(i / stages - 1) & 1u, abort,
+                                     kWaitLimitNs);
+        if (!got) record_timeout(abort);
       }
+      if (__shfl_sync(0xFFFFFFFFu, got ? 1 : 0, 0) == 0) break;
+      if (lane == 0 && !armed) ptx::mbar_arrive_expect_tx(fb, tx);
+      if (i < nkb) {
+        if (lane == 0) {
+          if (!armed) ptx::tma_load_3d(dst, &maps.w, (kb0 + i) * BK, n0, q.e, fb);
+          ptx::tma_load_2d(dst + W_STAGE, mx, (kb0 + i) * BK, q.t0, fb);
+        }
+      } else if constexpr (LORA) {
+        const int d = (i - nkb) / per, j = (i - nkb) % per;
+        const int a = __ldg(p.list + rank + d * p.split);
+        int bx, hx;
+        lora_columns(p, j, bx, hx);
+        if (lane == 0) ptx::tma_load_3d(dst, &maps.lb, bx, n0, a, fb);
+        __syncwarp();
+        gather_h<1>(p, &maps.h, g, q.nn, a, hx, dst + W_STAGE, fb, lane);
+      }
+      ++issued;
+    }
+    if (lane == 0)
       for (int i = issued - 1; i >= 0 && i >= issued - stages; --i)
         ptx::mbar_wait_timeout(bar_empty + 8 * (i % stages),
                                static_cast<uint32_t>(i / stages) & 1u, kDrainLimitNs);
-    }
   } else if (warp == 1) {
     if (lane == 0) {
       bool ok = true;
       const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS, q.nn);
+      const uint32_t id16 = ptx::idesc_f16_f32(WROWS, q.nn, p.lora_dtype == kBF16);
       int s = 0;
       uint32_t ph = 0;
-      for (int i = 0; i < nkb; ++i) {
+      for (int i = 0; i < nst; ++i) {
         if (!ptx::mbar_wait_bounded(bar_full + 8 * s, ph, abort, kWaitLimitNs)) {
           record_timeout(abort);
           ok = false;
@@ -744,12 +808,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         ptx::tc_fence_after();
         const uint32_t st = sbase + static_cast<uint32_t>(s) * stage_bytes;
-        const uint64_t adesc = ptx::sw128_kmajor_desc(st);
-        const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
+        if (i < nkb) {
+          const uint64_t adesc = ptx::sw128_kmajor_desc(st);
+          const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
 #pragma unroll
-        for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-          const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
-          ptx::mma_f8f6f4(tmem, adesc + koff, bdesc + koff, idesc, (i | kk) != 0 ? 1u : 0u);
+          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+            const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
+            ptx::mma_f8f6f4(tmem, adesc + koff, bdesc + koff, idesc, (i | kk) != 0 ? 1u : 0u);
+          }
+        } else if constexpr (LORA) {
+          lora_mma<1>(p, tmem + acc_l, st, id16, (i - nkb) % per, i == nkb);
         }
         ptx::mma_commit(bar_empty + 8 * s);
         if (++s == stages) {
@@ -762,68 +830,62 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
     }
   } else {
+    // xs (adapters: and hscale, ids) of the tokens, weight scales and biases: of the rows
+    // reduced here, or with adapters of all the tile's rows
     const int et = threadIdx.x - 64;
-    for (int i = et; i < cnt; i += NUM_THREADS - 64) e_xs[i] = __ldg(p.xs + q.t0 + i);
+    for (int i = et; i < cnt; i += NUM_THREADS - 64) {
+      e_xs[i] = __ldg(p.xs + q.t0 + i);
+      if constexpr (LORA) {
+        const int id = __ldg(p.ids + q.t0 + i);
+        const bool has = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L);
+        e_id[i] = has ? id : -1;
+        e_hs[i] = has ? __ldg(p.hscale + q.t0 + i) : 0.0f;
+      }
+    }
     for (int i = et; i < r1 - r0; i += NUM_THREADS - 64) {
       const int n = n0 + r0 + i;
       const int64_t wn = static_cast<int64_t>(q.e) * p.N + n;
       e_ws[i] = n < p.N ? __ldg(p.ws + wn) : 0.0f;
       e_b[i] = n < p.N ? load_bias(p.bias, p.bias_dtype, wn) : 0.0f;
     }
-    if constexpr (LORA) {
-      // The adapters' part of the rows reduced here, while the weights stream: one task is 4
-      // rows of one token, with that token's adapter only.
-      const uint16_t *lb = reinterpret_cast<const uint16_t *>(p.lora_b);
-      const bool f16 = p.lora_dtype == kF16;
-      for (int idx = et; idx < cnt * quads; idx += NUM_THREADS - 64) {
-        const int m = idx / quads, qd = idx - m * quads;
-        const int id = __ldg(p.ids + q.t0 + m);
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L)) {
-          const float *hr = p.h + static_cast<int64_t>(q.t0 + m) * p.R;
-          const int nb = n0 + r0 + 4 * qd;
-          for (int rc = 0; rc < p.R; rc += 8) {
-            const float4 h0 = *reinterpret_cast<const float4 *>(hr + rc);
-            const float4 h1 = *reinterpret_cast<const float4 *>(hr + rc + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float bw[8];
-              unpack8(__ldg(reinterpret_cast<const uint4 *>(
-                          lb + (static_cast<int64_t>(id) * p.N + min(nb + i, p.N - 1)) * p.R + rc)),
-                      f16, bw);
-              s[i] = fmaf(h0.x, bw[0], s[i]);
-              s[i] = fmaf(h0.y, bw[1], s[i]);
-              s[i] = fmaf(h0.z, bw[2], s[i]);
-              s[i] = fmaf(h0.w, bw[3], s[i]);
-              s[i] = fmaf(h1.x, bw[4], s[i]);
-              s[i] = fmaf(h1.y, bw[5], s[i]);
-              s[i] = fmaf(h1.z, bw[6], s[i]);
-              s[i] = fmaf(h1.w, bw[7], s[i]);
-            }
-          }
-        }
-        *reinterpret_cast<float4 *>(lora + m * R + 4 * qd) = make_float4(s[0], s[1], s[2], s[3]);
-      }
-    }
-    // TMEM (lane = weight row, column = token) -> part[token][row], fp32
     const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const int n = n0 + row;
+    const float w = LORA && n < p.N ? __ldg(p.ws + n) : 1.0f;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    // TMEM (lane = weight row, column = token) -> part[token][row], fp32: the K-blocks' sums
+    // as they are, or with adapters dequantized, plus the sums of this CTA's adapters
     const bool ok = ptx::mbar_wait_bounded(bar_acc, 0, abort, kWaitLimitNs);
     if (!ok && lane == 0) record_timeout(abort);
     ptx::tc_fence_after();
-    const int row = quarter * 32 + lane;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     for (int c = 0; c < q.nn; c += 16) {
-      uint32_t r[16];
-      if (ok) {
-        ptx::tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                    static_cast<uint32_t>(c),
-                                r);
-        ptx::tmem_wait_ld();
-      } else {
+      uint32_t r[16], l[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = 0u;
+      for (int j = 0; j < 16; ++j) r[j] = l[j] = 0u;
+      if (ok) {
+        ptx::tmem_ld_32x32b_x16(t_row + static_cast<uint32_t>(c), r);
+        if (LORA && mine > 0) ptx::tmem_ld_32x32b_x16(t_row + acc_l + static_cast<uint32_t>(c), l);
+        ptx::tmem_wait_ld();
       }
 #pragma unroll
-      for (int j = 0; j < 16; ++j) part[(c + j) * WROWS + row] = __uint_as_float(r[j]);
+      for (int j = 0; j < 16; ++j) {
+        float v = __uint_as_float(r[j]);
+        if constexpr (LORA) {
+          const int i = min(c + j, cnt - 1);
+          v = v * e_xs[i] * w;
+          float s = __uint_as_float(l[j]);
+          const int id = e_id[i];
+          if (adapters > 1 && mine > 0 && !is_finite(s) && id >= 0 && n < p.N) {
+            // this CTA's adapter's sum again, or nothing
+            s = 0.0f;
+            for (int d = rank; d < adapters; d += p.split)
+              if (__ldg(p.list + d) == id) s = exact_sum(p, q.t0 + i, id, n);
+          }
+          v = id >= 0 ? fmaf(s, e_hs[i], v) : v;
+        }
+        part[(c + j) * WROWS + row] = v;
+      }
     }
     ptx::tc_fence_before();
   }
@@ -856,8 +918,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int nl = 4 * qd + i;
       const int n = n0 + r0 + nl;
       if (n >= p.N) break;
-      float val = fmaf(a[i] * xs, e_ws[nl], e_b[nl]);
-      if constexpr (LORA) val += lora[m * R + nl];
+      const float val = LORA ? a[i] + e_b[nl] : fmaf(a[i] * xs, e_ws[nl], e_b[nl]);
       store_out(p.out, p.out_dtype, static_cast<int64_t>(q.t0 + m) * p.N + n, val);
     }
   }
@@ -976,14 +1037,12 @@ int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const D
   p.split = (p.k_blocks + p.kps - 1) / p.kps;
   const uint32_t stage = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
   const uint32_t part = static_cast<uint32_t>(p.tok_cap) * WROWS * 4;
-  const uint32_t rows = static_cast<uint32_t>(((WROWS + p.split - 1) / p.split + 3) & ~3);
-  const uint32_t lora = LORA ? static_cast<uint32_t>(p.tok_cap) * rows * 4 : 0;
   const uint32_t tab = static_cast<uint32_t>(p.E + 1) * 8 + SPLIT_EPI;
-  const uint32_t room = SPLIT_SMEM - 2048 - part - lora - tab;
-  p.stages = std::max(1, std::min({static_cast<int>(room / stage), SPLIT_STAGES, p.kps}));
+  const uint32_t room = SPLIT_SMEM - 2048 - part - tab;
+  p.stages = std::max(1, std::min({static_cast<int>(room / stage), SPLIT_STAGES,
+                                   LORA ? SPLIT_STAGES : p.kps}));
   p.off_part = static_cast<uint32_t>(p.stages) * stage;
-  p.off_lora = p.off_part + part;
-  p.off_tab = p.off_lora + lora;
+  p.off_tab = p.off_part + part;
   const size_t smem = p.off_tab + tab + 1024;
   const cudaError_t e = launch(reinterpret_cast<const void *>(&split_kernel<LORA>), maps, p,
                                tiles * p.split, p.split, smem, stream, pdl);
@@ -1026,7 +1085,7 @@ int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl) {
     return 4;
   }
   maps.lb = maps.w;
-  for (auto &h : maps.h) h = maps.x[0];
+  maps.h = maps.x[0];
   Params p = {};
   p.xs = a.xs;
   p.ws = a.ws;
@@ -1073,15 +1132,10 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   bool ok = make_common_maps(&maps, a.xq, a.wq, a.M, a.N, a.K, 1, &err);
-  if (few) {
-    maps.lb = maps.w;
-    for (auto &h : maps.h) h = maps.x[0];
-  } else {
-    ok = ok && make_tmap_3d_sw128(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2,
-                                  64, WROWS, &err);
-    for (int i = 0; ok && i < H_MAPS; ++i)
-      ok = make_tmap_2d_sw128(&maps.h[i], t16, w.hl, 2 * rp, a.M, 4 * rp, 64, 16 * (i + 1), &err);
-  }
+  ok = ok &&
+       make_tmap_3d_sw128(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2, 64, WROWS,
+                          &err) &&
+       make_tmap_2d_sw128(&maps.h, t16, w.hl, 2 * rp, a.M + 1, 4 * rp, 64, 1, &err);
   if (!ok) {
     set_error(std::string(op) + ": " + err);
     return 4;
@@ -1105,10 +1159,10 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   p.L = static_cast<int>(a.L);
   p.R = static_cast<int>(a.R);
   p.rank_pad = static_cast<int>(rp);
-  p.tile_adapter = w.tile_adapter;
+  p.count = w.count;
+  p.list = w.list;
   p.hl = w.hl;
   p.hscale = w.hscale;
-  p.h = w.h;
   if (few) {
     const int64_t wb = (a.N + WROWS - 1) / WROWS;
     if (wb > 0x3fffffLL) {

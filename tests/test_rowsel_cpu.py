@@ -110,8 +110,9 @@ def test_lora_workspace_size(api):
     size = api.lora_workspace_size
     assert size(0, 32, 16) == 0
     assert size(5, 64, 0) == api.workspace_size(5, 64)
+    # h in two parts with the rank padded to 16 and a row of zeros, a scale per row, the
+    # adapters' count and list (160 entries) of each token tile
     base = api.workspace_size(128, 64)
-    assert size(128, 64, 24) - base == 128 * 24 * 4          # h in fp32
+    assert size(128, 64, 24) - base == 129 * 2 * 32 * 2 + 512 + 256 + 768 + (-129 * 128) % 256
     base = api.workspace_size(1000, 64)
-    # two parts of the rank padded to 16, a scale per row, an adapter per tile of 160 tokens
-    assert size(1000, 64, 24) - base == 1000 * 2 * 32 * 2 + 4096 + 256
+    assert size(1000, 64, 24) - base == 1001 * 128 + 128 + 4096 + 256 + 7 * 160 * 4 + 128 - 0

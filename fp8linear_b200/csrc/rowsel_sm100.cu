@@ -297,6 +297,11 @@ __device__ __forceinline__ bool is_finite(float v) { return fabsf(v) <= 3.402823
 
 // ---------------------------------------------------------------- persistent kernel
 
+// Epilogue staging, per warp: 32 tokens x 32 columns of 16 bits, rows 80 bytes apart (eight
+// rows' 16-byte pieces hit all banks once).
+constexpr int BOX_PITCH = 80;
+constexpr uint32_t BOX_BYTES = 32 * BOX_PITCH;
+
 template <int CG, bool LORA>
 struct Cfg {
   static constexpr int TOK_MAX = LORA ? kLoraTileTokens : CG == 2 ? 256 : 128;
@@ -311,7 +316,8 @@ struct Cfg {
   static constexpr uint32_t TMEM_COLS = CG == 1 && !LORA ? 256 : 512;
   static constexpr uint32_t OFF_PAR = STAGES * STAGE;
   static constexpr uint32_t PAR_WARP = TOK_MAX * 4u * (LORA ? 3u : 1u);  // xs (hscale, ids)
-  static constexpr uint32_t OFF_TAB = OFF_PAR + EPI_WARPS * PAR_WARP;
+  static constexpr uint32_t OFF_BOX = OFF_PAR + EPI_WARPS * PAR_WARP;
+  static constexpr uint32_t OFF_TAB = OFF_BOX + EPI_WARPS * BOX_BYTES;
   static constexpr int TAB = LORA ? 2 : kMaxExperts + 1;
   static constexpr uint32_t OFF_BAR = (OFF_TAB + 2 * TAB * 4 + 7u) & ~7u;
   static constexpr uint32_t NUM_BARS = 2 * STAGES + 5;  // full, empty, tfull, tempty, drain
@@ -559,12 +565,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    // TMEM lane = weight row, column = token: a thread holds one output column, a warp
-    // stores 32 adjacent columns (64 bytes) of a token at a time.
+    // TMEM lane = weight row (output column), TMEM column = token. A warp takes its 32
+    // columns of 32 tokens at a time as matrix fragments (lane 4i + t: columns i + 8k, tokens
+    // 8g + 2t, + 1), transposes them through shared memory (stmatrix) and stores 64-byte
+    // pieces of the tokens' rows, 16 bytes a lane.
     const int quarter = warp & 3;
-    float *e_xs = reinterpret_cast<float *>(smem + C::OFF_PAR + (warp - 2) * C::PAR_WARP);
+    const int ew = warp - 2;
+    float *e_xs = reinterpret_cast<float *>(smem + C::OFF_PAR + ew * C::PAR_WARP);
     float *e_hs = e_xs + C::TOK_MAX;
     int *e_id = reinterpret_cast<int *>(e_hs + C::TOK_MAX);
+    const uint8_t *box = smem + C::OFF_BOX + ew * BOX_BYTES;
+    const uint32_t box_st = sbase + C::OFF_BOX + ew * BOX_BYTES +
+                            static_cast<uint32_t>((lane & 7) * BOX_PITCH + (lane >> 3) * 16);
+    const int fi = lane >> 2, ft = lane & 3;
+    const bool wide = p.N % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
     int it = 0;
     int e = 0;
     for (int t = group; t < num_tiles; t += n_groups, ++it) {
@@ -572,23 +586,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int acc = it & 1;
       const uint32_t acc_phase = (it >> 1) & 1;
       const int cnt = q.t1 - q.t0;
-      const int n = (q.wb * CG + static_cast<int>(rank)) * WROWS + quarter * 32 + lane;
-      const bool live = n < p.N;
-      const int64_t wn = static_cast<int64_t>(q.e) * p.N + min(n, p.N - 1);
+      const int n0 = (q.wb * CG + static_cast<int>(rank)) * WROWS + quarter * 32;
       int adapters = 0;
       if constexpr (LORA) adapters = __ldg(p.count + q.tb);
       __syncwarp();
-      for (int i = lane; i < cnt; i += 32) {
-        e_xs[i] = __ldg(p.xs + q.t0 + i);
+      for (int i = lane; i < ((cnt + 31) & ~31); i += 32) {
+        e_xs[i] = i < cnt ? __ldg(p.xs + q.t0 + i) : 0.0f;
         if constexpr (LORA) {
-          const int id = __ldg(p.ids + q.t0 + i);
+          const int id = i < cnt ? __ldg(p.ids + q.t0 + i) : -1;
           const bool has = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L);
           e_id[i] = has ? id : -1;
           e_hs[i] = has ? __ldg(p.hscale + q.t0 + i) : 0.0f;
         }
       }
-      const float w = __ldg(p.ws + wn);
-      const float b = load_bias(p.bias, p.bias_dtype, wn);
+      float w[4], b[4];  // of columns fi + 8k
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t wn = static_cast<int64_t>(q.e) * p.N + min(n0 + fi + 8 * k, p.N - 1);
+        w[k] = __ldg(p.ws + wn);
+        b[k] = load_bias(p.bias, p.bias_dtype, wn);
+      }
       __syncwarp();
       if (!ptx::mbar_wait_bounded(bar_tfull + 8 * acc, acc_phase, abort, kWaitLimitNs)) {
         if (lane == 0) record_timeout(abort);
@@ -596,34 +613,93 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
       ptx::tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-#pragma unroll 1
-      for (int c = 0; c < cnt; c += 32) {
-        uint32_t r[32];
-        ptx::tmem_ld_32x32b_x32(t_row + (acc ? C::ACC1 : 0u) + static_cast<uint32_t>(c), r);
+      const uint32_t t_acc = t_row + (acc ? C::ACC1 : 0u);
+      constexpr uint32_t kHalf = 16u << 16;  // TMEM lanes 16-31 of the quarter
+      // (columns all past N: nothing to store)
+      for (int c = 0; c < cnt && n0 < p.N; c += 32) {
+        uint32_t r[2][16];
+        ptx::tmem_ld_16x256b_x4(t_acc + static_cast<uint32_t>(c), r[0]);
+        ptx::tmem_ld_16x256b_x4(t_acc + kHalf + static_cast<uint32_t>(c), r[1]);
         ptx::tmem_wait_ld();
-        float v[32];
+        float2 v[4][4];  // [g][k]: tokens 8g + 2t, + 1 of column i + 8k
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[j]) * e_xs[min(c + j, cnt - 1)], w, b);
+        for (int g = 0; g < 4; ++g) {
+          const float2 xs = *reinterpret_cast<const float2 *>(e_xs + c + 8 * g + 2 * ft);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t *a = r[k >> 1] + 4 * g + 2 * (k & 1);
+            v[g][k] = ptx::fma2(
+                ptx::mul2(make_float2(__uint_as_float(a[0]), __uint_as_float(a[1])), xs),
+                make_float2(w[k], w[k]), make_float2(b[k], b[k]));
+          }
+        }
         if constexpr (LORA) {
           if (adapters > 0) {
-            ptx::tmem_ld_32x32b_x32(t_row + C::ACC_L + static_cast<uint32_t>(c), r);
+            ptx::tmem_ld_16x256b_x4(t_row + C::ACC_L + static_cast<uint32_t>(c), r[0]);
+            ptx::tmem_ld_16x256b_x4(t_row + C::ACC_L + kHalf + static_cast<uint32_t>(c), r[1]);
             ptx::tmem_wait_ld();
+            float2 odd = make_float2(0.0f, 0.0f);  // NaN if any sum is not finite
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int i = min(c + j, cnt - 1);
-              float s = __uint_as_float(r[j]);
-              const int id = e_id[i];
-              if (adapters > 1 && !is_finite(s) && id >= 0 && live)
-                s = exact_sum(p, q.t0 + i, id, n);
-              v[j] = id >= 0 ? fmaf(s, e_hs[i], v[j]) : v[j];
+            for (int i = 0; i < 32; i += 2)
+              odd = ptx::fma2(make_float2(__uint_as_float(r[i >> 4][i & 15]),
+                                          __uint_as_float(r[i >> 4][(i & 15) + 1])),
+                              make_float2(0.0f, 0.0f), odd);
+            if (odd.x + odd.y != 0.0f) {
+              // (every sum of the lane anew: rows without an adapter get zero)
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const int i = c + 8 * g + 2 * ft + h;
+                    const int id = e_id[i], n = n0 + fi + 8 * k;
+                    uint32_t &s = r[k >> 1][4 * g + 2 * (k & 1) + h];
+                    if (id < 0 || n >= p.N)
+                      s = 0;
+                    else if (adapters > 1 && !is_finite(__uint_as_float(s)))
+                      s = __float_as_uint(exact_sum(p, q.t0 + i, id, n));
+                  }
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float2 hs = *reinterpret_cast<const float2 *>(e_hs + c + 8 * g + 2 * ft);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t *a = r[k >> 1] + 4 * g + 2 * (k & 1);
+                v[g][k] = ptx::fma2(make_float2(__uint_as_float(a[0]), __uint_as_float(a[1])), hs,
+                                    v[g][k]);
+              }
             }
           }
         }
-        if (live) {
+        __syncwarp();  // the box before has been read
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < cnt)
-              store_out(p.out, p.out_dtype, static_cast<int64_t>(q.t0 + c + j) * p.N + n, v[j]);
+        for (int g = 0; g < 4; ++g) {
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            o[k] = p.out_dtype == kF16 ? ptx::pack_f16x2(v[g][k].x, v[g][k].y)
+                                       : ptx::pack_bf16x2(v[g][k].x, v[g][k].y);
+          ptx::stsm_x4_trans(box_st + static_cast<uint32_t>(8 * g * BOX_PITCH), o[0], o[1], o[2],
+                             o[3]);
+        }
+        __syncwarp();
+        uint16_t *out = reinterpret_cast<uint16_t *>(p.out) +
+                        static_cast<int64_t>(q.t0 + c) * p.N + n0;
+        if (wide) {
+          const int col = ft * 8;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int m = 8 * i + fi;
+            if (c + m < cnt && n0 + col < p.N)
+              *reinterpret_cast<uint4 *>(out + static_cast<int64_t>(m) * p.N + col) =
+                  *reinterpret_cast<const uint4 *>(box + m * BOX_PITCH + col * 2);
+          }
+        } else if (n0 + lane < p.N) {
+          for (int m = 0; m < 32 && c + m < cnt; ++m)
+            out[static_cast<int64_t>(m) * p.N + lane] =
+                *reinterpret_cast<const uint16_t *>(box + m * BOX_PITCH + lane * 2);
         }
       }
       ptx::tc_fence_before();

@@ -186,27 +186,28 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl);
 cudaError_t read_rowsel_status(unsigned int *bits, bool clear);
 
 // ---- lora_sm100.cu
-// The adapters' intermediate h and the adapters of each token tile of the GEMM, in the
-// workspace:
-//   hl [M + 1][2 * rank_pad] of x's type: h / hscale as a high and a low part, h = hscale *
-//   (hi + lo) to fp32's last bits; row M is zeros, the row that the GEMM's gathers take for
-//   tokens of another adapter; hscale fp32 [M], powers of two;
-//   count int [tiles]: how many adapters the tile's tokens have, tokens without any aside;
-//   list int [tiles][kLoraTileTokens]: which.
+// The adapters' intermediate h and, for more than kLoraRowsMaxM rows, the plan of the GEMM's
+// token tiles, in the workspace:
+//   hl [M][2 * rank_pad] of x's type: h / hscale as a high and a low part, h = hscale *
+//   (hi + lo) to fp32's last bits; hscale fp32 [M], powers of two. Rows without an adapter
+//   are not written;
+//   plan int4: plan[0].x tiles follow, each {first token, end, adapter, 0}. A run of at least
+//   kLoraMixed rows with one adapter is cut into tiles of its own (adapter -1: none), of at
+//   most kLoraTileTokens; what lies between such runs goes in tiles of at most kLoraMixed
+//   tokens with any adapters (adapter -2).
 inline int64_t lora_rank_pad(int64_t R) { return (R + 15) / 16 * 16; }
-constexpr int kLoraTileTokens = 160;  // tokens per tile of the GEMM with adapters, at most
-inline int64_t lora_tiles(int64_t M) {
-  return M <= kLoraRowsMaxM ? 1 : (M + kLoraTileTokens - 1) / kLoraTileTokens;
-}
-inline int64_t lora_tile_tokens(int64_t M) {
-  const int64_t nt = lora_tiles(M);
-  return ((M + nt - 1) / nt + 31) / 32 * 32;
+constexpr int kLoraTileTokens = 160;
+constexpr int kLoraMixed = 32;
+// Entries of the plan at most: runs of one adapter, kLoraTileTokens each but for their last
+// tiles (M / 32 runs); as many gaps between them and one more; kLoraMixed tokens each but for
+// their last tiles.
+inline int64_t lora_plan_max(int64_t M) {
+  return M <= kLoraRowsMaxM ? 0 : 1 + M / kLoraTileTokens + 3 * (M / kLoraMixed) + 1;
 }
 struct LoraWorkspace {
   void *hl = nullptr;
   float *hscale = nullptr;
-  int *count = nullptr;
-  int *list = nullptr;
+  int4 *plan = nullptr;
   size_t bytes = 0;
 };
 LoraWorkspace lora_workspace(void *base, int64_t M, int64_t R);

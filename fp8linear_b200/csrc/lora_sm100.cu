@@ -45,9 +45,11 @@ struct Params {
   int M, K, L, R, rank_pad;
   void *hl;
   float *hscale;
-  int *count, *list;
-  int gemm_tiles, gemm_tile_tokens;
+  int4 *plan;      // null: not wanted
   int split, kps, k_blocks;
+  int x_rows;      // rows of x's box
+  int stages;
+  uint32_t off_part;
   int par;  // clusters per tile, each with every par-th pass
 };
 
@@ -58,15 +60,12 @@ __device__ __forceinline__ bool has_adapter(const Params &p, int id) {
 constexpr int ROWS = 128;
 constexpr int KB = 64;     // 16-bit elements per K-block: one 128-byte swizzle row
 constexpr int COLS = 128;  // columns (adapters x rank_pad) per pass
-constexpr int STAGES = 4;
-constexpr int NUM_THREADS = 192;
-constexpr uint32_t X_STAGE = ROWS * 128;
+constexpr int MAX_STAGES = 8;
+constexpr int NUM_THREADS = 224;  // producer, MMA, 4 x TMEM, plan
 constexpr uint32_t A_STAGE = COLS * 128;
-constexpr uint32_t STAGE = X_STAGE + A_STAGE;
-constexpr uint32_t OFF_PART = STAGES * STAGE;  // fp32 [ROWS][rank_pad + 1]
-constexpr uint32_t SMEM_BYTES = OFF_PART + ROWS * (kLoraMaxRank + 1) * 4 + 1024;
 constexpr int MAX_SPLIT = 8;
-static_assert(SMEM_BYTES <= 231424, "shared memory budget (the static part is below 2 KB)");
+// dynamic: the ring of (x_rows + COLS) x 128 bytes, then fp32 [ROWS][rank_pad + 1]
+constexpr uint32_t SMEM_MAX = 232448 - 4096;  // (the static part is below 3 KB)
 
 __device__ __forceinline__ void record_timeout(volatile int *abort) {
   if (!*abort) {
@@ -83,21 +82,24 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = ptx::smem_u32(smem);
-  __shared__ alignas(8) uint64_t s_bar[2 * STAGES + 3];
+  __shared__ alignas(8) uint64_t s_bar[2 * MAX_STAGES + 3];
   __shared__ uint32_t s_slot;
   __shared__ int s_abort;
-  __shared__ int s_id[ROWS];     // adapter of each row, -1: none
+  __shared__ alignas(16) int s_id[ROWS];  // adapter of each row, -1: none
   __shared__ int s_first[ROWS];  // the row's adapter appears first at this row of the tile
   __shared__ int s_rank[ROWS];   // .. and is this one of the tile's adapters
   __shared__ int s_list[ROWS];   // the tile's adapters
   __shared__ int s_count[5];
   const uint32_t bar_full = ptx::smem_u32(s_bar);
-  const uint32_t bar_empty = bar_full + 8 * STAGES;
-  const uint32_t bar_acc = bar_empty + 8 * STAGES;
+  const uint32_t bar_empty = bar_full + 8 * MAX_STAGES;
+  const uint32_t bar_acc = bar_empty + 8 * MAX_STAGES;
   const uint32_t bar_free = bar_acc + 8;
   const uint32_t bar_drain = bar_free + 8;
   volatile int *abort = &s_abort;
-  float *part = reinterpret_cast<float *>(smem + OFF_PART);
+  float *part = reinterpret_cast<float *>(smem + p.off_part);
+  const int stages = p.stages;
+  const uint32_t x_stage = static_cast<uint32_t>(p.x_rows) * 128;
+  const uint32_t stage_bytes = x_stage + A_STAGE;
   const int pitch = p.rank_pad + 1;  // odd: a column of it hits all banks
 
   ptx::grid_launch_dependents();
@@ -110,7 +112,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   if (threadIdx.x == 0) {
     ptx::prefetch_tmap(&tmap_x);
     ptx::prefetch_tmap(&tmap_a);
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < stages; ++s) {
       ptx::mbar_init(bar_full + 8 * s, 1);
       ptx::mbar_init(bar_empty + 8 * s, 1);
     }
@@ -136,10 +138,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t tmem = *const_cast<volatile uint32_t *>(&s_slot);
   bool first = false;
   if (me < ROWS) {
-    int f = me;
-    if (s_id[me] >= 0)
-      for (f = 0; s_id[f] != s_id[me]; ++f) {
+    int f;
+    // the lowest row with the same id: within the warp, then among the rows of those before
+    const int id = s_id[me];
+    f = (me & ~31) + __ffs(static_cast<int>(__match_any_sync(0xFFFFFFFFu, id))) - 1;
+    if (id >= 0) {
+#pragma unroll 1
+      for (int j = 0; j < (me & ~31); j += 4) {
+        const int4 v = *reinterpret_cast<const int4 *>(s_id + j);
+        if (v.x == id || v.y == id || v.z == id || v.w == id) {
+          f = v.x == id ? j : v.y == id ? j + 1 : v.z == id ? j + 2 : j + 3;
+          break;
+        }
       }
+    }
     first = s_id[me] >= 0 && f == me;
     s_first[me] = f;
     const uint32_t votes = __ballot_sync(0xFFFFFFFFu, first);
@@ -178,23 +190,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             break;
           }
           const uint32_t fb = bar_full + 8 * stage;
-          const uint32_t dst = sbase + static_cast<uint32_t>(stage) * STAGE;
-          ptx::mbar_arrive_expect_tx(fb, X_STAGE + static_cast<uint32_t>(nd * p.rank_pad) * 128u);
+          const uint32_t dst = sbase + static_cast<uint32_t>(stage) * stage_bytes;
+          ptx::mbar_arrive_expect_tx(fb, x_stage + static_cast<uint32_t>(nd * p.rank_pad) * 128u);
           ptx::tma_load_2d(dst, &tmap_x, (kb0 + i) * KB, m0, fb);
           for (int d = 0; d < nd; ++d)  // ranks past R read as zero
-            ptx::tma_load_3d(dst + X_STAGE + static_cast<uint32_t>(d * p.rank_pad) * 128u, &tmap_a,
+            ptx::tma_load_3d(dst + x_stage + static_cast<uint32_t>(d * p.rank_pad) * 128u, &tmap_a,
                              (kb0 + i) * KB, 0, s_list[d0 + d], fb);
           ++issued;
-          if (++stage == STAGES) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      const uint32_t n_drain = issued < STAGES ? issued : STAGES;
+      const uint32_t n_drain = min(issued, static_cast<uint32_t>(stages));
       for (uint32_t i = 0; i < n_drain; ++i) {
         if (stage == 0) {
-          stage = STAGES - 1;
+          stage = stages - 1;
           phase ^= 1u;
         } else {
           --stage;
@@ -224,14 +236,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             break;
           }
           ptx::tc_fence_after();
-          const uint32_t st = sbase + static_cast<uint32_t>(stage) * STAGE;
+          const uint32_t st = sbase + static_cast<uint32_t>(stage) * stage_bytes;
           const uint64_t adesc = ptx::sw128_kmajor_desc(st);
-          const uint64_t bdesc = ptx::sw128_kmajor_desc(st + X_STAGE);
+          const uint64_t bdesc = ptx::sw128_kmajor_desc(st + x_stage);
 #pragma unroll
           for (int kk = 0; kk < KB / 16; ++kk)
             ptx::mma_f16<1>(tmem, adesc + 2 * kk, bdesc + 2 * kk, idesc, (i | kk) != 0 ? 1u : 0u);
           ptx::mma_commit(bar_empty + 8 * stage);
-          if (++stage == STAGES) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
@@ -241,7 +253,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       ptx::mma_commit(bar_drain);
       ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
     }
-  } else {
+  } else if (warp < 6) {
     // TMEM lane = row: keep the columns of the row's own adapter
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
@@ -273,6 +285,74 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar_free);
     }
+  } else if (p.plan != nullptr && blockIdx.x == 0) {
+    // The plan of the GEMM's token tiles. A run of at least kLoraMixed (32) rows crosses a
+    // border between blocks of 32 rows, so of a block's runs only the one carried in and the
+    // one carried on can be long.
+    ptx::grid_dependency_wait();
+    int n = 0;
+    auto emit = [&](int t0, int t1, int a) {
+      ++n;
+      if (lane == 0) p.plan[n] = make_int4(t0, t1, a, 0);
+    };
+    int open = -1, open_end = 0;  // rows of short runs not yet in a tile
+    auto flush = [&]() {
+      if (open >= 0 && open < open_end) emit(open, open_end, -2);
+      open = -1;
+    };
+    auto add_short = [&](int s, int e) {
+      if (s == e) return;
+      if (open < 0) open = s;
+      open_end = e;
+      for (; open_end - open >= kLoraMixed; open += kLoraMixed) emit(open, open + kLoraMixed, -2);
+      if (open == open_end) open = -1;
+    };
+    auto add_run = [&](int s, int e, int a) {
+      if (e - s < kLoraMixed) {
+        add_short(s, e);
+        return;
+      }
+      flush();
+      const int nt = (e - s + kLoraTileTokens - 1) / kLoraTileTokens;
+      const int per = ((e - s + nt - 1) / nt + 31) / 32 * 32;
+      for (int t = s; t < e; t += per) emit(t, min(e, t + per), a);
+    };
+    int start = 0, cur = -1;  // the run carried on
+    constexpr int AHEAD = 8;  // blocks loaded together, one such batch before it is read
+    int ids[AHEAD], next[AHEAD];
+    auto fetch = [&](int b) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int m = b + 32 * k + lane;
+        next[k] = m < p.M ? __ldg(p.ids + m) : -1;
+      }
+    };
+    fetch(0);
+    for (int b0 = 0; b0 < p.M; b0 += 32 * AHEAD) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) ids[k] = has_adapter(p, next[k]) ? next[k] : -1;
+      fetch(b0 + 32 * AHEAD);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int b = b0 + 32 * k;
+        int before = __shfl_up_sync(0xFFFFFFFFu, ids[k], 1);
+        if (lane == 0) before = cur;
+        const uint32_t edges = __ballot_sync(0xFFFFFFFFu, b + lane < p.M && ids[k] != before);
+        if (edges != 0) {
+          const int first = __ffs(static_cast<int>(edges)) - 1;
+          const int last = 31 - __clz(static_cast<int>(edges));
+          add_run(start, b + first, cur);
+          add_short(b + first, b + last);
+          start = b + last;
+        }
+        cur = __shfl_sync(0xFFFFFFFFu, ids[k], 31);
+      }
+    }
+    // (past M the lanes hold -1; the run's own id is its first row's)
+    const int tail = __ldg(p.ids + min(start, p.M - 1));
+    add_run(start, p.M, has_adapter(p, tail) ? tail : -1);
+    flush();
+    if (lane == 0) p.plan[0] = make_int4(n, 0, 0, 0);
   }
 
   __syncwarp();
@@ -297,8 +377,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       v[i] = 0.0f;
       if (c < p.R) {
         const uint32_t at = part_base + static_cast<uint32_t>(row * pitch + c) * 4u;
-        for (int s = 0; s < p.split; ++s)
-          v[i] += ptx::ld_shared_cluster_f32(ptx::map_shared_rank(at, s));
+        float part_of[MAX_SPLIT];
+#pragma unroll
+        for (int s = 0; s < MAX_SPLIT; ++s)
+          if (s < p.split) part_of[s] = ptx::ld_shared_cluster_f32(ptx::map_shared_rank(at, s));
+#pragma unroll
+        for (int s = 0; s < MAX_SPLIT; ++s)
+          if (s < p.split) v[i] += part_of[s];
         v[i] *= sc;
         const float a = fabsf(v[i]);
         if (a <= 3.402823466e38f) top = fmaxf(top, a);  // finite values only
@@ -336,30 +421,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     if (lane == 0)
       p.hscale[m0 + row] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
   }
-  // Row M of hl: zeros.
-  if (blockIdx.x == 0)
-    for (int c = threadIdx.x; c < 2 * p.rank_pad; c += NUM_THREADS)
-      reinterpret_cast<uint16_t *>(p.hl)[static_cast<int64_t>(p.M) * (2 * p.rank_pad) + c] = 0;
-  // The adapters of each token tile of the GEMM, a warp to a tile: 32 tokens at a time, the
-  // first of each id among them looks the id up in the list and appends it.
-  for (int t = static_cast<int>(blockIdx.x) * (NUM_THREADS / 32) + warp; t < p.gemm_tiles;
-       t += static_cast<int>(gridDim.x) * (NUM_THREADS / 32)) {
-    const int t0 = t * p.gemm_tile_tokens, t1 = min(p.M, t0 + p.gemm_tile_tokens);
-    int *list = p.list + static_cast<int64_t>(t) * kLoraTileTokens;
-    int n = 0;
-    for (int b = t0; b < t1; b += 32) {
-      const int id = b + lane < t1 ? __ldg(p.ids + b + lane) : -1;
-      const uint32_t same = __match_any_sync(0xFFFFFFFFu, id);
-      bool add = has_adapter(p, id) && (same & ((1u << lane) - 1u)) == 0;
-      for (int i = 0; i < n && add; ++i) add = *const_cast<volatile int *>(list + i) != id;
-      const uint32_t votes = __ballot_sync(0xFFFFFFFFu, add);
-      if (add) list[n + __popc(votes & ((1u << lane) - 1u))] = id;
-      n += __popc(votes);
-      __syncwarp();
-    }
-    if (lane == 0) p.count[t] = n;
-  }
-
   ptx::cluster_sync();  // peers may still be reading this CTA's partial sums
   if (warp == 1) {
     ptx::tc_fence_after();
@@ -374,14 +435,12 @@ size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 LoraWorkspace lora_workspace(void *base, int64_t M, int64_t R) {
   LoraWorkspace w;
   uint8_t *b = static_cast<uint8_t *>(base);
-  const size_t hl = lora::align256(static_cast<size_t>(M + 1) * 2 * lora_rank_pad(R) * 2);
+  const size_t hl = lora::align256(static_cast<size_t>(M) * 2 * lora_rank_pad(R) * 2);
   const size_t sc = lora::align256(static_cast<size_t>(M) * 4);
-  const size_t ct = lora::align256(static_cast<size_t>(lora_tiles(M)) * 4);
   w.hl = b;
   w.hscale = reinterpret_cast<float *>(b + hl);
-  w.count = reinterpret_cast<int *>(b + hl + sc);
-  w.list = reinterpret_cast<int *>(b + hl + sc + ct);
-  w.bytes = hl + sc + ct + lora::align256(static_cast<size_t>(lora_tiles(M)) * kLoraTileTokens * 4);
+  w.plan = M <= kLoraRowsMaxM ? nullptr : reinterpret_cast<int4 *>(b + hl + sc);
+  w.bytes = hl + sc + lora::align256(static_cast<size_t>(lora_plan_max(M)) * sizeof(int4));
   return w;
 }
 
@@ -403,13 +462,10 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   p.rank_pad = static_cast<int>(lora_rank_pad(a.R));
   p.hl = w.hl;
   p.hscale = w.hscale;
-  p.count = w.count;
-  p.list = w.list;
+  p.plan = w.plan;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cudaError_t e;
-  p.gemm_tiles = static_cast<int>(lora_tiles(a.M));
-  p.gemm_tile_tokens = static_cast<int>(lora_tile_tokens(a.M));
   p.k_blocks = static_cast<int>((a.K + KB - 1) / KB);
   const int64_t tiles = (a.M + ROWS - 1) / ROWS;
   // K-splits while CTAs are left over, four K-blocks at least for each
@@ -421,11 +477,17 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   const int64_t most = (std::min<int64_t>(a.L, ROWS) + COLS / p.rank_pad - 1) / (COLS / p.rank_pad);
   p.par = static_cast<int>(
       std::max<int64_t>(1, std::min<int64_t>(dev.sm_count / (tiles * p.split), most)));
+  p.x_rows = static_cast<int>(std::min<int64_t>((a.M + 7) / 8 * 8, ROWS));
+  const uint32_t part = ROWS * (static_cast<uint32_t>(p.rank_pad) + 1) * 4;
+  const uint32_t stage = static_cast<uint32_t>(p.x_rows) * 128 + A_STAGE;
+  p.stages = static_cast<int>(std::min<uint32_t>((SMEM_MAX - 1024 - part) / stage, MAX_STAGES));
+  p.off_part = static_cast<uint32_t>(p.stages) * stage;
   const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   std::string err;
   CUtensorMap tx, ta;
-  if (!make_tmap_2d_sw128(&tx, t16, a.x, a.K, a.M, a.K * 2, KB, ROWS, &err) ||
+  if (!make_tmap_2d_sw128(&tx, t16, a.x, a.K, a.M, a.K * 2, KB, static_cast<uint32_t>(p.x_rows),
+                          &err) ||
       !make_tmap_3d_sw128(&ta, t16, a.lora_a, a.K, a.R, a.L, a.K * 2, a.R * a.K * 2, KB,
                           static_cast<uint32_t>(p.rank_pad), &err)) {
     set_error("fp8_linear_lora: " + err);
@@ -437,7 +499,7 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
     std::lock_guard<std::mutex> lock(mu);
     if (!set[dev.device & 63]) {
       e = cudaFuncSetAttribute(down_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(SMEM_BYTES));
+                               static_cast<int>(SMEM_MAX));
       if (e != cudaSuccess) {
         set_error(std::string("fp8_linear_lora: kernel setup: ") + cudaGetErrorString(e));
         return 4;
@@ -456,7 +518,7 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   cfg.numAttrs = 2;
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.par * p.split));
   cfg.blockDim = dim3(NUM_THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.dynamicSmemBytes = p.off_part + part + 1024;
   e = cudaLaunchKernelEx(&cfg, down_tile_kernel, tx, ta, p);
   if (e != cudaSuccess) {
     set_error(std::string("fp8_linear_lora: launch failed: ") + cudaGetErrorString(e));

@@ -16,8 +16,9 @@
 //       tokens; CG = 1: 128 x up to 128, for groups of few rows), TMA ring, two TMEM
 //       accumulators, epilogue of one tile under the main loop of the next.
 //   split_kernel<LORA>  when all tiles together do not fill the GPU: a cluster of CTAs per
-//       tile splits K and adds its partial tiles through distributed shared memory, in rank
-//       order (the result does not depend on timing).
+//       tile splits K; each CTA adds up a share of the tile's rows, of which the others push
+//       their partial sums into its shared memory, in rank order (the result does not depend
+//       on timing).
 //
 // Rows outside the experts' ranges are written as zeros. Offsets are clamped to [0, M] and to
 // their running maximum, so that no value of them leads outside a tensor.
@@ -47,6 +48,7 @@ constexpr int NUM_THREADS = 192;
 constexpr int EPI_WARPS = 4;
 constexpr uint32_t W_STAGE = WROWS * BK;  // 16 KB
 constexpr int X_MAPS = 8;                 // token boxes of 16, 32, .. 128 rows
+constexpr int H_MAPS = kLoraTileTokens / 32;  // boxes of the adapters' h: 16, 32, .. 80 rows
 constexpr uint64_t kWaitLimitNs = 4000000000ull;
 constexpr uint64_t kDrainLimitNs = 1000000000ull;
 
@@ -54,7 +56,7 @@ struct Maps {
   CUtensorMap x[X_MAPS];  // xq [M][K], box 128 B x 16 (i + 1) rows
   CUtensorMap w;          // wq [E][N][K], box 128 B x 128 rows x 1
   CUtensorMap lb;         // lora_b [L][N][R], box 64 x 128 rows x 1
-  CUtensorMap h;          // hl [M + 1][2 rank_pad], box 64 x 1 (gathered)
+  CUtensorMap h[H_MAPS];  // hl [M][2 rank_pad], box 64 x 16 (i + 1) rows
 };
 
 struct Params {
@@ -72,14 +74,16 @@ struct Params {
   // split_kernel
   int split, kps, stages;
   int tok_cap;        // tokens per tile at most
-  uint32_t off_part;  // shared-memory offsets
+  uint32_t off_ring;  // shared-memory offsets
+  uint32_t off_part;
+  uint32_t off_lora;
   uint32_t off_tab;
   // adapters
   const int *ids;
   const void *lora_b;
   int lora_dtype;
   int L, R, rank_pad;
-  const int *count, *list;  // adapters of each token tile
+  const int4 *plan;  // token tiles (persist_kernel)
   const void *hl;
   const float *hscale;
 };
@@ -126,7 +130,7 @@ __device__ __forceinline__ void build_groups(const Params &p, int tok_max, int *
     __syncthreads();
     return;
   }
-  for (int i = threadIdx.x; i <= E; i += NUM_THREADS)
+  for (int i = threadIdx.x; i <= E; i += blockDim.x)
     row[i] = min(max(__ldg(p.offsets + i), 0), p.M);
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -168,6 +172,7 @@ struct Tile {
   int t0, t1;  // tokens
   int nn;      // MMA N: tokens padded to a multiple of 16 x CG
   int tb;      // token block within the group
+  int adapter; // of all its tokens, -1: none, -2: several
 };
 
 // Tile t of the table; `e` is a group at or before the tile's (advanced to it).
@@ -193,8 +198,41 @@ __device__ __forceinline__ Tile find_tile(const Params &p, int tok_max, const in
   q.t0 = r0 + q.tb * per;
   q.t1 = min(r0 + rows, q.t0 + per);
   q.nn = (q.t1 - q.t0 + 16 * CG - 1) / (16 * CG) * (16 * CG);
+  q.adapter = -1;
   return q;
 }
+
+// The tiles of a call with adapters, from the plan. Each step also loads the next tile's
+// entry, which is then at hand without a wait.
+struct PlanWalk {
+  int n_tb, num_tiles;
+  int4 next;
+
+  __device__ __forceinline__ int token_block(const Params &p, int t) const {
+    return p.M >= p.N ? t / p.n_wb : t % n_tb;
+  }
+  __device__ __forceinline__ void load(const Params &p, int t) {
+    if (t < num_tiles) next = __ldg(p.plan + 1 + token_block(p, t));
+  }
+  __device__ __forceinline__ void start(const Params &p, int t) {
+    n_tb = __ldg(&p.plan->x);
+    num_tiles = n_tb * p.n_wb;
+    load(p, t);
+  }
+  template <int CG>
+  __device__ __forceinline__ Tile take(const Params &p, int t, int step) {
+    Tile q;
+    q.e = 0;
+    q.tb = token_block(p, t);
+    q.wb = p.M >= p.N ? t - q.tb * p.n_wb : t / n_tb;
+    q.t0 = next.x;
+    q.t1 = next.y;
+    q.adapter = next.z;
+    q.nn = (q.t1 - q.t0 + 16 * CG - 1) / (16 * CG) * (16 * CG);
+    load(p, t + step);
+    return q;
+  }
+};
 
 // Zeros to the rows that no group holds; the `n` threads from `first` of every CTA.
 __device__ __forceinline__ void zero_rows(const Params &p, const int *row, int first, int n) {
@@ -209,91 +247,194 @@ __device__ __forceinline__ void zero_rows(const Params &p, const int *row, int f
 
 // ---------------------------------------------------------------- adapters
 //
-// A token tile's adapters are taken one after the other, as further stages of the ring: the
-// adapter's B rows beside the tile's h, in which tokens of other adapters are rows of zeros
-// (gathered from the zero row of hl). Their products add up in one accumulator. 64 16-bit
-// elements are the 128 bytes of a stage's row: up to rank 32 the high and the low part of h
-// share a stage, above it each 64 values of the rank take one for either part.
+// A tile whose tokens all have one adapter takes it on the tensor cores, as further stages of
+// the ring: the adapter's B rows beside the tokens' h, into an accumulator of their own. 64
+// 16-bit elements are the 128 bytes of a stage's row: up to rank 32 the high and the low part
+// of h share a stage, above it each 64 values of the rank take one for either part.
 //
-// 0 * B is zero only for finite B: an infinity or NaN in an adapter also makes NaN of the
-// tokens that are not its own. So in a tile of several adapters the epilogue computes every
-// sum that is not finite once more (exact_sum), with the token's own adapter alone.
+// Tokens of short runs (decoding requests) are taken by the epilogue warps on warp-level
+// tensor cores while the tile's main loop runs (adapter_sums): there every adapter's product
+// is a tile of its own (8 tokens wide), from which each token keeps only its own adapter's
+// column. Adding the adapters up in one accumulator over tokens masked with zeros would need
+// as many passes, and 0 * inf would carry one adapter's infinities to all tokens of the tile.
 
 __device__ __forceinline__ int lora_stages(const Params &p) {
   return p.rank_pad <= 32 ? 1 : 2 * ((p.rank_pad + 63) / 64);
 }
 
-// Rows 4 * lane .. + 3 of a token tile half (lanes up to rows / 4), with their adapters.
-struct GatherRows {
-  int row[4];
-  int id[4];
-};
-
-__device__ __forceinline__ GatherRows gather_rows(const Params &p, int first, int end, int lane) {
-  GatherRows g;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    g.row[i] = first + 4 * lane + i;
-    g.id[i] = g.row[i] < end ? __ldg(p.ids + g.row[i]) : -1;
-  }
-  return g;
-}
-
-// Stage `j` (of lora_stages) of adapter `a`: columns of B and of hl.
+// Stage `j` (of lora_stages): columns of B and of hl.
 __device__ __forceinline__ void lora_columns(const Params &p, int j, int &bx, int &hx) {
   const int chunks = (p.rank_pad + 63) / 64;
   bx = (j % chunks) * 64;
   hx = (j / chunks) * p.rank_pad + bx;
 }
 
-template <int CG>
-__device__ __forceinline__ void gather_h(const Params &p, const CUtensorMap *map,
-                                         const GatherRows &g, int rows, int a, int x,
-                                         uint32_t dst, uint32_t bar, int lane) {
-  if (4 * lane < rows) {
-    int r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = g.id[i] == a ? g.row[i] : p.M;
-    ptx::tma_gather4<CG>(dst + static_cast<uint32_t>(lane) * 4 * BK, map, x, r[0], r[1], r[2],
-                         r[3], bar);
-  }
-}
-
-// The MMAs of stage `j` of an adapter; `first`: nothing in the accumulator counts yet.
+// The MMAs of stage `j` of an adapter.
 template <int CG>
 __device__ __forceinline__ void lora_mma(const Params &p, uint32_t d, uint32_t stage, uint32_t idesc,
-                                         int j, bool first) {
+                                         int j) {
   const uint64_t adesc = ptx::sw128_kmajor_desc(stage);
   const uint64_t bdesc = ptx::sw128_kmajor_desc(stage + W_STAGE);
   int bx, hx;
   lora_columns(p, j, bx, hx);
   const int steps = min(64, p.rank_pad - bx) / 16;  // 16 elements: 32 bytes
   for (int kk = 0; kk < steps; ++kk)
-    ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + 2 * kk, idesc, first && kk == 0 ? 0u : 1u);
+    ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + 2 * kk, idesc, (j | kk) != 0 ? 1u : 0u);
   if (p.rank_pad <= 32)  // the low part, next to the high part
     for (int kk = 0; kk < steps; ++kk)
       ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + 2 * (kk + steps), idesc, 1u);
 }
 
-__device__ __forceinline__ float load16(const uint16_t *v, bool f16) {
-  const uint16_t b = __ldg(v);
-  return f16 ? __half2float(__ushort_as_half(b)) : __uint_as_float(static_cast<uint32_t>(b) << 16);
+// The ring of B boxes for adapter_sums: 128 weight rows x 64 ranks, 128-byte swizzle. A warp
+// of its own fills it (feed), the four epilogue warps read it; both go through the tokens
+// eight at a time, through the adapters of eight in the order of their first tokens, and
+// through the rank 64 at a time. `count` boxes have been through the ring.
+constexpr int SUM_SLOTS = 3;
+constexpr int SUM_RANK = 64;
+constexpr int SUM_BARS = 2 * SUM_SLOTS;  // full, empty
+struct SumRing {
+  uint32_t slots;  // shared-memory addresses
+  uint32_t bars;
+  volatile int *abort;
+  uint32_t count;
+};
+
+// Lane l of a warp has the adapter of token l % 8 of eight (-1: none); bits 0-7 of the
+// result are the tokens whose adapter no earlier one of them has.
+__device__ __forceinline__ uint32_t first_tokens(int id) {
+  const uint32_t same = __match_any_sync(0xFFFFFFFFu, id) & 0xFFu;
+  const int lane = threadIdx.x & 31;
+  return __ballot_sync(0xFFFFFFFFu, id >= 0 && lane < 8 && __ffs(static_cast<int>(same)) - 1 == lane) &
+         0xFFu;
 }
 
-// sum_r (hi + lo)[token][r] * B[id][n][r], on CUDA cores.
-__device__ __noinline__ float exact_sum(const Params &p, int token, int id, int n) {
+__device__ __forceinline__ int token_id(const Params &p, int i, int end) {
+  const int id = i < end ? __ldg(p.ids + i) : -1;
+  return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L) ? id : -1;
+}
+
+// The boxes for tokens [t0, t1) and weight rows n0 ..; by a whole warp. False when a wait ran
+// out (nothing is issued after that).
+__device__ __forceinline__ bool feed_sums(const Params &p, const CUtensorMap *map, SumRing &ring,
+                                          int t0, int t1, int n0) {
+  const int lane = threadIdx.x & 31;
+  int next = token_id(p, t0 + (lane & 7), t1);
+  for (int i = t0; i < t1; i += 8) {
+    const int id = next;
+    next = token_id(p, i + 8 + (lane & 7), t1);
+    for (uint32_t todo = first_tokens(id); todo != 0; todo &= todo - 1) {
+      const int a = __shfl_sync(0xFFFFFFFFu, id, __ffs(static_cast<int>(todo)) - 1);
+      for (int rc = 0; rc < p.R; rc += SUM_RANK) {
+        const uint32_t s = ring.count % SUM_SLOTS;
+        int ok = 1;
+        if (lane == 0) {
+          if (ptx::mbar_wait_bounded(ring.bars + 8 * (SUM_SLOTS + s),
+                                     (ring.count / SUM_SLOTS & 1u) ^ 1u, ring.abort,
+                                     kWaitLimitNs)) {
+            ptx::mbar_arrive_expect_tx(ring.bars + 8 * s, W_STAGE);
+            ptx::tma_load_3d(ring.slots + s * W_STAGE, map, rc, n0, a, ring.bars + 8 * s);
+          } else {
+            record_timeout(ring.abort);
+            ok = 0;
+          }
+        }
+        if (__shfl_sync(0xFFFFFFFFu, ok, 0) == 0) return false;
+        ++ring.count;
+      }
+    }
+  }
+  return true;
+}
+
+// Waits (bounded) until every box issued has landed and been read.
+__device__ __forceinline__ void drain_sums(const SumRing &ring) {
+  if ((threadIdx.x & 31) != 0) return;
+  for (uint32_t i = ring.count > SUM_SLOTS ? ring.count - SUM_SLOTS : 0; i < ring.count; ++i)
+    ptx::mbar_wait_timeout(ring.bars + 8 * (SUM_SLOTS + i % SUM_SLOTS), (i / SUM_SLOTS) & 1u,
+                           kDrainLimitNs);
+}
+
+// For eight tokens i0 .. (below t1) and the 32 weight rows `quarter` of the boxes: the sums
+// sum_r (hi + lo)[token][r] * B[adapter of the token][row][r], as matrix fragments: lane
+// 4i + t gets tokens 2t, 2t + 1 of rows i + 8k in s[k]; zero for tokens without an adapter. By
+// one epilogue warp; false when a wait ran out.
+__device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring, int i0, int t1,
+                                             int quarter, float2 (&s)[4]) {
+  const int lane = threadIdx.x & 31;
   const bool f16 = p.lora_dtype == kF16;
-  const uint16_t *h = reinterpret_cast<const uint16_t *>(p.hl) +
-                      static_cast<int64_t>(token) * (2 * p.rank_pad);
-  const uint16_t *b = reinterpret_cast<const uint16_t *>(p.lora_b) +
-                      (static_cast<int64_t>(id) * p.N + n) * p.R;
-  float s = 0.0f;
-  for (int r = 0; r < p.R; ++r)
-    s = fmaf(load16(h + r, f16) + load16(h + p.rank_pad + r, f16), load16(b + r, f16), s);
-  return s;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s[k] = make_float2(0.0f, 0.0f);
+  const int id = token_id(p, i0 + (lane & 7), t1);
+  uint32_t todo = first_tokens(id);
+  if (todo == 0) return true;
+  // B operand of the product: h of token lane / 4, ranks 16j + 2t, + 1 and 16j + 8 + 2t, + 1,
+  // high and low part (tokens without an adapter: zero, their h is not written)
+  uint32_t h[kLoraMaxRank / 16][4];
+  const bool has = __shfl_sync(0xFFFFFFFFu, id, lane >> 2) >= 0;
+  const uint32_t *hr = reinterpret_cast<const uint32_t *>(p.hl) +
+                       static_cast<int64_t>(i0 + (lane >> 2)) * p.rank_pad + (lane & 3);
+#pragma unroll
+  for (int j = 0; j < kLoraMaxRank / 16; ++j) {
+    const bool in = has && 16 * j < p.rank_pad;
+    h[j][0] = in ? __ldg(hr + 8 * j) : 0u;
+    h[j][1] = in ? __ldg(hr + 8 * j + 4) : 0u;
+    h[j][2] = in ? __ldg(hr + p.rank_pad / 2 + 8 * j) : 0u;
+    h[j][3] = in ? __ldg(hr + p.rank_pad / 2 + 8 * j + 4) : 0u;
+  }
+  const int id0 = __shfl_sync(0xFFFFFFFFu, id, 2 * (lane & 3));
+  const int id1 = __shfl_sync(0xFFFFFFFFu, id, 2 * (lane & 3) + 1);
+  // ldmatrix: lane 8m + i has row i + 8 (m % 2) of a 16-row tile, 16-byte column 2j + m / 2
+  const uint32_t row = static_cast<uint32_t>(quarter * 32 + (lane & 7) + (lane & 8));
+  const uint32_t col = static_cast<uint32_t>(lane >> 4);
+  for (; todo != 0; todo &= todo - 1) {
+    const int a = __shfl_sync(0xFFFFFFFFu, id, __ffs(static_cast<int>(todo)) - 1);
+    float d[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[m][e] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kLoraMaxRank / SUM_RANK; ++c) {
+      if (c * SUM_RANK >= p.R) break;
+      const uint32_t slot = ring.count % SUM_SLOTS;
+      if (!ptx::mbar_wait_bounded(ring.bars + 8 * slot, ring.count / SUM_SLOTS & 1u, ring.abort,
+                                  kWaitLimitNs)) {
+        record_timeout(ring.abort);
+        return false;
+      }
+      const uint32_t box = ring.slots + slot * W_STAGE + row * 128;
+#pragma unroll
+      for (int j = 0; j < SUM_RANK / 16; ++j) {
+        if (c * SUM_RANK + 16 * j >= p.rank_pad) break;
+        const uint32_t *b = h[c * (SUM_RANK / 16) + j];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          uint32_t w[4];
+          ptx::ldsm_x4(box + m * 16 * 128 + (((2 * j + col) ^ (row & 7)) << 4), w);
+          if (f16) {
+            ptx::mma_f16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[0], b[1]);
+            ptx::mma_f16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[2], b[3]);
+          } else {
+            ptx::mma_bf16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[0], b[1]);
+            ptx::mma_bf16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[2], b[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ring.bars + 8 * (SUM_SLOTS + slot));
+      ++ring.count;
+    }
+    // d[m]: rows i + 16m (0, 1) and i + 16m + 8 (2, 3), tokens 2t (0, 2) and 2t + 1 (1, 3)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (id0 == a) s[k].x = d[k >> 1][2 * (k & 1)];
+      if (id1 == a) s[k].y = d[k >> 1][2 * (k & 1) + 1];
+    }
+  }
+  return true;
 }
 
-__device__ __forceinline__ bool is_finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // ---------------------------------------------------------------- persistent kernel
 
@@ -308,19 +449,21 @@ struct Cfg {
   static constexpr int X_ROWS = TOK_MAX / CG;  // tokens this CTA loads, at most
   static constexpr uint32_t X_STAGE = X_ROWS * BK;
   static constexpr uint32_t STAGE = W_STAGE + X_STAGE;
-  static constexpr int STAGES = LORA ? 7 : 6;
+  static constexpr int THREADS = NUM_THREADS + (LORA ? 32 : 0);  // + the warp that feeds B
+  static constexpr int STAGES = 6;
   // TMEM: two accumulators; the adapters' products have a third, which only the epilogue of
   // one tile holds at a time
   static constexpr uint32_t ACC1 = TOK_MAX;
   static constexpr uint32_t ACC_L = 2 * TOK_MAX;
   static constexpr uint32_t TMEM_COLS = CG == 1 && !LORA ? 256 : 512;
-  static constexpr uint32_t OFF_PAR = STAGES * STAGE;
-  static constexpr uint32_t PAR_WARP = TOK_MAX * 4u * (LORA ? 3u : 1u);  // xs (hscale, ids)
+  static constexpr uint32_t OFF_RING = STAGES * STAGE;
+  static constexpr uint32_t OFF_PAR = OFF_RING + (LORA ? SUM_SLOTS * W_STAGE : 0u);
+  static constexpr uint32_t PAR_WARP = TOK_MAX * 4u * (LORA ? 2u : 1u);  // xs (hscale)
   static constexpr uint32_t OFF_BOX = OFF_PAR + EPI_WARPS * PAR_WARP;
   static constexpr uint32_t OFF_TAB = OFF_BOX + EPI_WARPS * BOX_BYTES;
   static constexpr int TAB = LORA ? 2 : kMaxExperts + 1;
   static constexpr uint32_t OFF_BAR = (OFF_TAB + 2 * TAB * 4 + 7u) & ~7u;
-  static constexpr uint32_t NUM_BARS = 2 * STAGES + 5;  // full, empty, tfull, tempty, drain
+  static constexpr uint32_t NUM_BARS = 2 * STAGES + 5 + SUM_BARS;  // full, empty, tfull, tempty, drain, B
   static constexpr uint32_t OFF_SLOT = OFF_BAR + NUM_BARS * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_SLOT + 8 + 1024;
   static_assert(STAGE % 1024 == 0, "swizzle atoms need 1024 B alignment");
@@ -329,7 +472,7 @@ struct Cfg {
 };
 
 template <int CG, bool LORA>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
     persist_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using C = Cfg<CG, LORA>;
   extern __shared__ uint8_t smem_raw[];
@@ -341,6 +484,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t bar_tfull = bar_empty + C::STAGES * 8;
   const uint32_t bar_tempty = bar_tfull + 2 * 8;
   const uint32_t bar_drain = bar_tempty + 2 * 8;
+  const uint32_t bar_sum = bar_drain + 8;
   volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + C::OFF_SLOT);
   volatile int *abort = reinterpret_cast<volatile int *>(smem + C::OFF_SLOT + 4);
   int *g_row = reinterpret_cast<int *>(smem + C::OFF_TAB);
@@ -364,6 +508,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       ptx::mbar_init(bar_tempty + 8 * a, EPI_WARPS * CG);
     }
     ptx::mbar_init(bar_drain, 1);
+    for (int i = 0; i < SUM_SLOTS; ++i) {
+      ptx::mbar_init(bar_sum + 8 * i, 1);
+      ptx::mbar_init(bar_sum + 8 * (SUM_SLOTS + i), EPI_WARPS);
+    }
     *abort = 0;
     ptx::fence_mbar_init();
   }
@@ -377,90 +525,73 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
+  if (!LORA && p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
   if (p.pdl) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  if (!p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
+  if (!LORA && !p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
 
-  const int num_tiles = g_tile[p.E];
+  PlanWalk plan = {};
+  if constexpr (LORA) plan.start(p, group);
+  const int num_tiles = LORA ? plan.num_tiles : g_tile[p.E];
+  auto tile_at = [&](int t, int &e) -> Tile {
+    if constexpr (LORA)
+      return plan.template take<CG>(p, t, n_groups);
+    else
+      return find_tile<CG>(p, C::TOK_MAX, g_row, g_tile, t, e);
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    // (the whole warp: the rows of h are gathered by all lanes)
-    {
+    if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       uint32_t issued = 0;
       int e = 0;
-      // A free stage: false when the wait ran out.
-      auto take = [&]() -> bool {
-        bool got = true;
-        if (lane == 0) {
-          got = ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort, kWaitLimitNs);
-          if (!got) record_timeout(abort);
-        }
-        return LORA ? __shfl_sync(0xFFFFFFFFu, got ? 1 : 0, 0) != 0 : got;
-      };
-      auto next = [&]() {
-        ++issued;
-        if (++stage == C::STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      };
       bool ok = true;
-      for (int t = group; t < num_tiles && ok && (LORA || lane == 0); t += n_groups) {
-        const Tile q = find_tile<CG>(p, C::TOK_MAX, g_row, g_tile, t, e);
+      for (int t = group; t < num_tiles && ok; t += n_groups) {
+        const Tile q = tile_at(t, e);
         const int wrow = (q.wb * CG + static_cast<int>(rank)) * WROWS;
         const int xrows = q.nn / CG;
         const int xrow = q.t0 + static_cast<int>(rank) * xrows;
         const uint32_t tx = CG * W_STAGE + static_cast<uint32_t>(q.nn) * BK;
-        // both CTAs' bytes complete the leader's barrier; only the leader arms it
-        auto arm = [&](const CUtensorMap *m, int x, int z) {
+        // One stage: the weight box and the token box at the given coordinates.
+        auto load = [&](const CUtensorMap *mw, int wx, int wz, const CUtensorMap *mx, int xx) {
+          if (!ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort, kWaitLimitNs)) {
+            record_timeout(abort);
+            return false;
+          }
           const uint32_t fb = bar_full + 8 * stage;
           const uint32_t dst = sbase + static_cast<uint32_t>(stage) * C::STAGE;
-          if (leader) ptx::mbar_arrive_expect_tx(fb, tx);
-          if constexpr (CG == 1)
-            ptx::tma_load_3d(dst, m, x, wrow, z, fb);
-          else
-            ptx::tma_load_3d_pair(dst, m, x, wrow, z, ptx::map_shared_rank(fb, 0));
-        };
-        auto dst_x = [&]() { return sbase + static_cast<uint32_t>(stage) * C::STAGE + W_STAGE; };
-        auto bar_x = [&]() {
-          const uint32_t fb = bar_full + 8 * stage;
-          return CG == 1 ? fb : ptx::map_shared_rank(fb, 0);
-        };
-        const CUtensorMap *mx = &maps.x[xrows / 16 - 1];
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!(ok = take())) break;
-          if (lane == 0) {
-            arm(&maps.w, kb * BK, q.e);
-            if constexpr (CG == 1)
-              ptx::tma_load_2d(dst_x(), mx, kb * BK, xrow, bar_x());
-            else
-              ptx::tma_load_2d_pair(dst_x(), mx, kb * BK, xrow, bar_x());
+          if constexpr (CG == 1) {
+            ptx::mbar_arrive_expect_tx(fb, tx);
+            ptx::tma_load_3d(dst, mw, wx, wrow, wz, fb);
+            ptx::tma_load_2d(dst + W_STAGE, mx, xx, xrow, fb);
+          } else {
+            // both CTAs' bytes complete the leader's barrier; only the leader arms it
+            if (leader) ptx::mbar_arrive_expect_tx(fb, tx);
+            const uint32_t fl = ptx::map_shared_rank(fb, 0);
+            ptx::tma_load_3d_pair(dst, mw, wx, wrow, wz, fl);
+            ptx::tma_load_2d_pair(dst + W_STAGE, mx, xx, xrow, fl);
           }
-          next();
-        }
+          ++issued;
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          return true;
+        };
+        const int mi = xrows / 16 - 1;
+        for (int kb = 0; kb < p.k_blocks && ok; ++kb)
+          ok = load(&maps.w, kb * BK, q.e, &maps.x[mi], kb * BK);
         if constexpr (LORA) {
-          const int count = __ldg(p.count + q.tb), per = lora_stages(p);
-          GatherRows g;
-          if (count > 0) g = gather_rows(p, xrow, q.t1, lane);
-          for (int d = 0; d < count && ok; ++d) {
-            const int a = __ldg(p.list + static_cast<int64_t>(q.tb) * kLoraTileTokens + d);
-            for (int j = 0; j < per; ++j) {
-              if (!(ok = take())) break;
-              int bx, hx;
-              lora_columns(p, j, bx, hx);
-              if (lane == 0) arm(&maps.lb, bx, a);
-              __syncwarp();
-              gather_h<CG>(p, &maps.h, g, xrows, a, hx, dst_x(), bar_x(), lane);
-              next();
-            }
+          const int per = q.adapter >= 0 ? lora_stages(p) : 0;
+          for (int j = 0; j < per && ok; ++j) {
+            int bx, hx;
+            lora_columns(p, j, bx, hx);
+            ok = load(&maps.lb, bx, q.adapter, &maps.h[mi], hx);
           }
         }
       }
-      if (lane == 0) {
       // Drain: every load issued here has landed and been consumed.
       const uint32_t n_drain = issued < C::STAGES ? issued : C::STAGES;
       for (uint32_t i = 0; i < n_drain; ++i) {
@@ -471,7 +602,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           --stage;
         }
         ptx::mbar_wait_timeout(bar_empty + 8 * stage, phase, kDrainLimitNs);
-      }
       }
     }
   } else if (warp == 1) {
@@ -502,7 +632,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         return true;
       };
       for (int t = group; t < num_tiles && ok; t += n_groups, ++it) {
-        const Tile q = find_tile<CG>(p, C::TOK_MAX, g_row, g_tile, t, e);
+        const Tile q = tile_at(t, e);
         const int acc = it & 1;
         const uint32_t acc_phase = (it >> 1) & 1;
         if (!ptx::mbar_wait_bounded(bar_tempty + 8 * acc, acc_phase ^ 1u, abort, kWaitLimitNs)) {
@@ -529,8 +659,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           next_stage();
         }
         if constexpr (LORA) {
-          const int count = ok ? __ldg(p.count + q.tb) : 0;
-          if (count > 0) {
+          if (ok && q.adapter >= 0) {
             // the third accumulator is free once the epilogue of the tile before has let
             // its own go (the same arrival that this loop waits for one tile later)
             if (it > 0 && !ptx::mbar_wait_bounded(bar_tempty + 8 * (acc ^ 1),
@@ -542,10 +671,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             ptx::tc_fence_after();
             const uint32_t id16 = ptx::idesc_f16_f32(WROWS * CG, q.nn, p.lora_dtype == kBF16);
             const int per = lora_stages(p);
-            for (int i = 0; i < count * per; ++i) {
+            for (int j = 0; j < per; ++j) {
               if (!(ok = wait_full())) break;
               lora_mma<CG>(p, tmem_base + C::ACC_L, sbase + static_cast<uint32_t>(stage) * C::STAGE,
-                           id16, i % per, i == 0);
+                           id16, j);
               next_stage();
             }
           }
@@ -563,6 +692,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         ptx::mma_commit_pair(bar_drain);
       ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
     }
+  } else if (LORA && warp == 2 + EPI_WARPS) {
+    // ------------------------------------------------------------ B boxes of mixed tiles
+    SumRing ring = {sbase + C::OFF_RING, bar_sum, abort, 0};
+    int e = 0;
+    for (int t = group; t < num_tiles; t += n_groups) {
+      const Tile q = tile_at(t, e);
+      if (q.adapter == -2 && !feed_sums(p, &maps.lb, ring, q.t0, q.t1,
+                                        (q.wb * CG + static_cast<int>(rank)) * WROWS))
+        break;
+    }
+    drain_sums(ring);
   } else {
     // ------------------------------------------------------------ epilogue
     // TMEM lane = weight row (output column), TMEM column = token. A warp takes its 32
@@ -573,7 +713,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const int ew = warp - 2;
     float *e_xs = reinterpret_cast<float *>(smem + C::OFF_PAR + ew * C::PAR_WARP);
     float *e_hs = e_xs + C::TOK_MAX;
-    int *e_id = reinterpret_cast<int *>(e_hs + C::TOK_MAX);
+    SumRing ring = {sbase + C::OFF_RING, bar_sum, abort, 0};
     const uint8_t *box = smem + C::OFF_BOX + ew * BOX_BYTES;
     const uint32_t box_st = sbase + C::OFF_BOX + ew * BOX_BYTES +
                             static_cast<uint32_t>((lane & 7) * BOX_PITCH + (lane >> 3) * 16);
@@ -582,20 +722,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     int it = 0;
     int e = 0;
     for (int t = group; t < num_tiles; t += n_groups, ++it) {
-      const Tile q = find_tile<CG>(p, C::TOK_MAX, g_row, g_tile, t, e);
+      const Tile q = tile_at(t, e);
       const int acc = it & 1;
       const uint32_t acc_phase = (it >> 1) & 1;
       const int cnt = q.t1 - q.t0;
       const int n0 = (q.wb * CG + static_cast<int>(rank)) * WROWS + quarter * 32;
-      int adapters = 0;
-      if constexpr (LORA) adapters = __ldg(p.count + q.tb);
       __syncwarp();
       for (int i = lane; i < ((cnt + 31) & ~31); i += 32) {
         e_xs[i] = i < cnt ? __ldg(p.xs + q.t0 + i) : 0.0f;
         if constexpr (LORA) {
-          const int id = i < cnt ? __ldg(p.ids + q.t0 + i) : -1;
-          const bool has = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L);
-          e_id[i] = has ? id : -1;
+          const bool has =
+              q.adapter >= 0 ? i < cnt : q.adapter == -2 && token_id(p, q.t0 + i, q.t1) >= 0;
           e_hs[i] = has ? __ldg(p.hscale + q.t0 + i) : 0.0f;
         }
       }
@@ -607,6 +744,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         b[k] = load_bias(p.bias, p.bias_dtype, wn);
       }
       __syncwarp();
+      float2 sum[kLoraMixed / 8][4];  // a mixed tile's adapter sums, [g][k] as v below
+      if constexpr (LORA) {
+        if (q.adapter == -2) {
+          bool ok = true;
+#pragma unroll
+          for (int g = 0; g < kLoraMixed / 8; ++g)
+            ok = ok && adapter_sums(p, ring, q.t0 + 8 * g, q.t1, quarter, sum[g]);
+          if (!ok) break;
+        }
+      }
       if (!ptx::mbar_wait_bounded(bar_tfull + 8 * acc, acc_phase, abort, kWaitLimitNs)) {
         if (lane == 0) record_timeout(abort);
         break;
@@ -634,33 +781,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
         }
         if constexpr (LORA) {
-          if (adapters > 0) {
+          if (q.adapter >= 0) {
             ptx::tmem_ld_16x256b_x4(t_row + C::ACC_L + static_cast<uint32_t>(c), r[0]);
             ptx::tmem_ld_16x256b_x4(t_row + C::ACC_L + kHalf + static_cast<uint32_t>(c), r[1]);
             ptx::tmem_wait_ld();
-            float2 odd = make_float2(0.0f, 0.0f);  // NaN if any sum is not finite
-#pragma unroll
-            for (int i = 0; i < 32; i += 2)
-              odd = ptx::fma2(make_float2(__uint_as_float(r[i >> 4][i & 15]),
-                                          __uint_as_float(r[i >> 4][(i & 15) + 1])),
-                              make_float2(0.0f, 0.0f), odd);
-            if (odd.x + odd.y != 0.0f) {
-              // (every sum of the lane anew: rows without an adapter get zero)
-#pragma unroll
-              for (int g = 0; g < 4; ++g)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const int i = c + 8 * g + 2 * ft + h;
-                    const int id = e_id[i], n = n0 + fi + 8 * k;
-                    uint32_t &s = r[k >> 1][4 * g + 2 * (k & 1) + h];
-                    if (id < 0 || n >= p.N)
-                      s = 0;
-                    else if (adapters > 1 && !is_finite(__uint_as_float(s)))
-                      s = __float_as_uint(exact_sum(p, q.t0 + i, id, n));
-                  }
-            }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               const float2 hs = *reinterpret_cast<const float2 *>(e_hs + c + 8 * g + 2 * ft);
@@ -670,6 +794,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 v[g][k] = ptx::fma2(make_float2(__uint_as_float(a[0]), __uint_as_float(a[1])), hs,
                                     v[g][k]);
               }
+            }
+          } else if (q.adapter == -2) {  // (one chunk: cnt <= kLoraMixed)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float2 hs = *reinterpret_cast<const float2 *>(e_hs + 8 * g + 2 * ft);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[g][k] = ptx::fma2(sum[g][k], hs, v[g][k]);
             }
           }
         }
@@ -711,7 +842,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           ptx::mbar_arrive_cluster(ptx::map_shared_rank(bar_tempty + 8 * acc, 0));
       }
     }
-    zero_rows(p, g_row, 64, NUM_THREADS - 64);
+    if constexpr (!LORA) zero_rows(p, g_row, 64, 32 * EPI_WARPS);
   }
 
   __syncwarp();
@@ -727,44 +858,47 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 // ---------------------------------------------------------------- split-K kernel
 
 constexpr int SPLIT_TOK = 128;   // tokens per tile, at most
+constexpr int SPLIT_LORA_TOK = 64;  // with adapters, whose sums need room too
 constexpr int SPLIT_STAGES = 8;  // ring slots, at most
 constexpr int SPLIT_MAX = 8;     // CTAs per cluster, at most (portable)
-constexpr uint32_t SPLIT_EPI = (3 * SPLIT_TOK + 2 * WROWS) * 4;  // xs, ws, bias, hscale, ids
+constexpr int SPLIT_COST = 12;   // a tile's set-up and reduction, in K-blocks
+constexpr uint32_t SPLIT_EPI = (2 * SPLIT_TOK + 2 * WROWS) * 4;  // xs, ws, bias, hscale
 constexpr uint32_t SPLIT_SMEM = 232448;
 
 template <bool LORA>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = ptx::smem_u32(smem);
-  __shared__ alignas(8) uint64_t s_bar[2 * SPLIT_STAGES + 2];
+  __shared__ alignas(8) uint64_t s_bar[2 * SPLIT_STAGES + 2 + SUM_BARS];
   __shared__ uint32_t s_slot;
   __shared__ int s_abort;
   const uint32_t bar_full = ptx::smem_u32(s_bar);
   const uint32_t bar_empty = bar_full + 8 * SPLIT_STAGES;
   const uint32_t bar_acc = bar_empty + 8 * SPLIT_STAGES;
   const uint32_t bar_drain = bar_acc + 8;
+  const uint32_t bar_sum = bar_drain + 8;
   volatile uint32_t *tmem_slot = &s_slot;
   volatile int *abort = &s_abort;
-  float *part = reinterpret_cast<float *>(smem + p.off_part);  // [tokens][WROWS]
+  // partial sums of the rows reduced here: [CTA they come from][token][R rows]
+  float *part = reinterpret_cast<float *>(smem + p.off_part);
+  float *lora = reinterpret_cast<float *>(smem + p.off_lora);  // [tokens of this CTA][WROWS]
   int *g_row = reinterpret_cast<int *>(smem + p.off_tab);
   int *g_tile = g_row + p.E + 1;
-  float *e_xs = reinterpret_cast<float *>(g_tile + p.E + 1);  // [SPLIT_TOK]
+  float *e_xs = reinterpret_cast<float *>(
+      smem + ((p.off_tab + static_cast<uint32_t>(p.E + 1) * 8 + 15u) & ~15u));  // [SPLIT_TOK]
   float *e_ws = e_xs + SPLIT_TOK;                              // [WROWS]
   float *e_b = e_ws + WROWS;
-  float *e_hs = e_b + WROWS;                              // [SPLIT_TOK]
-  int *e_id = reinterpret_cast<int *>(e_hs + SPLIT_TOK);  // [SPLIT_TOK]
+  float *e_hs = e_b + WROWS;  // [SPLIT_TOK]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
   const int stages = p.stages;
   const uint32_t stage_bytes = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
-  // TMEM: the accumulator, and behind it the adapters'
-  const uint32_t acc_l = static_cast<uint32_t>(p.tok_cap);
   uint32_t tmem_cols = 32;
-  while (tmem_cols < (LORA ? 2 : 1) * static_cast<uint32_t>(p.tok_cap)) tmem_cols <<= 1;
+  while (tmem_cols < static_cast<uint32_t>(p.tok_cap)) tmem_cols <<= 1;
 
   if (threadIdx.x == 0) {
     ptx::prefetch_tmap(&maps.w);
@@ -774,6 +908,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
     ptx::mbar_init(bar_acc, 1);
     ptx::mbar_init(bar_drain, 1);
+    for (int i = 0; i < SUM_SLOTS; ++i) {
+      ptx::mbar_init(bar_sum + 8 * i, 1);
+      ptx::mbar_init(bar_sum + 8 * (SUM_SLOTS + i), EPI_WARPS);
+    }
     s_abort = 0;
     ptx::fence_mbar_init();
   }
@@ -783,7 +921,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   if (t >= g_tile[p.E]) {  // the whole cluster: fewer tiles than clusters
     if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    zero_rows(p, g_row, 0, NUM_THREADS);
+    zero_rows(p, g_row, 0, blockDim.x);
     return;
   }
   int ge = 0;
@@ -814,6 +952,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  ptx::cluster_arrive_release();  // (waited for before the first push: all CTAs have started)
   if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
@@ -824,59 +963,44 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int quads = r1 > r0 ? (r1 - r0) >> 2 : 0;
   const int n0 = q.wb * WROWS;
 
-  // This CTA's adapters: every split-th of the tile's, as stages behind its K-blocks.
-  const int adapters = LORA ? __ldg(p.count) : 0;
-  const int mine = LORA && adapters > rank ? (adapters - rank + p.split - 1) / p.split : 0;
-  const int per = LORA ? lora_stages(p) : 0;
-  const int nst = nkb + mine * per;
+  // Adapters: the cluster's CTAs share out the tokens, eight at a time.
+  const int per_cta = LORA ? ((cnt + 7) / 8 + p.split - 1) / p.split * 8 : 0;
+  const int a0 = min(cnt, rank * per_cta), a1 = min(cnt, a0 + per_cta);
 
   if (warp == 0) {
-    GatherRows g;
-    if (LORA && mine > 0) g = gather_rows(p, q.t0, q.t1, lane);
-    int issued = 0;
-    for (int i = 0; i < nst; ++i) {
-      const int s = i % stages;
-      const uint32_t fb = bar_full + 8 * s;
-      const uint32_t dst = sbase + static_cast<uint32_t>(s) * stage_bytes;
-      // (the first K-blocks' stages are armed, their weight boxes under way)
-      const bool armed = i < nkb && i < stages;
-      bool got = true;
-      if (lane == 0 && i >= stages) {
-        got = ptx::mbar_wait_bounded(bar_empty + 8 * s,
-                                     static_cast<uint32_t>(i / stages - 1) & 1u, abort,
-                                     kWaitLimitNs);
-        if (!got) record_timeout(abort);
-      }
-      if (__shfl_sync(0xFFFFFFFFu, got ? 1 : 0, 0) == 0) break;
-      if (lane == 0 && !armed) ptx::mbar_arrive_expect_tx(fb, tx);
-      if (i < nkb) {
-        if (lane == 0) {
-          if (!armed) ptx::tma_load_3d(dst, &maps.w, (kb0 + i) * BK, n0, q.e, fb);
-          ptx::tma_load_2d(dst + W_STAGE, mx, (kb0 + i) * BK, q.t0, fb);
+    if (lane == 0) {
+      int issued = 0;
+      int s = 0;
+      uint32_t ph = 1;
+      for (int i = 0; i < nkb; ++i) {
+        const uint32_t fb = bar_full + 8 * s;
+        const uint32_t dst = sbase + static_cast<uint32_t>(s) * stage_bytes;
+        if (i >= stages) {  // (the first stages are armed, their weight boxes under way)
+          if (!ptx::mbar_wait_bounded(bar_empty + 8 * s, ph, abort, kWaitLimitNs)) {
+            record_timeout(abort);
+            break;
+          }
+          ptx::mbar_arrive_expect_tx(fb, tx);
+          ptx::tma_load_3d(dst, &maps.w, (kb0 + i) * BK, n0, q.e, fb);
         }
-      } else if constexpr (LORA) {
-        const int d = (i - nkb) / per, j = (i - nkb) % per;
-        const int a = __ldg(p.list + rank + d * p.split);
-        int bx, hx;
-        lora_columns(p, j, bx, hx);
-        if (lane == 0) ptx::tma_load_3d(dst, &maps.lb, bx, n0, a, fb);
-        __syncwarp();
-        gather_h<1>(p, &maps.h, g, q.nn, a, hx, dst + W_STAGE, fb, lane);
+        ptx::tma_load_2d(dst + W_STAGE, mx, (kb0 + i) * BK, q.t0, fb);
+        ++issued;
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1u;
+        }
       }
-      ++issued;
-    }
-    if (lane == 0)
       for (int i = issued - 1; i >= 0 && i >= issued - stages; --i)
         ptx::mbar_wait_timeout(bar_empty + 8 * (i % stages),
                                static_cast<uint32_t>(i / stages) & 1u, kDrainLimitNs);
+    }
   } else if (warp == 1) {
     if (lane == 0) {
       bool ok = true;
       const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS, q.nn);
-      const uint32_t id16 = ptx::idesc_f16_f32(WROWS, q.nn, p.lora_dtype == kBF16);
       int s = 0;
       uint32_t ph = 0;
-      for (int i = 0; i < nst; ++i) {
+      for (int i = 0; i < nkb; ++i) {
         if (!ptx::mbar_wait_bounded(bar_full + 8 * s, ph, abort, kWaitLimitNs)) {
           record_timeout(abort);
           ok = false;
@@ -884,16 +1008,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         ptx::tc_fence_after();
         const uint32_t st = sbase + static_cast<uint32_t>(s) * stage_bytes;
-        if (i < nkb) {
-          const uint64_t adesc = ptx::sw128_kmajor_desc(st);
-          const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
+        const uint64_t adesc = ptx::sw128_kmajor_desc(st);
+        const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
 #pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-            const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
-            ptx::mma_f8f6f4(tmem, adesc + koff, bdesc + koff, idesc, (i | kk) != 0 ? 1u : 0u);
-          }
-        } else if constexpr (LORA) {
-          lora_mma<1>(p, tmem + acc_l, st, id16, (i - nkb) % per, i == nkb);
+        for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+          const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
+          ptx::mma_f8f6f4(tmem, adesc + koff, bdesc + koff, idesc, (i | kk) != 0 ? 1u : 0u);
         }
         ptx::mma_commit(bar_empty + 8 * s);
         if (++s == stages) {
@@ -905,20 +1025,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       ptx::mma_commit(bar_drain);
       ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
     }
+  } else if (LORA && warp == 2 + EPI_WARPS) {
+    SumRing ring = {sbase + p.off_ring, bar_sum, abort, 0};
+    feed_sums(p, &maps.lb, ring, q.t0 + a0, q.t0 + a1, n0);
+    drain_sums(ring);
   } else {
-    // xs (adapters: and hscale, ids) of the tokens, weight scales and biases: of the rows
-    // reduced here, or with adapters of all the tile's rows
+    // xs (adapters: and hscale) of the tokens, weight scales and biases of the rows reduced
+    // here
     const int et = threadIdx.x - 64;
-    for (int i = et; i < cnt; i += NUM_THREADS - 64) {
-      e_xs[i] = __ldg(p.xs + q.t0 + i);
-      if constexpr (LORA) {
-        const int id = __ldg(p.ids + q.t0 + i);
-        const bool has = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.L);
-        e_id[i] = has ? id : -1;
-        e_hs[i] = has ? __ldg(p.hscale + q.t0 + i) : 0.0f;
-      }
+    for (int i = et; i < q.nn; i += 128) {
+      e_xs[i] = i < cnt ? __ldg(p.xs + q.t0 + i) : 0.0f;
+      if constexpr (LORA)
+        e_hs[i] = token_id(p, q.t0 + i, q.t1) >= 0 ? __ldg(p.hscale + q.t0 + i) : 0.0f;
     }
-    for (int i = et; i < r1 - r0; i += NUM_THREADS - 64) {
+    for (int i = et; i < r1 - r0; i += 128) {
       const int n = n0 + r0 + i;
       const int64_t wn = static_cast<int64_t>(q.e) * p.N + n;
       e_ws[i] = n < p.N ? __ldg(p.ws + wn) : 0.0f;
@@ -928,65 +1048,77 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const int row = quarter * 32 + lane;
     const int n = n0 + row;
     const float w = LORA && n < p.N ? __ldg(p.ws + n) : 1.0f;
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    // TMEM (lane = weight row, column = token) -> part[token][row], fp32: the K-blocks' sums
-    // as they are, or with adapters dequantized, plus the sums of this CTA's adapters
+    epilogue_sync();  // xs and hscale are in shared memory
+    if constexpr (LORA) {
+      // (a warp writes and reads back its own rows only; after a wait that ran out, whatever)
+      SumRing ring = {sbase + p.off_ring, bar_sum, abort, 0};
+      bool ok = true;
+      for (int i = a0; i < a1 && ok; i += 8) {
+        float2 s[4];
+        ok = adapter_sums(p, ring, q.t0 + i, q.t0 + a1, quarter, s);
+        float *to = lora + (i - a0 + 2 * (lane & 3)) * WROWS + quarter * 32 + (lane >> 2);
+        const float2 hs = *reinterpret_cast<const float2 *>(e_hs + i + 2 * (lane & 3));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          to[8 * k] = s[k].x * hs.x;
+          to[8 * k + WROWS] = s[k].y * hs.y;
+        }
+      }
+      __syncwarp();
+    }
+    // TMEM (lane = weight row, column = token) -> the part of the CTA that reduces the row,
+    // fp32: the K-blocks' sums as they are, or with adapters dequantized and added to the
+    // adapters' sums
     const bool ok = ptx::mbar_wait_bounded(bar_acc, 0, abort, kWaitLimitNs);
     if (!ok && lane == 0) record_timeout(abort);
     ptx::tc_fence_after();
+    ptx::cluster_wait_acquire();
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t dst = ptx::map_shared_rank(
+        ptx::smem_u32(part) +
+            static_cast<uint32_t>(rank * p.tok_cap * R + row % R) * 4u,
+        static_cast<uint32_t>(row / R));
+#pragma unroll 1
     for (int c = 0; c < q.nn; c += 16) {
-      uint32_t r[16], l[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) r[j] = l[j] = 0u;
+      uint32_t r[16];
       if (ok) {
         ptx::tmem_ld_32x32b_x16(t_row + static_cast<uint32_t>(c), r);
-        if (LORA && mine > 0) ptx::tmem_ld_32x32b_x16(t_row + acc_l + static_cast<uint32_t>(c), l);
         ptx::tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = 0u;
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         float v = __uint_as_float(r[j]);
         if constexpr (LORA) {
-          const int i = min(c + j, cnt - 1);
-          v = v * e_xs[i] * w;
-          float s = __uint_as_float(l[j]);
-          const int id = e_id[i];
-          if (adapters > 1 && mine > 0 && !is_finite(s) && id >= 0 && n < p.N) {
-            // this CTA's adapter's sum again, or nothing
-            s = 0.0f;
-            for (int d = rank; d < adapters; d += p.split)
-              if (__ldg(p.list + d) == id) s = exact_sum(p, q.t0 + i, id, n);
-          }
-          v = id >= 0 ? fmaf(s, e_hs[i], v) : v;
+          v = v * e_xs[c + j] * w;
+          if (c + j >= a0 && c + j < a1) v += lora[(c + j - a0) * WROWS + row];
         }
-        part[(c + j) * WROWS + row] = v;
+        if (c + j < cnt) ptx::st_shared_cluster_f32(dst + static_cast<uint32_t>((c + j) * R) * 4u, v);
       }
     }
     ptx::tc_fence_before();
   }
+  if (warp < 2 || warp >= 2 + EPI_WARPS) ptx::cluster_wait_acquire();
 
   __syncwarp();
   __syncthreads();
-  ptx::cluster_sync();  // every CTA's partial tile is in its shared memory
+  ptx::cluster_sync();  // the partial sums of this CTA's rows have arrived
 
-  const uint32_t part_base = ptx::smem_u32(part);
-  for (int idx = threadIdx.x; idx < cnt * quads; idx += NUM_THREADS) {
+  for (int idx = threadIdx.x; idx < cnt * quads; idx += blockDim.x) {
     const int m = idx / quads;
     const int qd = idx - m * quads;
-    const uint32_t off = static_cast<uint32_t>(m * WROWS + r0 + 4 * qd) * 4u;
-    float4 v[SPLIT_MAX];
-#pragma unroll
-    for (int s = 0; s < SPLIT_MAX; ++s)
-      if (s < p.split) v[s] = ptx::ld_shared_cluster_v4(ptx::map_shared_rank(part_base + off, s));
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < SPLIT_MAX; ++s)
       if (s < p.split) {
-        a[0] += v[s].x;
-        a[1] += v[s].y;
-        a[2] += v[s].z;
-        a[3] += v[s].w;
+        const float4 v =
+            *reinterpret_cast<const float4 *>(part + (s * p.tok_cap + m) * R + 4 * qd);
+        a[0] += v.x;
+        a[1] += v.y;
+        a[2] += v.z;
+        a[3] += v.w;
       }
     const float xs = e_xs[m];
 #pragma unroll
@@ -998,9 +1130,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       store_out(p.out, p.out_dtype, static_cast<int64_t>(q.t0 + m) * p.N + n, val);
     }
   }
-  zero_rows(p, g_row, 0, NUM_THREADS);
+  zero_rows(p, g_row, 0, blockDim.x);
 
-  ptx::cluster_sync();  // peers may still be reading this CTA's partial tile
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc<1>(tmem, tmem_cols);
@@ -1030,7 +1161,7 @@ LaunchInfo &persist_info(const DeviceInfo &dev) {
     if (li.err == cudaSuccess && CG == 2) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(dev.sm_count / CG * CG);
-      cfg.blockDim = dim3(NUM_THREADS);
+      cfg.blockDim = dim3(Cfg<CG, LORA>::THREADS);
       cfg.dynamicSmemBytes = Cfg<CG, LORA>::SMEM_BYTES;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1053,11 +1184,11 @@ int launch_failed(const char *op, cudaError_t e) {
   return 4;
 }
 
-cudaError_t launch(const void *kernel, const Maps &maps, const Params &p, int ctas, int cluster,
-                   size_t smem, cudaStream_t stream, bool pdl) {
+cudaError_t launch(const void *kernel, const Maps &maps, const Params &p, int ctas, int threads,
+                   int cluster, size_t smem, cudaStream_t stream, bool pdl) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -1088,46 +1219,92 @@ int launch_persist(const char *op, const Maps &maps, Params &p, int64_t tiles,
   const int groups = static_cast<int>(std::min<int64_t>(tiles, li.max_groups));
   const cudaError_t e =
       launch(reinterpret_cast<const void *>(&persist_kernel<CG, LORA>), maps, p, groups * CG,
-             CG == 2 ? 2 : 0, Cfg<CG, LORA>::SMEM_BYTES, stream, pdl);
+             Cfg<CG, LORA>::THREADS, CG == 2 ? 2 : 0, Cfg<CG, LORA>::SMEM_BYTES, stream, pdl);
   return e == cudaSuccess ? 0 : launch_failed(op, e);
+}
+
+// Clusters of each size that the GPU holds at once with one CTA per SM (a size that does not
+// divide the SMs of a GPC leaves some of them over).
+struct SplitInfo {
+  bool ready = false;
+  cudaError_t err = cudaSuccess;
+  int clusters[SPLIT_MAX + 1] = {};
+};
+
+template <bool LORA>
+SplitInfo &split_info(const DeviceInfo &dev) {
+  static SplitInfo info[64];
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  SplitInfo &si = info[dev.device & 63];
+  if (!si.ready) {
+    si.ready = true;
+    // (the static barriers take a little of the 227 KB)
+    si.err = cudaFuncSetAttribute(split_kernel<LORA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  SPLIT_SMEM - 1024);
+    si.clusters[1] = dev.sm_count;
+    for (int s = 2; s <= SPLIT_MAX && si.err == cudaSuccess; ++s) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(static_cast<unsigned>(dev.sm_count / s * s));
+      cfg.blockDim = dim3(NUM_THREADS + (LORA ? 32 : 0));
+      cfg.dynamicSmemBytes = SPLIT_SMEM - 1024;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = static_cast<unsigned>(s);
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      si.err = cudaOccupancyMaxActiveClusters(&si.clusters[s], split_kernel<LORA>, &cfg);
+    }
+  }
+  return si;
 }
 
 template <bool LORA>
 int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const DeviceInfo &dev,
                  cudaStream_t stream, bool pdl) {
-  static bool set[64];
-  static std::mutex mu;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!set[dev.device & 63]) {
-      // (the static barriers take a little of the 227 KB)
-      const cudaError_t e = cudaFuncSetAttribute(
-          split_kernel<LORA>, cudaFuncAttributeMaxDynamicSharedMemorySize, SPLIT_SMEM - 1024);
-      if (e != cudaSuccess) return launch_failed(op, e);
-      set[dev.device & 63] = true;
+  SplitInfo &si = split_info<LORA>(dev);
+  if (si.err != cudaSuccess) return launch_failed(op, si.err);
+  // The K-split that takes the least time: waves of clusters, each as long as its K-blocks
+  // and a set-up and reduction worth about SPLIT_COST of them; at least two K-blocks a CTA.
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= SPLIT_MAX && s <= std::max(1, p.k_blocks / 2); ++s) {
+    if (si.clusters[s] < 1) continue;
+    const int64_t waves = (tiles + si.clusters[s] - 1) / si.clusters[s];
+    const int64_t cost = waves * ((p.k_blocks + s - 1) / s + SPLIT_COST);
+    if (cost < least) {
+      least = cost;
+      best = s;
     }
   }
-  // K-splits: as many CTAs as the GPU holds, at least two K-blocks for each
-  int split = std::max(1, std::min({dev.sm_count / tiles, SPLIT_MAX, (p.k_blocks + 1) / 2}));
-  p.kps = (p.k_blocks + split - 1) / split;
+  p.kps = (p.k_blocks + best - 1) / best;
   p.split = (p.k_blocks + p.kps - 1) / p.kps;
   const uint32_t stage = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
-  const uint32_t part = static_cast<uint32_t>(p.tok_cap) * WROWS * 4;
-  const uint32_t tab = static_cast<uint32_t>(p.E + 1) * 8 + SPLIT_EPI;
-  const uint32_t room = SPLIT_SMEM - 2048 - part - tab;
-  p.stages = std::max(1, std::min({static_cast<int>(room / stage), SPLIT_STAGES,
-                                   LORA ? SPLIT_STAGES : p.kps}));
-  p.off_part = static_cast<uint32_t>(p.stages) * stage;
-  p.off_tab = p.off_part + part;
+  const uint32_t rows = static_cast<uint32_t>(((WROWS + p.split - 1) / p.split + 3) & ~3);
+  const uint32_t part = static_cast<uint32_t>(p.split * p.tok_cap) * rows * 4;
+  const uint32_t lora =
+      LORA ? static_cast<uint32_t>((p.tok_cap / 8 + p.split - 1) / p.split * 8) * WROWS * 4 : 0;
+  const uint32_t tab = static_cast<uint32_t>(p.E + 1) * 8 + 16 + SPLIT_EPI;
+  const uint32_t ring = LORA ? SUM_SLOTS * W_STAGE : 0u;
+  const uint32_t room = SPLIT_SMEM - 2048 - ring - part - lora - tab;
+  p.stages = std::max(1, std::min({static_cast<int>(room / stage), SPLIT_STAGES, p.kps}));
+  p.off_ring = static_cast<uint32_t>(p.stages) * stage;
+  p.off_part = p.off_ring + ring;
+  p.off_lora = p.off_part + part;
+  p.off_tab = p.off_lora + lora;
   const size_t smem = p.off_tab + tab + 1024;
   const cudaError_t e = launch(reinterpret_cast<const void *>(&split_kernel<LORA>), maps, p,
-                               tiles * p.split, p.split, smem, stream, pdl);
+                               tiles * p.split, NUM_THREADS + (LORA ? 32 : 0), p.split, smem,
+                               stream, pdl);
   return e == cudaSuccess ? 0 : launch_failed(op, e);
 }
 
-bool make_common_maps(Maps *m, const uint8_t *xq, const uint8_t *wq, int64_t M, int64_t N,
+// `n` boxes of tokens: 16, 32, .. 16 n rows.
+bool make_common_maps(Maps *m, int n, const uint8_t *xq, const uint8_t *wq, int64_t M, int64_t N,
                       int64_t K, int64_t E, std::string *err) {
-  for (int i = 0; i < X_MAPS; ++i)
+  for (int i = 0; i < n; ++i)
     if (!make_tmap_2d_sw128(&m->x[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, K, M, K, BK, 16 * (i + 1),
                             err))
       return false;
@@ -1154,14 +1331,6 @@ int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl) {
   const char *op = "fp8_grouped_gemm";
   DeviceInfo dev;
   if (!check_device(op, &dev)) return 5;
-  std::string err;
-  Maps maps;
-  if (!make_common_maps(&maps, a.xq, a.wq, a.M, a.N, a.K, a.E, &err)) {
-    set_error(std::string(op) + ": " + err);
-    return 4;
-  }
-  maps.lb = maps.w;
-  maps.h = maps.x[0];
   Params p = {};
   p.xs = a.xs;
   p.ws = a.ws;
@@ -1184,12 +1353,18 @@ int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl) {
     set_error(std::string(op) + ": too many output tiles");
     return 2;
   }
-  p.n_wb = static_cast<int>(wb1);
-  if (ub1 <= dev.sm_count) {
-    p.tok_cap = static_cast<int>(std::min<int64_t>((a.M + 15) / 16 * 16, SPLIT_TOK));
-    return launch_split<false>(op, maps, p, static_cast<int>(ub1), dev, stream, pdl);
+  const bool split = ub1 <= dev.sm_count;
+  const bool pairs = !split && a.M / live >= 48;
+  p.tok_cap = split ? static_cast<int>(std::min<int64_t>((a.M + 15) / 16 * 16, SPLIT_TOK)) : 128;
+  std::string err;
+  Maps maps = {};
+  if (!make_common_maps(&maps, p.tok_cap / 16, a.xq, a.wq, a.M, a.N, a.K, a.E, &err)) {
+    set_error(std::string(op) + ": " + err);
+    return 4;
   }
-  if (a.M / live < 48) return launch_persist<1, false>(op, maps, p, ub1, dev, stream, pdl);
+  p.n_wb = static_cast<int>(wb1);
+  if (split) return launch_split<false>(op, maps, p, static_cast<int>(ub1), dev, stream, pdl);
+  if (!pairs) return launch_persist<1, false>(op, maps, p, ub1, dev, stream, pdl);
   const int64_t wb2 = (a.N + 2 * WROWS - 1) / (2 * WROWS);
   p.n_wb = static_cast<int>(wb2);
   return launch_persist<2, false>(op, maps, p, wb2 * (live + a.M / 256), dev, stream, pdl);
@@ -1200,22 +1375,9 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   const char *op = "fp8_linear_lora";
   DeviceInfo dev;
   if (!check_device(op, &dev)) return 5;
-  std::string err;
-  Maps maps;
   const LoraWorkspace w = lora_workspace(a.workspace, a.M, a.R);
   const int64_t rp = lora_rank_pad(a.R);
   const bool few = a.M <= kLoraRowsMaxM;
-  const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  bool ok = make_common_maps(&maps, a.xq, a.wq, a.M, a.N, a.K, 1, &err);
-  ok = ok &&
-       make_tmap_3d_sw128(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2, 64, WROWS,
-                          &err) &&
-       make_tmap_2d_sw128(&maps.h, t16, w.hl, 2 * rp, a.M + 1, 4 * rp, 64, 1, &err);
-  if (!ok) {
-    set_error(std::string(op) + ": " + err);
-    return 4;
-  }
   Params p = {};
   p.xs = a.xs;
   p.ws = a.ws;
@@ -1235,27 +1397,38 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   p.L = static_cast<int>(a.L);
   p.R = static_cast<int>(a.R);
   p.rank_pad = static_cast<int>(rp);
-  p.count = w.count;
-  p.list = w.list;
+  p.plan = w.plan;
   p.hl = w.hl;
   p.hscale = w.hscale;
-  if (few) {
-    const int64_t wb = (a.N + WROWS - 1) / WROWS;
-    if (wb > 0x3fffffLL) {
-      set_error(std::string(op) + ": too many output tiles");
-      return 2;
-    }
-    p.n_wb = static_cast<int>(wb);
-    p.tok_cap = static_cast<int>((a.M + 15) / 16 * 16);
-    return launch_split<true>(op, maps, p, static_cast<int>(wb), dev, stream, pdl);
-  }
-  const int64_t wb = (a.N + 2 * WROWS - 1) / (2 * WROWS);
-  const int64_t tiles = wb * lora_tiles(a.M);
+  const int rows = few ? WROWS : 2 * WROWS;
+  const int64_t wb = (a.N + rows - 1) / rows;
+  // the plan's tiles at most (and every product within int32)
+  const int64_t tiles =
+      wb * (few ? (a.M + SPLIT_LORA_TOK - 1) / SPLIT_LORA_TOK : lora_plan_max(a.M));
   if (tiles > 0x3fffffffLL) {
     set_error(std::string(op) + ": too many output tiles");
     return 2;
   }
   p.n_wb = static_cast<int>(wb);
+  p.tok_cap = few ? static_cast<int>(std::min<int64_t>((a.M + 15) / 16 * 16, SPLIT_LORA_TOK))
+                  : kLoraTileTokens;
+  std::string err;
+  Maps maps = {};
+  const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  bool ok = make_common_maps(&maps, few ? p.tok_cap / 16 : H_MAPS, a.xq, a.wq, a.M, a.N, a.K, 1,
+                             &err);
+  ok = ok && make_tmap_3d_sw128(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2, 64,
+                                WROWS, &err);
+  if (!few) {
+    for (int i = 0; ok && i < H_MAPS; ++i)
+      ok = make_tmap_2d_sw128(&maps.h[i], t16, w.hl, 2 * rp, a.M, 4 * rp, 64, 16 * (i + 1), &err);
+  }
+  if (!ok) {
+    set_error(std::string(op) + ": " + err);
+    return 4;
+  }
+  if (few) return launch_split<true>(op, maps, p, static_cast<int>(tiles), dev, stream, pdl);
   return launch_persist<2, true>(op, maps, p, tiles, dev, stream, pdl);
 }
 

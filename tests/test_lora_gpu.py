@@ -93,17 +93,11 @@ def test_ids_outside_the_adapters_mean_none(M):
 
 @pytest.mark.parametrize("M", [3, 128, 160, 700])
 def test_one_request_does_not_reach_anothers_rows(M):
-    """Infinities and NaN in an adapter or a row stay with that adapter's rows or that row.
-
-    The other requests' rows keep the bound of the clean call, not its bits: tensor cores
-    multiply an adapter's B with zeros for the tile's other tokens, and sums that 0 * inf or
-    0 * NaN spoiled are computed again as one fp32 FMA chain over the rank. R such steps lose
-    at most R * 2^-24 of the magnitudes' sum, which (R + 16) * 2^-23 of lora_ref covers."""
+    """Infinities and NaN in an adapter or a row stay with that adapter's rows or that row."""
     x, wq, ws, a, b, sc, bias = make(M, M, 160, 264, 3, 16, bias=torch.bfloat16)
     ids = torch.arange(M, device="cuda", dtype=torch.int32) * 3 // M
     good = f.fp8_linear_lora(x, wq, ws, a, b, ids, sc, bias)
-    ref, err = lora_ref(x, wq, ws, a, b, ids, sc, bias)
-    check(good, ref, err)
+    check(good, *lora_ref(x, wq, ws, a, b, ids, sc, bias))
     for where in ("a", "b", "scaling"):
         a2, b2, s2 = a.clone(), b.clone(), sc.clone()
         if where == "a":
@@ -115,9 +109,7 @@ def test_one_request_does_not_reach_anothers_rows(M):
         got = f.fp8_linear_lora(x, wq, ws, a2, b2, ids, s2, bias)
         hit = ids == 1
         assert not torch.isfinite(got[hit]).any()
-        check(got[~hit], ref[~hit], err[~hit])
-        if where != "b":
-            assert torch.equal(got[~hit], good[~hit])
+        assert torch.equal(got[~hit], good[~hit])
     x2 = x.clone()
     x2[0, 5] = float("nan")  # ignored by the quantizer's maximum, not by the adapter
     got = f.fp8_linear_lora(x2, wq, ws, a, b, ids, sc, bias)

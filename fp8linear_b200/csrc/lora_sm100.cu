@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int pitch = p.rank_pad + 1;  // odd: a column of it hits all banks
 
   ptx::grid_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
   const int cluster = static_cast<int>(blockIdx.x) / p.split;
   const int m0 = cluster / p.par * ROWS;
@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = *const_cast<volatile uint32_t *>(&s_slot);
+  const uint32_t tmem = static_cast<uint32_t>(
+      ptx::uniform(static_cast<int>(*const_cast<volatile uint32_t *>(&s_slot))));
   bool first = false;
   if (me < ROWS) {
     int f;
@@ -215,41 +216,44 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int ps = ps0; ps < passes && ok; ps += p.par) {
-        const int nd = min(per_pass, distinct - ps * per_pass);
-        const uint32_t idesc = ptx::idesc_f16_f32(ROWS, nd * p.rank_pad, p.dtype == kBF16);
-        if (ps > ps0 && !ptx::mbar_wait_bounded(
-                            bar_free, static_cast<uint32_t>((ps - ps0) / p.par - 1) & 1u, abort,
-                            kWaitLimitNs)) {
-          record_timeout(abort);
-          break;
-        }
-        ptx::tc_fence_after();
-        for (int i = 0; i < nkb; ++i) {
-          if (!ptx::mbar_wait_bounded(bar_full + 8 * stage, phase, abort, kWaitLimitNs)) {
-            record_timeout(abort);
-            ok = false;
-            break;
-          }
-          ptx::tc_fence_after();
-          const uint32_t st = sbase + static_cast<uint32_t>(stage) * stage_bytes;
-          const uint64_t adesc = ptx::sw128_kmajor_desc(st);
-          const uint64_t bdesc = ptx::sw128_kmajor_desc(st + x_stage);
+    // The whole warp goes through the loop, one elected lane issues: the MMAs' operands stay
+    // in uniform registers.
+    const bool elected = ptx::elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+      const bool got = ptx::mbar_wait_bounded(bar, parity, abort, kWaitLimitNs);
+      if (!__all_sync(0xFFFFFFFFu, got)) {
+        if (elected) record_timeout(abort);
+        return false;
+      }
+      ptx::tc_fence_after();
+      return true;
+    };
+    for (int ps = ps0; ps < passes && ok; ps += p.par) {
+      const int nd = ptx::uniform(min(per_pass, distinct - ps * per_pass));
+      const uint32_t idesc = ptx::idesc_f16_f32(ROWS, nd * p.rank_pad, p.dtype == kBF16);
+      if (ps > ps0 && !wait(bar_free, static_cast<uint32_t>((ps - ps0) / p.par - 1) & 1u)) break;
+      for (int i = 0; i < nkb; ++i) {
+        if (!(ok = wait(bar_full + 8 * stage, phase))) break;
+        const uint32_t st = sbase + static_cast<uint32_t>(stage) * stage_bytes;
+        const uint64_t adesc = ptx::sw128_kmajor_desc(st);
+        const uint64_t bdesc = ptx::sw128_kmajor_desc(st + x_stage);
+        if (elected) {
 #pragma unroll
           for (int kk = 0; kk < KB / 16; ++kk)
             ptx::mma_f16<1>(tmem, adesc + 2 * kk, bdesc + 2 * kk, idesc, (i | kk) != 0 ? 1u : 0u);
           ptx::mma_commit(bar_empty + 8 * stage);
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
         }
-        if (ok) ptx::mma_commit(bar_acc);
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
+      if (ok && elected) ptx::mma_commit(bar_acc);
+    }
+    if (elected) {
       ptx::mma_commit(bar_drain);
       ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
     }

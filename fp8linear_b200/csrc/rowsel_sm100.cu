@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
   int *g_row = reinterpret_cast<int *>(smem + C::OFF_TAB);
   int *g_tile = g_row + C::TAB;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = ptx::uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? ptx::cluster_ctarank() : 0u;  // 0 = leader (issues MMAs)
   const bool leader = rank == 0;
@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
   __syncthreads();
   if constexpr (CG == 2) ptx::cluster_sync();  // peer barriers initialised before any signal
   ptx::tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = static_cast<uint32_t>(ptx::uniform(static_cast<int>(*tmem_slot)));
 
   if (!LORA && p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
   if (p.pdl) ptx::grid_dependency_wait();
@@ -606,7 +606,11 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0 && leader) {
+    // The whole warp goes through the loop, one elected lane issues: in a branch of one lane
+    // the operands of every MMA go through per-thread registers first, about 125 cycles an
+    // MMA whatever its N (tiles of 16 tokens took the time of tiles of 256).
+    if (leader) {
+      const bool elected = ptx::elect_one();
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;
@@ -614,83 +618,88 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
       bool ok = true;
       auto next_stage = [&]() {
         // the stage is reusable (in both CTAs) once its MMAs have read it
-        if constexpr (CG == 1)
-          ptx::mma_commit(bar_empty + 8 * stage);
-        else
-          ptx::mma_commit_pair_mc(bar_empty + 8 * stage, 0x3);
+        if (elected) {
+          if constexpr (CG == 1)
+            ptx::mma_commit(bar_empty + 8 * stage);
+          else
+            ptx::mma_commit_pair_mc(bar_empty + 8 * stage, 0x3);
+        }
         if (++stage == C::STAGES) {
           stage = 0;
           phase ^= 1u;
         }
       };
-      auto wait_full = [&]() -> bool {
-        if (!ptx::mbar_wait_bounded(bar_full + 8 * stage, phase, abort, kWaitLimitNs)) {
-          record_timeout(abort);
+      // (every lane waits; a wait that runs out does so for all)
+      auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        const bool got = ptx::mbar_wait_bounded(bar, parity, abort, kWaitLimitNs);
+        if (!__all_sync(0xFFFFFFFFu, got)) {
+          if (elected) record_timeout(abort);
           return false;
         }
         ptx::tc_fence_after();
         return true;
       };
-      for (int t = group; t < num_tiles && ok; t += n_groups, ++it) {
+      for (int t = group; t < num_tiles; t += n_groups, ++it) {
         const Tile q = tile_at(t, e);
+        const int nn = ptx::uniform(q.nn);
         const int acc = it & 1;
         const uint32_t acc_phase = (it >> 1) & 1;
-        if (!ptx::mbar_wait_bounded(bar_tempty + 8 * acc, acc_phase ^ 1u, abort, kWaitLimitNs)) {
-          record_timeout(abort);
-          break;
-        }
-        ptx::tc_fence_after();
+        if (!wait(bar_tempty + 8 * acc, acc_phase ^ 1u)) break;
         const uint32_t d = tmem_base + (acc ? C::ACC1 : 0u);
-        const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS * CG, q.nn);
+        const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS * CG, nn);
         for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!(ok = wait_full())) break;
+          if (!(ok = wait(bar_full + 8 * stage, phase))) break;
           const uint32_t st = sbase + static_cast<uint32_t>(stage) * C::STAGE;
           const uint64_t adesc = ptx::sw128_kmajor_desc(st);
           const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
+          if (elected) {
 #pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-            const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
-            const uint32_t accumulate = (kb | kk) != 0 ? 1u : 0u;
-            if constexpr (CG == 1)
-              ptx::mma_f8f6f4(d, adesc + koff, bdesc + koff, idesc, accumulate);
-            else
-              ptx::mma_f8f6f4_pair(d, adesc + koff, bdesc + koff, idesc, accumulate);
+            for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+              const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
+              const uint32_t accumulate = (kb | kk) != 0 ? 1u : 0u;
+              if constexpr (CG == 1)
+                ptx::mma_f8f6f4(d, adesc + koff, bdesc + koff, idesc, accumulate);
+              else
+                ptx::mma_f8f6f4_pair(d, adesc + koff, bdesc + koff, idesc, accumulate);
+            }
           }
           next_stage();
         }
         if constexpr (LORA) {
-          if (ok && q.adapter >= 0) {
+          const int adapter = ptx::uniform(q.adapter);
+          if (ok && adapter >= 0) {
             // the third accumulator is free once the epilogue of the tile before has let
             // its own go (the same arrival that this loop waits for one tile later)
-            if (it > 0 && !ptx::mbar_wait_bounded(bar_tempty + 8 * (acc ^ 1),
-                                                  static_cast<uint32_t>((it - 1) >> 1) & 1u, abort,
-                                                  kWaitLimitNs)) {
-              record_timeout(abort);
+            if (it > 0 &&
+                !wait(bar_tempty + 8 * (acc ^ 1), static_cast<uint32_t>((it - 1) >> 1) & 1u))
               break;
-            }
-            ptx::tc_fence_after();
-            const uint32_t id16 = ptx::idesc_f16_f32(WROWS * CG, q.nn, p.lora_dtype == kBF16);
+            const uint32_t id16 = ptx::idesc_f16_f32(WROWS * CG, nn, p.lora_dtype == kBF16);
             const int per = lora_stages(p);
             for (int j = 0; j < per; ++j) {
-              if (!(ok = wait_full())) break;
-              lora_mma<CG>(p, tmem_base + C::ACC_L, sbase + static_cast<uint32_t>(stage) * C::STAGE,
-                           id16, j);
+              if (!(ok = wait(bar_full + 8 * stage, phase))) break;
+              if (elected)
+                lora_mma<CG>(p, tmem_base + C::ACC_L,
+                             sbase + static_cast<uint32_t>(stage) * C::STAGE, id16, j);
               next_stage();
             }
           }
         }
         if (!ok) break;
-        if constexpr (CG == 1)
-          ptx::mma_commit(bar_tfull + 8 * acc);
-        else
-          ptx::mma_commit_pair_mc(bar_tfull + 8 * acc, 0x3);
+        if (elected) {
+          if constexpr (CG == 1)
+            ptx::mma_commit(bar_tfull + 8 * acc);
+          else
+            ptx::mma_commit_pair_mc(bar_tfull + 8 * acc, 0x3);
+        }
       }
       // No MMA may still be running when the CTAs free TMEM.
-      if constexpr (CG == 1)
-        ptx::mma_commit(bar_drain);
-      else
-        ptx::mma_commit_pair(bar_drain);
-      ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
+      if (elected) {
+        if constexpr (CG == 1)
+          ptx::mma_commit(bar_drain);
+        else
+          ptx::mma_commit_pair(bar_drain);
+        ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
+      }
     }
   } else if (LORA && warp == 2 + EPI_WARPS) {
     // ------------------------------------------------------------ B boxes of mixed tiles
@@ -893,7 +902,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
   float *e_b = e_ws + WROWS;
   float *e_hs = e_b + WROWS;  // [SPLIT_TOK]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
   const int stages = p.stages;
   const uint32_t stage_bytes = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
@@ -951,7 +960,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = static_cast<uint32_t>(ptx::uniform(static_cast<int>(*tmem_slot)));
   ptx::cluster_arrive_release();  // (waited for before the first push: all CTAs have started)
   if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -995,32 +1004,37 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
                                static_cast<uint32_t>(i / stages) & 1u, kDrainLimitNs);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = true;
-      const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS, q.nn);
-      int s = 0;
-      uint32_t ph = 0;
-      for (int i = 0; i < nkb; ++i) {
-        if (!ptx::mbar_wait_bounded(bar_full + 8 * s, ph, abort, kWaitLimitNs)) {
-          record_timeout(abort);
-          ok = false;
-          break;
-        }
-        ptx::tc_fence_after();
-        const uint32_t st = sbase + static_cast<uint32_t>(s) * stage_bytes;
-        const uint64_t adesc = ptx::sw128_kmajor_desc(st);
-        const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
+    // (the whole warp, one elected lane issues: see persist_kernel)
+    const bool elected = ptx::elect_one();
+    bool ok = true;
+    const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS, ptx::uniform(q.nn));
+    int s = 0;
+    uint32_t ph = 0;
+    for (int i = 0; i < nkb; ++i) {
+      const bool got = ptx::mbar_wait_bounded(bar_full + 8 * s, ph, abort, kWaitLimitNs);
+      if (!__all_sync(0xFFFFFFFFu, got)) {
+        if (elected) record_timeout(abort);
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after();
+      const uint32_t st = sbase + static_cast<uint32_t>(s) * stage_bytes;
+      const uint64_t adesc = ptx::sw128_kmajor_desc(st);
+      const uint64_t bdesc = ptx::sw128_kmajor_desc(st + W_STAGE);
+      if (elected) {
 #pragma unroll
         for (int kk = 0; kk < BK / UMMA_K; ++kk) {
           const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
           ptx::mma_f8f6f4(tmem, adesc + koff, bdesc + koff, idesc, (i | kk) != 0 ? 1u : 0u);
         }
         ptx::mma_commit(bar_empty + 8 * s);
-        if (++s == stages) {
-          s = 0;
-          ph ^= 1u;
-        }
       }
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1u;
+      }
+    }
+    if (elected) {
       if (ok) ptx::mma_commit(bar_acc);
       ptx::mma_commit(bar_drain);
       ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);

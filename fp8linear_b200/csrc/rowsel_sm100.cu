@@ -736,21 +736,29 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
       const uint32_t acc_phase = (it >> 1) & 1;
       const int cnt = q.t1 - q.t0;
       const int n0 = (q.wb * CG + static_cast<int>(rank)) * WROWS + quarter * 32;
-      __syncwarp();
-      for (int i = lane; i < ((cnt + 31) & ~31); i += 32) {
-        e_xs[i] = i < cnt ? __ldg(p.xs + q.t0 + i) : 0.0f;
-        if constexpr (LORA) {
-          const bool has =
-              q.adapter >= 0 ? i < cnt : q.adapter == -2 && token_id(p, q.t0 + i, q.t1) >= 0;
-          e_hs[i] = has ? __ldg(p.hscale + q.t0 + i) : 0.0f;
-        }
-      }
+      // all loads at once, then to shared memory: one latency a tile (in a loop that stored
+      // each before the next it took 7000 cycles a tile, more than its main loop)
       float w[4], b[4];  // of columns fi + 8k
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int64_t wn = static_cast<int64_t>(q.e) * p.N + min(n0 + fi + 8 * k, p.N - 1);
         w[k] = __ldg(p.ws + wn);
         b[k] = load_bias(p.bias, p.bias_dtype, wn);
+      }
+      float xs[C::TOK_MAX / 32], hs[C::TOK_MAX / 32];
+#pragma unroll
+      for (int k = 0; k < C::TOK_MAX / 32; ++k) {
+        const int i = 32 * k + lane;
+        xs[k] = i < cnt ? __ldg(p.xs + q.t0 + i) : 0.0f;
+        hs[k] = LORA && q.adapter >= 0 && i < cnt ? __ldg(p.hscale + q.t0 + i) : 0.0f;
+      }
+      if (LORA && q.adapter == -2 && token_id(p, q.t0 + lane, q.t1) >= 0)  // (at most 32)
+        hs[0] = __ldg(p.hscale + q.t0 + lane);
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < C::TOK_MAX / 32; ++k) {
+        e_xs[32 * k + lane] = xs[k];
+        if constexpr (LORA) e_hs[32 * k + lane] = hs[k];
       }
       __syncwarp();
       float2 sum[kLoraMixed / 8][4];  // a mixed tile's adapter sums, [g][k] as v below

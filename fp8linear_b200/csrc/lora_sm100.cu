@@ -74,6 +74,17 @@ __device__ __forceinline__ void record_timeout(volatile int *abort) {
   }
 }
 
+// A whole warp waits; copies and MMAs go out from one elected lane of it (operands in uniform
+// registers).
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort,
+                                          bool elected) {
+  if (__all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(bar, parity))) return true;
+  const bool got = ptx::mbar_wait_bounded(bar, parity, abort, kWaitLimitNs);
+  if (__all_sync(0xFFFFFFFFu, got)) return true;
+  if (elected) record_timeout(abort);
+  return false;
+}
+
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     down_tile_kernel(const __grid_constant__ CUtensorMap tmap_x,
                      const __grid_constant__ CUtensorMap tmap_a,
@@ -177,57 +188,51 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int nkb = min(p.k_blocks, kb0 + p.kps) - kb0;  // >= 1 (the host's split)
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t issued = 0;
-      bool ok = true;
-      for (int ps = ps0; ps < passes && ok; ps += p.par) {
-        const int d0 = ps * per_pass, nd = min(per_pass, distinct - d0);
-        for (int i = 0; i < nkb; ++i) {
-          if (!ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort, kWaitLimitNs)) {
-            record_timeout(abort);
-            ok = false;
-            break;
-          }
-          const uint32_t fb = bar_full + 8 * stage;
-          const uint32_t dst = sbase + static_cast<uint32_t>(stage) * stage_bytes;
+    const bool elected = ptx::elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t issued = 0;
+    bool ok = true;
+    for (int ps = ps0; ps < passes && ok; ps += p.par) {
+      const int d0 = ps * per_pass, nd = min(per_pass, distinct - d0);
+      for (int i = 0; i < nkb; ++i) {
+        if (!(ok = warp_wait(bar_empty + 8 * stage, phase ^ 1u, abort, elected))) break;
+        const uint32_t fb = bar_full + 8 * stage;
+        const uint32_t dst = sbase + static_cast<uint32_t>(stage) * stage_bytes;
+        if (elected) {
           ptx::mbar_arrive_expect_tx(fb, x_stage + static_cast<uint32_t>(nd * p.rank_pad) * 128u);
           ptx::tma_load_2d(dst, &tmap_x, (kb0 + i) * KB, m0, fb);
-          for (int d = 0; d < nd; ++d)  // ranks past R read as zero
+        }
+        for (int d = 0; d < nd; ++d) {  // ranks past R read as zero
+          const int a = ptx::uniform(s_list[d0 + d]);
+          if (elected)
             ptx::tma_load_3d(dst + x_stage + static_cast<uint32_t>(d * p.rank_pad) * 128u, &tmap_a,
-                             (kb0 + i) * KB, 0, s_list[d0 + d], fb);
-          ++issued;
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+                             (kb0 + i) * KB, 0, a, fb);
         }
-      }
-      const uint32_t n_drain = min(issued, static_cast<uint32_t>(stages));
-      for (uint32_t i = 0; i < n_drain; ++i) {
-        if (stage == 0) {
-          stage = stages - 1;
+        ++issued;
+        if (++stage == stages) {
+          stage = 0;
           phase ^= 1u;
-        } else {
-          --stage;
         }
-        ptx::mbar_wait_timeout(bar_empty + 8 * stage, phase, kDrainLimitNs);
       }
     }
+    const uint32_t n_drain = min(issued, static_cast<uint32_t>(stages));
+    for (uint32_t i = 0; i < n_drain; ++i) {
+      if (stage == 0) {
+        stage = stages - 1;
+        phase ^= 1u;
+      } else {
+        --stage;
+      }
+      ptx::mbar_wait_timeout(bar_empty + 8 * stage, phase, kDrainLimitNs);
+    }
   } else if (warp == 1) {
-    // The whole warp goes through the loop, one elected lane issues: the MMAs' operands stay
-    // in uniform registers.
     const bool elected = ptx::elect_one();
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
-      const bool got = ptx::mbar_wait_bounded(bar, parity, abort, kWaitLimitNs);
-      if (!__all_sync(0xFFFFFFFFu, got)) {
-        if (elected) record_timeout(abort);
-        return false;
-      }
+      if (!warp_wait(bar, parity, abort, elected)) return false;
       ptx::tc_fence_after();
       return true;
     };

@@ -114,6 +114,19 @@ __device__ __forceinline__ void record_timeout(volatile int *abort) {
   }
 }
 
+// A whole warp waits for a barrier's phase. The roles that issue TMA copies and MMAs keep the
+// warp converged and issue from one elected lane: in a branch of one lane the operands of each
+// copy or MMA go through per-thread registers first, which made an MMA take 125 cycles
+// whatever its N and a stage's two copies 400.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort,
+                                          bool elected) {
+  if (__all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(bar, parity))) return true;
+  const bool got = ptx::mbar_wait_bounded(bar, parity, abort, kWaitLimitNs);
+  if (__all_sync(0xFFFFFFFFu, got)) return true;
+  if (elected) record_timeout(abort);
+  return false;
+}
+
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // The groups' rows and tiles, in shared memory: row[e] .. row[e + 1] are the rows of group e,
@@ -318,6 +331,7 @@ __device__ __forceinline__ int token_id(const Params &p, int i, int end) {
 __device__ __forceinline__ bool feed_sums(const Params &p, const CUtensorMap *map, SumRing &ring,
                                           int t0, int t1, int n0) {
   const int lane = threadIdx.x & 31;
+  const bool elected = ptx::elect_one();
   int next = token_id(p, t0 + (lane & 7), t1);
   for (int i = t0; i < t1; i += 8) {
     const int id = next;
@@ -326,19 +340,13 @@ __device__ __forceinline__ bool feed_sums(const Params &p, const CUtensorMap *ma
       const int a = __shfl_sync(0xFFFFFFFFu, id, __ffs(static_cast<int>(todo)) - 1);
       for (int rc = 0; rc < p.R; rc += SUM_RANK) {
         const uint32_t s = ring.count % SUM_SLOTS;
-        int ok = 1;
-        if (lane == 0) {
-          if (ptx::mbar_wait_bounded(ring.bars + 8 * (SUM_SLOTS + s),
-                                     (ring.count / SUM_SLOTS & 1u) ^ 1u, ring.abort,
-                                     kWaitLimitNs)) {
-            ptx::mbar_arrive_expect_tx(ring.bars + 8 * s, W_STAGE);
-            ptx::tma_load_3d(ring.slots + s * W_STAGE, map, rc, n0, a, ring.bars + 8 * s);
-          } else {
-            record_timeout(ring.abort);
-            ok = 0;
-          }
+        if (!warp_wait(ring.bars + 8 * (SUM_SLOTS + s), (ring.count / SUM_SLOTS & 1u) ^ 1u, ring.abort,
+                       elected))
+          return false;
+        if (elected) {
+          ptx::mbar_arrive_expect_tx(ring.bars + 8 * s, W_STAGE);
+          ptx::tma_load_3d(ring.slots + s * W_STAGE, map, rc, n0, a, ring.bars + 8 * s);
         }
-        if (__shfl_sync(0xFFFFFFFFu, ok, 0) == 0) return false;
         ++ring.count;
       }
     }
@@ -542,73 +550,69 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t issued = 0;
-      int e = 0;
-      bool ok = true;
-      for (int t = group; t < num_tiles && ok; t += n_groups) {
-        const Tile q = tile_at(t, e);
-        const int wrow = (q.wb * CG + static_cast<int>(rank)) * WROWS;
-        const int xrows = q.nn / CG;
-        const int xrow = q.t0 + static_cast<int>(rank) * xrows;
-        const uint32_t tx = CG * W_STAGE + static_cast<uint32_t>(q.nn) * BK;
-        // One stage: the weight box and the token box at the given coordinates.
-        auto load = [&](const CUtensorMap *mw, int wx, int wz, const CUtensorMap *mx, int xx) {
-          if (!ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort, kWaitLimitNs)) {
-            record_timeout(abort);
-            return false;
-          }
-          const uint32_t fb = bar_full + 8 * stage;
-          const uint32_t dst = sbase + static_cast<uint32_t>(stage) * C::STAGE;
+    const bool elected = ptx::elect_one();
+    // both CTAs' bytes of a stage complete the leader's barrier
+    const uint32_t full_leader = CG == 1 ? bar_full : ptx::map_shared_rank(bar_full, 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t issued = 0;
+    int e = 0;
+    bool ok = true;
+    for (int t = group; t < num_tiles && ok; t += n_groups) {
+      const Tile q = tile_at(t, e);
+      const int nn = ptx::uniform(q.nn);
+      const int wz = ptx::uniform(q.e);
+      const int wrow = (ptx::uniform(q.wb) * CG + static_cast<int>(rank)) * WROWS;
+      const int xrow = ptx::uniform(q.t0) + static_cast<int>(rank) * (nn / CG);
+      const int mi = nn / CG / 16 - 1;
+      const uint32_t tx = CG * W_STAGE + static_cast<uint32_t>(nn) * BK;
+      // One stage: the weight box and the token box at the given coordinates.
+      auto load = [&](const CUtensorMap *mw, int wx, int z, const CUtensorMap *mx, int xx) {
+        if (!warp_wait(bar_empty + 8 * stage, phase ^ 1u, abort, elected)) return false;
+        const uint32_t dst = sbase + static_cast<uint32_t>(stage) * C::STAGE;
+        const uint32_t fl = full_leader + 8 * stage;
+        if (elected) {
+          if (leader) ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, tx);
           if constexpr (CG == 1) {
-            ptx::mbar_arrive_expect_tx(fb, tx);
-            ptx::tma_load_3d(dst, mw, wx, wrow, wz, fb);
-            ptx::tma_load_2d(dst + W_STAGE, mx, xx, xrow, fb);
+            ptx::tma_load_3d(dst, mw, wx, wrow, z, fl);
+            ptx::tma_load_2d(dst + W_STAGE, mx, xx, xrow, fl);
           } else {
-            // both CTAs' bytes complete the leader's barrier; only the leader arms it
-            if (leader) ptx::mbar_arrive_expect_tx(fb, tx);
-            const uint32_t fl = ptx::map_shared_rank(fb, 0);
-            ptx::tma_load_3d_pair(dst, mw, wx, wrow, wz, fl);
+            ptx::tma_load_3d_pair(dst, mw, wx, wrow, z, fl);
             ptx::tma_load_2d_pair(dst + W_STAGE, mx, xx, xrow, fl);
           }
-          ++issued;
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
-          return true;
-        };
-        const int mi = xrows / 16 - 1;
-        for (int kb = 0; kb < p.k_blocks && ok; ++kb)
-          ok = load(&maps.w, kb * BK, q.e, &maps.x[mi], kb * BK);
-        if constexpr (LORA) {
-          const int per = q.adapter >= 0 ? lora_stages(p) : 0;
-          for (int j = 0; j < per && ok; ++j) {
-            int bx, hx;
-            lora_columns(p, j, bx, hx);
-            ok = load(&maps.lb, bx, q.adapter, &maps.h[mi], hx);
-          }
         }
-      }
-      // Drain: every load issued here has landed and been consumed.
-      const uint32_t n_drain = issued < C::STAGES ? issued : C::STAGES;
-      for (uint32_t i = 0; i < n_drain; ++i) {
-        if (stage == 0) {
-          stage = C::STAGES - 1;
+        ++issued;
+        if (++stage == C::STAGES) {
+          stage = 0;
           phase ^= 1u;
-        } else {
-          --stage;
         }
-        ptx::mbar_wait_timeout(bar_empty + 8 * stage, phase, kDrainLimitNs);
+        return true;
+      };
+      for (int kb = 0; kb < p.k_blocks && ok; ++kb)
+        ok = load(&maps.w, kb * BK, wz, &maps.x[mi], kb * BK);
+      if constexpr (LORA) {
+        const int adapter = ptx::uniform(q.adapter);
+        const int per = adapter >= 0 ? lora_stages(p) : 0;
+        for (int j = 0; j < per && ok; ++j) {
+          int bx, hx;
+          lora_columns(p, j, bx, hx);
+          ok = load(&maps.lb, bx, adapter, &maps.h[mi], hx);
+        }
       }
+    }
+    // Drain: every load issued here has landed and been consumed.
+    const uint32_t n_drain = issued < C::STAGES ? issued : C::STAGES;
+    for (uint32_t i = 0; i < n_drain; ++i) {
+      if (stage == 0) {
+        stage = C::STAGES - 1;
+        phase ^= 1u;
+      } else {
+        --stage;
+      }
+      ptx::mbar_wait_timeout(bar_empty + 8 * stage, phase, kDrainLimitNs);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    // The whole warp goes through the loop, one elected lane issues: in a branch of one lane
-    // the operands of every MMA go through per-thread registers first, about 125 cycles an
-    // MMA whatever its N (tiles of 16 tokens took the time of tiles of 256).
     if (leader) {
       const bool elected = ptx::elect_one();
       int stage = 0;
@@ -629,13 +633,8 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
           phase ^= 1u;
         }
       };
-      // (every lane waits; a wait that runs out does so for all)
       auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
-        const bool got = ptx::mbar_wait_bounded(bar, parity, abort, kWaitLimitNs);
-        if (!__all_sync(0xFFFFFFFFu, got)) {
-          if (elected) record_timeout(abort);
-          return false;
-        }
+        if (!warp_wait(bar, parity, abort, elected)) return false;
         ptx::tc_fence_after();
         return true;
       };
@@ -946,21 +945,23 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
   const int kb0 = rank * p.kps;
   const int nkb = min(p.k_blocks, kb0 + p.kps) - kb0;  // >= 1 (the host's split)
   const int cnt = q.t1 - q.t0;
-  const CUtensorMap *mx = &maps.x[q.nn / 16 - 1];
-  const uint32_t tx = W_STAGE + static_cast<uint32_t>(q.nn) * BK;
+  const CUtensorMap *mx = &maps.x[ptx::uniform(q.nn) / 16 - 1];
+  const uint32_t tx = W_STAGE + static_cast<uint32_t>(ptx::uniform(q.nn)) * BK;
 
+  const int nn = ptx::uniform(q.nn);
+  const int we = ptx::uniform(q.e), wrow = ptx::uniform(q.wb) * WROWS, xrow = ptx::uniform(q.t0);
   // The first stages' weight boxes go out at once: before the dependency wait where the
   // weights cannot depend on the kernel before (pre_w).
-  auto weights_first = [&]() {
+  if (warp == 0) {
     const int n = min(stages, nkb);
-    for (int i = 0; i < n; ++i) {
-      const uint32_t fb = bar_full + 8 * i;
-      ptx::mbar_arrive_expect_tx(fb, tx);
-      ptx::tma_load_3d(sbase + static_cast<uint32_t>(i) * stage_bytes, &maps.w, (kb0 + i) * BK,
-                       q.wb * WROWS, q.e, fb);
-    }
-  };
-  if (threadIdx.x == 0) weights_first();
+    if (ptx::elect_one())
+      for (int i = 0; i < n; ++i) {
+        const uint32_t fb = bar_full + 8 * i;
+        ptx::mbar_arrive_expect_tx(fb, tx);
+        ptx::tma_load_3d(sbase + static_cast<uint32_t>(i) * stage_bytes, &maps.w, (kb0 + i) * BK,
+                         wrow, we, fb);
+      }
+  }
   if (warp == 1) {
     ptx::tmem_alloc<1>(ptx::smem_u32(&s_slot), tmem_cols);
     ptx::tmem_relinquish<1>();
@@ -985,46 +986,39 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
   const int a0 = min(cnt, rank * per_cta), a1 = min(cnt, a0 + per_cta);
 
   if (warp == 0) {
-    if (lane == 0) {
-      int issued = 0;
-      int s = 0;
-      uint32_t ph = 1;
-      for (int i = 0; i < nkb; ++i) {
-        const uint32_t fb = bar_full + 8 * s;
-        const uint32_t dst = sbase + static_cast<uint32_t>(s) * stage_bytes;
-        if (i >= stages) {  // (the first stages are armed, their weight boxes under way)
-          if (!ptx::mbar_wait_bounded(bar_empty + 8 * s, ph, abort, kWaitLimitNs)) {
-            record_timeout(abort);
-            break;
-          }
+    const bool elected = ptx::elect_one();
+    int issued = 0;
+    int s = 0;
+    uint32_t ph = 1;
+    for (int i = 0; i < nkb; ++i) {
+      const uint32_t fb = bar_full + 8 * s;
+      const uint32_t dst = sbase + static_cast<uint32_t>(s) * stage_bytes;
+      const bool refill = i >= stages;  // (the first are armed, their weight boxes under way)
+      if (refill && !warp_wait(bar_empty + 8 * s, ph, abort, elected)) break;
+      if (elected) {
+        if (refill) {
           ptx::mbar_arrive_expect_tx(fb, tx);
-          ptx::tma_load_3d(dst, &maps.w, (kb0 + i) * BK, n0, q.e, fb);
+          ptx::tma_load_3d(dst, &maps.w, (kb0 + i) * BK, wrow, we, fb);
         }
-        ptx::tma_load_2d(dst + W_STAGE, mx, (kb0 + i) * BK, q.t0, fb);
-        ++issued;
-        if (++s == stages) {
-          s = 0;
-          ph ^= 1u;
-        }
+        ptx::tma_load_2d(dst + W_STAGE, mx, (kb0 + i) * BK, xrow, fb);
       }
-      for (int i = issued - 1; i >= 0 && i >= issued - stages; --i)
-        ptx::mbar_wait_timeout(bar_empty + 8 * (i % stages),
-                               static_cast<uint32_t>(i / stages) & 1u, kDrainLimitNs);
+      ++issued;
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1u;
+      }
     }
+    for (int i = issued - 1; i >= 0 && i >= issued - stages; --i)
+      ptx::mbar_wait_timeout(bar_empty + 8 * (i % stages), static_cast<uint32_t>(i / stages) & 1u,
+                             kDrainLimitNs);
   } else if (warp == 1) {
-    // (the whole warp, one elected lane issues: see persist_kernel)
     const bool elected = ptx::elect_one();
     bool ok = true;
-    const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS, ptx::uniform(q.nn));
+    const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS, nn);
     int s = 0;
     uint32_t ph = 0;
     for (int i = 0; i < nkb; ++i) {
-      const bool got = ptx::mbar_wait_bounded(bar_full + 8 * s, ph, abort, kWaitLimitNs);
-      if (!__all_sync(0xFFFFFFFFu, got)) {
-        if (elected) record_timeout(abort);
-        ok = false;
-        break;
-      }
+      if (!(ok = warp_wait(bar_full + 8 * s, ph, abort, elected))) break;
       ptx::tc_fence_after();
       const uint32_t st = sbase + static_cast<uint32_t>(s) * stage_bytes;
       const uint64_t adesc = ptx::sw128_kmajor_desc(st);

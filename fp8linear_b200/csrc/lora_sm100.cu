@@ -4,9 +4,9 @@
 // GEMM (rowsel_sm100.cu), which adds h . B^T before its one rounding.
 //
 // tcgen05 (kind::f16) on tiles of 128 rows. All of a tile's adapters stand side by side on the
-// MMA's N side (rank_pad columns each, 128 columns a pass), and each row keeps the columns of
+// MMA's N side (rank_pad columns each, 256 columns a pass), and each row keeps the columns of
 // its own; rows never mix, so an adapter's infinities and NaN stay with its rows. When the
-// tiles are few, a cluster splits K and the passes go to clusters of their own.
+// tiles are few, a cluster splits K.
 //
 // The GEMM's tensor cores take h in x's 16-bit type. h is a sum, so it keeps fp32's accuracy:
 // it goes as a high and a low part, h / hscale = hi + lo (bf16: 2^-17 relative; f16: hscale,
@@ -48,9 +48,9 @@ struct Params {
   int4 *plan;      // null: not wanted
   int split, kps, k_blocks;
   int x_rows;      // rows of x's box
-  int stages;
+  int cols;        // columns per pass
   uint32_t off_part;
-  int par;  // clusters per tile, each with every par-th pass
+  int tiles, clusters, max_passes;
 };
 
 __device__ __forceinline__ bool has_adapter(const Params &p, int id) {
@@ -59,12 +59,12 @@ __device__ __forceinline__ bool has_adapter(const Params &p, int id) {
 
 constexpr int ROWS = 128;
 constexpr int KB = 64;     // 16-bit elements per K-block: one 128-byte swizzle row
-constexpr int COLS = 128;  // columns (adapters x rank_pad) per pass
+constexpr int COLS = 256;  // columns (adapters x rank_pad) per pass, at most
 constexpr int MAX_STAGES = 8;
 constexpr int NUM_THREADS = 224;  // producer, MMA, 4 x TMEM, plan
-constexpr uint32_t A_STAGE = COLS * 128;
 constexpr int MAX_SPLIT = 8;
-// dynamic: the ring of (x_rows + COLS) x 128 bytes, then fp32 [ROWS][rank_pad + 1]
+// dynamic: the ring, cut anew for each item into stages of x_rows + columns rows of 128 bytes,
+// then fp32 [ROWS][rank_pad + 1]
 constexpr uint32_t SMEM_MAX = 232448 - 4096;  // (the static part is below 3 KB)
 
 __device__ __forceinline__ void record_timeout(volatile int *abort) {
@@ -85,6 +85,99 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return false;
 }
 
+// The plan of the GEMM's token tiles, by one warp. A run of at least kLoraMixed (32) rows
+// crosses a border between blocks of 32 rows, so of a block's runs only the one carried in and
+// the one carried on can be long.
+__device__ __forceinline__ void make_plan(const Params &p, int lane) {
+  int n = 0;
+  auto emit = [&](int t0, int t1, int a) {
+    ++n;
+    if (lane == 0) p.plan[n] = make_int4(t0, t1, a, 0);
+  };
+  int open = -1, open_end = 0;  // rows of short runs not yet in a tile
+  auto flush = [&]() {
+    if (open >= 0 && open < open_end) emit(open, open_end, -2);
+    open = -1;
+  };
+  auto add_short = [&](int s, int e) {
+    if (s == e) return;
+    if (open < 0) open = s;
+    open_end = e;
+    for (; open_end - open >= kLoraMixed; open += kLoraMixed) emit(open, open + kLoraMixed, -2);
+    if (open == open_end) open = -1;
+  };
+  auto add_run = [&](int s, int e, int a) {
+    if (e - s < kLoraMixed) {
+      add_short(s, e);
+      return;
+    }
+    flush();
+    const int nt = (e - s + kLoraTileTokens - 1) / kLoraTileTokens;
+    const int per = ((e - s + nt - 1) / nt + 31) / 32 * 32;
+    for (int t = s; t < e; t += per) emit(t, min(e, t + per), a);
+  };
+  int start = 0, cur = -1;  // the run carried on
+  constexpr int AHEAD = 8;  // blocks loaded together, one such batch before it is read
+  int ids[AHEAD], next[AHEAD];
+  auto fetch = [&](int b) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int m = b + 32 * k + lane;
+      next[k] = m < p.M ? __ldg(p.ids + m) : -1;
+    }
+  };
+  fetch(0);
+  for (int b0 = 0; b0 < p.M; b0 += 32 * AHEAD) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) ids[k] = has_adapter(p, next[k]) ? next[k] : -1;
+    fetch(b0 + 32 * AHEAD);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int b = b0 + 32 * k;
+      int before = __shfl_up_sync(0xFFFFFFFFu, ids[k], 1);
+      if (lane == 0) before = cur;
+      const uint32_t edges = __ballot_sync(0xFFFFFFFFu, b + lane < p.M && ids[k] != before);
+      if (edges != 0) {
+        const int first = __ffs(static_cast<int>(edges)) - 1;
+        const int last = 31 - __clz(static_cast<int>(edges));
+        add_run(start, b + first, cur);
+        add_short(b + first, b + last);
+        start = b + last;
+      }
+      cur = __shfl_sync(0xFFFFFFFFu, ids[k], 31);
+    }
+  }
+  // (past M the lanes hold -1; the run's own id is its first row's)
+  const int tail = __ldg(p.ids + min(start, p.M - 1));
+  add_run(start, p.M, has_adapter(p, tail) ? tail : -1);
+  flush();
+  if (lane == 0) p.plan[0] = make_int4(n, 0, 0, 0);
+}
+
+// At most how many adapters the 128 rows from m0 have, by a whole warp: exact where an
+// adapter's rows lie together.
+__device__ __forceinline__ int adapters_at_most(const Params &p, int m0, int lane) {
+  int id[ROWS / 32];
+#pragma unroll
+  for (int j = 0; j < ROWS / 32; ++j) {
+    const int m = m0 + 32 * j + lane;
+    id[j] = m < p.M ? __ldg(p.ids + m) : -1;
+    if (!has_adapter(p, id[j])) id[j] = -1;
+  }
+  int n = 0, before = -1;  // the last row's of the 32 before
+#pragma unroll
+  for (int j = 0; j < ROWS / 32; ++j) {
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, id[j]);
+    n += __popc(__ballot_sync(0xFFFFFFFFu, id[j] >= 0 && id[j] != before &&
+                                               __ffs(static_cast<int>(same)) - 1 == lane));
+    before = __shfl_sync(0xFFFFFFFFu, id[j], 31);
+  }
+  return n;
+}
+
+// Work comes in items (tile of 128 rows, pass over p.cols columns of its adapters). Item (t, ps)
+// is cluster (t + ps) % p.clusters's: a tile of one adapter is its own cluster's only item,
+// the passes of a tile of many (decoding requests) spread over the neighbours.
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     down_tile_kernel(const __grid_constant__ CUtensorMap tmap_x,
                      const __grid_constant__ CUtensorMap tmap_a,
@@ -93,42 +186,43 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = ptx::smem_u32(smem);
-  __shared__ alignas(8) uint64_t s_bar[2 * MAX_STAGES + 3];
+  __shared__ alignas(8) uint64_t s_bar[2 * MAX_STAGES + 2];
   __shared__ uint32_t s_slot;
   __shared__ int s_abort;
   __shared__ alignas(16) int s_id[ROWS];  // adapter of each row, -1: none
   __shared__ int s_first[ROWS];  // the row's adapter appears first at this row of the tile
   __shared__ int s_rank[ROWS];   // .. and is this one of the tile's adapters
   __shared__ int s_list[ROWS];   // the tile's adapters
-  __shared__ int s_count[5];
+  __shared__ int s_count[ROWS / 32];
+  __shared__ int s_todo[ROWS];   // pass ps of tile (cluster - ps) may have work
   const uint32_t bar_full = ptx::smem_u32(s_bar);
   const uint32_t bar_empty = bar_full + 8 * MAX_STAGES;
   const uint32_t bar_acc = bar_empty + 8 * MAX_STAGES;
-  const uint32_t bar_free = bar_acc + 8;
-  const uint32_t bar_drain = bar_free + 8;
+  const uint32_t bar_drain = bar_acc + 8;
   volatile int *abort = &s_abort;
   float *part = reinterpret_cast<float *>(smem + p.off_part);
-  const int stages = p.stages;
   const uint32_t x_stage = static_cast<uint32_t>(p.x_rows) * 128;
-  const uint32_t stage_bytes = x_stage + A_STAGE;
   const int pitch = p.rank_pad + 1;  // odd: a column of it hits all banks
+  const int per_pass = p.cols / p.rank_pad;
 
   ptx::grid_launch_dependents();
   const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
   const int cluster = static_cast<int>(blockIdx.x) / p.split;
-  const int m0 = cluster / p.par * ROWS;
-  const int ps0 = cluster % p.par;
+  // the tile whose pass ps is this cluster's (tiles or above: none)
+  auto tile_of = [&](int ps) {
+    const int t = cluster - ps % p.clusters;
+    return t < 0 ? t + p.clusters : t;
+  };
 
   if (threadIdx.x == 0) {
     ptx::prefetch_tmap(&tmap_x);
     ptx::prefetch_tmap(&tmap_a);
-    for (int s = 0; s < stages; ++s) {
+    for (int s = 0; s < MAX_STAGES; ++s) {
       ptx::mbar_init(bar_full + 8 * s, 1);
       ptx::mbar_init(bar_empty + 8 * s, 1);
     }
     ptx::mbar_init(bar_acc, 1);
-    ptx::mbar_init(bar_free, 4);
     ptx::mbar_init(bar_drain, 1);
     s_abort = 0;
     ptx::fence_mbar_init();
@@ -137,70 +231,84 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     ptx::tmem_alloc<1>(ptx::smem_u32(&s_slot), COLS);
     ptx::tmem_relinquish<1>();
   }
-  // The tile's adapters, in the order of their first rows.
-  const int me = threadIdx.x;
-  if (me < ROWS) {
-    const int id = m0 + me < p.M ? __ldg(p.ids + m0 + me) : -1;
-    s_id[me] = has_adapter(p, id) ? id : -1;
+  for (int ps = warp; ps < p.max_passes; ps += NUM_THREADS / 32) {
+    const int t = tile_of(ps);
+    const int n = t < p.tiles ? adapters_at_most(p, t * ROWS, lane) : 0;
+    if (lane == 0) s_todo[ps] = n > ps * per_pass;
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = static_cast<uint32_t>(
       ptx::uniform(static_cast<int>(*const_cast<volatile uint32_t *>(&s_slot))));
-  bool first = false;
-  if (me < ROWS) {
-    int f;
-    // the lowest row with the same id: within the warp, then among the rows of those before
-    const int id = s_id[me];
-    f = (me & ~31) + __ffs(static_cast<int>(__match_any_sync(0xFFFFFFFFu, id))) - 1;
-    if (id >= 0) {
-#pragma unroll 1
-      for (int j = 0; j < (me & ~31); j += 4) {
-        const int4 v = *reinterpret_cast<const int4 *>(s_id + j);
-        if (v.x == id || v.y == id || v.z == id || v.w == id) {
-          f = v.x == id ? j : v.y == id ? j + 1 : v.z == id ? j + 2 : j + 3;
-          break;
-        }
-      }
-    }
-    first = s_id[me] >= 0 && f == me;
-    s_first[me] = f;
-    const uint32_t votes = __ballot_sync(0xFFFFFFFFu, first);
-    s_rank[me] = __popc(votes & ((1u << lane) - 1u));
-    if (lane == 0) s_count[warp] = __popc(votes);
-  }
-  __syncthreads();
-  int before = 0, distinct = 0;
-  for (int w = 0; w < ROWS / 32; ++w) {
-    if (w < warp) before += s_count[w];
-    distinct += s_count[w];
-  }
-  if (me < ROWS) {
-    s_rank[me] += before;
-    if (first) s_list[s_rank[me]] = s_id[me];
-  }
-  __syncthreads();
 
-  const int per_pass = COLS / p.rank_pad;
-  const int passes = (distinct + per_pass - 1) / per_pass;
   const int kb0 = rank * p.kps;
   const int nkb = min(p.k_blocks, kb0 + p.kps) - kb0;  // >= 1 (the host's split)
+  bool plan_open = p.plan != nullptr && blockIdx.x == 0;  // this CTA's last warp has it to make
+  const bool elected = ptx::elect_one();
+  uint32_t phases = 0;  // bit s: of stage s, in the producer and the MMA warp
+  uint32_t used = 0;       // .. that have been used
+  uint32_t items = 0;
+  bool ok = true;
 
-  if (warp == 0) {
-    const bool elected = ptx::elect_one();
+  for (int ps = 0; ps < p.max_passes; ++ps) {
+    if (s_todo[ps] == 0) continue;
+    const int m0 = tile_of(ps) * ROWS;
+    // The tile's adapters, in the order of their first rows.
+    const int me = threadIdx.x;
+    if (me < ROWS) {
+      const int id = m0 + me < p.M ? __ldg(p.ids + m0 + me) : -1;
+      s_id[me] = has_adapter(p, id) ? id : -1;
+    }
+    __syncthreads();
+    bool first = false;
+    if (me < ROWS) {
+      // the lowest row with the same id: within the warp, then among the rows of those before
+      const int id = s_id[me];
+      int f = (me & ~31) + __ffs(static_cast<int>(__match_any_sync(0xFFFFFFFFu, id))) - 1;
+      if (id >= 0) {
+#pragma unroll 1
+        for (int j = 0; j < (me & ~31); j += 4) {
+          const int4 v = *reinterpret_cast<const int4 *>(s_id + j);
+          if (v.x == id || v.y == id || v.z == id || v.w == id) {
+            f = v.x == id ? j : v.y == id ? j + 1 : v.z == id ? j + 2 : j + 3;
+            break;
+          }
+        }
+      }
+      first = id >= 0 && f == me;
+      s_first[me] = f;
+      const uint32_t votes = __ballot_sync(0xFFFFFFFFu, first);
+      s_rank[me] = __popc(votes & ((1u << lane) - 1u));
+      if (lane == 0) s_count[warp] = __popc(votes);
+    }
+    __syncthreads();
+    int before = 0, distinct = 0;
+#pragma unroll
+    for (int w = 0; w < ROWS / 32; ++w) {
+      if (w < warp) before += s_count[w];
+      distinct += s_count[w];
+    }
+    if (me < ROWS) {
+      s_rank[me] += before;
+      if (first) s_list[s_rank[me]] = s_id[me];
+    }
+    __syncthreads();
+    const int d0 = ps * per_pass, nd = ptx::uniform(min(per_pass, distinct - d0));
+    if (nd <= 0) continue;  // (in the whole cluster)
+    // (every item leaves the ring empty)
+    const uint32_t tx = x_stage + static_cast<uint32_t>(nd * p.rank_pad) * 128u;
+    const int stages = ptx::uniform(static_cast<int>(min(p.off_part / tx, static_cast<uint32_t>(MAX_STAGES))));
     int stage = 0;
-    uint32_t phase = 0;
-    uint32_t issued = 0;
-    bool ok = true;
-    for (int ps = ps0; ps < passes && ok; ps += p.par) {
-      const int d0 = ps * per_pass, nd = min(per_pass, distinct - d0);
-      for (int i = 0; i < nkb; ++i) {
-        if (!(ok = warp_wait(bar_empty + 8 * stage, phase ^ 1u, abort, elected))) break;
+
+    if (warp == 0) {
+      for (int i = 0; i < nkb && ok; ++i) {
+        if (!(ok = warp_wait(bar_empty + 8 * stage, (phases >> stage & 1u) ^ 1u, abort, elected)))
+          break;
         const uint32_t fb = bar_full + 8 * stage;
-        const uint32_t dst = sbase + static_cast<uint32_t>(stage) * stage_bytes;
+        const uint32_t dst = sbase + static_cast<uint32_t>(stage) * tx;
         if (elected) {
-          ptx::mbar_arrive_expect_tx(fb, x_stage + static_cast<uint32_t>(nd * p.rank_pad) * 128u);
+          ptx::mbar_arrive_expect_tx(fb, tx);
           ptx::tma_load_2d(dst, &tmap_x, (kb0 + i) * KB, m0, fb);
         }
         for (int d = 0; d < nd; ++d) {  // ranks past R read as zero
@@ -209,40 +317,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             ptx::tma_load_3d(dst + x_stage + static_cast<uint32_t>(d * p.rank_pad) * 128u, &tmap_a,
                              (kb0 + i) * KB, 0, a, fb);
         }
-        ++issued;
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        phases ^= 1u << stage;
+        used |= 1u << stage;
+        if (++stage == stages) stage = 0;
       }
-    }
-    const uint32_t n_drain = min(issued, static_cast<uint32_t>(stages));
-    for (uint32_t i = 0; i < n_drain; ++i) {
-      if (stage == 0) {
-        stage = stages - 1;
-        phase ^= 1u;
-      } else {
-        --stage;
-      }
-      ptx::mbar_wait_timeout(bar_empty + 8 * stage, phase, kDrainLimitNs);
-    }
-  } else if (warp == 1) {
-    const bool elected = ptx::elect_one();
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
-      if (!warp_wait(bar, parity, abort, elected)) return false;
-      ptx::tc_fence_after();
-      return true;
-    };
-    for (int ps = ps0; ps < passes && ok; ps += p.par) {
-      const int nd = ptx::uniform(min(per_pass, distinct - ps * per_pass));
+    } else if (warp == 1) {
       const uint32_t idesc = ptx::idesc_f16_f32(ROWS, nd * p.rank_pad, p.dtype == kBF16);
-      if (ps > ps0 && !wait(bar_free, static_cast<uint32_t>((ps - ps0) / p.par - 1) & 1u)) break;
-      for (int i = 0; i < nkb; ++i) {
-        if (!(ok = wait(bar_full + 8 * stage, phase))) break;
-        const uint32_t st = sbase + static_cast<uint32_t>(stage) * stage_bytes;
+      ptx::tc_fence_after();
+      for (int i = 0; i < nkb && ok; ++i) {
+        if (!(ok = warp_wait(bar_full + 8 * stage, phases >> stage & 1u, abort, elected))) break;
+        ptx::tc_fence_after();
+        const uint32_t st = sbase + static_cast<uint32_t>(stage) * tx;
         const uint64_t adesc = ptx::sw128_kmajor_desc(st);
         const uint64_t bdesc = ptx::sw128_kmajor_desc(st + x_stage);
         if (elected) {
@@ -251,31 +336,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             ptx::mma_f16<1>(tmem, adesc + 2 * kk, bdesc + 2 * kk, idesc, (i | kk) != 0 ? 1u : 0u);
           ptx::mma_commit(bar_empty + 8 * stage);
         }
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        phases ^= 1u << stage;
+        if (++stage == stages) stage = 0;
       }
       if (ok && elected) ptx::mma_commit(bar_acc);
-    }
-    if (elected) {
-      ptx::mma_commit(bar_drain);
-      ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
-    }
-  } else if (warp < 6) {
-    // TMEM lane = row: keep the columns of the row's own adapter
-    const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;
-    const int mine = s_id[row] >= 0 ? s_rank[s_first[row]] : -1;
-    for (int ps = ps0; ps < passes; ps += p.par) {
-      const int d0 = ps * per_pass, nd = min(per_pass, distinct - d0);
-      if (!ptx::mbar_wait_bounded(bar_acc, static_cast<uint32_t>((ps - ps0) / p.par) & 1u, abort,
-                                  kWaitLimitNs)) {
-        if (lane == 0) record_timeout(abort);
-        break;
+    } else if (warp < 6) {
+      // TMEM lane = row: keep the columns of the row's own adapter
+      const int quarter = warp & 3;
+      const int row = quarter * 32 + lane;
+      const int mine = s_id[row] >= 0 ? s_rank[s_first[row]] : -1;
+      if (ok && !ptx::mbar_wait_bounded(bar_acc, items & 1u, abort, kWaitLimitNs)) {
+        record_timeout(abort);
+        ok = false;
       }
+      ok = __all_sync(0xFFFFFFFFu, ok);
       ptx::tc_fence_after();
-      for (int d = 0; d < nd; ++d) {
+      for (int d = 0; d < nd && ok; ++d) {
         const bool keep = mine == d0 + d;
         if (!__any_sync(0xFFFFFFFFu, keep)) continue;
         for (int c = 0; c < p.rank_pad; c += 16) {
@@ -291,146 +367,96 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
       ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar_free);
+    } else if (plan_open) {
+      ptx::grid_dependency_wait();
+      make_plan(p, lane);
+      plan_open = false;
     }
-  } else if (p.plan != nullptr && blockIdx.x == 0) {
-    // The plan of the GEMM's token tiles. A run of at least kLoraMixed (32) rows crosses a
-    // border between blocks of 32 rows, so of a block's runs only the one carried in and the
-    // one carried on can be long.
+    ++items;
+
+    __syncwarp();
+    __syncthreads();
+    ptx::cluster_sync();  // every CTA's partial sums are in its shared memory
     ptx::grid_dependency_wait();
-    int n = 0;
-    auto emit = [&](int t0, int t1, int a) {
-      ++n;
-      if (lane == 0) p.plan[n] = make_int4(t0, t1, a, 0);
-    };
-    int open = -1, open_end = 0;  // rows of short runs not yet in a tile
-    auto flush = [&]() {
-      if (open >= 0 && open < open_end) emit(open, open_end, -2);
-      open = -1;
-    };
-    auto add_short = [&](int s, int e) {
-      if (s == e) return;
-      if (open < 0) open = s;
-      open_end = e;
-      for (; open_end - open >= kLoraMixed; open += kLoraMixed) emit(open, open + kLoraMixed, -2);
-      if (open == open_end) open = -1;
-    };
-    auto add_run = [&](int s, int e, int a) {
-      if (e - s < kLoraMixed) {
-        add_short(s, e);
-        return;
-      }
-      flush();
-      const int nt = (e - s + kLoraTileTokens - 1) / kLoraTileTokens;
-      const int per = ((e - s + nt - 1) / nt + 31) / 32 * 32;
-      for (int t = s; t < e; t += per) emit(t, min(e, t + per), a);
-    };
-    int start = 0, cur = -1;  // the run carried on
-    constexpr int AHEAD = 8;  // blocks loaded together, one such batch before it is read
-    int ids[AHEAD], next[AHEAD];
-    auto fetch = [&](int b) {
+
+    const uint32_t part_base = ptx::smem_u32(part);
+    const bool f16 = p.dtype == kF16;
+    const bool fine = *abort == 0;
+    for (int row = rank + warp * p.split; row < ROWS && fine; row += NUM_THREADS / 32 * p.split) {
+      const int id = s_id[row];
+      if (id < 0 || s_rank[s_first[row]] / per_pass != ps) continue;
+      const float sc = __ldg(p.scaling + id);
+      float v[kLoraMaxRank / 32];
+      float top = 0.0f;
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int m = b + 32 * k + lane;
-        next[k] = m < p.M ? __ldg(p.ids + m) : -1;
-      }
-    };
-    fetch(0);
-    for (int b0 = 0; b0 < p.M; b0 += 32 * AHEAD) {
+      for (int i = 0; i < kLoraMaxRank / 32; ++i) {
+        const int c = i * 32 + lane;
+        v[i] = 0.0f;
+        if (c < p.R) {
+          const uint32_t at = part_base + static_cast<uint32_t>(row * pitch + c) * 4u;
+          float part_of[MAX_SPLIT];
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) ids[k] = has_adapter(p, next[k]) ? next[k] : -1;
-      fetch(b0 + 32 * AHEAD);
+          for (int s = 0; s < MAX_SPLIT; ++s)
+            if (s < p.split) part_of[s] = ptx::ld_shared_cluster_f32(ptx::map_shared_rank(at, s));
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int b = b0 + 32 * k;
-        int before = __shfl_up_sync(0xFFFFFFFFu, ids[k], 1);
-        if (lane == 0) before = cur;
-        const uint32_t edges = __ballot_sync(0xFFFFFFFFu, b + lane < p.M && ids[k] != before);
-        if (edges != 0) {
-          const int first = __ffs(static_cast<int>(edges)) - 1;
-          const int last = 31 - __clz(static_cast<int>(edges));
-          add_run(start, b + first, cur);
-          add_short(b + first, b + last);
-          start = b + last;
+          for (int s = 0; s < MAX_SPLIT; ++s)
+            if (s < p.split) v[i] += part_of[s];
+          v[i] *= sc;
+          const float a = fabsf(v[i]);
+          if (a <= 3.402823466e38f) top = fmaxf(top, a);  // finite values only
         }
-        cur = __shfl_sync(0xFFFFFFFFu, ids[k], 31);
       }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+      // f16: the row divided by 2^ex, its largest finite value's exponent (exact)
+      int ex = 0;
+      if (f16 && top > 0.0f)
+        ex = min(126, max(-126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+      const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+      const int64_t base = static_cast<int64_t>(m0 + row) * (2 * p.rank_pad);
+#pragma unroll
+      for (int i = 0; i < kLoraMaxRank / 32; ++i) {
+        const int c = i * 32 + lane;
+        if (c >= p.rank_pad) break;
+        const float t = v[i] * inv;
+        // an infinity or NaN is the high part's alone
+        if (f16) {
+          const __half hi = __float2half_rn(t);
+          const float back = __half2float(hi);
+          __half *dst = reinterpret_cast<__half *>(p.hl) + base;
+          dst[c] = hi;
+          dst[p.rank_pad + c] = __float2half_rn(fabsf(back) <= 65504.0f ? t - back : 0.0f);
+        } else {
+          const __nv_bfloat16 hi = __float2bfloat16_rn(t);
+          const float back = __bfloat162float(hi);
+          __nv_bfloat16 *dst = reinterpret_cast<__nv_bfloat16 *>(p.hl) + base;
+          dst[c] = hi;
+          dst[p.rank_pad + c] =
+              __float2bfloat16_rn(fabsf(back) <= 3.402823466e38f ? t - back : 0.0f);
+        }
+      }
+      if (lane == 0)
+        p.hscale[m0 + row] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
     }
-    // (past M the lanes hold -1; the run's own id is its first row's)
-    const int tail = __ldg(p.ids + min(start, p.M - 1));
-    add_run(start, p.M, has_adapter(p, tail) ? tail : -1);
-    flush();
-    if (lane == 0) p.plan[0] = make_int4(n, 0, 0, 0);
+
+    // (peers may still be reading this CTA's partial sums, its own warps the lists)
+    ptx::cluster_sync();
   }
 
+  ptx::grid_dependency_wait();  // the GEMM's wait for this kernel covers the quantizer too
+  if (warp == 6 && plan_open) make_plan(p, lane);
+  if (warp == 0) {
+    // (after a wait that ran out: no copy may be under way when the CTA ends)
+    for (int s = 0; s < MAX_STAGES; ++s)
+      if (*abort && (used >> s & 1u))
+        ptx::mbar_wait_timeout(bar_empty + 8 * s, (phases >> s & 1u) ^ 1u, kDrainLimitNs);
+  } else if (warp == 1 && elected) {
+    ptx::mma_commit(bar_drain);
+    ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
+  }
   __syncwarp();
+  ptx::tc_fence_before();
   __syncthreads();
-  ptx::cluster_sync();  // every CTA's partial sums are in its shared memory
-  ptx::grid_dependency_wait();
-
-  // Row by row: add the K-splits in rank order, scale, split into the two parts. CTA `rank`
-  // of the cluster has rows rank, rank + split, ..; a warp has a row, a lane four values.
-  const uint32_t part_base = ptx::smem_u32(part);
-  const bool f16 = p.dtype == kF16;
-  const bool fine = *abort == 0;
-  for (int row = rank + warp * p.split; row < ROWS && fine; row += NUM_THREADS / 32 * p.split) {
-    const int id = s_id[row];
-    if (id < 0 || s_rank[s_first[row]] / per_pass % p.par != ps0) continue;
-    const float sc = __ldg(p.scaling + id);
-    float v[kLoraMaxRank / 32];
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kLoraMaxRank / 32; ++i) {
-      const int c = i * 32 + lane;
-      v[i] = 0.0f;
-      if (c < p.R) {
-        const uint32_t at = part_base + static_cast<uint32_t>(row * pitch + c) * 4u;
-        float part_of[MAX_SPLIT];
-#pragma unroll
-        for (int s = 0; s < MAX_SPLIT; ++s)
-          if (s < p.split) part_of[s] = ptx::ld_shared_cluster_f32(ptx::map_shared_rank(at, s));
-#pragma unroll
-        for (int s = 0; s < MAX_SPLIT; ++s)
-          if (s < p.split) v[i] += part_of[s];
-        v[i] *= sc;
-        const float a = fabsf(v[i]);
-        if (a <= 3.402823466e38f) top = fmaxf(top, a);  // finite values only
-      }
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    // f16: the row divided by 2^ex, its largest finite value's exponent (exact)
-    int ex = 0;
-    if (f16 && top > 0.0f)
-      ex = min(126, max(-126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
-    const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-    const int64_t base = static_cast<int64_t>(m0 + row) * (2 * p.rank_pad);
-#pragma unroll
-    for (int i = 0; i < kLoraMaxRank / 32; ++i) {
-      const int c = i * 32 + lane;
-      if (c >= p.rank_pad) break;
-      const float t = v[i] * inv;
-      // an infinity or NaN is the high part's alone
-      if (f16) {
-        const __half hi = __float2half_rn(t);
-        const float back = __half2float(hi);
-        __half *dst = reinterpret_cast<__half *>(p.hl) + base;
-        dst[c] = hi;
-        dst[p.rank_pad + c] = __float2half_rn(fabsf(back) <= 65504.0f ? t - back : 0.0f);
-      } else {
-        const __nv_bfloat16 hi = __float2bfloat16_rn(t);
-        const float back = __bfloat162float(hi);
-        __nv_bfloat16 *dst = reinterpret_cast<__nv_bfloat16 *>(p.hl) + base;
-        dst[c] = hi;
-        dst[p.rank_pad + c] =
-            __float2bfloat16_rn(fabsf(back) <= 3.402823466e38f ? t - back : 0.0f);
-      }
-    }
-    if (lane == 0)
-      p.hscale[m0 + row] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
-  }
-  ptx::cluster_sync();  // peers may still be reading this CTA's partial sums
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc<1>(tmem, COLS);
@@ -482,15 +508,18 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
       1, std::min<int64_t>({dev.sm_count / tiles, MAX_SPLIT, (p.k_blocks + 3) / 4})));
   p.kps = (p.k_blocks + split - 1) / split;
   p.split = (p.k_blocks + p.kps - 1) / p.kps;
-  // passes side by side while CTAs are left over still
-  const int64_t most = (std::min<int64_t>(a.L, ROWS) + COLS / p.rank_pad - 1) / (COLS / p.rank_pad);
-  p.par = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(dev.sm_count / (tiles * p.split), most)));
+  // a cluster per tile, and further ones for the passes of tiles with many adapters while CTAs
+  // are left over still
+  // (few rows: narrower passes, that more clusters share them)
+  p.cols = a.M <= ROWS ? 128 : COLS;
+  const int per_pass = p.cols / p.rank_pad;
+  p.tiles = static_cast<int>(tiles);
+  p.max_passes = static_cast<int>((std::min<int64_t>(a.L, ROWS) + per_pass - 1) / per_pass);
+  p.clusters = static_cast<int>(std::max<int64_t>(
+      tiles, std::min<int64_t>(dev.sm_count / p.split, tiles * p.max_passes)));
   p.x_rows = static_cast<int>(std::min<int64_t>((a.M + 7) / 8 * 8, ROWS));
   const uint32_t part = ROWS * (static_cast<uint32_t>(p.rank_pad) + 1) * 4;
-  const uint32_t stage = static_cast<uint32_t>(p.x_rows) * 128 + A_STAGE;
-  p.stages = static_cast<int>(std::min<uint32_t>((SMEM_MAX - 1024 - part) / stage, MAX_STAGES));
-  p.off_part = static_cast<uint32_t>(p.stages) * stage;
+  p.off_part = (SMEM_MAX - 1024 - part) / 1024 * 1024;
   const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   std::string err;
@@ -525,7 +554,7 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.par * p.split));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.clusters * p.split));
   cfg.blockDim = dim3(NUM_THREADS);
   cfg.dynamicSmemBytes = p.off_part + part + 1024;
   e = cudaLaunchKernelEx(&cfg, down_tile_kernel, tx, ta, p);

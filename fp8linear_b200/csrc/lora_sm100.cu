@@ -46,7 +46,7 @@ struct Params {
   void *hl;
   float *hscale;
   int4 *plan;      // null: not wanted
-  int split, kps, k_blocks;
+  int split, k_blocks;
   int x_rows;      // rows of x's box
   int cols;        // columns per pass
   uint32_t off_part;
@@ -175,6 +175,86 @@ __device__ __forceinline__ int adapters_at_most(const Params &p, int m0, int lan
   return n;
 }
 
+// An item's sums, row by row: the K-splits' parts added in rank order, scaled, and split into
+// the two 16-bit parts. CTA `rank` of the S of a cluster has rows rank, rank + S, ..; a warp
+// has two rows at a time, a lane values 2 lane, + 1 and 64 more of each. (All loads are
+// unconditional, so that they run side by side: behind branches they took 1 us a row pair.)
+template <int S>
+__device__ __forceinline__ void finish_rows(const Params &p, const float *part, int pitch,
+                                            const int *live, const float *scaling, int m0,
+                                            int rank, int warp, int lane) {
+  const bool f16 = p.dtype == kF16;
+  uint32_t from[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    from[s] = S == 1 ? ptx::smem_u32(part) : ptx::map_shared_rank(ptx::smem_u32(part), s);
+  int col[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) col[i] = (i >> 1) * 64 + 2 * lane + (i & 1);
+  for (int r0 = 2 * warp; rank + r0 * S < ROWS; r0 += 2 * (NUM_THREADS / 32)) {
+    int row[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) row[h] = min(rank + (r0 + h) * S, ROWS - 1);
+    const bool on[2] = {live[row[0]] != 0, live[row[1]] != 0 && rank + (r0 + 1) * S < ROWS};
+    if (!on[0] && !on[1]) continue;  // uniform in the warp
+    float t[2][4][S];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const uint32_t at =
+              from[s] + static_cast<uint32_t>(row[h] * pitch + min(col[i], p.rank_pad - 1)) * 4u;
+          t[h][i][s] = S == 1 ? ptx::ld_shared_f32(at) : ptx::ld_shared_cluster_f32(at);
+        }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; ++s) v[i] += t[h][i][s];
+        v[i] = col[i] < p.R ? v[i] * scaling[row[h]] : 0.0f;
+      }
+      if (!on[h]) continue;
+      // f16: the row divided by 2^ex, its largest finite value's exponent (exact)
+      int ex = 0;
+      if (f16) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (fabsf(v[i]) <= 3.402823466e38f) top = fmaxf(top, fabsf(v[i]));
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+        if (top > 0.0f)
+          ex = min(126, max(-126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+      }
+      const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+      uint32_t *dst = reinterpret_cast<uint32_t *>(p.hl) +
+                      static_cast<int64_t>(m0 + row[h]) * p.rank_pad + lane;
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        if (col[i] >= p.rank_pad) break;
+        // an infinity or NaN is the high part's alone
+        float hi[2], lo[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float w = v[i + j] * inv;
+          hi[j] = f16 ? __half2float(__float2half_rn(w)) : __bfloat162float(__float2bfloat16_rn(w));
+          lo[j] = fabsf(hi[j]) <= (f16 ? 65504.0f : 3.402823466e38f) ? w - hi[j] : 0.0f;
+        }
+        dst[16 * i] = f16 ? ptx::pack_f16x2(hi[0], hi[1]) : ptx::pack_bf16x2(hi[0], hi[1]);
+        dst[p.rank_pad / 2 + 16 * i] =
+            f16 ? ptx::pack_f16x2(lo[0], lo[1]) : ptx::pack_bf16x2(lo[0], lo[1]);
+      }
+      if (lane == 0)
+        p.hscale[m0 + row[h]] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+    }
+  }
+}
+
 // Work comes in items (tile of 128 rows, pass over p.cols columns of its adapters). Item (t, ps)
 // is cluster (t + ps) % p.clusters's: a tile of one adapter is its own cluster's only item,
 // the passes of a tile of many (decoding requests) spread over the neighbours.
@@ -193,6 +273,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __shared__ int s_first[ROWS];  // the row's adapter appears first at this row of the tile
   __shared__ int s_rank[ROWS];   // .. and is this one of the tile's adapters
   __shared__ int s_list[ROWS];   // the tile's adapters
+  __shared__ int s_live[ROWS];   // the row's sums are this item's
+  __shared__ float s_scaling[ROWS];
   __shared__ int s_count[ROWS / 32];
   __shared__ int s_todo[ROWS];   // pass ps of tile (cluster - ps) may have work
   const uint32_t bar_full = ptx::smem_u32(s_bar);
@@ -242,8 +324,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t tmem = static_cast<uint32_t>(
       ptx::uniform(static_cast<int>(*const_cast<volatile uint32_t *>(&s_slot))));
 
-  const int kb0 = rank * p.kps;
-  const int nkb = min(p.k_blocks, kb0 + p.kps) - kb0;  // >= 1 (the host's split)
+  const int kb0 = rank * p.k_blocks / p.split;  // (split <= k_blocks)
+  const int nkb = (rank + 1) * p.k_blocks / p.split - kb0;
   bool plan_open = p.plan != nullptr && blockIdx.x == 0;  // this CTA's last warp has it to make
   const bool elected = ptx::elect_one();
   uint32_t phases = 0;  // bit s: of stage s, in the producer and the MMA warp
@@ -259,6 +341,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     if (me < ROWS) {
       const int id = m0 + me < p.M ? __ldg(p.ids + m0 + me) : -1;
       s_id[me] = has_adapter(p, id) ? id : -1;
+      s_scaling[me] = has_adapter(p, id) ? __ldg(p.scaling + id) : 0.0f;
     }
     __syncthreads();
     bool first = false;
@@ -296,6 +379,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     __syncthreads();
     const int d0 = ps * per_pass, nd = ptx::uniform(min(per_pass, distinct - d0));
     if (nd <= 0) continue;  // (in the whole cluster)
+    if (me < ROWS) {  // (read after the barriers below)
+      const int r = s_rank[s_first[me]];
+      s_live[me] = s_id[me] >= 0 && r >= d0 && r < d0 + nd;
+    }
     // (every item leaves the ring empty)
     const uint32_t tx = x_stage + static_cast<uint32_t>(nd * p.rank_pad) * 128u;
     const int stages = ptx::uniform(static_cast<int>(min(p.off_part / tx, static_cast<uint32_t>(MAX_STAGES))));
@@ -379,64 +466,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     ptx::cluster_sync();  // every CTA's partial sums are in its shared memory
     ptx::grid_dependency_wait();
 
-    const uint32_t part_base = ptx::smem_u32(part);
-    const bool f16 = p.dtype == kF16;
-    const bool fine = *abort == 0;
-    for (int row = rank + warp * p.split; row < ROWS && fine; row += NUM_THREADS / 32 * p.split) {
-      const int id = s_id[row];
-      if (id < 0 || s_rank[s_first[row]] / per_pass != ps) continue;
-      const float sc = __ldg(p.scaling + id);
-      float v[kLoraMaxRank / 32];
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kLoraMaxRank / 32; ++i) {
-        const int c = i * 32 + lane;
-        v[i] = 0.0f;
-        if (c < p.R) {
-          const uint32_t at = part_base + static_cast<uint32_t>(row * pitch + c) * 4u;
-          float part_of[MAX_SPLIT];
-#pragma unroll
-          for (int s = 0; s < MAX_SPLIT; ++s)
-            if (s < p.split) part_of[s] = ptx::ld_shared_cluster_f32(ptx::map_shared_rank(at, s));
-#pragma unroll
-          for (int s = 0; s < MAX_SPLIT; ++s)
-            if (s < p.split) v[i] += part_of[s];
-          v[i] *= sc;
-          const float a = fabsf(v[i]);
-          if (a <= 3.402823466e38f) top = fmaxf(top, a);  // finite values only
-        }
+    if (*abort == 0) {
+      switch (p.split) {
+        case 1: finish_rows<1>(p, part, pitch, s_live, s_scaling, m0, rank, warp, lane); break;
+        case 2: finish_rows<2>(p, part, pitch, s_live, s_scaling, m0, rank, warp, lane); break;
+        case 4: finish_rows<4>(p, part, pitch, s_live, s_scaling, m0, rank, warp, lane); break;
+        default: finish_rows<8>(p, part, pitch, s_live, s_scaling, m0, rank, warp, lane);
       }
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-      // f16: the row divided by 2^ex, its largest finite value's exponent (exact)
-      int ex = 0;
-      if (f16 && top > 0.0f)
-        ex = min(126, max(-126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
-      const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-      const int64_t base = static_cast<int64_t>(m0 + row) * (2 * p.rank_pad);
-#pragma unroll
-      for (int i = 0; i < kLoraMaxRank / 32; ++i) {
-        const int c = i * 32 + lane;
-        if (c >= p.rank_pad) break;
-        const float t = v[i] * inv;
-        // an infinity or NaN is the high part's alone
-        if (f16) {
-          const __half hi = __float2half_rn(t);
-          const float back = __half2float(hi);
-          __half *dst = reinterpret_cast<__half *>(p.hl) + base;
-          dst[c] = hi;
-          dst[p.rank_pad + c] = __float2half_rn(fabsf(back) <= 65504.0f ? t - back : 0.0f);
-        } else {
-          const __nv_bfloat16 hi = __float2bfloat16_rn(t);
-          const float back = __bfloat162float(hi);
-          __nv_bfloat16 *dst = reinterpret_cast<__nv_bfloat16 *>(p.hl) + base;
-          dst[c] = hi;
-          dst[p.rank_pad + c] =
-              __float2bfloat16_rn(fabsf(back) <= 3.402823466e38f ? t - back : 0.0f);
-        }
-      }
-      if (lane == 0)
-        p.hscale[m0 + row] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
     }
 
     // (peers may still be reading this CTA's partial sums, its own warps the lists)
@@ -479,6 +515,45 @@ LoraWorkspace lora_workspace(void *base, int64_t M, int64_t R) {
   return w;
 }
 
+namespace lora {
+
+// Clusters of 1, 2, 4 and 8 CTAs that the GPU holds at once.
+struct DownInfo {
+  bool ready = false;
+  cudaError_t err = cudaSuccess;
+  int clusters[MAX_SPLIT + 1] = {};
+};
+
+const DownInfo &down_info(const DeviceInfo &dev) {
+  static DownInfo info[64];
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  DownInfo &di = info[dev.device & 63];
+  if (!di.ready) {
+    di.ready = true;
+    di.err = cudaFuncSetAttribute(down_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(SMEM_MAX));
+    di.clusters[1] = dev.sm_count;
+    for (int s = 2; s <= MAX_SPLIT && di.err == cudaSuccess; s *= 2) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(static_cast<unsigned>(dev.sm_count / s * s));
+      cfg.blockDim = dim3(NUM_THREADS);
+      cfg.dynamicSmemBytes = SMEM_MAX;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = static_cast<unsigned>(s);
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      di.err = cudaOccupancyMaxActiveClusters(&di.clusters[s], down_tile_kernel, &cfg);
+    }
+  }
+  return di;
+}
+
+}  // namespace lora
+
 int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   using namespace lora;
   DeviceInfo dev;
@@ -503,11 +578,17 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   cudaError_t e;
   p.k_blocks = static_cast<int>((a.K + KB - 1) / KB);
   const int64_t tiles = (a.M + ROWS - 1) / ROWS;
-  // K-splits while CTAs are left over, four K-blocks at least for each
-  const int split = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>({dev.sm_count / tiles, MAX_SPLIT, (p.k_blocks + 3) / 4})));
-  p.kps = (p.k_blocks + split - 1) / split;
-  p.split = (p.k_blocks + p.kps - 1) / p.kps;
+  const DownInfo &di = down_info(dev);
+  if (di.err != cudaSuccess) {
+    set_error(std::string("fp8_linear_lora: kernel setup: ") + cudaGetErrorString(di.err));
+    return 4;
+  }
+  // K-splits (1, 2, 4 or 8) while there is room for all tiles' clusters, four K-blocks at
+  // least for each
+  int split = 1;
+  for (int s = 2; s <= MAX_SPLIT && 4 * s <= p.k_blocks + 3; s *= 2)
+    if (di.clusters[s] >= tiles) split = s;
+  p.split = split;
   // a cluster per tile, and further ones for the passes of tiles with many adapters while CTAs
   // are left over still
   // (few rows: narrower passes, that more clusters share them)
@@ -516,7 +597,7 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   p.tiles = static_cast<int>(tiles);
   p.max_passes = static_cast<int>((std::min<int64_t>(a.L, ROWS) + per_pass - 1) / per_pass);
   p.clusters = static_cast<int>(std::max<int64_t>(
-      tiles, std::min<int64_t>(dev.sm_count / p.split, tiles * p.max_passes)));
+      tiles, std::min<int64_t>(di.clusters[split], tiles * p.max_passes)));
   p.x_rows = static_cast<int>(std::min<int64_t>((a.M + 7) / 8 * 8, ROWS));
   const uint32_t part = ROWS * (static_cast<uint32_t>(p.rank_pad) + 1) * 4;
   p.off_part = (SMEM_MAX - 1024 - part) / 1024 * 1024;
@@ -526,24 +607,10 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   CUtensorMap tx, ta;
   if (!make_tmap_2d_sw128(&tx, t16, a.x, a.K, a.M, a.K * 2, KB, static_cast<uint32_t>(p.x_rows),
                           &err) ||
-      !make_tmap_3d_sw128(&ta, t16, a.lora_a, a.K, a.R, a.L, a.K * 2, a.R * a.K * 2, KB,
-                          static_cast<uint32_t>(p.rank_pad), &err)) {
+      !make_tmap_3d_swizzled(&ta, t16, a.lora_a, a.K, a.R, a.L, a.K * 2, a.R * a.K * 2, KB,
+                             static_cast<uint32_t>(p.rank_pad), 128, &err)) {
     set_error("fp8_linear_lora: " + err);
     return 4;
-  }
-  static bool set[64];
-  static std::mutex mu;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!set[dev.device & 63]) {
-      e = cudaFuncSetAttribute(down_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(SMEM_MAX));
-      if (e != cudaSuccess) {
-        set_error(std::string("fp8_linear_lora: kernel setup: ") + cudaGetErrorString(e));
-        return 4;
-      }
-      set[dev.device & 63] = true;
-    }
   }
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -527,6 +527,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // 32-bit load from another CTA's shared memory (a shared::cluster address).
 __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t addr) {
   float v;

@@ -56,6 +56,7 @@ struct Maps {
   CUtensorMap x[X_MAPS];  // xq [M][K], box 128 B x 16 (i + 1) rows
   CUtensorMap w;          // wq [E][N][K], box 128 B x 128 rows x 1
   CUtensorMap lb;         // lora_b [L][N][R], box 64 x 128 rows x 1
+  CUtensorMap ls;         // the same for adapter_sums, box sum_width(R) x 128 rows x 1
   CUtensorMap h[H_MAPS];  // hl [M][2 rank_pad], box 64 x 16 (i + 1) rows
 };
 
@@ -298,18 +299,42 @@ __device__ __forceinline__ void lora_mma(const Params &p, uint32_t d, uint32_t s
       ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + 2 * (kk + steps), idesc, 1u);
 }
 
-// The ring of B boxes for adapter_sums: 128 weight rows x 64 ranks, 128-byte swizzle. A warp
-// of its own fills it (feed), the four epilogue warps read it; both go through the tokens
-// eight at a time, through the adapters of eight in the order of their first tokens, and
-// through the rank 64 at a time. `count` boxes have been through the ring.
-constexpr int SUM_SLOTS = 3;
+// The ring of B boxes for adapter_sums: 128 weight rows x 64 ranks (32 or 16 where the rank
+// fits), rows of 128, 64 or 32 bytes swizzled over as many; 48 KB of it, so that three to
+// eight boxes are under way. A warp of its own fills it (feed_sums), the four epilogue warps
+// read it; both go through the tokens eight at a time, through the adapters of eight in the
+// order of their first tokens, and through the rank a box at a time. `count` boxes have been
+// through the ring.
+constexpr uint32_t SUM_RING = 3 * W_STAGE;
+constexpr int SUM_SLOTS_MAX = 8;
 constexpr int SUM_RANK = 64;
-constexpr int SUM_BARS = 2 * SUM_SLOTS;  // full, empty
+constexpr int SUM_BARS = 2 * SUM_SLOTS_MAX;  // full, empty
+__host__ __device__ constexpr int sum_width(int rank) { return rank > 32 ? 64 : rank > 16 ? 32 : 16; }
+__device__ __forceinline__ uint32_t sum_slots(int rank) {
+  return rank > 32 ? 3u : rank > 16 ? 6u : 8u;
+}
 struct SumRing {
   uint32_t slots;  // shared-memory addresses
   uint32_t bars;
   volatile int *abort;
+  uint32_t n;       // slots
+  uint32_t box;     // bytes of one
+  uint32_t slot;    // the next, and its phase
+  uint32_t phase;
   uint32_t count;
+
+  __device__ __forceinline__ SumRing(const Params &p, uint32_t s, uint32_t b, volatile int *a)
+      : slots(s), bars(b), abort(a), n(sum_slots(p.R)),
+        box(static_cast<uint32_t>(sum_width(p.R)) * 2u * WROWS), slot(0), phase(0), count(0) {}
+  __device__ __forceinline__ uint32_t full() const { return bars + 8 * slot; }
+  __device__ __forceinline__ uint32_t empty() const { return bars + 8 * (SUM_SLOTS_MAX + slot); }
+  __device__ __forceinline__ void next() {
+    ++count;
+    if (++slot == n) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
 };
 
 // Lane l of a warp has the adapter of token l % 8 of eight (-1: none); bits 0-7 of the
@@ -339,15 +364,12 @@ __device__ __forceinline__ bool feed_sums(const Params &p, const CUtensorMap *ma
     for (uint32_t todo = first_tokens(id); todo != 0; todo &= todo - 1) {
       const int a = __shfl_sync(0xFFFFFFFFu, id, __ffs(static_cast<int>(todo)) - 1);
       for (int rc = 0; rc < p.R; rc += SUM_RANK) {
-        const uint32_t s = ring.count % SUM_SLOTS;
-        if (!warp_wait(ring.bars + 8 * (SUM_SLOTS + s), (ring.count / SUM_SLOTS & 1u) ^ 1u, ring.abort,
-                       elected))
-          return false;
+        if (!warp_wait(ring.empty(), ring.phase ^ 1u, ring.abort, elected)) return false;
         if (elected) {
-          ptx::mbar_arrive_expect_tx(ring.bars + 8 * s, W_STAGE);
-          ptx::tma_load_3d(ring.slots + s * W_STAGE, map, rc, n0, a, ring.bars + 8 * s);
+          ptx::mbar_arrive_expect_tx(ring.full(), ring.box);
+          ptx::tma_load_3d(ring.slots + ring.slot * ring.box, map, rc, n0, a, ring.full());
         }
-        ++ring.count;
+        ring.next();
       }
     }
   }
@@ -355,11 +377,16 @@ __device__ __forceinline__ bool feed_sums(const Params &p, const CUtensorMap *ma
 }
 
 // Waits (bounded) until every box issued has landed and been read.
-__device__ __forceinline__ void drain_sums(const SumRing &ring) {
-  if ((threadIdx.x & 31) != 0) return;
-  for (uint32_t i = ring.count > SUM_SLOTS ? ring.count - SUM_SLOTS : 0; i < ring.count; ++i)
-    ptx::mbar_wait_timeout(ring.bars + 8 * (SUM_SLOTS + i % SUM_SLOTS), (i / SUM_SLOTS) & 1u,
-                           kDrainLimitNs);
+__device__ __forceinline__ void drain_sums(SumRing &ring) {
+  for (uint32_t i = min(ring.count, ring.n); i > 0; --i) {
+    if (ring.slot == 0) {
+      ring.slot = ring.n - 1;
+      ring.phase ^= 1u;
+    } else {
+      --ring.slot;
+    }
+    ptx::mbar_wait_timeout(ring.empty(), ring.phase, kDrainLimitNs);
+  }
 }
 
 // For eight tokens i0 .. (below t1) and the 32 weight rows `quarter` of the boxes: the sums
@@ -394,6 +421,10 @@ __device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring, int
   // ldmatrix: lane 8m + i has row i + 8 (m % 2) of a 16-row tile, 16-byte column 2j + m / 2
   const uint32_t row = static_cast<uint32_t>(quarter * 32 + (lane & 7) + (lane & 8));
   const uint32_t col = static_cast<uint32_t>(lane >> 4);
+  // 16-byte column c of a row lies at c ^ swizzle: address bits 7.. of the row's own (the same
+  // for rows 16 apart)
+  const uint32_t row_bytes = ring.box / WROWS;
+  const uint32_t swizzle = row * row_bytes / 128 & (row_bytes / 16 - 1);
   for (; todo != 0; todo &= todo - 1) {
     const int a = __shfl_sync(0xFFFFFFFFu, id, __ffs(static_cast<int>(todo)) - 1);
     float d[2][4];
@@ -404,13 +435,11 @@ __device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring, int
 #pragma unroll
     for (int c = 0; c < kLoraMaxRank / SUM_RANK; ++c) {
       if (c * SUM_RANK >= p.R) break;
-      const uint32_t slot = ring.count % SUM_SLOTS;
-      if (!ptx::mbar_wait_bounded(ring.bars + 8 * slot, ring.count / SUM_SLOTS & 1u, ring.abort,
-                                  kWaitLimitNs)) {
+      if (!ptx::mbar_wait_bounded(ring.full(), ring.phase, ring.abort, kWaitLimitNs)) {
         record_timeout(ring.abort);
         return false;
       }
-      const uint32_t box = ring.slots + slot * W_STAGE + row * 128;
+      const uint32_t box = ring.slots + ring.slot * ring.box + row * row_bytes;
 #pragma unroll
       for (int j = 0; j < SUM_RANK / 16; ++j) {
         if (c * SUM_RANK + 16 * j >= p.rank_pad) break;
@@ -418,7 +447,7 @@ __device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring, int
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           uint32_t w[4];
-          ptx::ldsm_x4(box + m * 16 * 128 + (((2 * j + col) ^ (row & 7)) << 4), w);
+          ptx::ldsm_x4(box + m * 16 * row_bytes + (((2 * j + col) ^ swizzle) << 4), w);
           if (f16) {
             ptx::mma_f16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[0], b[1]);
             ptx::mma_f16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[2], b[3]);
@@ -429,8 +458,8 @@ __device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring, int
         }
       }
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ring.bars + 8 * (SUM_SLOTS + slot));
-      ++ring.count;
+      if (lane == 0) ptx::mbar_arrive(ring.empty());
+      ring.next();
     }
     // d[m]: rows i + 16m (0, 1) and i + 16m + 8 (2, 3), tokens 2t (0, 2) and 2t + 1 (1, 3)
 #pragma unroll
@@ -465,7 +494,7 @@ struct Cfg {
   static constexpr uint32_t ACC_L = 2 * TOK_MAX;
   static constexpr uint32_t TMEM_COLS = CG == 1 && !LORA ? 256 : 512;
   static constexpr uint32_t OFF_RING = STAGES * STAGE;
-  static constexpr uint32_t OFF_PAR = OFF_RING + (LORA ? SUM_SLOTS * W_STAGE : 0u);
+  static constexpr uint32_t OFF_PAR = OFF_RING + (LORA ? SUM_RING : 0u);
   static constexpr uint32_t PAR_WARP = TOK_MAX * 4u * (LORA ? 2u : 1u);  // xs (hscale)
   static constexpr uint32_t OFF_BOX = OFF_PAR + EPI_WARPS * PAR_WARP;
   static constexpr uint32_t OFF_TAB = OFF_BOX + EPI_WARPS * BOX_BYTES;
@@ -516,9 +545,9 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
       ptx::mbar_init(bar_tempty + 8 * a, EPI_WARPS * CG);
     }
     ptx::mbar_init(bar_drain, 1);
-    for (int i = 0; i < SUM_SLOTS; ++i) {
+    for (int i = 0; i < SUM_SLOTS_MAX; ++i) {
       ptx::mbar_init(bar_sum + 8 * i, 1);
-      ptx::mbar_init(bar_sum + 8 * (SUM_SLOTS + i), EPI_WARPS);
+      ptx::mbar_init(bar_sum + 8 * (SUM_SLOTS_MAX + i), EPI_WARPS);
     }
     *abort = 0;
     ptx::fence_mbar_init();
@@ -702,11 +731,11 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
     }
   } else if (LORA && warp == 2 + EPI_WARPS) {
     // ------------------------------------------------------------ B boxes of mixed tiles
-    SumRing ring = {sbase + C::OFF_RING, bar_sum, abort, 0};
+    SumRing ring(p, sbase + C::OFF_RING, bar_sum, abort);
     int e = 0;
     for (int t = group; t < num_tiles; t += n_groups) {
       const Tile q = tile_at(t, e);
-      if (q.adapter == -2 && !feed_sums(p, &maps.lb, ring, q.t0, q.t1,
+      if (q.adapter == -2 && !feed_sums(p, &maps.ls, ring, q.t0, q.t1,
                                         (q.wb * CG + static_cast<int>(rank)) * WROWS))
         break;
     }
@@ -721,7 +750,7 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
     const int ew = warp - 2;
     float *e_xs = reinterpret_cast<float *>(smem + C::OFF_PAR + ew * C::PAR_WARP);
     float *e_hs = e_xs + C::TOK_MAX;
-    SumRing ring = {sbase + C::OFF_RING, bar_sum, abort, 0};
+    SumRing ring(p, sbase + C::OFF_RING, bar_sum, abort);
     const uint8_t *box = smem + C::OFF_BOX + ew * BOX_BYTES;
     const uint32_t box_st = sbase + C::OFF_BOX + ew * BOX_BYTES +
                             static_cast<uint32_t>((lane & 7) * BOX_PITCH + (lane >> 3) * 16);
@@ -924,9 +953,9 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     }
     ptx::mbar_init(bar_acc, 1);
     ptx::mbar_init(bar_drain, 1);
-    for (int i = 0; i < SUM_SLOTS; ++i) {
+    for (int i = 0; i < SUM_SLOTS_MAX; ++i) {
       ptx::mbar_init(bar_sum + 8 * i, 1);
-      ptx::mbar_init(bar_sum + 8 * (SUM_SLOTS + i), EPI_WARPS);
+      ptx::mbar_init(bar_sum + 8 * (SUM_SLOTS_MAX + i), EPI_WARPS);
     }
     s_abort = 0;
     ptx::fence_mbar_init();
@@ -1042,8 +1071,8 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
       ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
     }
   } else if (LORA && warp == 2 + EPI_WARPS) {
-    SumRing ring = {sbase + p.off_ring, bar_sum, abort, 0};
-    feed_sums(p, &maps.lb, ring, q.t0 + a0, q.t0 + a1, n0);
+    SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
+    feed_sums(p, &maps.ls, ring, q.t0 + a0, q.t0 + a1, n0);
     drain_sums(ring);
   } else {
     // xs (adapters: and hscale) of the tokens, weight scales and biases of the rows reduced
@@ -1067,7 +1096,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     epilogue_sync();  // xs and hscale are in shared memory
     if constexpr (LORA) {
       // (a warp writes and reads back its own rows only; after a wait that ran out, whatever)
-      SumRing ring = {sbase + p.off_ring, bar_sum, abort, 0};
+      SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
       bool ok = true;
       for (int i = a0; i < a1 && ok; i += 8) {
         float2 s[4];
@@ -1303,7 +1332,7 @@ int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const D
   const uint32_t lora =
       LORA ? static_cast<uint32_t>((p.tok_cap / 8 + p.split - 1) / p.split * 8) * WROWS * 4 : 0;
   const uint32_t tab = static_cast<uint32_t>(p.E + 1) * 8 + 16 + SPLIT_EPI;
-  const uint32_t ring = LORA ? SUM_SLOTS * W_STAGE : 0u;
+  const uint32_t ring = LORA ? SUM_RING : 0u;
   const uint32_t room = SPLIT_SMEM - 2048 - ring - part - lora - tab;
   p.stages = std::max(1, std::min({static_cast<int>(room / stage), SPLIT_STAGES, p.kps}));
   p.off_ring = static_cast<uint32_t>(p.stages) * stage;
@@ -1324,8 +1353,8 @@ bool make_common_maps(Maps *m, int n, const uint8_t *xq, const uint8_t *wq, int6
     if (!make_tmap_2d_sw128(&m->x[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, K, M, K, BK, 16 * (i + 1),
                             err))
       return false;
-  return make_tmap_3d_sw128(&m->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, K, N, E, K, N * K, BK, WROWS,
-                            err);
+  return make_tmap_3d_swizzled(&m->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, K, N, E, K, N * K, BK,
+                               WROWS, 128, err);
 }
 
 }  // namespace rowsel
@@ -1434,9 +1463,12 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   bool ok = make_common_maps(&maps, few ? p.tok_cap / 16 : H_MAPS, a.xq, a.wq, a.M, a.N, a.K, 1,
                              &err);
-  ok = ok && make_tmap_3d_sw128(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2, 64,
-                                WROWS, &err);
+  const int sw = sum_width(static_cast<int>(a.R));
+  ok = ok && make_tmap_3d_swizzled(&maps.ls, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2,
+                                   static_cast<uint32_t>(sw), WROWS, sw * 2, &err);
   if (!few) {
+    ok = ok && make_tmap_3d_swizzled(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2,
+                                     64, WROWS, 128, &err);
     for (int i = 0; ok && i < H_MAPS; ++i)
       ok = make_tmap_2d_sw128(&maps.h[i], t16, w.hl, 2 * rp, a.M, 4 * rp, 64, 16 * (i + 1), &err);
   }

@@ -389,74 +389,93 @@ __device__ __forceinline__ void drain_sums(SumRing &ring) {
   }
 }
 
-// For eight tokens i0 .. (below t1) and the 32 weight rows `quarter` of the boxes: the sums
+// Eight tokens' adapters (as token_id gives them) and h, the B operand of their products: h of
+// token lane / 4, ranks 16j + 2t, + 1 and 16j + 8 + 2t, + 1, high and low part, t = lane % 4
+// (zero past the rank and for tokens without an adapter, whose h is not written).
+template <int J>
+struct EightTokens {
+  int id;
+  uint32_t h[J][4];
+
+  __device__ __forceinline__ void load(const Params &p, int i0, int t1) {
+    const int lane = threadIdx.x & 31;
+    id = token_id(p, i0 + (lane & 7), t1);
+    const bool has = __shfl_sync(0xFFFFFFFFu, id, lane >> 2) >= 0;
+    const uint32_t *hr = reinterpret_cast<const uint32_t *>(p.hl) +
+                         static_cast<int64_t>(i0 + (lane >> 2)) * p.rank_pad + (lane & 3);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const bool in = has && 16 * j < p.rank_pad;
+      h[j][0] = in ? __ldg(hr + 8 * j) : 0u;
+      h[j][1] = in ? __ldg(hr + 8 * j + 4) : 0u;
+      h[j][2] = in ? __ldg(hr + p.rank_pad / 2 + 8 * j) : 0u;
+      h[j][3] = in ? __ldg(hr + p.rank_pad / 2 + 8 * j + 4) : 0u;
+    }
+  }
+};
+
+__device__ __forceinline__ void mma_16x8x16(bool f16, float (&d)[4], const uint32_t (&a)[4],
+                                            uint32_t b0, uint32_t b1) {
+  if (f16)
+    ptx::mma_f16_16x8x16(d, a[0], a[1], a[2], a[3], b0, b1);
+  else
+    ptx::mma_bf16_16x8x16(d, a[0], a[1], a[2], a[3], b0, b1);
+}
+
+// For the eight tokens `now` and the 32 weight rows `quarter` of the boxes: the sums
 // sum_r (hi + lo)[token][r] * B[adapter of the token][row][r], as matrix fragments: lane
-// 4i + t gets tokens 2t, 2t + 1 of rows i + 8k in s[k]; zero for tokens without an adapter. By
-// one epilogue warp; false when a wait ran out.
-__device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring, int i0, int t1,
-                                             int quarter, float2 (&s)[4]) {
+// 4i + t gets tokens 2t, 2t + 1 of rows i + 8k in s[k]; zero for tokens without an adapter. C
+// boxes of 16 J ranks an adapter. By one epilogue warp; false when a wait ran out. The high
+// and the low part have accumulators of their own and a box's fragments are read before its
+// first MMA, so that the chain of dependent MMAs is J long: in one chain with reads between
+// them a box of 32 ranks took 740 cycles.
+template <int J, int C>
+__device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring,
+                                             const EightTokens<J * C> &now, int quarter,
+                                             float2 (&s)[4]) {
   const int lane = threadIdx.x & 31;
   const bool f16 = p.lora_dtype == kF16;
+  const int id = now.id;
 #pragma unroll
   for (int k = 0; k < 4; ++k) s[k] = make_float2(0.0f, 0.0f);
-  const int id = token_id(p, i0 + (lane & 7), t1);
-  uint32_t todo = first_tokens(id);
-  if (todo == 0) return true;
-  // B operand of the product: h of token lane / 4, ranks 16j + 2t, + 1 and 16j + 8 + 2t, + 1,
-  // high and low part (tokens without an adapter: zero, their h is not written)
-  uint32_t h[kLoraMaxRank / 16][4];
-  const bool has = __shfl_sync(0xFFFFFFFFu, id, lane >> 2) >= 0;
-  const uint32_t *hr = reinterpret_cast<const uint32_t *>(p.hl) +
-                       static_cast<int64_t>(i0 + (lane >> 2)) * p.rank_pad + (lane & 3);
-#pragma unroll
-  for (int j = 0; j < kLoraMaxRank / 16; ++j) {
-    const bool in = has && 16 * j < p.rank_pad;
-    h[j][0] = in ? __ldg(hr + 8 * j) : 0u;
-    h[j][1] = in ? __ldg(hr + 8 * j + 4) : 0u;
-    h[j][2] = in ? __ldg(hr + p.rank_pad / 2 + 8 * j) : 0u;
-    h[j][3] = in ? __ldg(hr + p.rank_pad / 2 + 8 * j + 4) : 0u;
-  }
   const int id0 = __shfl_sync(0xFFFFFFFFu, id, 2 * (lane & 3));
   const int id1 = __shfl_sync(0xFFFFFFFFu, id, 2 * (lane & 3) + 1);
-  // ldmatrix: lane 8m + i has row i + 8 (m % 2) of a 16-row tile, 16-byte column 2j + m / 2
+  // ldmatrix: lane 8m + i has row i + 8 (m % 2) of a 16-row tile, 16-byte column 2j + m / 2;
+  // column c of a row lies at c ^ swizzle: address bits 7.. of the row's own (the same for
+  // rows 16 apart)
+  constexpr uint32_t kRow = 32 * J;  // bytes
   const uint32_t row = static_cast<uint32_t>(quarter * 32 + (lane & 7) + (lane & 8));
   const uint32_t col = static_cast<uint32_t>(lane >> 4);
-  // 16-byte column c of a row lies at c ^ swizzle: address bits 7.. of the row's own (the same
-  // for rows 16 apart)
-  const uint32_t row_bytes = ring.box / WROWS;
-  const uint32_t swizzle = row * row_bytes / 128 & (row_bytes / 16 - 1);
-  for (; todo != 0; todo &= todo - 1) {
+  const uint32_t swizzle = row * kRow / 128 & (kRow / 16 - 1);
+#pragma unroll 1
+  for (uint32_t todo = first_tokens(id); todo != 0; todo &= todo - 1) {
     const int a = __shfl_sync(0xFFFFFFFFu, id, __ffs(static_cast<int>(todo)) - 1);
-    float d[2][4];
+    float d[2][2][4];  // [16-row tile][high, low]
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) d[m][e] = 0.0f;
+      for (int e = 0; e < 8; ++e) d[m][e >> 2][e & 3] = 0.0f;
 #pragma unroll
-    for (int c = 0; c < kLoraMaxRank / SUM_RANK; ++c) {
-      if (c * SUM_RANK >= p.R) break;
+    for (int c = 0; c < C; ++c) {
       if (!ptx::mbar_wait_bounded(ring.full(), ring.phase, ring.abort, kWaitLimitNs)) {
         record_timeout(ring.abort);
         return false;
       }
-      const uint32_t box = ring.slots + ring.slot * ring.box + row * row_bytes;
+      const uint32_t box = ring.slots + ring.slot * ring.box + row * kRow;
+      uint32_t w[2][J][4];
 #pragma unroll
-      for (int j = 0; j < SUM_RANK / 16; ++j) {
-        if (c * SUM_RANK + 16 * j >= p.rank_pad) break;
-        const uint32_t *b = h[c * (SUM_RANK / 16) + j];
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          ptx::ldsm_x4(box + m * 16 * kRow + (((2 * j + col) ^ swizzle) << 4), w[m][j]);
+#pragma unroll
+      for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          uint32_t w[4];
-          ptx::ldsm_x4(box + m * 16 * row_bytes + (((2 * j + col) ^ swizzle) << 4), w);
-          if (f16) {
-            ptx::mma_f16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[0], b[1]);
-            ptx::mma_f16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[2], b[3]);
-          } else {
-            ptx::mma_bf16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[0], b[1]);
-            ptx::mma_bf16_16x8x16(d[m], w[0], w[1], w[2], w[3], b[2], b[3]);
-          }
+          const uint32_t(&h)[4] = now.h[c * J + j];
+          mma_16x8x16(f16, d[m][0], w[m][j], h[0], h[1]);
+          mma_16x8x16(f16, d[m][1], w[m][j], h[2], h[3]);
         }
-      }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ring.empty());
       ring.next();
@@ -464,11 +483,39 @@ __device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring, int
     // d[m]: rows i + 16m (0, 1) and i + 16m + 8 (2, 3), tokens 2t (0, 2) and 2t + 1 (1, 3)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (id0 == a) s[k].x = d[k >> 1][2 * (k & 1)];
-      if (id1 == a) s[k].y = d[k >> 1][2 * (k & 1) + 1];
+      const int e = 2 * (k & 1);
+      if (id0 == a) s[k].x = d[k >> 1][0][e] + d[k >> 1][1][e];
+      if (id1 == a) s[k].y = d[k >> 1][0][e + 1] + d[k >> 1][1][e + 1];
     }
   }
   return true;
+}
+
+// All tokens [t0, t1) so, eight at a time: to(i, s) takes the sums of the tokens from t0 + i.
+template <int J, int C, class To>
+__device__ __forceinline__ bool token_sums(const Params &p, SumRing &ring, int t0, int t1,
+                                           int quarter, To &&to) {
+  EightTokens<J * C> now;
+  now.load(p, t0, t1);
+#pragma unroll 1
+  for (int i = 0; t0 + i < t1; i += 8) {
+    EightTokens<J * C> next;  // (under way meanwhile)
+    next.load(p, t0 + i + 8, t1);
+    float2 s[4];
+    if (!adapter_sums<J, C>(p, ring, now, quarter, s)) return false;
+    to(i, s);
+    now = next;
+  }
+  return true;
+}
+
+template <class To>
+__device__ __forceinline__ bool token_sums(const Params &p, SumRing &ring, int t0, int t1,
+                                           int quarter, To &&to) {
+  if (p.R > 64) return token_sums<4, 2>(p, ring, t0, t1, quarter, to);
+  if (p.R > 32) return token_sums<4, 1>(p, ring, t0, t1, quarter, to);
+  if (p.R > 16) return token_sums<2, 1>(p, ring, t0, t1, quarter, to);
+  return token_sums<1, 1>(p, ring, t0, t1, quarter, to);
 }
 
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -792,10 +839,18 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
       float2 sum[kLoraMixed / 8][4];  // a mixed tile's adapter sums, [g][k] as v below
       if constexpr (LORA) {
         if (q.adapter == -2) {
-          bool ok = true;
 #pragma unroll
           for (int g = 0; g < kLoraMixed / 8; ++g)
-            ok = ok && adapter_sums(p, ring, q.t0 + 8 * g, q.t1, quarter, sum[g]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[g][k] = make_float2(0.0f, 0.0f);
+          // (the index of a register array has to be known: one of four gets the sums)
+          const bool ok = token_sums(p, ring, q.t0, q.t1, quarter, [&](int i, float2(&s)[4]) {
+#pragma unroll
+            for (int g = 0; g < kLoraMixed / 8; ++g)
+              if (i == 8 * g)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum[g][k] = s[k];
+          });
           if (!ok) break;
         }
       }
@@ -1097,18 +1152,15 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     if constexpr (LORA) {
       // (a warp writes and reads back its own rows only; after a wait that ran out, whatever)
       SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
-      bool ok = true;
-      for (int i = a0; i < a1 && ok; i += 8) {
-        float2 s[4];
-        ok = adapter_sums(p, ring, q.t0 + i, q.t0 + a1, quarter, s);
-        float *to = lora + (i - a0 + 2 * (lane & 3)) * WROWS + quarter * 32 + (lane >> 2);
-        const float2 hs = *reinterpret_cast<const float2 *>(e_hs + i + 2 * (lane & 3));
+      token_sums(p, ring, q.t0 + a0, q.t0 + a1, quarter, [&](int i, float2(&s)[4]) {
+        float *to = lora + (i + 2 * (lane & 3)) * WROWS + quarter * 32 + (lane >> 2);
+        const float2 hs = *reinterpret_cast<const float2 *>(e_hs + a0 + i + 2 * (lane & 3));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           to[8 * k] = s[k].x * hs.x;
           to[8 * k + WROWS] = s[k].y * hs.y;
         }
-      }
+      });
       __syncwarp();
     }
     // TMEM (lane = weight row, column = token) -> the part of the CTA that reduces the row,

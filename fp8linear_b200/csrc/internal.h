@@ -191,18 +191,19 @@ cudaError_t read_rowsel_status(unsigned int *bits, bool clear);
 //   hl [M][2 * rank_pad] of x's type: h / hscale as a high and a low part, h = hscale *
 //   (hi + lo) to fp32's last bits; hscale fp32 [M], powers of two. Rows without an adapter
 //   are not written;
-//   plan int4: plan[0].x tiles follow, each {first token, end, adapter, 0}. A run of at least
+//   plan int4: {tiles of one adapter, tiles of several}, then the tiles {first token, end,
+//   adapter, 0}, those of several adapters from entry lora_plan_mixed(M) on. A run of at least
 //   kLoraMixed rows with one adapter is cut into tiles of its own (adapter -1: none), of at
 //   most kLoraTileTokens; what lies between such runs goes in tiles of at most kLoraMixed
 //   tokens with any adapters (adapter -2).
 inline int64_t lora_rank_pad(int64_t R) { return (R + 15) / 16 * 16; }
 constexpr int kLoraTileTokens = 160;
 constexpr int kLoraMixed = 32;
-// Entries of the plan at most: runs of one adapter, kLoraTileTokens each but for their last
-// tiles (M / 32 runs); as many gaps between them and one more; kLoraMixed tokens each but for
-// their last tiles.
+// At most M / 32 runs, of kLoraTileTokens each but for their last tiles; as many gaps between
+// them and one more, of kLoraMixed tokens each but for their last tiles.
+inline int64_t lora_plan_mixed(int64_t M) { return 1 + M / kLoraTileTokens + M / kLoraMixed; }
 inline int64_t lora_plan_max(int64_t M) {
-  return M <= kLoraRowsMaxM ? 0 : 1 + M / kLoraTileTokens + 3 * (M / kLoraMixed) + 1;
+  return M <= kLoraRowsMaxM ? 0 : lora_plan_mixed(M) + 2 * (M / kLoraMixed) + 1;
 }
 struct LoraWorkspace {
   void *hl = nullptr;

@@ -46,6 +46,7 @@ struct Params {
   void *hl;
   float *hscale;
   int4 *plan;      // null: not wanted
+  int plan_mixed;
   int split, k_blocks;
   int x_rows;      // rows of x's box
   int cols;        // columns per pass
@@ -89,10 +90,11 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // crosses a border between blocks of 32 rows, so of a block's runs only the one carried in and
 // the one carried on can be long.
 __device__ __forceinline__ void make_plan(const Params &p, int lane) {
-  int n = 0;
+  int n_one = 0, n_mixed = 0;
   auto emit = [&](int t0, int t1, int a) {
-    ++n;
-    if (lane == 0) p.plan[n] = make_int4(t0, t1, a, 0);
+    const int at = a == -2 ? p.plan_mixed + n_mixed : 1 + n_one;
+    ++(a == -2 ? n_mixed : n_one);
+    if (lane == 0) p.plan[at] = make_int4(t0, t1, a, 0);
   };
   int open = -1, open_end = 0;  // rows of short runs not yet in a tile
   auto flush = [&]() {
@@ -151,7 +153,7 @@ __device__ __forceinline__ void make_plan(const Params &p, int lane) {
   const int tail = __ldg(p.ids + min(start, p.M - 1));
   add_run(start, p.M, has_adapter(p, tail) ? tail : -1);
   flush();
-  if (lane == 0) p.plan[0] = make_int4(n, 0, 0, 0);
+  if (lane == 0) p.plan[0] = make_int4(n_one, n_mixed, 0, 0);
 }
 
 // At most how many adapters the 128 rows from m0 have, by a whole warp: exact where an
@@ -573,6 +575,7 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   p.hl = w.hl;
   p.hscale = w.hscale;
   p.plan = w.plan;
+  p.plan_mixed = static_cast<int>(lora_plan_mixed(a.M));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cudaError_t e;
@@ -591,8 +594,9 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   p.split = split;
   // a cluster per tile, and further ones for the passes of tiles with many adapters while CTAs
   // are left over still
-  // (few rows: narrower passes, that more clusters share them)
-  p.cols = a.M <= ROWS ? 128 : COLS;
+  // (few tiles: narrower passes, that more clusters share them; many: a tile at the border of
+  // two requests in one pass)
+  p.cols = split >= 4 ? COLS / 2 : COLS;
   const int per_pass = p.cols / p.rank_pad;
   p.tiles = static_cast<int>(tiles);
   p.max_passes = static_cast<int>((std::min<int64_t>(a.L, ROWS) + per_pass - 1) / per_pass);

@@ -85,6 +85,7 @@ struct Params {
   int lora_dtype;
   int L, R, rank_pad;
   const int4 *plan;  // token tiles (persist_kernel)
+  int plan_mixed;    // .. of several adapters: from this entry on
   const void *hl;
   const float *hscale;
 };
@@ -185,7 +186,6 @@ struct Tile {
   int wb;      // block of weight rows
   int t0, t1;  // tokens
   int nn;      // MMA N: tokens padded to a multiple of 16 x CG
-  int tb;      // token block within the group
   int adapter; // of all its tokens, -1: none, -2: several
 };
 
@@ -202,43 +202,51 @@ __device__ __forceinline__ Tile find_tile(const Params &p, int tok_max, const in
   const int l = t - tile[e];
   // The larger operand of the group streams once, the tiles that run side by side share the
   // smaller one through L2.
+  int tb;
   if (rows >= p.N) {
-    q.tb = l / p.n_wb;
-    q.wb = l - q.tb * p.n_wb;
+    tb = l / p.n_wb;
+    q.wb = l - tb * p.n_wb;
   } else {
     q.wb = l / n_tb;
-    q.tb = l - q.wb * n_tb;
+    tb = l - q.wb * n_tb;
   }
-  q.t0 = r0 + q.tb * per;
+  q.t0 = r0 + tb * per;
   q.t1 = min(r0 + rows, q.t0 + per);
   q.nn = (q.t1 - q.t0 + 16 * CG - 1) / (16 * CG) * (16 * CG);
   q.adapter = -1;
   return q;
 }
 
-// The tiles of a call with adapters, from the plan. Each step also loads the next tile's
-// entry, which is then at hand without a wait.
+// The tiles of a call with adapters, from the plan: first those of several adapters (they take
+// longest, and this way no CTA pair gets a second one before all have one), then the others
+// in the order of find_tile. Each step also loads the next tile's entry, which is then at hand
+// without a wait.
 struct PlanWalk {
-  int n_tb, num_tiles;
+  int n_one, first_one, num_tiles;  // token blocks and first tile of one adapter
   int4 next;
 
-  __device__ __forceinline__ int token_block(const Params &p, int t) const {
-    return p.M >= p.N ? t / p.n_wb : t % n_tb;
+  __device__ __forceinline__ int weight_block(const Params &p, int t) const {
+    if (t < first_one) return t % p.n_wb;
+    return p.M >= p.N ? (t - first_one) % p.n_wb : (t - first_one) / n_one;
   }
   __device__ __forceinline__ void load(const Params &p, int t) {
-    if (t < num_tiles) next = __ldg(p.plan + 1 + token_block(p, t));
+    if (t >= num_tiles) return;
+    const int l = t - first_one;
+    next = __ldg(p.plan + (l < 0 ? p.plan_mixed + t / p.n_wb
+                                 : 1 + (p.M >= p.N ? l / p.n_wb : l % n_one)));
   }
   __device__ __forceinline__ void start(const Params &p, int t) {
-    n_tb = __ldg(&p.plan->x);
-    num_tiles = n_tb * p.n_wb;
+    const int4 head = __ldg(p.plan);
+    n_one = head.x;
+    first_one = head.y * p.n_wb;
+    num_tiles = first_one + n_one * p.n_wb;
     load(p, t);
   }
   template <int CG>
   __device__ __forceinline__ Tile take(const Params &p, int t, int step) {
     Tile q;
     q.e = 0;
-    q.tb = token_block(p, t);
-    q.wb = p.M >= p.N ? t - q.tb * p.n_wb : t / n_tb;
+    q.wb = weight_block(p, t);
     q.t0 = next.x;
     q.t1 = next.y;
     q.adapter = next.z;
@@ -1495,6 +1503,7 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   p.R = static_cast<int>(a.R);
   p.rank_pad = static_cast<int>(rp);
   p.plan = w.plan;
+  p.plan_mixed = static_cast<int>(lora_plan_mixed(a.M));
   p.hl = w.hl;
   p.hscale = w.hscale;
   const int rows = few ? WROWS : 2 * WROWS;

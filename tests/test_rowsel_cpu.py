@@ -111,10 +111,10 @@ def test_lora_workspace_size(api):
     assert size(0, 32, 16) == 0
     assert size(5, 64, 0) == api.workspace_size(5, 64)
     # h in two parts with the rank padded to 16 and a scale per row; above 128 rows the plan of
-    # the token tiles (16 bytes each; at most one of 160 tokens a full 160, and for each 32
-    # rows a run's last tile, a gap's and a gap's last); all rounded up to 256 bytes
+    # the token tiles (16 bytes each: a header, tiles of 160 and one per 32 rows for the runs'
+    # ends, two per 32 rows and one for the gaps); all rounded up to 256 bytes
     base = api.workspace_size(128, 64)
     assert size(128, 64, 24) - base == 128 * 2 * 32 * 2 + 512
     base = api.workspace_size(1000, 64)
-    plan = 16 * (1 + 1000 // 160 + 3 * (1000 // 32) + 1)
+    plan = 16 * (1 + 1000 // 160 + 1000 // 32 + 2 * (1000 // 32) + 1)
     assert size(1000, 64, 24) - base == 1000 * 128 + 4096 + (plan + 255) // 256 * 256

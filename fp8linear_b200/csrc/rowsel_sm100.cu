@@ -936,9 +936,11 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
                   *reinterpret_cast<const uint4 *>(box + m * BOX_PITCH + col * 2);
           }
         } else if (n0 + lane < p.N) {
-          for (int m = 0; m < 32 && c + m < cnt; ++m)
-            out[static_cast<int64_t>(m) * p.N + lane] =
-                *reinterpret_cast<const uint16_t *>(box + m * BOX_PITCH + lane * 2);
+#pragma unroll 8
+          for (int m = 0; m < 32; ++m) {
+            const uint16_t v = *reinterpret_cast<const uint16_t *>(box + m * BOX_PITCH + lane * 2);
+            if (c + m < cnt) out[static_cast<int64_t>(m) * p.N + lane] = v;
+          }
         }
       }
       ptx::tc_fence_before();
@@ -1211,28 +1213,60 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
   __syncthreads();
   ptx::cluster_sync();  // the partial sums of this CTA's rows have arrived
 
-  for (int idx = threadIdx.x; idx < cnt * quads; idx += blockDim.x) {
-    const int m = idx / quads;
-    const int qd = idx - m * quads;
+  // A task is 4 rows (output columns) of one token: 8 bytes of output.
+  const bool wide = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
+  const int step = static_cast<int>(blockDim.x);
+  const int step_m = quads > 0 ? step / quads : 0, step_q = step - step_m * quads;
+  int m = quads > 0 ? static_cast<int>(threadIdx.x) / quads : cnt;
+  int qd = static_cast<int>(threadIdx.x) - m * quads;
+#pragma unroll 2
+  while (m < cnt) {
+    float4 v[SPLIT_MAX];
+#pragma unroll
+    for (int s = 0; s < SPLIT_MAX; ++s)
+      if (s < p.split)
+        v[s] = *reinterpret_cast<const float4 *>(part + (s * p.tok_cap + m) * R + 4 * qd);
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < SPLIT_MAX; ++s)
       if (s < p.split) {
-        const float4 v =
-            *reinterpret_cast<const float4 *>(part + (s * p.tok_cap + m) * R + 4 * qd);
-        a[0] += v.x;
-        a[1] += v.y;
-        a[2] += v.z;
-        a[3] += v.w;
+        a[0] += v[s].x;
+        a[1] += v[s].y;
+        a[2] += v[s].z;
+        a[3] += v[s].w;
       }
     const float xs = e_xs[m];
+    const float4 w = *reinterpret_cast<const float4 *>(e_ws + 4 * qd);
+    const float4 b = *reinterpret_cast<const float4 *>(e_b + 4 * qd);
+    if constexpr (LORA) {
+      a[0] += b.x;
+      a[1] += b.y;
+      a[2] += b.z;
+      a[3] += b.w;
+    } else {
+      a[0] = fmaf(a[0] * xs, w.x, b.x);
+      a[1] = fmaf(a[1] * xs, w.y, b.y);
+      a[2] = fmaf(a[2] * xs, w.z, b.z);
+      a[3] = fmaf(a[3] * xs, w.w, b.w);
+    }
+    const int n = n0 + r0 + 4 * qd;
+    const int64_t o = static_cast<int64_t>(q.t0 + m) * p.N + n;
+    if (wide) {
+      if (n < p.N)
+        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p.out) + o) =
+            p.out_dtype == kF16
+                ? make_uint2(ptx::pack_f16x2(a[0], a[1]), ptx::pack_f16x2(a[2], a[3]))
+                : make_uint2(ptx::pack_bf16x2(a[0], a[1]), ptx::pack_bf16x2(a[2], a[3]));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int nl = 4 * qd + i;
-      const int n = n0 + r0 + nl;
-      if (n >= p.N) break;
-      const float val = LORA ? a[i] + e_b[nl] : fmaf(a[i] * xs, e_ws[nl], e_b[nl]);
-      store_out(p.out, p.out_dtype, static_cast<int64_t>(q.t0 + m) * p.N + n, val);
+      for (int i = 0; i < 4; ++i)
+        if (n + i < p.N) store_out(p.out, p.out_dtype, o + i, a[i]);
+    }
+    m += step_m;
+    qd += step_q;
+    if (qd >= quads) {
+      qd -= quads;
+      ++m;
     }
   }
   zero_rows(p, g_row, 0, blockDim.x);
@@ -1366,24 +1400,29 @@ SplitInfo &split_info(const DeviceInfo &dev) {
   return si;
 }
 
-template <bool LORA>
-int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const DeviceInfo &dev,
-                 cudaStream_t stream, bool pdl) {
-  SplitInfo &si = split_info<LORA>(dev);
-  if (si.err != cudaSuccess) return launch_failed(op, si.err);
-  // The K-split that takes the least time: waves of clusters, each as long as its K-blocks
-  // and a set-up and reduction worth about SPLIT_COST of them; at least two K-blocks a CTA.
+// The K-split that takes the least time: waves of clusters, each as long as its K-blocks and a
+// set-up and reduction worth about SPLIT_COST of them; at least two K-blocks a CTA.
+int best_split(const SplitInfo &si, int64_t tiles, int k_blocks) {
   int best = 1;
   int64_t least = INT64_MAX;
-  for (int s = 1; s <= SPLIT_MAX && s <= std::max(1, p.k_blocks / 2); ++s) {
+  for (int s = 1; s <= SPLIT_MAX && s <= std::max(1, k_blocks / 2); ++s) {
     if (si.clusters[s] < 1) continue;
     const int64_t waves = (tiles + si.clusters[s] - 1) / si.clusters[s];
-    const int64_t cost = waves * ((p.k_blocks + s - 1) / s + SPLIT_COST);
+    const int64_t cost = waves * ((k_blocks + s - 1) / s + SPLIT_COST);
     if (cost < least) {
       least = cost;
       best = s;
     }
   }
+  return best;
+}
+
+template <bool LORA>
+int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const DeviceInfo &dev,
+                 cudaStream_t stream, bool pdl) {
+  SplitInfo &si = split_info<LORA>(dev);
+  if (si.err != cudaSuccess) return launch_failed(op, si.err);
+  const int best = best_split(si, tiles, p.k_blocks);
   p.kps = (p.k_blocks + best - 1) / best;
   p.split = (p.k_blocks + p.kps - 1) / p.kps;
   const uint32_t stage = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
@@ -1458,8 +1497,14 @@ int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl) {
     set_error(std::string(op) + ": too many output tiles");
     return 2;
   }
-  const bool split = ub1 <= dev.sm_count;
-  const bool pairs = !split && a.M / live >= 48;
+  // Few tiles: split K, where that gives every tile two CTAs at least (one alone is faster in
+  // the persistent kernel: 512 rows of 4 experts, 2048 x 2048, 17.0 us against 9.4). CTA pairs
+  // from 100 rows an expert on: 16 experts of 4096 x 4096 with 64 rows each take 48.3 us with
+  // single CTAs and 48.7 with pairs, with 128 rows 55.1 and 52.8, with 256 rows 88.8 and 67.6.
+  const SplitInfo &si = split_info<false>(dev);
+  if (si.err != cudaSuccess) return launch_failed(op, si.err);
+  const bool split = ub1 <= dev.sm_count && best_split(si, ub1, p.k_blocks) > 1;
+  const bool pairs = !split && a.M / live >= 100;
   p.tok_cap = split ? static_cast<int>(std::min<int64_t>((a.M + 15) / 16 * 16, SPLIT_TOK)) : 128;
   std::string err;
   Maps maps = {};

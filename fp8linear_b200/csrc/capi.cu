@@ -807,10 +807,12 @@ int fp8lin_fp8_linear_lora(const void *x, int x_dtype, const void *wq, const flo
   a.N = N;
   a.K = K;
   a.workspace = xq + fp8lin_linear_workspace_size(M, K);
-  // the kernels before are this call's quantizer and down projection
+  // the kernels before are this call's quantizer and, if any, down projection
   a.weights_before_wait = true;
-  rc = launch_lora_down(a, s);
-  if (rc != FP8LIN_OK) return rc;
+  if (!lora_own_down(M, N, K, R)) {
+    rc = launch_lora_down(a, s);
+    if (rc != FP8LIN_OK) return rc;
+  }
   return launch_lora_gemm(a, s, true);
 }
 

@@ -182,6 +182,10 @@ struct LoraArgs {
   void *workspace;       // lora_workspace_bytes(M, R), 256-byte aligned
   bool weights_before_wait = false;
 };
+// A call of few tokens and ranks has no down projection of its own: the GEMM's CTAs multiply
+// their K ranges of x and A, each weight tile's anew. The K-split's CTAs decide.
+constexpr int kLoraOwnTokens = 8;
+bool lora_own_down(int64_t M, int64_t N, int64_t K, int64_t R);
 int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl);
 cudaError_t read_rowsel_status(unsigned int *bits, bool clear);
 

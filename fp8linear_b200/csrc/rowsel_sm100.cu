@@ -88,6 +88,12 @@ struct Params {
   int plan_mixed;    // .. of several adapters: from this entry on
   const void *hl;
   const float *hscale;
+  // few tokens: the down projection is the GEMM's own (split_kernel)
+  int own_down;
+  const void *x;       // [M][K] of lora_dtype
+  const void *lora_a;  // [L][R][K]
+  const float *scaling;
+  int K;
 };
 
 __device__ __forceinline__ float load_bias(const void *bias, int dtype, int64_t n) {
@@ -524,6 +530,91 @@ __device__ __forceinline__ bool token_sums(const Params &p, SumRing &ring, int t
   if (p.R > 32) return token_sums<4, 1>(p, ring, t0, t1, quarter, to);
   if (p.R > 16) return token_sums<2, 1>(p, ring, t0, t1, quarter, to);
   return token_sums<1, 1>(p, ring, t0, t1, quarter, to);
+}
+
+// Eight 16-bit values as floats.
+__device__ __forceinline__ void unpack8(const uint4 &v, bool f16, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (f16) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    } else {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+
+// A few tokens' adapters without a down projection of their own (a launch, and a wait for it,
+// longer than all of this): a CTA of the K-split multiplies its K range of x with that of A
+// and the result with B; the partial results add up with the partial tiles, since both
+// products are linear. CUDA cores, fp32 throughout. Nothing here depends on the quantizer, so
+// it comes before the dependency wait. out[m][row] for the CTA's 128 rows; `h`: M x R floats
+// of shared memory.
+constexpr int OWN_TOKENS = kLoraOwnTokens;
+__device__ __forceinline__ void own_adapter_sums(const Params &p, int k0, int k1, int n, float *h,
+                                                 float *out, int et, int row) {
+  const bool f16 = p.lora_dtype == kF16;
+  const int warp = et >> 5, lane = et & 31;
+  const int chunks = p.K / 8;  // 16-byte chunks of a row of x or A; K % 16 == 0
+  const int c1 = min(k1, p.K) / 8;
+  const uint4 *x4 = reinterpret_cast<const uint4 *>(p.x);
+  const uint4 *a4 = reinterpret_cast<const uint4 *>(p.lora_a);
+  // four values of h at a time (R % 8 == 0: of one token), so that their loads run side by side
+#pragma unroll 1
+  for (int v = 4 * warp; v < p.M * p.R; v += 4 * EPI_WARPS) {
+    const int m = v / p.R, r = v - m * p.R;
+    const int id = token_id(p, m, p.M);
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (id >= 0) {
+#pragma unroll 2
+      for (int c = k0 / 8 + lane; c < c1; c += 32) {
+        float xv[8];
+        uint4 av[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          av[i] = __ldg(a4 + (static_cast<int64_t>(id) * p.R + r + i) * chunks + c);
+        unpack8(__ldg(x4 + static_cast<int64_t>(m) * chunks + c), f16, xv);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[8];
+          unpack8(av[i], f16, f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[i] = fmaf(xv[j], f[j], s[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s[i] += __shfl_xor_sync(0xFFFFFFFFu, s[i], d);
+      const float sc = __ldg(p.scaling + id);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] *= sc;
+    }
+    if (lane == 0) *reinterpret_cast<float4 *>(h + v) = make_float4(s[0], s[1], s[2], s[3]);
+  }
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  const uint16_t *lb = reinterpret_cast<const uint16_t *>(p.lora_b);
+#pragma unroll 1
+  for (int m = 0; m < p.M; ++m) {
+    const int id = token_id(p, m, p.M);
+    float s = 0.0f;
+    if (id >= 0) {
+      const uint4 *b4 = reinterpret_cast<const uint4 *>(
+          lb + (static_cast<int64_t>(id) * p.N + min(n, p.N - 1)) * p.R);
+#pragma unroll 4
+      for (int c = 0; c < p.R / 8; ++c) {
+        float f[8];
+        unpack8(__ldg(b4 + c), f16, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(h[m * p.R + 8 * c + j], f[j], s);
+      }
+    }
+    out[m * WROWS + row] = s;
+  }
 }
 
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -1065,6 +1156,11 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
   ptx::tc_fence_after();
   const uint32_t tmem = static_cast<uint32_t>(ptx::uniform(static_cast<int>(*tmem_slot)));
   ptx::cluster_arrive_release();  // (waited for before the first push: all CTAs have started)
+  if (LORA && p.own_down && warp >= 2 && warp < 2 + EPI_WARPS) {
+    const int row = (warp & 3) * 32 + lane;
+    own_adapter_sums(p, kb0 * BK, (kb0 + nkb) * BK, q.wb * WROWS + row,
+                     reinterpret_cast<float *>(smem + p.off_ring), lora, threadIdx.x - 64, row);
+  }
   if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
@@ -1075,9 +1171,11 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
   const int quads = r1 > r0 ? (r1 - r0) >> 2 : 0;
   const int n0 = q.wb * WROWS;
 
-  // Adapters: the cluster's CTAs share out the tokens, eight at a time.
+  // Adapters: the cluster's CTAs share out the tokens, eight at a time (own_down: all tokens,
+  // but only this CTA's K range of them).
+  const bool own = LORA && p.own_down;
   const int per_cta = LORA ? ((cnt + 7) / 8 + p.split - 1) / p.split * 8 : 0;
-  const int a0 = min(cnt, rank * per_cta), a1 = min(cnt, a0 + per_cta);
+  const int a0 = own ? 0 : min(cnt, rank * per_cta), a1 = own ? cnt : min(cnt, a0 + per_cta);
 
   if (warp == 0) {
     const bool elected = ptx::elect_one();
@@ -1137,7 +1235,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     }
   } else if (LORA && warp == 2 + EPI_WARPS) {
     SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
-    feed_sums(p, &maps.ls, ring, q.t0 + a0, q.t0 + a1, n0);
+    if (!own) feed_sums(p, &maps.ls, ring, q.t0 + a0, q.t0 + a1, n0);
     drain_sums(ring);
   } else {
     // xs (adapters: and hscale) of the tokens, weight scales and biases of the rows reduced
@@ -1146,7 +1244,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     for (int i = et; i < q.nn; i += 128) {
       e_xs[i] = i < cnt ? __ldg(p.xs + q.t0 + i) : 0.0f;
       if constexpr (LORA)
-        e_hs[i] = token_id(p, q.t0 + i, q.t1) >= 0 ? __ldg(p.hscale + q.t0 + i) : 0.0f;
+        e_hs[i] = !own && token_id(p, q.t0 + i, q.t1) >= 0 ? __ldg(p.hscale + q.t0 + i) : 0.0f;
     }
     for (int i = et; i < r1 - r0; i += 128) {
       const int n = n0 + r0 + i;
@@ -1159,7 +1257,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     const int n = n0 + row;
     const float w = LORA && n < p.N ? __ldg(p.ws + n) : 1.0f;
     epilogue_sync();  // xs and hscale are in shared memory
-    if constexpr (LORA) {
+    if (LORA && !own) {
       // (a warp writes and reads back its own rows only; after a wait that ran out, whatever)
       SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
       token_sums(p, ring, q.t0 + a0, q.t0 + a1, quarter, [&](int i, float2(&s)[4]) {
@@ -1429,7 +1527,10 @@ int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const D
   const uint32_t rows = static_cast<uint32_t>(((WROWS + p.split - 1) / p.split + 3) & ~3);
   const uint32_t part = static_cast<uint32_t>(p.split * p.tok_cap) * rows * 4;
   const uint32_t lora =
-      LORA ? static_cast<uint32_t>((p.tok_cap / 8 + p.split - 1) / p.split * 8) * WROWS * 4 : 0;
+      LORA ? static_cast<uint32_t>(std::max((p.tok_cap / 8 + p.split - 1) / p.split * 8,
+                                            p.own_down ? OWN_TOKENS : 0)) *
+                 WROWS * 4
+           : 0;
   const uint32_t tab = static_cast<uint32_t>(p.E + 1) * 8 + 16 + SPLIT_EPI;
   const uint32_t ring = LORA ? SUM_RING : 0u;
   const uint32_t room = SPLIT_SMEM - 2048 - ring - part - lora - tab;
@@ -1520,6 +1621,23 @@ int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl) {
   return launch_persist<2, false>(op, maps, p, wb2 * (live + a.M / 256), dev, stream, pdl);
 }
 
+// Down to here a CTA's values of h times its K-blocks are done before the K-blocks have
+// arrived: 4096 -> 4096 (8 K-blocks a CTA), one token, rank 16: 10.2 us against 16.0 with a down
+// projection of its own; two tokens 12.2 against 16.7; one token, rank 64: 15.7 against 16.5,
+// rank 128: 22.5 against 17.3.
+constexpr int64_t OWN_WORK = 384;
+
+bool lora_own_down(int64_t M, int64_t N, int64_t K, int64_t R) {
+  using namespace rowsel;
+  DeviceInfo dev;
+  if (M > kLoraOwnTokens || !current_device_info(&dev)) return false;
+  const SplitInfo &si = split_info<true>(dev);
+  if (si.err != cudaSuccess) return false;
+  const int k_blocks = static_cast<int>((K + BK - 1) / BK);
+  const int split = best_split(si, (N + WROWS - 1) / WROWS, k_blocks);
+  return M * R * ((k_blocks + split - 1) / split) <= OWN_WORK;
+}
+
 int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   using namespace rowsel;
   const char *op = "fp8_linear_lora";
@@ -1547,6 +1665,11 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   p.L = static_cast<int>(a.L);
   p.R = static_cast<int>(a.R);
   p.rank_pad = static_cast<int>(rp);
+  p.own_down = lora_own_down(a.M, a.N, a.K, a.R) ? 1 : 0;
+  p.x = a.x;
+  p.lora_a = a.lora_a;
+  p.scaling = a.scaling;
+  p.K = static_cast<int>(a.K);
   p.plan = w.plan;
   p.plan_mixed = static_cast<int>(lora_plan_mixed(a.M));
   p.hl = w.hl;

@@ -71,6 +71,18 @@ def test_lora(K, N, L, R, pairs, dtype):
     check(out, *lora_ref(x, wq, ws, a, b, ids, sc, bias))
 
 
+@pytest.mark.parametrize("M,K,R", [(1, 16, 128), (1, 4112, 128), (2, 2064, 64), (7, 144, 16),
+                                   (8, 1040, 16), (8, 1040, 24), (9, 1040, 8), (1, 272, 8)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_tokens(M, K, R, dtype):
+    """Both sides of the border below which the GEMM computes x . A^T itself."""
+    x, wq, ws, a, b, sc, bias = make(M + K + R, M, K, 392, 5, R, dtype, bias=torch.float32)
+    ids = (torch.arange(M, device="cuda", dtype=torch.int32) * 2) % 6 - 1
+    ids[0] = 4
+    check(f.fp8_linear_lora(x, wq, ws, a, b, ids, sc, bias),
+          *lora_ref(x, wq, ws, a, b, ids, sc, bias))
+
+
 @pytest.mark.parametrize("M", [5, 128, 129, 1000])
 def test_rows_in_any_order(M):
     g = torch.Generator(device="cuda").manual_seed(M)

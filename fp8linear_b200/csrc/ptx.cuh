@@ -144,6 +144,13 @@ __device__ __forceinline__ void tma_prefetch_2d(const void *tmap, int32_t x, int
                : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch_3d(const void *tmap, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
 // Brings `bytes` contiguous bytes at `src` into L2 (address 16-byte aligned, size a
 // multiple of 16). L2 is where every SM's accesses to device memory meet, so a prefetch
 // issued before a programmatic dependency wait is safe even for data the previous kernel

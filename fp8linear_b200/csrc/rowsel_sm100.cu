@@ -371,6 +371,14 @@ __device__ __forceinline__ bool feed_sums(const Params &p, const CUtensorMap *ma
                                           int t0, int t1, int n0) {
   const int lane = threadIdx.x & 31;
   const bool elected = ptx::elect_one();
+  // all of them into L2 first: three to eight boxes under way do not cover a trip to memory
+  for (int i = t0; i < t1; i += 32) {
+    const int id = token_id(p, i + lane, t1);
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, id);
+    if (id >= 0 && __ffs(static_cast<int>(same)) - 1 == lane)
+      for (int rc = 0; rc < p.R; rc += SUM_RANK) ptx::tma_prefetch_3d(map, rc, n0, id);
+    __syncwarp();
+  }
   int next = token_id(p, t0 + (lane & 7), t1);
   for (int i = t0; i < t1; i += 8) {
     const int id = next;
@@ -708,7 +716,31 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
   ptx::tc_fence_after();
   const uint32_t tmem_base = static_cast<uint32_t>(ptx::uniform(static_cast<int>(*tmem_slot)));
 
-  if (!LORA && p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
+  // Weights and offsets that cannot depend on the kernel before: the first tile's first weight
+  // boxes go out at once, their stages armed for the token boxes too.
+  int ahead = 0;
+  if (!LORA && p.pre_w) {
+    build_groups(p, C::TOK_MAX, g_row, g_tile);
+    if (warp == 0 && group < g_tile[p.E]) {
+      int e = 0;
+      const Tile q = find_tile<CG>(p, C::TOK_MAX, g_row, g_tile, group, e);
+      const uint32_t tx = CG * W_STAGE + static_cast<uint32_t>(ptx::uniform(q.nn)) * BK;
+      const int wz = ptx::uniform(q.e);
+      const int wrow = (ptx::uniform(q.wb) * CG + static_cast<int>(rank)) * WROWS;
+      const uint32_t fl = CG == 1 ? bar_full : ptx::map_shared_rank(bar_full, 0);
+      ahead = min(C::STAGES, p.k_blocks);
+      if (ptx::elect_one())
+        for (int s = 0; s < ahead; ++s) {
+          if (leader) ptx::mbar_arrive_expect_tx(bar_full + 8 * s, tx);
+          const uint32_t dst = sbase + static_cast<uint32_t>(s) * C::STAGE;
+          if constexpr (CG == 1)
+            ptx::tma_load_3d(dst, &maps.w, s * BK, wrow, wz, fl + 8 * s);
+          else
+            ptx::tma_load_3d_pair(dst, &maps.w, s * BK, wrow, wz, fl + 8 * s);
+        }
+      __syncwarp();
+    }
+  }
   if (p.pdl) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   if (!LORA && !p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
@@ -747,15 +779,19 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
         const uint32_t dst = sbase + static_cast<uint32_t>(stage) * C::STAGE;
         const uint32_t fl = full_leader + 8 * stage;
         if (elected) {
-          if (leader) ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, tx);
-          if constexpr (CG == 1) {
-            ptx::tma_load_3d(dst, mw, wx, wrow, z, fl);
-            ptx::tma_load_2d(dst + W_STAGE, mx, xx, xrow, fl);
-          } else {
-            ptx::tma_load_3d_pair(dst, mw, wx, wrow, z, fl);
-            ptx::tma_load_2d_pair(dst + W_STAGE, mx, xx, xrow, fl);
+          if (ahead == 0) {
+            if (leader) ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, tx);
+            if constexpr (CG == 1)
+              ptx::tma_load_3d(dst, mw, wx, wrow, z, fl);
+            else
+              ptx::tma_load_3d_pair(dst, mw, wx, wrow, z, fl);
           }
+          if constexpr (CG == 1)
+            ptx::tma_load_2d(dst + W_STAGE, mx, xx, xrow, fl);
+          else
+            ptx::tma_load_2d_pair(dst + W_STAGE, mx, xx, xrow, fl);
         }
+        if (ahead > 0) --ahead;  // (armed, its weights under way)
         ++issued;
         if (++stage == C::STAGES) {
           stage = 0;
@@ -1027,11 +1063,14 @@ __global__ void __launch_bounds__(Cfg<CG, LORA>::THREADS, 1)
                   *reinterpret_cast<const uint4 *>(box + m * BOX_PITCH + col * 2);
           }
         } else if (n0 + lane < p.N) {
-#pragma unroll 8
-          for (int m = 0; m < 32; ++m) {
-            const uint16_t v = *reinterpret_cast<const uint16_t *>(box + m * BOX_PITCH + lane * 2);
-            if (c + m < cnt) out[static_cast<int64_t>(m) * p.N + lane] = v;
-          }
+          uint16_t v[32];
+#pragma unroll
+          for (int m = 0; m < 32; ++m)
+            v[m] = *reinterpret_cast<const uint16_t *>(box + m * BOX_PITCH + lane * 2);
+          uint16_t *to = out + lane;
+#pragma unroll
+          for (int m = 0; m < 32; ++m, to += p.N)
+            if (c + m < cnt) *to = v[m];
         }
       }
       ptx::tc_fence_before();

@@ -889,10 +889,10 @@ bool make_tmap_2d_sw128(CUtensorMap *map, CUtensorMapDataType dtype, const void 
                             CU_TENSOR_MAP_SWIZZLE_128B, err);
 }
 
-bool make_tmap_3d_sw128(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
-                        uint64_t inner, uint64_t mid, uint64_t outer, uint64_t mid_bytes,
-                        uint64_t outer_bytes, uint32_t box_inner, uint32_t box_mid,
-                        std::string *err) {
+bool make_tmap_3d_swizzled(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
+                           uint64_t inner, uint64_t mid, uint64_t outer, uint64_t mid_bytes,
+                           uint64_t outer_bytes, uint32_t box_inner, uint32_t box_mid,
+                           int swizzle, std::string *err) {
   auto fn = gemm::encode_fn();
   if (!fn) {
     *err = "cuTensorMapEncodeTiled is unavailable (driver entry point query failed)";
@@ -903,7 +903,10 @@ bool make_tmap_3d_sw128(CUtensorMap *map, CUtensorMapDataType dtype, const void 
   cuuint32_t box[3] = {box_inner, box_mid, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, dtype, 3, const_cast<void *>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                  : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                  : CU_TENSOR_MAP_SWIZZLE_32B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     *err = "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(static_cast<int>(r));

@@ -224,11 +224,12 @@ cudaError_t read_lora_status(unsigned int *bits, bool clear);
 
 // ---- tensor maps
 // 3-D map over an array of `dtype` (inner, mid, outer) with byte strides mid_bytes and
-// outer_bytes, box box_inner x box_mid x 1, 128-byte swizzle.
-bool make_tmap_3d_sw128(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
-                        uint64_t inner, uint64_t mid, uint64_t outer, uint64_t mid_bytes,
-                        uint64_t outer_bytes, uint32_t box_inner, uint32_t box_mid,
-                        std::string *err);
+// outer_bytes, box box_inner x box_mid x 1, swizzled over 128, 64 or 32 bytes (at least the
+// box's rows).
+bool make_tmap_3d_swizzled(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
+                           uint64_t inner, uint64_t mid, uint64_t outer, uint64_t mid_bytes,
+                           uint64_t outer_bytes, uint32_t box_inner, uint32_t box_mid,
+                           int swizzle, std::string *err);
 // 2-D form with any element type and row pitch, 128-byte swizzle.
 bool make_tmap_2d_sw128(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
                         uint64_t inner, uint64_t outer, uint64_t row_bytes, uint32_t box_inner,

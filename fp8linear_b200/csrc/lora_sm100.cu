@@ -611,8 +611,8 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   CUtensorMap tx, ta;
   if (!make_tmap_2d_sw128(&tx, t16, a.x, a.K, a.M, a.K * 2, KB, static_cast<uint32_t>(p.x_rows),
                           &err) ||
-      !make_tmap_3d_sw128(&ta, t16, a.lora_a, a.K, a.R, a.L, a.K * 2, a.R * a.K * 2, KB,
-                          static_cast<uint32_t>(p.rank_pad), &err)) {
+      !make_tmap_3d_swizzled(&ta, t16, a.lora_a, a.K, a.R, a.L, a.K * 2, a.R * a.K * 2, KB,
+                             static_cast<uint32_t>(p.rank_pad), 128, &err)) {
     set_error("fp8_linear_lora: " + err);
     return 4;
   }

@@ -74,7 +74,8 @@ struct Params {
   // split_kernel
   int split, kps, stages;
   int tok_cap;        // tokens per tile at most
-  uint32_t off_part;  // shared-memory offsets
+  uint32_t off_ring;  // shared-memory offsets
+  uint32_t off_part;
   uint32_t off_lora;
   uint32_t off_tab;
   // adapters
@@ -276,45 +277,60 @@ __device__ __forceinline__ void zero_rows(const Params &p, const int *row, int f
 // A tile whose tokens all have one adapter takes it on the tensor cores, as further stages of
 // the ring: the adapter's B rows beside the tokens' h, into an accumulator of their own. 64
 // 16-bit elements are the 128 bytes of a stage's row: up to rank 32 the high and the low part
-// of h share a stage, above it each 64 values of the rank take one for either part.
+// of h share a stage's box, above it each 64 values of the rank take a stage for either part.
 //
-// A tile of tokens of short runs (decoding requests) takes its adapters one after the other in
-// the same way, each into a window of TMEM columns of its own for all the tile's tokens; the
-// epilogue keeps the columns of the adapter's own tokens while further adapters come in. The
+// A tile of tokens of short runs (decoding requests) takes its adapters one after the other,
+// each into a window of TMEM columns of its own for all the tile's tokens; their h is loaded
+// once and the stages bring B alone (with h in every stage all CTAs kept asking for the same
+// few lines: 64 tokens of 27 adapters took 35 us). The epilogue keeps the columns of the adapter's own tokens while further adapters come in. The
 // columns of the other tokens are never read, so that an adapter's infinities stay with its
 // tokens (which one accumulator over tokens masked with zeros would not do: 0 * inf). Warp-level
 // MMAs on the epilogue warps took 0.8 us an adapter at rank 64.
 
-// The stages of an adapter: stage(bx, hx, steps, first) with the columns of B and of hl
-// and the 16-element steps; false ends them. (Nested counted loops: with the columns computed
-// from a stage's number by division, and MMAs in a loop of unknown length, a stage took 0.7 us.)
+// The stages of an adapter that is a whole tile's: stage(bx, hx, steps, first) with the columns
+// of B and of hl and the 16-element steps; false ends them. (Nested counted loops: with the
+// columns computed from a stage's number by division, and MMAs in a loop of unknown length, a
+// stage took 0.7 us.)
 template <class Stage>
 __device__ __forceinline__ bool adapter_stages(int rank_pad, Stage &&stage) {
-  if (rank_pad <= 32) return stage(0, 0, rank_pad / 16, true);
-  for (int part = 0; part < 2; ++part)
+  for (int part = 0; part < (rank_pad <= 32 ? 1 : 2); ++part)
     for (int bx = 0; bx < rank_pad; bx += 64)
       if (!stage(bx, part * rank_pad + bx, min(4, (rank_pad - bx) / 16), part + bx == 0))
         return false;
   return true;
 }
 
-// The MMAs of a stage; `first`: nothing in the accumulator counts yet. `packed` (rank up to
-// 32): the low part of h follows the high part in the same box.
+// d (+)= B . h^T for up to 64 ranks: B at `b`, h at `h`; `low`: where the low part of h lies,
+// as a descriptor offset from the high part (0: not in this stage). `first`: nothing in the
+// accumulator counts yet.
 template <int CG>
-__device__ __forceinline__ void lora_mma(uint32_t d, uint32_t stage, uint32_t idesc, int steps,
-                                         bool first, bool packed) {
-  const uint64_t adesc = ptx::sw128_kmajor_desc(stage);
-  const uint64_t bdesc = ptx::sw128_kmajor_desc(stage + W_STAGE);
+__device__ __forceinline__ void lora_mma(uint32_t d, uint32_t b, uint32_t h, uint32_t idesc,
+                                         int steps, bool first, uint32_t low) {
+  const uint64_t adesc = ptx::sw128_kmajor_desc(b);
+  const uint64_t bdesc = ptx::sw128_kmajor_desc(h);
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk)  // 16 elements: 32 bytes
     if (kk < steps)
       ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + 2 * kk, idesc, first && kk == 0 ? 0u : 1u);
-  if (packed) {
-    const uint64_t low = bdesc + 2 * static_cast<uint64_t>(steps);
+  if (low != 0) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-      if (kk < steps) ptx::mma_f16<CG>(d, adesc + 2 * kk, low + 2 * kk, idesc, 1u);
+    for (int kk = 0; kk < 4; ++kk)
+      if (kk < steps) ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + low + 2 * kk, idesc, 1u);
   }
+}
+
+// A mixed tile's h in shared memory: boxes of 64 columns (`rows` rows of 128 bytes), those of
+// the high part and behind them those of the low part; up to rank 32 one box has both.
+__device__ __forceinline__ int h_boxes(int rank_pad) {
+  return rank_pad <= 32 ? 1 : (rank_pad + 63) / 64 * 2;
+}
+__device__ __forceinline__ int h_column(int rank_pad, int box) {
+  const int half = (rank_pad + 63) / 64;
+  return box < half ? box * 64 : rank_pad + (box - half) * 64;
+}
+__device__ __forceinline__ uint32_t h_low(int rank_pad, int rows) {
+  return rank_pad <= 32 ? static_cast<uint32_t>(rank_pad / 8)
+                        : static_cast<uint32_t>((rank_pad + 63) / 64 * rows * BK / 16);
 }
 
 __device__ __forceinline__ int token_id(const Params &p, int i, int end) {
@@ -353,6 +369,228 @@ __device__ __forceinline__ void keep_columns(uint32_t base, uint32_t mask, float
     out[c0 * pitch] = __uint_as_float(v0);
     if (c1 >= 0) out[c1 * pitch] = __uint_as_float(v1);
   }
+}
+
+// The ring of B boxes for adapter_sums: 128 weight rows x 64 ranks (32 or 16 where the rank
+// fits), rows of 128, 64 or 32 bytes swizzled over as many; 48 KB of it, so that three to
+// eight boxes are under way. A warp of its own fills it (feed_sums), the four epilogue warps
+// read it; both go through the tokens eight at a time, through the adapters of eight in the
+// order of their first tokens, and through the rank a box at a time. `count` boxes have been
+// through the ring.
+constexpr uint32_t SUM_RING = 3 * W_STAGE;
+constexpr int SUM_SLOTS_MAX = 8;
+constexpr int SUM_RANK = 64;
+constexpr int SUM_BARS = 2 * SUM_SLOTS_MAX;  // full, empty
+__host__ __device__ constexpr int sum_width(int rank) { return rank > 32 ? 64 : rank > 16 ? 32 : 16; }
+__device__ __forceinline__ uint32_t sum_slots(int rank) {
+  return rank > 32 ? 3u : rank > 16 ? 6u : 8u;
+}
+struct SumRing {
+  uint32_t slots;  // shared-memory addresses
+  uint32_t bars;
+  volatile int *abort;
+  uint32_t n;       // slots
+  uint32_t box;     // bytes of one
+  uint32_t slot;    // the next, and its phase
+  uint32_t phase;
+  uint32_t count;
+
+  __device__ __forceinline__ SumRing(const Params &p, uint32_t s, uint32_t b, volatile int *a)
+      : slots(s), bars(b), abort(a), n(sum_slots(p.R)),
+        box(static_cast<uint32_t>(sum_width(p.R)) * 2u * WROWS), slot(0), phase(0), count(0) {}
+  __device__ __forceinline__ uint32_t full() const { return bars + 8 * slot; }
+  __device__ __forceinline__ uint32_t empty() const { return bars + 8 * (SUM_SLOTS_MAX + slot); }
+  __device__ __forceinline__ void next() {
+    ++count;
+    if (++slot == n) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// Lane l of a warp has the adapter of token l % 8 of eight (-1: none); bits 0-7 of the
+// result are the tokens whose adapter no earlier one of them has.
+__device__ __forceinline__ uint32_t first_tokens(int id) {
+  const uint32_t same = __match_any_sync(0xFFFFFFFFu, id) & 0xFFu;
+  const int lane = threadIdx.x & 31;
+  return __ballot_sync(0xFFFFFFFFu, id >= 0 && lane < 8 && __ffs(static_cast<int>(same)) - 1 == lane) &
+         0xFFu;
+}
+
+// The boxes for tokens [t0, t1) and weight rows n0 ..; by a whole warp. False when a wait ran
+// out (nothing is issued after that).
+__device__ __forceinline__ bool feed_sums(const Params &p, const CUtensorMap *map, SumRing &ring,
+                                          int t0, int t1, int n0) {
+  const int lane = threadIdx.x & 31;
+  const bool elected = ptx::elect_one();
+  // all of them into L2 first: three to eight boxes under way do not cover a trip to memory
+  for (int i = t0; i < t1; i += 32) {
+    const int id = token_id(p, i + lane, t1);
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, id);
+    if (id >= 0 && __ffs(static_cast<int>(same)) - 1 == lane)
+      for (int rc = 0; rc < p.R; rc += SUM_RANK) ptx::tma_prefetch_3d(map, rc, n0, id);
+    __syncwarp();
+  }
+  int next = token_id(p, t0 + (lane & 7), t1);
+  for (int i = t0; i < t1; i += 8) {
+    const int id = next;
+    next = token_id(p, i + 8 + (lane & 7), t1);
+    for (uint32_t todo = first_tokens(id); todo != 0; todo &= todo - 1) {
+      const int a = __shfl_sync(0xFFFFFFFFu, id, __ffs(static_cast<int>(todo)) - 1);
+      for (int rc = 0; rc < p.R; rc += SUM_RANK) {
+        if (!warp_wait(ring.empty(), ring.phase ^ 1u, ring.abort, elected)) return false;
+        if (elected) {
+          ptx::mbar_arrive_expect_tx(ring.full(), ring.box);
+          ptx::tma_load_3d(ring.slots + ring.slot * ring.box, map, rc, n0, a, ring.full());
+        }
+        ring.next();
+      }
+    }
+  }
+  return true;
+}
+
+// Waits (bounded) until every box issued has landed and been read.
+__device__ __forceinline__ void drain_sums(SumRing &ring) {
+  for (uint32_t i = min(ring.count, ring.n); i > 0; --i) {
+    if (ring.slot == 0) {
+      ring.slot = ring.n - 1;
+      ring.phase ^= 1u;
+    } else {
+      --ring.slot;
+    }
+    ptx::mbar_wait_timeout(ring.empty(), ring.phase, kDrainLimitNs);
+  }
+}
+
+// Eight tokens' adapters (as token_id gives them) and h, the B operand of their products: h of
+// token lane / 4, ranks 16j + 2t, + 1 and 16j + 8 + 2t, + 1, high and low part, t = lane % 4
+// (zero past the rank and for tokens without an adapter, whose h is not written).
+template <int J>
+struct EightTokens {
+  int id;
+  uint32_t h[J][4];
+
+  __device__ __forceinline__ void load(const Params &p, int i0, int t1) {
+    const int lane = threadIdx.x & 31;
+    id = token_id(p, i0 + (lane & 7), t1);
+    const bool has = __shfl_sync(0xFFFFFFFFu, id, lane >> 2) >= 0;
+    const uint32_t *hr = reinterpret_cast<const uint32_t *>(p.hl) +
+                         static_cast<int64_t>(i0 + (lane >> 2)) * p.rank_pad + (lane & 3);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const bool in = has && 16 * j < p.rank_pad;
+      h[j][0] = in ? __ldg(hr + 8 * j) : 0u;
+      h[j][1] = in ? __ldg(hr + 8 * j + 4) : 0u;
+      h[j][2] = in ? __ldg(hr + p.rank_pad / 2 + 8 * j) : 0u;
+      h[j][3] = in ? __ldg(hr + p.rank_pad / 2 + 8 * j + 4) : 0u;
+    }
+  }
+};
+
+__device__ __forceinline__ void mma_16x8x16(bool f16, float (&d)[4], const uint32_t (&a)[4],
+                                            uint32_t b0, uint32_t b1) {
+  if (f16)
+    ptx::mma_f16_16x8x16(d, a[0], a[1], a[2], a[3], b0, b1);
+  else
+    ptx::mma_bf16_16x8x16(d, a[0], a[1], a[2], a[3], b0, b1);
+}
+
+// For the eight tokens `now` and the 32 weight rows `quarter` of the boxes: the sums
+// sum_r (hi + lo)[token][r] * B[adapter of the token][row][r], as matrix fragments: lane
+// 4i + t gets tokens 2t, 2t + 1 of rows i + 8k in s[k]; zero for tokens without an adapter. C
+// boxes of 16 J ranks an adapter. By one epilogue warp; false when a wait ran out. The high
+// and the low part have accumulators of their own and a box's fragments are read before its
+// first MMA, so that the chain of dependent MMAs is J long: in one chain with reads between
+// them a box of 32 ranks took 740 cycles.
+template <int J, int C>
+__device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring,
+                                             const EightTokens<J * C> &now, int quarter,
+                                             float2 (&s)[4]) {
+  const int lane = threadIdx.x & 31;
+  const bool f16 = p.lora_dtype == kF16;
+  const int id = now.id;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s[k] = make_float2(0.0f, 0.0f);
+  const int id0 = __shfl_sync(0xFFFFFFFFu, id, 2 * (lane & 3));
+  const int id1 = __shfl_sync(0xFFFFFFFFu, id, 2 * (lane & 3) + 1);
+  // ldmatrix: lane 8m + i has row i + 8 (m % 2) of a 16-row tile, 16-byte column 2j + m / 2;
+  // column c of a row lies at c ^ swizzle: address bits 7.. of the row's own (the same for
+  // rows 16 apart)
+  constexpr uint32_t kRow = 32 * J;  // bytes
+  const uint32_t row = static_cast<uint32_t>(quarter * 32 + (lane & 7) + (lane & 8));
+  const uint32_t col = static_cast<uint32_t>(lane >> 4);
+  const uint32_t swizzle = row * kRow / 128 & (kRow / 16 - 1);
+#pragma unroll 1
+  for (uint32_t todo = first_tokens(id); todo != 0; todo &= todo - 1) {
+    const int a = __shfl_sync(0xFFFFFFFFu, id, __ffs(static_cast<int>(todo)) - 1);
+    float d[2][2][4];  // [16-row tile][high, low]
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[m][e >> 2][e & 3] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (!ptx::mbar_wait_bounded(ring.full(), ring.phase, ring.abort, kWaitLimitNs)) {
+        record_timeout(ring.abort);
+        return false;
+      }
+      const uint32_t box = ring.slots + ring.slot * ring.box + row * kRow;
+      uint32_t w[2][J][4];
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          ptx::ldsm_x4(box + m * 16 * kRow + (((2 * j + col) ^ swizzle) << 4), w[m][j]);
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const uint32_t(&h)[4] = now.h[c * J + j];
+          mma_16x8x16(f16, d[m][0], w[m][j], h[0], h[1]);
+          mma_16x8x16(f16, d[m][1], w[m][j], h[2], h[3]);
+        }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ring.empty());
+      ring.next();
+    }
+    // d[m]: rows i + 16m (0, 1) and i + 16m + 8 (2, 3), tokens 2t (0, 2) and 2t + 1 (1, 3)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int e = 2 * (k & 1);
+      if (id0 == a) s[k].x = d[k >> 1][0][e] + d[k >> 1][1][e];
+      if (id1 == a) s[k].y = d[k >> 1][0][e + 1] + d[k >> 1][1][e + 1];
+    }
+  }
+  return true;
+}
+
+// All tokens [t0, t1) so, eight at a time: to(i, s) takes the sums of the tokens from t0 + i.
+template <int J, int C, class To>
+__device__ __forceinline__ bool token_sums(const Params &p, SumRing &ring, int t0, int t1,
+                                           int quarter, To &&to) {
+  EightTokens<J * C> now;
+  now.load(p, t0, t1);
+#pragma unroll 1
+  for (int i = 0; t0 + i < t1; i += 8) {
+    EightTokens<J * C> next;  // (under way meanwhile)
+    next.load(p, t0 + i + 8, t1);
+    float2 s[4];
+    if (!adapter_sums<J, C>(p, ring, now, quarter, s)) return false;
+    to(i, s);
+    now = next;
+  }
+  return true;
+}
+
+template <class To>
+__device__ __forceinline__ bool token_sums(const Params &p, SumRing &ring, int t0, int t1,
+                                           int quarter, To &&to) {
+  if (p.R > 64) return token_sums<4, 2>(p, ring, t0, t1, quarter, to);
+  if (p.R > 32) return token_sums<4, 1>(p, ring, t0, t1, quarter, to);
+  if (p.R > 16) return token_sums<2, 1>(p, ring, t0, t1, quarter, to);
+  return token_sums<1, 1>(p, ring, t0, t1, quarter, to);
 }
 
 // Eight 16-bit values as floats.
@@ -473,10 +711,13 @@ struct Cfg {
   // the fragments' reads
   static constexpr uint32_t OFF_SUM = OFF_BOX + EPI_WARPS * BOX_BYTES;
   static constexpr int WINDOWS = TOK_MAX / kLoraMixed;  // .. of TMEM columns, in ACC_L's place
-  static constexpr uint32_t OFF_TAB = OFF_SUM + (LORA ? kLoraMixed * SUM_PITCH * 4u : 0u);
+  // .. and their h: four boxes of this CTA's tokens
+  static constexpr uint32_t OFF_H = (OFF_SUM + (LORA ? kLoraMixed * SUM_PITCH * 4u : 0u) + 1023u) &
+                                    ~1023u;
+  static constexpr uint32_t OFF_TAB = OFF_H + (LORA ? 4u * (kLoraMixed / CG) * BK : 0u);
   static constexpr int TAB = LORA ? 2 : kMaxExperts + 1;
   static constexpr uint32_t OFF_BAR = (OFF_TAB + 2 * TAB * 4 + 7u) & ~7u;
-  static constexpr uint32_t NUM_BARS = 2 * STAGES + 5 + 2 * WINDOWS;  // full, empty, tfull, tempty, drain, windows
+  static constexpr uint32_t NUM_BARS = 2 * STAGES + 7 + 2 * WINDOWS;  // full, empty, tfull, tempty, drain, h, windows
   static constexpr uint32_t OFF_SLOT = OFF_BAR + NUM_BARS * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_SLOT + 8 + 1024;
   static_assert(STAGE % 1024 == 0, "swizzle atoms need 1024 B alignment");
@@ -497,7 +738,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t bar_tfull = bar_empty + C::STAGES * 8;
   const uint32_t bar_tempty = bar_tfull + 2 * 8;
   const uint32_t bar_drain = bar_tempty + 2 * 8;
-  const uint32_t bar_wfull = bar_drain + 8;
+  const uint32_t bar_h = bar_drain + 8;  // full, empty
+  const uint32_t bar_wfull = bar_h + 2 * 8;
   const uint32_t bar_wempty = bar_wfull + 8 * C::WINDOWS;
   volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + C::OFF_SLOT);
   volatile int *abort = reinterpret_cast<volatile int *>(smem + C::OFF_SLOT + 4);
@@ -522,6 +764,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       ptx::mbar_init(bar_tempty + 8 * a, EPI_WARPS * CG);
     }
     ptx::mbar_init(bar_drain, 1);
+    ptx::mbar_init(bar_h, 1);
+    ptx::mbar_init(bar_h + 8, 1);
     for (int i = 0; i < C::WINDOWS; ++i) {
       ptx::mbar_init(bar_wfull + 8 * i, 1);
       ptx::mbar_init(bar_wempty + 8 * i, EPI_WARPS * CG);
@@ -586,6 +830,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     int stage = 0;
     uint32_t phase = 0;
     uint32_t issued = 0;
+    uint32_t hphase = 0;
     int e = 0;
     bool ok = true;
     for (int t = group; t < num_tiles && ok; t += n_groups) {
@@ -596,23 +841,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int xrow = ptx::uniform(q.t0) + static_cast<int>(rank) * (nn / CG);
       const int mi = nn / CG / 16 - 1;
       const uint32_t tx = CG * W_STAGE + static_cast<uint32_t>(nn) * BK;
-      // One stage: the weight box and the token box at the given coordinates.
+      // One stage: the weight box and the token box (mx null: none) at the given coordinates.
       auto load = [&](const CUtensorMap *mw, int wx, int z, const CUtensorMap *mx, int xx) {
         if (!warp_wait(bar_empty + 8 * stage, phase ^ 1u, abort, elected)) return false;
         const uint32_t dst = sbase + static_cast<uint32_t>(stage) * C::STAGE;
         const uint32_t fl = full_leader + 8 * stage;
         if (elected) {
           if (ahead == 0) {
-            if (leader) ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, tx);
+            if (leader)
+              ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, mx != nullptr ? tx : CG * W_STAGE);
             if constexpr (CG == 1)
               ptx::tma_load_3d(dst, mw, wx, wrow, z, fl);
             else
               ptx::tma_load_3d_pair(dst, mw, wx, wrow, z, fl);
           }
-          if constexpr (CG == 1)
-            ptx::tma_load_2d(dst + W_STAGE, mx, xx, xrow, fl);
-          else
-            ptx::tma_load_2d_pair(dst + W_STAGE, mx, xx, xrow, fl);
+          if (mx != nullptr) {
+            if constexpr (CG == 1)
+              ptx::tma_load_2d(dst + W_STAGE, mx, xx, xrow, fl);
+            else
+              ptx::tma_load_2d_pair(dst + W_STAGE, mx, xx, xrow, fl);
+          }
         }
         if (ahead > 0) --ahead;  // (armed, its weights under way)
         ++issued;
@@ -625,21 +873,39 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       for (int kb = 0; kb < p.k_blocks && ok; ++kb)
         ok = load(&maps.w, kb * BK, wz, &maps.x[mi], kb * BK);
       if constexpr (LORA) {
-        auto load_adapter = [&](int a) {
-          ok = ok && adapter_stages(p.rank_pad, [&](int bx, int hx, int, bool) {
-                 return load(&maps.lb, bx, a, &maps.h[mi], hx);
-               });
-        };
         const int adapter = ptx::uniform(q.adapter);
-        if (adapter >= 0) load_adapter(adapter);
-        if (adapter == -2) {
+        if (adapter >= 0)
+          ok = ok && adapter_stages(p.rank_pad, [&](int bx, int hx, int, bool) {
+                 return load(&maps.lb, bx, adapter, &maps.h[mi], hx);
+               });
+        if (adapter == -2 && ok) {
           const TokenAdapters ta(p, q.t0, q.t1);
-          for (uint32_t todo = ta.leaders; todo != 0 && ok; todo &= todo - 1)
-            load_adapter(__shfl_sync(0xFFFFFFFFu, ta.id, __ffs(static_cast<int>(todo)) - 1));
+          if (ta.leaders != 0) {
+            if (!(ok = warp_wait(bar_h + 8, hphase ^ 1u, abort, elected))) break;
+            const int boxes = h_boxes(p.rank_pad);
+            if (elected) {
+              const uint32_t bytes = static_cast<uint32_t>(nn / CG) * BK;
+              const uint32_t hl = CG == 1 ? bar_h : ptx::map_shared_rank(bar_h, 0);
+              if (leader) ptx::mbar_arrive_expect_tx(bar_h, CG * bytes * static_cast<uint32_t>(boxes));
+              for (int i = 0; i < boxes; ++i) {
+                const uint32_t dst = sbase + C::OFF_H + static_cast<uint32_t>(i) * bytes;
+                if constexpr (CG == 1)
+                  ptx::tma_load_2d(dst, &maps.h[mi], h_column(p.rank_pad, i), xrow, hl);
+                else
+                  ptx::tma_load_2d_pair(dst, &maps.h[mi], h_column(p.rank_pad, i), xrow, hl);
+              }
+            }
+            hphase ^= 1u;
+          }
+          for (uint32_t todo = ta.leaders; todo != 0 && ok; todo &= todo - 1) {
+            const int a = __shfl_sync(0xFFFFFFFFu, ta.id, __ffs(static_cast<int>(todo)) - 1);
+            for (int bx = 0; bx < p.R && ok; bx += 64) ok = load(&maps.lb, bx, a, nullptr, 0);
+          }
         }
       }
     }
     // Drain: every load issued here has landed and been consumed.
+    if (LORA && !ok) ptx::mbar_wait_timeout(bar_h + 8, hphase ^ 1u, kDrainLimitNs);
     const uint32_t n_drain = issued < C::STAGES ? issued : C::STAGES;
     for (uint32_t i = 0; i < n_drain; ++i) {
       if (stage == 0) {
@@ -657,7 +923,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       int window = 0;
-      uint32_t wphase = 0;
+      uint32_t wphase = 0, hphase = 0;
       int it = 0;
       int e = 0;
       bool ok = true;
@@ -714,23 +980,35 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 !wait(bar_tempty + 8 * (acc ^ 1), static_cast<uint32_t>((it - 1) >> 1) & 1u))
               break;
             const uint32_t id16 = ptx::idesc_f16_f32(WROWS * CG, nn, p.lora_dtype == kBF16);
-            auto product = [&](uint32_t dl) {
-              ok = ok && adapter_stages(p.rank_pad, [&](int, int, int steps, bool first) {
-                     if (!wait(bar_full + 8 * stage, phase)) return false;
-                     if (elected)
-                       lora_mma<CG>(dl, sbase + static_cast<uint32_t>(stage) * C::STAGE, id16,
-                                    steps, first, p.rank_pad <= 32);
-                     next_stage();
-                     return true;
-                   });
-            };
             if (adapter >= 0) {
-              product(tmem_base + C::ACC_L);
+              const uint32_t low = p.rank_pad <= 32 ? h_low(p.rank_pad, 0) : 0u;
+              ok = adapter_stages(p.rank_pad, [&](int, int, int steps, bool first) {
+                if (!wait(bar_full + 8 * stage, phase)) return false;
+                const uint32_t st = sbase + static_cast<uint32_t>(stage) * C::STAGE;
+                if (elected)
+                  lora_mma<CG>(tmem_base + C::ACC_L, st, st + W_STAGE, id16, steps, first, low);
+                next_stage();
+                return true;
+              });
             } else {
               const TokenAdapters ta(p, q.t0, q.t1);
+              const uint32_t low = h_low(p.rank_pad, nn / CG);
+              if (ta.leaders != 0) {
+                if (!(ok = wait(bar_h, hphase))) break;
+                hphase ^= 1u;
+              }
               for (int i = __popc(ta.leaders); i > 0 && ok; --i) {
                 if (!(ok = wait(bar_wempty + 8 * window, wphase ^ 1u))) break;
-                product(tmem_base + C::ACC_L + static_cast<uint32_t>(window * kLoraMixed));
+                uint32_t h = sbase + C::OFF_H;
+                for (int bx = 0; bx < p.R; bx += 64, h += static_cast<uint32_t>(nn / CG) * BK) {
+                  if (!(ok = wait(bar_full + 8 * stage, phase))) break;
+                  if (elected)
+                    lora_mma<CG>(
+                        tmem_base + C::ACC_L + static_cast<uint32_t>(window * kLoraMixed),
+                        sbase + static_cast<uint32_t>(stage) * C::STAGE, h, id16,
+                        min(4, (p.rank_pad - bx) / 16), bx == 0, low);
+                  next_stage();
+                }
                 if (ok && elected) {
                   if constexpr (CG == 1)
                     ptx::mma_commit(bar_wfull + 8 * window);
@@ -741,6 +1019,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                   window = 0;
                   wphase ^= 1u;
                 }
+              }
+              if (ta.leaders != 0 && elected) {  // h may be overwritten
+                if constexpr (CG == 1)
+                  ptx::mma_commit(bar_h + 8);
+                else
+                  ptx::mma_commit_pair_mc(bar_h + 8, 0x3);
               }
             }
           }
@@ -961,7 +1245,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
 constexpr int SPLIT_TOK = 128;   // tokens per tile, at most
 constexpr int SPLIT_LORA_TOK = 64;  // with adapters, whose sums need room too
-constexpr int SPLIT_WINDOWS = 4;    // adapters' products under way
 constexpr int SPLIT_STAGES = 8;  // ring slots, at most
 constexpr int SPLIT_MAX = 8;     // CTAs per cluster, at most (portable)
 constexpr int SPLIT_COST = 12;   // a tile's set-up and reduction, in K-blocks
@@ -969,31 +1252,25 @@ constexpr uint32_t SPLIT_EPI = (2 * SPLIT_TOK + 2 * WROWS) * 4;  // xs, ws, bias
 constexpr uint32_t SPLIT_SMEM = 232448;
 
 template <bool LORA>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = ptx::smem_u32(smem);
-  __shared__ alignas(8) uint64_t s_bar[2 * SPLIT_STAGES + 2 + 2 * SPLIT_WINDOWS];
+  __shared__ alignas(8) uint64_t s_bar[2 * SPLIT_STAGES + 2 + SUM_BARS];
   __shared__ uint32_t s_slot;
   __shared__ int s_abort;
-  __shared__ int s_id[SPLIT_LORA_TOK];            // adapter of each token of the tile, -1: none
-  __shared__ int s_adapter[SPLIT_LORA_TOK];       // the tile's adapters
-  __shared__ uint32_t s_mask[2][SPLIT_LORA_TOK];  // .. and their tokens
-  __shared__ int s_adapters;
-  __shared__ alignas(16) float s_own[LORA ? OWN_WORK : 1];
   const uint32_t bar_full = ptx::smem_u32(s_bar);
   const uint32_t bar_empty = bar_full + 8 * SPLIT_STAGES;
   const uint32_t bar_acc = bar_empty + 8 * SPLIT_STAGES;
   const uint32_t bar_drain = bar_acc + 8;
-  const uint32_t bar_wfull = bar_drain + 8;
-  const uint32_t bar_wempty = bar_wfull + 8 * SPLIT_WINDOWS;
+  const uint32_t bar_sum = bar_drain + 8;
   volatile uint32_t *tmem_slot = &s_slot;
   volatile int *abort = &s_abort;
   // partial sums of the rows reduced here: [CTA they come from][token][R rows]
   float *part = reinterpret_cast<float *>(smem + p.off_part);
-  float *lora = reinterpret_cast<float *>(smem + p.off_lora);  // [tokens][WROWS]
+  float *lora = reinterpret_cast<float *>(smem + p.off_lora);  // [tokens of this CTA][WROWS]
   int *g_row = reinterpret_cast<int *>(smem + p.off_tab);
   int *g_tile = g_row + p.E + 1;
   float *e_xs = reinterpret_cast<float *>(
@@ -1006,27 +1283,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int rank = static_cast<int>(ptx::cluster_ctarank());
   const int stages = p.stages;
   const uint32_t stage_bytes = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
-  // TMEM: the accumulator, with adapters also SPLIT_WINDOWS windows as wide
-  const uint32_t cols = static_cast<uint32_t>(p.tok_cap) * (LORA ? 1 + SPLIT_WINDOWS : 1);
   uint32_t tmem_cols = 32;
-  while (tmem_cols < cols) tmem_cols <<= 1;
+  while (tmem_cols < static_cast<uint32_t>(p.tok_cap)) tmem_cols <<= 1;
 
-  const bool own = LORA && p.own_down;
   if (threadIdx.x == 0) {
     ptx::prefetch_tmap(&maps.w);
-    if (LORA && !own) {
-      ptx::prefetch_tmap(&maps.lb);
-      ptx::prefetch_tmap(&maps.h[0]);
-    }
     for (int s = 0; s < stages; ++s) {
       ptx::mbar_init(bar_full + 8 * s, 1);
       ptx::mbar_init(bar_empty + 8 * s, 1);
     }
     ptx::mbar_init(bar_acc, 1);
     ptx::mbar_init(bar_drain, 1);
-    for (int i = 0; i < SPLIT_WINDOWS; ++i) {
-      ptx::mbar_init(bar_wfull + 8 * i, 1);
-      ptx::mbar_init(bar_wempty + 8 * i, EPI_WARPS);
+    for (int i = 0; i < SUM_SLOTS_MAX; ++i) {
+      ptx::mbar_init(bar_sum + 8 * i, 1);
+      ptx::mbar_init(bar_sum + 8 * (SUM_SLOTS_MAX + i), EPI_WARPS);
     }
     s_abort = 0;
     ptx::fence_mbar_init();
@@ -1066,37 +1336,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     ptx::tmem_alloc<1>(ptx::smem_u32(&s_slot), tmem_cols);
     ptx::tmem_relinquish<1>();
   }
-  if (LORA && !own && warp == 2) {
-    // the tile's adapters in the order of their first tokens, two tokens a lane
-    const int id[2] = {token_id(p, q.t0 + lane, q.t1), token_id(p, q.t0 + 32 + lane, q.t1)};
-    s_id[lane] = id[0];
-    s_id[32 + lane] = id[1];
-    __syncwarp();
-    int n = 0;
-    for (int i = 0; i < cnt; ++i) {
-      const int a = s_id[i];  // (the same for all lanes)
-      const uint32_t m0 = __ballot_sync(0xFFFFFFFFu, id[0] == a);
-      const uint32_t m1 = __ballot_sync(0xFFFFFFFFu, id[1] == a);
-      const int first = m0 != 0 ? __ffs(static_cast<int>(m0)) - 1 : 31 + __ffs(static_cast<int>(m1));
-      if (a < 0 || first != i) continue;
-      if (lane == 0) {
-        s_adapter[n] = a;
-        s_mask[0][n] = m0;
-        s_mask[1][n] = m1;
-      }
-      ++n;
-    }
-    if (lane == 0) s_adapters = n;
-  }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = static_cast<uint32_t>(ptx::uniform(static_cast<int>(*tmem_slot)));
   ptx::cluster_arrive_release();  // (waited for before the first push: all CTAs have started)
-  if (own && warp >= 2) {
+  if (LORA && p.own_down && warp >= 2 && warp < 2 + EPI_WARPS) {
     const int row = (warp & 3) * 32 + lane;
     own_adapter_sums(p, kb0 * BK, (kb0 + nkb) * BK, q.wb * WROWS + row,
-                     s_own, lora, threadIdx.x - 64, row);
+                     reinterpret_cast<float *>(smem + p.off_ring), lora, threadIdx.x - 64, row);
   }
   if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -1108,29 +1356,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int quads = r1 > r0 ? (r1 - r0) >> 2 : 0;
   const int n0 = q.wb * WROWS;
 
-  // Adapters: every split-th of the tile's is this CTA's, as stages behind its K-blocks, each
-  // into a window of TMEM columns.
-  const int all = LORA && !own ? s_adapters : 0;
-  const int mine = all > rank ? ptx::uniform((all - rank + p.split - 1) / p.split) : 0;
+  // Adapters: the cluster's CTAs share out the tokens, eight at a time (own_down: all tokens,
+  // but only this CTA's K range of them).
+  const bool own = LORA && p.own_down;
+  const int per_cta = LORA ? ((cnt + 7) / 8 + p.split - 1) / p.split * 8 : 0;
+  const int a0 = own ? 0 : min(cnt, rank * per_cta), a1 = own ? cnt : min(cnt, a0 + per_cta);
 
   if (warp == 0) {
     const bool elected = ptx::elect_one();
     int issued = 0;
     int s = 0;
     uint32_t ph = 1;
-    auto next = [&]() {
-      ++issued;
-      if (++s == stages) {
-        s = 0;
-        ph ^= 1u;
-      }
-    };
-    bool ok = true;
     for (int i = 0; i < nkb; ++i) {
       const uint32_t fb = bar_full + 8 * s;
       const uint32_t dst = sbase + static_cast<uint32_t>(s) * stage_bytes;
       const bool refill = i >= stages;  // (the first are armed, their weight boxes under way)
-      if (refill && !(ok = warp_wait(bar_empty + 8 * s, ph, abort, elected))) break;
+      if (refill && !warp_wait(bar_empty + 8 * s, ph, abort, elected)) break;
       if (elected) {
         if (refill) {
           ptx::mbar_arrive_expect_tx(fb, tx);
@@ -1138,24 +1379,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         ptx::tma_load_2d(dst + W_STAGE, mx, (kb0 + i) * BK, xrow, fb);
       }
-      next();
-    }
-    if constexpr (LORA) {
-      const CUtensorMap *mh = &maps.h[nn / 16 - 1];
-      for (int d = 0; d < mine && ok; ++d) {
-        const int a = ptx::uniform(s_adapter[rank + d * p.split]);
-        ok = adapter_stages(p.rank_pad, [&](int bx, int hx, int, bool) {
-          if (issued >= stages && !warp_wait(bar_empty + 8 * s, ph, abort, elected)) return false;
-          const uint32_t fb = bar_full + 8 * s;
-          const uint32_t dst = sbase + static_cast<uint32_t>(s) * stage_bytes;
-          if (elected) {
-            ptx::mbar_arrive_expect_tx(fb, tx);
-            ptx::tma_load_3d(dst, &maps.lb, bx, wrow, a, fb);
-            ptx::tma_load_2d(dst + W_STAGE, mh, hx, xrow, fb);
-          }
-          next();
-          return true;
-        });
+      ++issued;
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1u;
       }
     }
     for (int i = issued - 1; i >= 0 && i >= issued - stages; --i)
@@ -1167,13 +1394,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t idesc = ptx::idesc_e4m3_f32(WROWS, nn);
     int s = 0;
     uint32_t ph = 0;
-    auto next = [&]() {
-      if (elected) ptx::mma_commit(bar_empty + 8 * s);
-      if (++s == stages) {
-        s = 0;
-        ph ^= 1u;
-      }
-    };
     for (int i = 0; i < nkb; ++i) {
       if (!(ok = warp_wait(bar_full + 8 * s, ph, abort, elected))) break;
       ptx::tc_fence_after();
@@ -1186,45 +1406,30 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           const uint64_t koff = static_cast<uint64_t>((kk * UMMA_K) >> 4);
           ptx::mma_f8f6f4(tmem, adesc + koff, bdesc + koff, idesc, (i | kk) != 0 ? 1u : 0u);
         }
+        ptx::mma_commit(bar_empty + 8 * s);
       }
-      next();
-    }
-    if (ok && elected) ptx::mma_commit(bar_acc);
-    if constexpr (LORA) {
-      const uint32_t id16 = ptx::idesc_f16_f32(WROWS, nn, p.lora_dtype == kBF16);
-      int window = 0;
-      uint32_t wphase = 1;
-      for (int d = 0; d < mine && ok; ++d) {
-        if (!(ok = warp_wait(bar_wempty + 8 * window, wphase, abort, elected))) break;
-        const uint32_t dl = tmem + static_cast<uint32_t>((1 + window) * p.tok_cap);
-        ok = adapter_stages(p.rank_pad, [&](int, int, int steps, bool first) {
-          if (!warp_wait(bar_full + 8 * s, ph, abort, elected)) return false;
-          ptx::tc_fence_after();
-          if (elected)
-            lora_mma<1>(dl, sbase + static_cast<uint32_t>(s) * stage_bytes, id16, steps, first,
-                        p.rank_pad <= 32);
-          next();
-          return true;
-        });
-        if (ok && elected) ptx::mma_commit(bar_wfull + 8 * window);
-        if (++window == SPLIT_WINDOWS) {
-          window = 0;
-          wphase ^= 1u;
-        }
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1u;
       }
     }
     if (elected) {
+      if (ok) ptx::mma_commit(bar_acc);
       ptx::mma_commit(bar_drain);
       ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
     }
+  } else if (LORA && warp == 2 + EPI_WARPS) {
+    SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
+    if (!own) feed_sums(p, &maps.lb, ring, q.t0 + a0, q.t0 + a1, n0);
+    drain_sums(ring);
   } else {
     // xs (adapters: and hscale) of the tokens, weight scales and biases of the rows reduced
     // here
     const int et = threadIdx.x - 64;
     for (int i = et; i < q.nn; i += 128) {
       e_xs[i] = i < cnt ? __ldg(p.xs + q.t0 + i) : 0.0f;
-      if constexpr (LORA)  // (own sums come scaled)
-        e_hs[i] = own ? 1.0f : i < cnt && s_id[i] >= 0 ? __ldg(p.hscale + q.t0 + i) : 0.0f;
+      if constexpr (LORA)
+        e_hs[i] = !own && token_id(p, q.t0 + i, q.t1) >= 0 ? __ldg(p.hscale + q.t0 + i) : 0.0f;
     }
     for (int i = et; i < r1 - r0; i += 128) {
       const int n = n0 + r0 + i;
@@ -1237,33 +1442,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const int n = n0 + row;
     const float w = LORA && n < p.N ? __ldg(p.ws + n) : 1.0f;
     epilogue_sync();  // xs and hscale are in shared memory
-    const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    bool ok = true;
     if (LORA && !own) {
-      // This CTA's adapters' sums, as they come, to lora[token][row]; zero for the tokens of
-      // the others' (a warp writes and reads back its own rows only).
-      float *to = lora + row;
-      for (int i = 0; i < cnt; ++i) to[i * WROWS] = 0.0f;
-      for (int d = 0; d < mine && ok; ++d) {
-        const int window = d % SPLIT_WINDOWS;
-        if (!(ok = warp_wait(bar_wfull + 8 * window, static_cast<uint32_t>(d / SPLIT_WINDOWS) & 1u,
-                             abort, lane == 0)))
-          break;
-        ptx::tc_fence_after();
-        const uint32_t base = t_row + static_cast<uint32_t>((1 + window) * p.tok_cap);
-        keep_columns(base, s_mask[0][rank + d * p.split], to, WROWS);
-        keep_columns(base + 32, s_mask[1][rank + d * p.split], to + 32 * WROWS, WROWS);
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar_wempty + 8 * window);
-      }
+      // (a warp writes and reads back its own rows only; after a wait that ran out, whatever)
+      SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
+      token_sums(p, ring, q.t0 + a0, q.t0 + a1, quarter, [&](int i, float2(&s)[4]) {
+        float *to = lora + (i + 2 * (lane & 3)) * WROWS + quarter * 32 + (lane >> 2);
+        const float2 hs = *reinterpret_cast<const float2 *>(e_hs + a0 + i + 2 * (lane & 3));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          to[8 * k] = s[k].x * hs.x;
+          to[8 * k + WROWS] = s[k].y * hs.y;
+        }
+      });
+      __syncwarp();
     }
     // TMEM (lane = weight row, column = token) -> the part of the CTA that reduces the row,
     // fp32: the K-blocks' sums as they are, or with adapters dequantized and added to the
     // adapters' sums
-    ok = ok && warp_wait(bar_acc, 0, abort, lane == 0);
+    const bool ok = ptx::mbar_wait_bounded(bar_acc, 0, abort, kWaitLimitNs);
+    if (!ok && lane == 0) record_timeout(abort);
     ptx::tc_fence_after();
     ptx::cluster_wait_acquire();
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t dst = ptx::map_shared_rank(
         ptx::smem_u32(part) +
             static_cast<uint32_t>(rank * p.tok_cap * R + row % R) * 4u,
@@ -1283,14 +1483,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         float v = __uint_as_float(r[j]);
         if constexpr (LORA) {
           v = v * e_xs[c + j] * w;
-          if (c + j < cnt) v = fmaf(lora[(c + j) * WROWS + row], e_hs[c + j], v);
+          if (c + j >= a0 && c + j < a1) v += lora[(c + j - a0) * WROWS + row];
         }
         if (c + j < cnt) ptx::st_shared_cluster_f32(dst + static_cast<uint32_t>((c + j) * R) * 4u, v);
       }
     }
     ptx::tc_fence_before();
   }
-  if (warp < 2) ptx::cluster_wait_acquire();
+  if (warp < 2 || warp >= 2 + EPI_WARPS) ptx::cluster_wait_acquire();
 
   __syncwarp();
   __syncthreads();
@@ -1461,15 +1661,15 @@ SplitInfo &split_info(const DeviceInfo &dev) {
   SplitInfo &si = info[dev.device & 63];
   if (!si.ready) {
     si.ready = true;
-    // (the static part takes a little of the 227 KB)
+    // (the static barriers take a little of the 227 KB)
     si.err = cudaFuncSetAttribute(split_kernel<LORA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  SPLIT_SMEM - 3072);
+                                  SPLIT_SMEM - 1024);
     si.clusters[1] = dev.sm_count;
     for (int s = 2; s <= SPLIT_MAX && si.err == cudaSuccess; ++s) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(static_cast<unsigned>(dev.sm_count / s * s));
-      cfg.blockDim = dim3(NUM_THREADS);
-      cfg.dynamicSmemBytes = SPLIT_SMEM - 3072;
+      cfg.blockDim = dim3(NUM_THREADS + (LORA ? 32 : 0));
+      cfg.dynamicSmemBytes = SPLIT_SMEM - 1024;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = static_cast<unsigned>(s);
@@ -1511,17 +1711,22 @@ int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const D
   const uint32_t stage = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
   const uint32_t rows = static_cast<uint32_t>(((WROWS + p.split - 1) / p.split + 3) & ~3);
   const uint32_t part = static_cast<uint32_t>(p.split * p.tok_cap) * rows * 4;
-  const uint32_t lora = LORA ? static_cast<uint32_t>(p.tok_cap) * WROWS * 4 : 0;
+  const uint32_t lora =
+      LORA ? static_cast<uint32_t>(std::max((p.tok_cap / 8 + p.split - 1) / p.split * 8,
+                                            p.own_down ? kLoraOwnTokens : 0)) *
+                 WROWS * 4
+           : 0;
   const uint32_t tab = static_cast<uint32_t>(p.E + 1) * 8 + 16 + SPLIT_EPI;
-  const uint32_t room = SPLIT_SMEM - 4096 - part - lora - tab;
-  p.stages = std::max(1, std::min({static_cast<int>(room / stage), SPLIT_STAGES,
-                                   LORA ? SPLIT_STAGES : p.kps}));
-  p.off_part = static_cast<uint32_t>(p.stages) * stage;
+  const uint32_t ring = LORA ? SUM_RING : 0u;
+  const uint32_t room = SPLIT_SMEM - 2048 - ring - part - lora - tab;
+  p.stages = std::max(1, std::min({static_cast<int>(room / stage), SPLIT_STAGES, p.kps}));
+  p.off_ring = static_cast<uint32_t>(p.stages) * stage;
+  p.off_part = p.off_ring + ring;
   p.off_lora = p.off_part + part;
   p.off_tab = p.off_lora + lora;
   const size_t smem = p.off_tab + tab + 1024;
   const cudaError_t e = launch(reinterpret_cast<const void *>(&split_kernel<LORA>), maps, p,
-                               tiles * p.split, NUM_THREADS, p.split, smem,
+                               tiles * p.split, NUM_THREADS + (LORA ? 32 : 0), p.split, smem,
                                stream, pdl);
   return e == cudaSuccess ? 0 : launch_failed(op, e);
 }
@@ -1533,8 +1738,8 @@ bool make_common_maps(Maps *m, int n, const uint8_t *xq, const uint8_t *wq, int6
     if (!make_tmap_2d_sw128(&m->x[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, K, M, K, BK, 16 * (i + 1),
                             err))
       return false;
-  return make_tmap_3d_sw128(&m->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, K, N, E, K, N * K, BK, WROWS,
-                            err);
+  return make_tmap_3d_swizzled(&m->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, K, N, E, K, N * K, BK,
+                               WROWS, 128, err);
 }
 
 }  // namespace rowsel
@@ -1666,11 +1871,16 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   bool ok = make_common_maps(&maps, few ? p.tok_cap / 16 : H_MAPS, a.xq, a.wq, a.M, a.N, a.K, 1,
                              &err);
-  ok = ok && make_tmap_3d_sw128(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2, 64,
-                                WROWS, &err);
-  if (!p.own_down)
-    for (int i = 0; ok && i < (few ? p.tok_cap / 16 : H_MAPS); ++i)
+  if (few) {
+    const int sw = sum_width(static_cast<int>(a.R));
+    ok = ok && make_tmap_3d_swizzled(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2,
+                                     static_cast<uint32_t>(sw), WROWS, sw * 2, &err);
+  } else {
+    ok = ok && make_tmap_3d_swizzled(&maps.lb, t16, a.lora_b, a.R, a.N, a.L, a.R * 2, a.N * a.R * 2,
+                                     64, WROWS, 128, &err);
+    for (int i = 0; ok && i < H_MAPS; ++i)
       ok = make_tmap_2d_sw128(&maps.h[i], t16, w.hl, 2 * rp, a.M, 4 * rp, 64, 16 * (i + 1), &err);
+  }
   if (!ok) {
     set_error(std::string(op) + ": " + err);
     return 4;

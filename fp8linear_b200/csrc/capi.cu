@@ -779,7 +779,7 @@ int fp8lin_fp8_linear_lora(const void *x, int x_dtype, const void *wq, const flo
       xq + round_up(static_cast<size_t>(M) * static_cast<size_t>(K), kWsAlign));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   L2Prefetch pf;
-  if (M <= kLoraRowsMaxM) {  // as fp8_linear: the weights come into L2 on the way
+  if (M <= kFewTokenMaxM) {  // the weights come into L2 on the way
     pf.ptr = wq;
     pf.bytes = N * K;
   }

@@ -55,7 +55,7 @@ constexpr uint64_t kDrainLimitNs = 1000000000ull;
 struct Maps {
   CUtensorMap x[X_MAPS];  // xq [M][K], box 128 B x 16 (i + 1) rows
   CUtensorMap w;          // wq [E][N][K], box 128 B x 128 rows x 1
-  CUtensorMap lb;         // lora_b [L][N][R], box 64 x 128 rows x 1
+  CUtensorMap lb;         // lora_b [L][N][R], box 64 (few tokens: sum_width(R)) x 128 rows x 1
   CUtensorMap h[H_MAPS];  // hl [M][2 rank_pad], box 64 x 16 (i + 1) rows
 };
 
@@ -281,11 +281,18 @@ __device__ __forceinline__ void zero_rows(const Params &p, const int *row, int f
 //
 // A tile of tokens of short runs (decoding requests) takes its adapters one after the other,
 // each into a window of TMEM columns of its own for all the tile's tokens; their h is loaded
-// once and the stages bring B alone (with h in every stage all CTAs kept asking for the same
-// few lines: 64 tokens of 27 adapters took 35 us). The epilogue keeps the columns of the adapter's own tokens while further adapters come in. The
-// columns of the other tokens are never read, so that an adapter's infinities stay with its
-// tokens (which one accumulator over tokens masked with zeros would not do: 0 * inf). Warp-level
-// MMAs on the epilogue warps took 0.8 us an adapter at rank 64.
+// once and the stages bring B alone. The epilogue keeps the columns of the adapter's own tokens
+// while further adapters come in. The columns of the other tokens are never read, so that an
+// adapter's infinities stay with its tokens (which one accumulator over tokens masked with
+// zeros would not do: 0 * inf).
+//
+// split_kernel, where the whole call is such tokens and a CTA has few K-blocks, takes the
+// adapters on the epilogue warps' own matrix instructions (adapter_sums below), with a ring of
+// B boxes that a further warp fills while the K-blocks run. Measured, both ways: 64 tokens of 27
+// adapters, 4096 -> 6144, rank 32: 29 us on the warps, 37 in TMEM windows behind the K-blocks of
+// one ring (whose order makes the two wait for one another); persist_kernel, 2000 tokens of
+// prompts and decodes, 4096 -> 4096, rank 64: 82 us on the warps (0.8 us an adapter, which
+// nothing hides in a pair that has one tile), 79 in windows; 16384 rows, rank 128: 351 and 337.
 
 // The stages of an adapter that is a whole tile's: stage(bx, hx, steps, first) with the columns
 // of B and of hl and the 16-element steps; false ends them. (Nested counted loops: with the
@@ -717,12 +724,13 @@ struct Cfg {
   static constexpr uint32_t OFF_TAB = OFF_H + (LORA ? 4u * (kLoraMixed / CG) * BK : 0u);
   static constexpr int TAB = LORA ? 2 : kMaxExperts + 1;
   static constexpr uint32_t OFF_BAR = (OFF_TAB + 2 * TAB * 4 + 7u) & ~7u;
-  static constexpr uint32_t NUM_BARS = 2 * STAGES + 7 + 2 * WINDOWS;  // full, empty, tfull, tempty, drain, h, windows
+  // full, empty, tfull, tempty, drain, h, windows
+  static constexpr uint32_t NUM_BARS = 2 * STAGES + 7 + 2 * WINDOWS;
   static constexpr uint32_t OFF_SLOT = OFF_BAR + NUM_BARS * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_SLOT + 8 + 1024;
   static_assert(STAGE % 1024 == 0, "swizzle atoms need 1024 B alignment");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
-  static_assert(!LORA || 3 * TOK_MAX <= 512, "TMEM budget");
+  static_assert(!LORA || (CG == 2 && 3 * TOK_MAX <= 512), "TMEM budget");
 };
 
 template <int CG, bool LORA>
@@ -884,16 +892,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             if (!(ok = warp_wait(bar_h + 8, hphase ^ 1u, abort, elected))) break;
             const int boxes = h_boxes(p.rank_pad);
             if (elected) {
-              const uint32_t bytes = static_cast<uint32_t>(nn / CG) * BK;
-              const uint32_t hl = CG == 1 ? bar_h : ptx::map_shared_rank(bar_h, 0);
+              const uint32_t bytes = static_cast<uint32_t>(nn / CG) * BK;  // (a multiple of 1024)
+              const uint32_t hl = ptx::map_shared_rank(bar_h, 0);
               if (leader) ptx::mbar_arrive_expect_tx(bar_h, CG * bytes * static_cast<uint32_t>(boxes));
-              for (int i = 0; i < boxes; ++i) {
-                const uint32_t dst = sbase + C::OFF_H + static_cast<uint32_t>(i) * bytes;
-                if constexpr (CG == 1)
-                  ptx::tma_load_2d(dst, &maps.h[mi], h_column(p.rank_pad, i), xrow, hl);
-                else
-                  ptx::tma_load_2d_pair(dst, &maps.h[mi], h_column(p.rank_pad, i), xrow, hl);
-              }
+              for (int i = 0; i < boxes; ++i)
+                ptx::tma_load_2d_pair(sbase + C::OFF_H + static_cast<uint32_t>(i) * bytes,
+                                      &maps.h[mi], h_column(p.rank_pad, i), xrow, hl);
             }
             hphase ^= 1u;
           }
@@ -1009,23 +1013,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                         min(4, (p.rank_pad - bx) / 16), bx == 0, low);
                   next_stage();
                 }
-                if (ok && elected) {
-                  if constexpr (CG == 1)
-                    ptx::mma_commit(bar_wfull + 8 * window);
-                  else
-                    ptx::mma_commit_pair_mc(bar_wfull + 8 * window, 0x3);
-                }
+                if (ok && elected) ptx::mma_commit_pair_mc(bar_wfull + 8 * window, 0x3);
                 if (++window == C::WINDOWS) {
                   window = 0;
                   wphase ^= 1u;
                 }
               }
-              if (ta.leaders != 0 && elected) {  // h may be overwritten
-                if constexpr (CG == 1)
-                  ptx::mma_commit(bar_h + 8);
-                else
-                  ptx::mma_commit_pair_mc(bar_h + 8, 0x3);
-              }
+              if (ta.leaders != 0 && elected)  // h may be overwritten
+                ptx::mma_commit_pair_mc(bar_h + 8, 0x3);
             }
           }
         }
@@ -1116,12 +1111,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                          mask, mine, SUM_PITCH);
             ptx::tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-              if constexpr (CG == 1)
-                ptx::mbar_arrive(bar_wempty + 8 * window);
-              else
-                ptx::mbar_arrive_cluster_relaxed(ptx::map_shared_rank(bar_wempty + 8 * window, 0));
-            }
+            if (lane == 0)
+              ptx::mbar_arrive_cluster_relaxed(ptx::map_shared_rank(bar_wempty + 8 * window, 0));
             if (++window == C::WINDOWS) {
               window = 0;
               wphase ^= 1u;
@@ -1243,11 +1234,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
 // ---------------------------------------------------------------- split-K kernel
 
-constexpr int SPLIT_TOK = 128;   // tokens per tile, at most
-constexpr int SPLIT_LORA_TOK = 64;  // with adapters, whose sums need room too
+// What bounds it: the latency of a short chain. One expert's row, 2048 -> 1024, 16 experts: 7.3
+// us with the quantizer, of which the 2 MB of weights would take 0.6 at the copy rate; 64
+// tokens with adapters, 4096 -> 6144: 29 us, three dependent launches, against 7.
+constexpr int SPLIT_TOK = 128;   // tokens per tile, at most (with adapters kLoraRowsMaxM)
 constexpr int SPLIT_STAGES = 8;  // ring slots, at most
 constexpr int SPLIT_MAX = 8;     // CTAs per cluster, at most (portable)
-constexpr int SPLIT_COST = 12;   // a tile's set-up and reduction, in K-blocks
+// A tile's set-up and reduction, in K-blocks (half or twice as much: the same times, within
+// 2%, at 1 to 64 tokens)
+constexpr int SPLIT_COST = 12;
 constexpr uint32_t SPLIT_EPI = (2 * SPLIT_TOK + 2 * WROWS) * 4;  // xs, ws, bias, hscale
 constexpr uint32_t SPLIT_SMEM = 232448;
 
@@ -1346,6 +1341,17 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     own_adapter_sums(p, kb0 * BK, (kb0 + nkb) * BK, q.wb * WROWS + row,
                      reinterpret_cast<float *>(smem + p.off_ring), lora, threadIdx.x - 64, row);
   }
+  // Adapters: the cluster's CTAs share out the tokens, eight at a time (own_down: all tokens,
+  // but only this CTA's K range of them).
+  const bool own = LORA && p.own_down;
+  const int per_cta = LORA ? ((cnt + 7) / 8 + p.split - 1) / p.split * 8 : 0;
+  const int a0 = own ? 0 : min(cnt, rank * per_cta), a1 = own ? cnt : min(cnt, a0 + per_cta);
+  // (B and ids are the call's own inputs: their boxes need no wait for the kernel before)
+  if (LORA && !own && warp == 2 + EPI_WARPS) {
+    SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
+    feed_sums(p, &maps.lb, ring, q.t0 + a0, q.t0 + a1, q.wb * WROWS);
+    drain_sums(ring);
+  }
   if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
@@ -1355,12 +1361,6 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
   const int r1 = min(WROWS, r0 + R);
   const int quads = r1 > r0 ? (r1 - r0) >> 2 : 0;
   const int n0 = q.wb * WROWS;
-
-  // Adapters: the cluster's CTAs share out the tokens, eight at a time (own_down: all tokens,
-  // but only this CTA's K range of them).
-  const bool own = LORA && p.own_down;
-  const int per_cta = LORA ? ((cnt + 7) / 8 + p.split - 1) / p.split * 8 : 0;
-  const int a0 = own ? 0 : min(cnt, rank * per_cta), a1 = own ? cnt : min(cnt, a0 + per_cta);
 
   if (warp == 0) {
     const bool elected = ptx::elect_one();
@@ -1418,11 +1418,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
       ptx::mma_commit(bar_drain);
       ptx::mbar_wait_timeout(bar_drain, 0, kDrainLimitNs);
     }
-  } else if (LORA && warp == 2 + EPI_WARPS) {
-    SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
-    if (!own) feed_sums(p, &maps.lb, ring, q.t0 + a0, q.t0 + a1, n0);
-    drain_sums(ring);
-  } else {
+  } else if (warp < 2 + EPI_WARPS) {
     // xs (adapters: and hscale) of the tokens, weight scales and biases of the rows reduced
     // here
     const int et = threadIdx.x - 64;
@@ -1857,14 +1853,13 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   const int64_t wb = (a.N + rows - 1) / rows;
   // the plan's tiles at most (and every product within int32)
   const int64_t tiles =
-      wb * (few ? (a.M + SPLIT_LORA_TOK - 1) / SPLIT_LORA_TOK : lora_plan_max(a.M));
+      wb * (few ? 1 : lora_plan_max(a.M));
   if (tiles > 0x3fffffffLL) {
     set_error(std::string(op) + ": too many output tiles");
     return 2;
   }
   p.n_wb = static_cast<int>(wb);
-  p.tok_cap = few ? static_cast<int>(std::min<int64_t>((a.M + 15) / 16 * 16, SPLIT_LORA_TOK))
-                  : kLoraTileTokens;
+  p.tok_cap = few ? static_cast<int>((a.M + 15) / 16 * 16) : kLoraTileTokens;
   std::string err;
   Maps maps = {};
   const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16

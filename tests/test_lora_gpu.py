@@ -48,7 +48,9 @@ CASES = [
     (4096, 1000, 8, 64, [(i % 8, 1) for i in range(64)]),
     (272, 2048, 5, 128, [(4, 100), (-1, 3), (0, 25)]),
     (128, 64, 1, 40, [(-1, 30)]),
-    # more than 128 rows: tensor cores
+    (1040, 384, 33, 32, [(i % 33, 1) for i in range(63)]),
+    (1040, 384, 33, 32, [(i % 33, 1) for i in range(65)]),
+    # more than 64 rows: tiles from the plan
     (16, 1, 1, 8, [(0, 129)]),
     (256, 320, 2, 16, [(0, 160), (1, 160)]),
     (1040, 257, 3, 8, [(0, 200), (-1, 31), (2, 1), (1, 400), (-1, 170)]),

@@ -94,6 +94,23 @@ def test_rows_in_any_order(M):
           *lora_ref(x, wq, ws, a, b, ids, sc, bias))
 
 
+@pytest.mark.parametrize("M", [65, 511, 512, 513, 1025, 5000])
+@pytest.mark.parametrize("longest", [2, 40, 700])
+def test_runs_of_any_lengths(M, longest):
+    """Long runs, short ones and none in turn, across every border of the token plan."""
+    g = torch.Generator().manual_seed(M + longest)
+    ids = []
+    while len(ids) < M:
+        n = int(torch.randint(1, longest + 1, (1,), generator=g))
+        if torch.rand(1, generator=g) < 0.3:
+            n = min(n, 3)
+        ids += [int(torch.randint(-1, 5, (1,), generator=g))] * n
+    ids = torch.tensor(ids[:M], dtype=torch.int32, device="cuda")
+    x, wq, ws, a, b, sc, bias = make(M, M, 48, 72, 5, 8, bias=torch.float32)
+    check(f.fp8_linear_lora(x, wq, ws, a, b, ids, sc, bias),
+          *lora_ref(x, wq, ws, a, b, ids, sc, bias))
+
+
 @pytest.mark.parametrize("M", [7, 300])
 def test_ids_outside_the_adapters_mean_none(M):
     x, wq, ws, a, b, sc, bias = make(M, M, 96, 136, 2, 8)

@@ -110,11 +110,11 @@ def test_lora_workspace_size(api):
     size = api.lora_workspace_size
     assert size(0, 32, 16) == 0
     assert size(5, 64, 0) == api.workspace_size(5, 64)
-    # h in two parts with the rank padded to 16 and a scale per row; above 128 rows the plan of
+    # h in two parts with the rank padded to 16 and a scale per row; above 64 rows the plan of
     # the token tiles (16 bytes each: a header, tiles of 160 and one per 32 rows for the runs'
     # ends, two per 32 rows and one for the gaps); all rounded up to 256 bytes
-    base = api.workspace_size(128, 64)
-    assert size(128, 64, 24) - base == 128 * 2 * 32 * 2 + 512
+    base = api.workspace_size(64, 64)
+    assert size(64, 64, 24) - base == 64 * 2 * 32 * 2 + 256
     base = api.workspace_size(1000, 64)
     plan = 16 * (1 + 1000 // 160 + 1000 // 32 + 2 * (1000 // 32) + 1)
     assert size(1000, 64, 24) - base == 1000 * 128 + 4096 + (plan + 255) // 256 * 256

@@ -62,10 +62,10 @@ constexpr int ROWS = 128;
 constexpr int KB = 64;     // 16-bit elements per K-block: one 128-byte swizzle row
 constexpr int COLS = 256;  // columns (adapters x rank_pad) per pass, at most
 constexpr int MAX_STAGES = 8;
-constexpr int NUM_THREADS = 224;  // producer, MMA, 4 x TMEM, plan
+constexpr int NUM_THREADS = 256;  // producer, MMA, 4 x TMEM, plan, and one more for the row sums
 constexpr int MAX_SPLIT = 8;
 // dynamic: the ring, cut anew for each item into stages of x_rows + columns rows of 128 bytes,
-// then fp32 [ROWS][rank_pad + 1]
+// then fp32 [ROWS][rank_pad + 4]
 constexpr uint32_t SMEM_MAX = 232448 - 4096;  // (the static part is below 3 KB)
 
 __device__ __forceinline__ void record_timeout(volatile int *abort) {
@@ -182,8 +182,8 @@ __device__ __forceinline__ int adapters_at_most(const Params &p, int m0, int lan
 
 // An item's sums, row by row: the K-splits' parts added in rank order, scaled, and split into
 // the two 16-bit parts. CTA `rank` of the S of a cluster has rows rank, rank + S, ..; a warp
-// has two rows at a time, a lane values 2 lane, + 1 and 64 more of each. (All loads are
-// unconditional, so that they run side by side: behind branches they took 1 us a row pair.)
+// has two rows at a time, a lane values 4 lane .. 4 lane + 3, one 16-byte load from each part
+// (4-byte loads took three times as long), all of them before the first is used.
 template <int S>
 __device__ __forceinline__ void finish_rows(const Params &p, const float *part, int pitch,
                                             const int *live, const float *scaling, int m0,
@@ -193,36 +193,34 @@ __device__ __forceinline__ void finish_rows(const Params &p, const float *part, 
 #pragma unroll
   for (int s = 0; s < S; ++s)
     from[s] = S == 1 ? ptx::smem_u32(part) : ptx::map_shared_rank(ptx::smem_u32(part), s);
-  int col[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) col[i] = (i >> 1) * 64 + 2 * lane + (i & 1);
+  const int col = 4 * lane;
   for (int r0 = 2 * warp; rank + r0 * S < ROWS; r0 += 2 * (NUM_THREADS / 32)) {
     int row[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) row[h] = min(rank + (r0 + h) * S, ROWS - 1);
     const bool on[2] = {live[row[0]] != 0, live[row[1]] != 0 && rank + (r0 + 1) * S < ROWS};
     if (!on[0] && !on[1]) continue;  // uniform in the warp
-    float t[2][4][S];
+    float4 t[2][S];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const uint32_t at =
-              from[s] + static_cast<uint32_t>(row[h] * pitch + min(col[i], p.rank_pad - 1)) * 4u;
-          t[h][i][s] = S == 1 ? ptx::ld_shared_f32(at) : ptx::ld_shared_cluster_f32(at);
-        }
+      for (int s = 0; s < S; ++s) {
+        const uint32_t at =
+            from[s] + static_cast<uint32_t>(row[h] * pitch + min(col, p.rank_pad - 4)) * 4u;
+        t[h][s] = S == 1 ? ptx::ld_shared_f32x4(at) : ptx::ld_shared_cluster_v4(at);
+      }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float v[4];
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < S; ++s) v[i] += t[h][i][s];
-        v[i] = col[i] < p.R ? v[i] * scaling[row[h]] : 0.0f;
+      for (int s = 0; s < S; ++s) {
+        v[0] += t[h][s].x;
+        v[1] += t[h][s].y;
+        v[2] += t[h][s].z;
+        v[3] += t[h][s].w;
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = col < p.R ? v[i] * scaling[row[h]] : 0.0f;  // R % 8 == 0
       if (!on[h]) continue;
       // f16: the row divided by 2^ex, its largest finite value's exponent (exact)
       int ex = 0;
@@ -237,22 +235,26 @@ __device__ __forceinline__ void finish_rows(const Params &p, const float *part, 
           ex = min(126, max(-126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
       }
       const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-      uint32_t *dst = reinterpret_cast<uint32_t *>(p.hl) +
-                      static_cast<int64_t>(m0 + row[h]) * p.rank_pad + lane;
+      if (col < p.rank_pad) {
+        uint32_t hi2[2], lo2[2];
 #pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        if (col[i] >= p.rank_pad) break;
-        // an infinity or NaN is the high part's alone
-        float hi[2], lo[2];
+        for (int i = 0; i < 4; i += 2) {
+          // an infinity or NaN is the high part's alone
+          float hi[2], lo[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float w = v[i + j] * inv;
-          hi[j] = f16 ? __half2float(__float2half_rn(w)) : __bfloat162float(__float2bfloat16_rn(w));
-          lo[j] = fabsf(hi[j]) <= (f16 ? 65504.0f : 3.402823466e38f) ? w - hi[j] : 0.0f;
+          for (int j = 0; j < 2; ++j) {
+            const float w = v[i + j] * inv;
+            hi[j] =
+                f16 ? __half2float(__float2half_rn(w)) : __bfloat162float(__float2bfloat16_rn(w));
+            lo[j] = fabsf(hi[j]) <= (f16 ? 65504.0f : 3.402823466e38f) ? w - hi[j] : 0.0f;
+          }
+          hi2[i / 2] = f16 ? ptx::pack_f16x2(hi[0], hi[1]) : ptx::pack_bf16x2(hi[0], hi[1]);
+          lo2[i / 2] = f16 ? ptx::pack_f16x2(lo[0], lo[1]) : ptx::pack_bf16x2(lo[0], lo[1]);
         }
-        dst[16 * i] = f16 ? ptx::pack_f16x2(hi[0], hi[1]) : ptx::pack_bf16x2(hi[0], hi[1]);
-        dst[p.rank_pad / 2 + 16 * i] =
-            f16 ? ptx::pack_f16x2(lo[0], lo[1]) : ptx::pack_bf16x2(lo[0], lo[1]);
+        uint32_t *dst = reinterpret_cast<uint32_t *>(p.hl) +
+                        static_cast<int64_t>(m0 + row[h]) * p.rank_pad + 2 * lane;
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(hi2[0], hi2[1]);
+        *reinterpret_cast<uint2 *>(dst + p.rank_pad / 2) = make_uint2(lo2[0], lo2[1]);
       }
       if (lane == 0)
         p.hscale[m0 + row[h]] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
@@ -292,7 +294,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   volatile int *abort = &s_abort;
   float *part = reinterpret_cast<float *>(smem + p.off_part);
   const uint32_t x_stage = static_cast<uint32_t>(p.x_rows) * 128;
-  const int pitch = p.rank_pad + 1;  // odd: a column of it hits all banks
+  // 16 bytes past a multiple of 64: eight rows' 16-byte pieces hit all banks
+  const int pitch = p.rank_pad + 4;
   const int per_pass = p.cols / p.rank_pad;
 
   ptx::grid_launch_dependents();
@@ -457,12 +460,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           ptx::tmem_wait_ld();
           if (keep) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) part[row * pitch + c + j] = __uint_as_float(r[j]);
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4 *>(part + row * pitch + c + j) =
+                  make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
+                              __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
           }
         }
       }
       ptx::tc_fence_before();
-    } else if (plan_open) {
+    } else if (warp == 6 && plan_open) {
       ptx::grid_dependency_wait();
       make_plan(p, lane);
       plan_open = false;
@@ -611,7 +617,7 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   p.clusters = static_cast<int>(std::max<int64_t>(
       tiles, std::min<int64_t>(di.clusters[split], tiles * p.max_passes)));
   p.x_rows = static_cast<int>(std::min<int64_t>((a.M + 7) / 8 * 8, ROWS));
-  const uint32_t part = ROWS * (static_cast<uint32_t>(p.rank_pad) + 1) * 4;
+  const uint32_t part = ROWS * (static_cast<uint32_t>(p.rank_pad) + 4) * 4;
   p.off_part = (SMEM_MAX - 1024 - part) / 1024 * 1024;
   const CUtensorMapDataType t16 = a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

@@ -123,10 +123,19 @@ __device__ __forceinline__ void make_plan(const Params &p, int lane) {
   // Blocks of 32 rows, AHEAD of them at a time, and as many loaded while those are looked at.
   // A row is compared with the one before it by a load of its own; most blocks have no border
   // between runs, which one vote shows for all of them. (The rows before through shuffles and a
-  // vote a block: 9216 rows took 24 us, twice as long as all sums.)
-  constexpr int AHEAD = 16;
+  // vote a block: 9216 rows took 24 us, twice as long as all sums; now 11, most of it the loads.)
+  constexpr int AHEAD = 32;
   int here[AHEAD], left[AHEAD];
   auto fetch = [&](int b) {
+    if (b > 0 && b <= p.M - 32 * AHEAD) {
+      const int *q = p.ids + b + lane;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        here[k] = __ldg(q + 32 * k);
+        left[k] = __ldg(q + 32 * k - 1);
+      }
+      return;
+    }
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       const int m = min(b + 32 * k + lane, p.M - 1);  // (a row past the end is no border)
@@ -138,9 +147,12 @@ __device__ __forceinline__ void make_plan(const Params &p, int lane) {
   for (int b0 = 0; b0 < p.M; b0 += 32 * AHEAD) {
     uint32_t mine = 0;  // bit k: a run starts at this lane's row of block k
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int id = has_adapter(p, here[k]) ? here[k] : -1;
-      if (id != (has_adapter(p, left[k]) ? left[k] : -1)) mine |= 1u << k;
+    for (int k = 0; k < AHEAD; ++k)
+      if (here[k] != left[k]) mine |= 1u << k;
+    if (__any_sync(0xFFFFFFFFu, mine != 0)) {  // (different ids may both mean none)
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (!has_adapter(p, here[k]) && !has_adapter(p, left[k])) mine &= ~(1u << k);
     }
     fetch(b0 + 32 * AHEAD);
     for (uint32_t todo = __reduce_or_sync(0xFFFFFFFFu, mine); todo != 0; todo &= todo - 1) {

@@ -87,16 +87,28 @@ int check_gemm_args(const void *xq, const float *xs, const void *wq, const float
   return FP8LIN_OK;
 }
 
-// The further arguments of the grouped forms, after check_gemm_args.
-int check_group_args(const int32_t *offsets, int64_t M, int64_t N, int64_t K, int64_t E,
-                     const char *op) {
+// What the kernels with weights per row ask beyond check_gemm_args: their indexes are int32, up to
+// a tile past the end, and they read scales and bias with plain loads.
+constexpr int64_t kRowselMaxDim = 0x7fffffffLL - 1023;
+
+int check_rowsel_args(const float *xs, const float *ws, const void *bias, int bias_dtype, int64_t M,
+                      int64_t N, int64_t K, const char *op) {
+  if (M > kRowselMaxDim || N > kRowselMaxDim || K > kRowselMaxDim)
+    return fail(FP8LIN_ERR_UNSUPPORTED,
+                std::string(op) + ": M, N and K must be at most 2^31 - 1024 (int32 indexes)");
+  if (!aligned(xs, 4) || !aligned(ws, 4) || (bias && !aligned(bias, bias_dtype == kF32 ? 4 : 2)))
+    return fail(FP8LIN_ERR_UNSUPPORTED,
+                std::string(op) + ": scales and bias must be aligned to their elements");
+  return FP8LIN_OK;
+}
+
+// The further arguments of the grouped forms, after check_rowsel_args.
+int check_group_args(const int32_t *offsets, int64_t M, int64_t N, int64_t E, const char *op) {
   const std::string o(op);
   if (E < 1 || E > kMaxExperts)
     return fail(FP8LIN_ERR_UNSUPPORTED, o + ": the number of experts must be 1 to " +
                                             std::to_string(kMaxExperts) + ", got " +
                                             std::to_string(E));
-  if (M > 0x7fffffffLL || N > 0x7fffffffLL || K > 0x7fffffffLL)
-    return fail(FP8LIN_ERR_UNSUPPORTED, o + ": dimensions must fit in int32");
   if (M == 0 || N == 0) return FP8LIN_OK;
   if (!offsets) return fail(FP8LIN_ERR_INVALID_ARGUMENT, o + ": null offsets");
   if (!aligned(offsets, 4)) return fail(FP8LIN_ERR_UNSUPPORTED, o + ": offsets must be 4-byte aligned");
@@ -697,7 +709,9 @@ int fp8lin_fp8_grouped_gemm(const void *xq, const float *x_scale, const void *wq
   clear_error();
   int rc = check_gemm_args(xq, x_scale, wq, w_scale, bias, bias_dtype, out, out_dtype, M, N, K,
                            "fp8_grouped_gemm");
-  if (rc == FP8LIN_OK) rc = check_group_args(offsets, M, N, K, E, "fp8_grouped_gemm");
+  if (rc == FP8LIN_OK)
+    rc = check_rowsel_args(x_scale, w_scale, bias, bias_dtype, M, N, K, "fp8_grouped_gemm");
+  if (rc == FP8LIN_OK) rc = check_group_args(offsets, M, N, E, "fp8_grouped_gemm");
   if (rc != FP8LIN_OK || M == 0 || N == 0) return rc;
   GroupedArgs a{static_cast<const uint8_t *>(xq), x_scale, static_cast<const uint8_t *>(wq),
                 w_scale, bias, bias ? bias_dtype : kNone, out, out_dtype, offsets, M, N, K, E};
@@ -713,7 +727,9 @@ int fp8lin_fp8_grouped_linear(const void *x, int x_dtype, const void *wq, const 
     return fail(FP8LIN_ERR_INVALID_ARGUMENT, "fp8_grouped_linear: x must be fp16 or bf16");
   int rc = check_gemm_args(reinterpret_cast<const void *>(16), w_scale, wq, w_scale, bias,
                            bias_dtype, out, out_dtype, M, N, K, "fp8_grouped_linear");
-  if (rc == FP8LIN_OK) rc = check_group_args(offsets, M, N, K, E, "fp8_grouped_linear");
+  if (rc == FP8LIN_OK)
+    rc = check_rowsel_args(nullptr, w_scale, bias, bias_dtype, M, N, K, "fp8_grouped_linear");
+  if (rc == FP8LIN_OK) rc = check_group_args(offsets, M, N, E, "fp8_grouped_linear");
   if (rc != FP8LIN_OK || M == 0 || N == 0) return rc;
   if (!x) return fail(FP8LIN_ERR_INVALID_ARGUMENT, "fp8_grouped_linear: null x");
   const size_t need = fp8lin_linear_workspace_size(M, K);
@@ -762,13 +778,17 @@ int fp8lin_fp8_linear_lora(const void *x, int x_dtype, const void *wq, const flo
     return fail(FP8LIN_ERR_UNSUPPORTED, o + ": the rank must be a multiple of 8 from 8 to " +
                                             std::to_string(kLoraMaxRank) + " (pad with zeros), got " +
                                             std::to_string(R));
-  if (M > 0x7fffffffLL || N > 0x7fffffffLL || K > 0x7fffffffLL || L > 0x7fffffffLL)
-    return fail(FP8LIN_ERR_UNSUPPORTED, o + ": dimensions must fit in int32");
+  rc = check_rowsel_args(scaling, w_scale, bias, bias_dtype, M, N, K, op);
+  if (rc != FP8LIN_OK) return rc;
+  if (L > 0x7fffffffLL)
+    return fail(FP8LIN_ERR_UNSUPPORTED, o + ": the number of adapters must fit in int32");
   if (M == 0 || N == 0) return FP8LIN_OK;
   if (!x || !lora_a || !lora_b || !adapters || !scaling)
     return fail(FP8LIN_ERR_INVALID_ARGUMENT, o + ": null pointer");
   if (!aligned(x, 16) || !aligned(lora_a, 16) || !aligned(lora_b, 16))
     return fail(FP8LIN_ERR_UNSUPPORTED, o + ": x, lora_a and lora_b must be 16-byte aligned");
+  if (!aligned(adapters, 4))
+    return fail(FP8LIN_ERR_UNSUPPORTED, o + ": adapters must be 4-byte aligned");
   const size_t need = fp8lin_fp8_linear_lora_workspace_size(M, K, R);
   if (!workspace || workspace_bytes < need || !aligned(workspace, kWsAlign))
     return fail(FP8LIN_ERR_WORKSPACE, o + ": workspace of " + std::to_string(need) +

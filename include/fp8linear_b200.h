@@ -375,8 +375,8 @@ FP8LIN_API int fp8lin_fp8_linear_noalloc(const void *x, int x_dtype, const void 
  *   offsets [E+1] int32 in device memory, never read on the host: clamped to [0, M] and to
  *   their running maximum (offsets that run backwards leave the later group empty)
  *   bias [E,N] BF16/F16/F32 or NULL; out [M,N] BF16 or F16
- * Requirements (checked): 1 <= E <= 1024, K % 16 == 0, K > 0, xq/wq 16-byte aligned, M, N and
- * K below 2^31. M == 0 or N == 0 is a no-op.
+ * Requirements (checked): 1 <= E <= 1024, K % 16 == 0, K > 0, xq/wq 16-byte aligned, the other
+ * arrays aligned to their elements, M, N and K at most 2^31 - 1024. M == 0 or N == 0 is a no-op.
  */
 FP8LIN_API int fp8lin_fp8_grouped_gemm(const void *xq, const float *x_scale, const void *wq,
                                        const float *w_scale, const int32_t *offsets,
@@ -404,7 +404,8 @@ FP8LIN_API int fp8lin_fp8_grouped_linear(const void *x, int x_dtype, const void 
  *   device memory; the others as fp8lin_fp8_linear
  *   workspace fp8lin_fp8_linear_lora_workspace_size(M, K, R) bytes, 256-byte aligned
  * Requirements (checked): R % 8 == 0, 8 <= R <= 128; x, wq, lora_a and lora_b 16-byte aligned;
- * K % 16 == 0; sizes below 2^31. L == 0 is fp8lin_fp8_linear. M == 0 or N == 0 is a no-op.
+ * K % 16 == 0; the other arrays aligned to their elements; M, N and K at most 2^31 - 1024.
+ * L == 0 is fp8lin_fp8_linear. M == 0 or N == 0 is a no-op.
  */
 FP8LIN_API size_t fp8lin_fp8_linear_lora_workspace_size(int64_t M, int64_t K, int64_t R);
 FP8LIN_API int fp8lin_fp8_linear_lora(const void *x, int x_dtype, const void *wq,

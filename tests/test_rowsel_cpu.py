@@ -69,7 +69,13 @@ def test_grouped_refusals(api):
     assert grouped(api, K=24) == 2 and grouped(api, K=0) == 2
     assert grouped(api, E=0) == 2 and grouped(api, E=1025) == 2
     assert "experts" in api.last_error()
-    assert grouped(api, M=2**31) == 2 and "int32" in api.last_error()
+    for dim in ("M", "N"):
+        for size in (2**31, 2**31 - 1023):
+            assert grouped(api, **{dim: size}) == 2 and "int32" in api.last_error()
+    assert grouped(api, K=2**31 - 16) == 2 and "int32" in api.last_error()
+    odd = ctypes.c_void_p(257)
+    assert grouped(api, xs=odd) == 2 and grouped(api, ws=odd) == 2
+    assert grouped(api, bias=odd, bd=0) == 2 and grouped(api, bias=ctypes.c_void_p(258), bd=2) == 2
     for name in ("xq", "xs", "wq", "ws", "off", "out"):
         assert grouped(api, **{name: None}) == 1, name
     assert grouped(api, xq=ctypes.c_void_p(264)) == 2 and grouped(api, off=ctypes.c_void_p(258)) == 2
@@ -96,7 +102,8 @@ def test_lora_refusals(api):
     assert call(K=40) == 2
     for R in (0, 4, 12, 136):
         assert call(R=R) == 2 and "rank" in api.last_error()
-    assert call(M=2**31) == 2 and call(L=2**31) == 2
+    assert call(M=2**31) == 2 and call(M=2**31 - 1023) == 2 and call(L=2**31) == 2
+    assert call(ids=ctypes.c_void_p(258)) == 2 and call(sc=ctypes.c_void_p(258)) == 2
     for name in ("x", "a", "b", "ids", "sc"):
         assert call(**{name: None}) == 1, name
     odd = ctypes.c_void_p(264)

@@ -619,10 +619,13 @@ int launch_lora_down(const LoraArgs &a, cudaStream_t stream) {
   p.split = split;
   // a cluster per tile, and further ones for the passes of tiles with many adapters while CTAs
   // are left over still
-  // (few tiles: narrower passes, that more clusters share them: 64 tokens of 27 adapters 29.2 us
-  // against 31.4, 2000 tokens 79 against 84; many: a tile at the border of two requests in one
-  // pass: 16384 rows, rank 128, 347 us against 373)
-  p.cols = split >= 4 ? COLS / 2 : COLS;
+  // Few tiles: four adapters a pass, so that more clusters share them (K 4096: 1000 tokens of
+  // prompts and decodes, rank 64, 55 us, with three 60, with two 67; 64 tokens, rank 16, 24.4, with
+  // eight 26.1; 4096 rows of 8 requests, rank 64, 78, with two 83; only where idle clusters happen to
+  // take all further passes, 2000 tokens at rank 64, 82 and with two 78). Many tiles: all columns, so
+  // that a tile at the border of two requests takes one pass (16384 rows, rank 128: 347 us, with one
+  // adapter a pass 373).
+  p.cols = split >= 4 ? std::min(COLS, 4 * p.rank_pad) : COLS;
   const int per_pass = p.cols / p.rank_pad;
   p.tiles = static_cast<int>(tiles);
   p.max_passes = static_cast<int>((std::min<int64_t>(a.L, ROWS) + per_pass - 1) / per_pass);

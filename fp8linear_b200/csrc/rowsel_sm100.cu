@@ -1236,7 +1236,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
 // What bounds it: the latency of a short chain. One expert's row, 2048 -> 1024, 16 experts: 7.3
 // us with the quantizer, of which the 2 MB of weights would take 0.6 at the copy rate; 64
-// tokens with adapters, 4096 -> 6144: 29 us, three dependent launches, against 7.
+// tokens with adapters, 4096 -> 6144: 28 us, three dependent launches, against 7.
 constexpr int SPLIT_TOK = 128;   // tokens per tile, at most (with adapters kLoraRowsMaxM)
 constexpr int SPLIT_STAGES = 8;  // ring slots, at most
 constexpr int SPLIT_MAX = 8;     // CTAs per cluster, at most (portable)

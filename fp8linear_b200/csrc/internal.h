@@ -195,14 +195,18 @@ cudaError_t read_rowsel_status(unsigned int *bits, bool clear);
 // ---- lora_sm100.cu
 // The adapters' intermediate h and, for more than kLoraRowsMaxM rows, the plan of the GEMM's
 // token tiles, in the workspace:
-//   hl [M][2 * rank_pad] of x's type: h / hscale as a high and a low part, h = hscale *
-//   (hi + lo) to fp32's last bits; hscale fp32 [M], powers of two. Rows without an adapter
-//   are not written;
+//   hl [M][2 * rank_pad] of x's type: h / hscale as a high part and 2^kLoraLowShift times the
+//   rest, h = hscale * (hi + lo / 2^kLoraLowShift) to 2^-16 of h in bf16, where hscale is 1, and to
+//   2^-22 of h or 2^-45 of the row's largest value, whichever is more, in fp16; hscale fp32 [M],
+//   powers of two. Rows without an adapter are not written;
 //   plan int4: {tiles of one adapter, tiles of several}, then the tiles {first token, end,
 //   adapter, 0}, those of several adapters from entry lora_plan_mixed(M) on. A run of at least
 //   kLoraMixed rows with one adapter is cut into tiles of its own (adapter -1: none), of at
 //   most kLoraTileTokens; what lies between such runs goes in tiles of at most kLoraMixed
 //   tokens with any adapters (adapter -2).
+// As far as the rest of a bf16 value can go without passing its high part's range; fp16, whose
+// range is the narrow one, would take 10.
+constexpr int kLoraLowShift = 7;
 inline int64_t lora_rank_pad(int64_t R) { return (R + 15) / 16 * 16; }
 // (Three accumulators of a tile's tokens have to fit in 512 TMEM columns. Of 128 tokens: rank 128,
 // 16384 rows, 371 us against 340, 9216 rows of a few requests 203 against 184, since the

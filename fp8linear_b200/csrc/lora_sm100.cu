@@ -8,10 +8,13 @@
 // its own; rows never mix, so an adapter's infinities and NaN stay with its rows. When the
 // tiles are few, a cluster splits K.
 //
-// The GEMM's tensor cores take h in x's 16-bit type. h is a sum, so it keeps fp32's accuracy:
-// it goes as a high and a low part, h / hscale = hi + lo (bf16: 2^-17 relative; f16: hscale,
-// a power of two, puts the row's largest value in [1, 2), the error is 2^-22 of it), at the
-// price of twice the rank in a product that is a few per cent of the whole.
+// The GEMM's tensor cores take h in x's 16-bit type. h is a sum, and B may bring up what is small
+// in it, so it goes with more bits than the type's, as a high and a low part,
+// h / hscale = hi + lo / 2^7, at the price of twice the rank in a product that is a few per cent
+// of the whole. bf16 has fp32's range (hscale = 1): 2^-16 of each value. f16: hscale, a power of
+// two, puts the row's largest value in [2^14, 2^15), and with the low part 2^7 times larger the
+// error is 2^-22 of a value down to 2^-23 of the row's largest, and 2^-45 of the largest below (with
+// the largest at 1 and a low part of the same scale it was 2^-25 of the largest).
 //
 // The kernel reads x, ids and A before the dependency wait (the kernel before is the call's
 // quantizer, which lets it launch only after its own wait) and writes after it.
@@ -234,7 +237,7 @@ __device__ __forceinline__ void finish_rows(const Params &p, const float *part, 
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = col < p.R ? v[i] * scaling[row[h]] : 0.0f;  // R % 8 == 0
       if (!on[h]) continue;
-      // f16: the row divided by 2^ex, its largest finite value's exponent (exact)
+      // f16: the row divided by 2^ex (exact), its largest finite value in [2^14, 2^15)
       int ex = 0;
       if (f16) {
         float top = 0.0f;
@@ -244,7 +247,7 @@ __device__ __forceinline__ void finish_rows(const Params &p, const float *part, 
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
         if (top > 0.0f)
-          ex = min(126, max(-126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+          ex = max(-126, static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14);
       }
       const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
       if (col < p.rank_pad) {
@@ -258,7 +261,9 @@ __device__ __forceinline__ void finish_rows(const Params &p, const float *part, 
             const float w = v[i + j] * inv;
             hi[j] =
                 f16 ? __half2float(__float2half_rn(w)) : __bfloat162float(__float2bfloat16_rn(w));
-            lo[j] = fabsf(hi[j]) <= (f16 ? 65504.0f : 3.402823466e38f) ? w - hi[j] : 0.0f;
+            lo[j] = fabsf(hi[j]) <= (f16 ? 65504.0f : 3.402823466e38f)
+                        ? (w - hi[j]) * (1 << kLoraLowShift)
+                        : 0.0f;
           }
           hi2[i / 2] = f16 ? ptx::pack_f16x2(hi[0], hi[1]) : ptx::pack_bf16x2(hi[0], hi[1]);
           lo2[i / 2] = f16 ? ptx::pack_f16x2(lo[0], lo[1]) : ptx::pack_bf16x2(lo[0], lo[1]);

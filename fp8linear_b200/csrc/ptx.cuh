@@ -385,6 +385,27 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
         : "memory");
 }
 
+// The same with the accumulator divided by 2^SHIFT first: D = A * B^T + D * 2^-SHIFT.
+template <int CG, int SHIFT>
+__device__ __forceinline__ void mma_f16_shift(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                              uint32_t idesc) {
+  static_assert(SHIFT >= 0 && SHIFT <= 15, "scale-input-d");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "n"(SHIFT)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "n"(SHIFT)
+        : "memory");
+}
+
 // Block-scaled (MXFP8) form: D (+)= (A * 2^(sfA)) * (B * 2^(sfB))^T with one e8m0 scale per
 // 32 K-elements of every row of A and B, read from TMEM at `sfa` / `sfb` (the byte of the
 // 32-bit scale word selected by bits 30-31 of the address and the instruction

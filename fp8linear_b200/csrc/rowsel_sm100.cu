@@ -278,6 +278,8 @@ __device__ __forceinline__ void zero_rows(const Params &p, const int *row, int f
 // the ring: the adapter's B rows beside the tokens' h, into an accumulator of their own. 64
 // 16-bit elements are the 128 bytes of a stage's row: up to rank 32 the high and the low part
 // of h share a stage's box, above it each 64 values of the rank take a stage for either part.
+// The low part, 2^kLoraLowShift times too large, comes first; the first MMA of the high part divides
+// the accumulator by as much.
 //
 // A tile of tokens of short runs (decoding requests) takes its adapters one after the other,
 // each into a window of TMEM columns of its own for all the tile's tokens; their h is loaded
@@ -294,36 +296,39 @@ __device__ __forceinline__ void zero_rows(const Params &p, const int *row, int f
 // prompts and decodes, 4096 -> 4096, rank 64: 82 us on the warps (0.8 us an adapter, which
 // nothing hides in a pair that has one tile), 79 in windows; 16384 rows, rank 128: 351 and 337.
 
-// The stages of an adapter that is a whole tile's: stage(bx, hx, steps, first) with the columns
-// of B and of hl and the 16-element steps; false ends them. (Nested counted loops: with the
-// columns computed from a stage's number by division, and MMAs in a loop of unknown length, a
-// stage took 0.7 us.)
+// What an MMA finds in the accumulator: nothing that counts, sums to add to, or the low part's
+// sums, to be divided by 2^kLoraLowShift.
+enum class Acc { kFresh, kAdd, kShift };
+
+// The stages of an adapter that is a whole tile's: stage(bx, hx, steps, acc) with the columns
+// of B and of hl, the 16-element steps and what the accumulator holds; false ends them. (Nested
+// counted loops: with the columns computed from a stage's number by division, and MMAs in a loop of
+// unknown length, a stage took 0.7 us.)
 template <class Stage>
 __device__ __forceinline__ bool adapter_stages(int rank_pad, Stage &&stage) {
-  for (int part = 0; part < (rank_pad <= 32 ? 1 : 2); ++part)
+  if (rank_pad <= 32) return stage(0, 0, rank_pad / 16, Acc::kFresh);
+  for (int part = 1; part >= 0; --part)
     for (int bx = 0; bx < rank_pad; bx += 64)
-      if (!stage(bx, part * rank_pad + bx, min(4, (rank_pad - bx) / 16), part + bx == 0))
+      if (!stage(bx, part * rank_pad + bx, min(4, (rank_pad - bx) / 16),
+                 bx != 0 ? Acc::kAdd : part != 0 ? Acc::kFresh : Acc::kShift))
         return false;
   return true;
 }
 
-// d (+)= B . h^T for up to 64 ranks: B at `b`, h at `h`; `low`: where the low part of h lies,
-// as a descriptor offset from the high part (0: not in this stage). `first`: nothing in the
-// accumulator counts yet.
+// d = d (as `acc` says) + B . h^T for up to 64 ranks: B at `b`, h at `h`.
 template <int CG>
-__device__ __forceinline__ void lora_mma(uint32_t d, uint32_t b, uint32_t h, uint32_t idesc,
-                                         int steps, bool first, uint32_t low) {
-  const uint64_t adesc = ptx::sw128_kmajor_desc(b);
-  const uint64_t bdesc = ptx::sw128_kmajor_desc(h);
+__device__ __forceinline__ void lora_mma(uint32_t d, uint32_t b, uint64_t hdesc, uint32_t idesc,
+                                         int steps, Acc acc) {
+  const uint64_t bdesc = ptx::sw128_kmajor_desc(b);
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk)  // 16 elements: 32 bytes
-    if (kk < steps)
-      ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + 2 * kk, idesc, first && kk == 0 ? 0u : 1u);
-  if (low != 0) {
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
-      if (kk < steps) ptx::mma_f16<CG>(d, adesc + 2 * kk, bdesc + low + 2 * kk, idesc, 1u);
-  }
+    if (kk < steps) {
+      if (kk == 0 && acc == Acc::kShift)
+        ptx::mma_f16_shift<CG, kLoraLowShift>(d, bdesc, hdesc, idesc);
+      else
+        ptx::mma_f16<CG>(d, bdesc + 2 * kk, hdesc + 2 * kk, idesc,
+                         kk == 0 && acc == Acc::kFresh ? 0u : 1u);
+    }
 }
 
 // A mixed tile's h in shared memory: boxes of 64 columns (`rows` rows of 128 bytes), those of
@@ -335,6 +340,7 @@ __device__ __forceinline__ int h_column(int rank_pad, int box) {
   const int half = (rank_pad + 63) / 64;
   return box < half ? box * 64 : rank_pad + (box - half) * 64;
 }
+// The low part's descriptor offset from the high part's.
 __device__ __forceinline__ uint32_t h_low(int rank_pad, int rows) {
   return rank_pad <= 32 ? static_cast<uint32_t>(rank_pad / 8)
                         : static_cast<uint32_t>((rank_pad + 63) / 64 * rows * BK / 16);
@@ -505,9 +511,9 @@ __device__ __forceinline__ void mma_16x8x16(bool f16, float (&d)[4], const uint3
 }
 
 // For the eight tokens `now` and the 32 weight rows `quarter` of the boxes: the sums
-// sum_r (hi + lo)[token][r] * B[adapter of the token][row][r], as matrix fragments: lane
-// 4i + t gets tokens 2t, 2t + 1 of rows i + 8k in s[k]; zero for tokens without an adapter. C
-// boxes of 16 J ranks an adapter. By one epilogue warp; false when a wait ran out. The high
+// sum_r (hi + lo / 2^kLoraLowShift)[token][r] * B[adapter of the token][row][r], as matrix
+// fragments: lane 4i + t gets tokens 2t, 2t + 1 of rows i + 8k in s[k]; zero for tokens without an
+// adapter. C boxes of 16 J ranks an adapter. By one epilogue warp; false when a wait ran out. The high
 // and the low part have accumulators of their own and a box's fragments are read before its
 // first MMA, so that the chain of dependent MMAs is J long: in one chain with reads between
 // them a box of 32 ranks took 740 cycles.
@@ -563,11 +569,12 @@ __device__ __forceinline__ bool adapter_sums(const Params &p, SumRing &ring,
       ring.next();
     }
     // d[m]: rows i + 16m (0, 1) and i + 16m + 8 (2, 3), tokens 2t (0, 2) and 2t + 1 (1, 3)
+    constexpr float kLow = 1.0f / (1 << kLoraLowShift);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int e = 2 * (k & 1);
-      if (id0 == a) s[k].x = d[k >> 1][0][e] + d[k >> 1][1][e];
-      if (id1 == a) s[k].y = d[k >> 1][0][e + 1] + d[k >> 1][1][e + 1];
+      if (id0 == a) s[k].x = fmaf(d[k >> 1][1][e], kLow, d[k >> 1][0][e]);
+      if (id1 == a) s[k].y = fmaf(d[k >> 1][1][e + 1], kLow, d[k >> 1][0][e + 1]);
     }
   }
   return true;
@@ -883,7 +890,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if constexpr (LORA) {
         const int adapter = ptx::uniform(q.adapter);
         if (adapter >= 0)
-          ok = ok && adapter_stages(p.rank_pad, [&](int bx, int hx, int, bool) {
+          ok = ok && adapter_stages(p.rank_pad, [&](int bx, int hx, int, Acc) {
                  return load(&maps.lb, bx, adapter, &maps.h[mi], hx);
                });
         if (adapter == -2 && ok) {
@@ -985,12 +992,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               break;
             const uint32_t id16 = ptx::idesc_f16_f32(WROWS * CG, nn, p.lora_dtype == kBF16);
             if (adapter >= 0) {
-              const uint32_t low = p.rank_pad <= 32 ? h_low(p.rank_pad, 0) : 0u;
-              ok = adapter_stages(p.rank_pad, [&](int, int, int steps, bool first) {
+              const uint32_t low = p.rank_pad <= 32 ? h_low(p.rank_pad, 0) : 0u;  // (one stage)
+              ok = adapter_stages(p.rank_pad, [&](int, int, int steps, Acc acc) {
                 if (!wait(bar_full + 8 * stage, phase)) return false;
                 const uint32_t st = sbase + static_cast<uint32_t>(stage) * C::STAGE;
-                if (elected)
-                  lora_mma<CG>(tmem_base + C::ACC_L, st, st + W_STAGE, id16, steps, first, low);
+                const uint64_t h = ptx::sw128_kmajor_desc(st + W_STAGE);
+                if (elected) {
+                  lora_mma<CG>(tmem_base + C::ACC_L, st, h + low, id16, steps, acc);
+                  if (low != 0) lora_mma<CG>(tmem_base + C::ACC_L, st, h, id16, steps, Acc::kShift);
+                }
                 next_stage();
                 return true;
               });
@@ -1003,16 +1013,30 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               }
               for (int i = __popc(ta.leaders); i > 0 && ok; --i) {
                 if (!(ok = wait(bar_wempty + 8 * window, wphase ^ 1u))) break;
-                uint32_t h = sbase + C::OFF_H;
-                for (int bx = 0; bx < p.R; bx += 64, h += static_cast<uint32_t>(nn / CG) * BK) {
-                  if (!(ok = wait(bar_full + 8 * stage, phase))) break;
-                  if (elected)
-                    lora_mma<CG>(
-                        tmem_base + C::ACC_L + static_cast<uint32_t>(window * kLoraMixed),
-                        sbase + static_cast<uint32_t>(stage) * C::STAGE, h, id16,
-                        min(4, (p.rank_pad - bx) / 16), bx == 0, low);
-                  next_stage();
+                // B's boxes (two above rank 64, in a stage each) with the low part, then with
+                // the high part
+                const uint32_t d =
+                    tmem_base + C::ACC_L + static_cast<uint32_t>(window * kLoraMixed);
+                const uint64_t h = ptx::sw128_kmajor_desc(sbase + C::OFF_H);
+                const uint64_t h1 = h + static_cast<uint32_t>(nn / CG) * BK / 16;
+                if (!(ok = wait(bar_full + 8 * stage, phase))) break;
+                const uint32_t b0 = sbase + static_cast<uint32_t>(stage) * C::STAGE;
+                uint32_t b1 = 0;
+                if (p.R > 64) {
+                  const bool wrap = stage + 1 == C::STAGES;
+                  const int s1 = wrap ? 0 : stage + 1;
+                  if (!(ok = wait(bar_full + 8 * s1, wrap ? phase ^ 1u : phase))) break;
+                  b1 = sbase + static_cast<uint32_t>(s1) * C::STAGE;
                 }
+                if (elected) {
+                  const int steps0 = min(4, p.rank_pad / 16), steps1 = p.rank_pad / 16 - 4;
+                  lora_mma<CG>(d, b0, h + low, id16, steps0, Acc::kFresh);
+                  if (b1 != 0) lora_mma<CG>(d, b1, h1 + low, id16, steps1, Acc::kAdd);
+                  lora_mma<CG>(d, b0, h, id16, steps0, Acc::kShift);
+                  if (b1 != 0) lora_mma<CG>(d, b1, h1, id16, steps1, Acc::kAdd);
+                }
+                next_stage();
+                if (b1 != 0) next_stage();
                 if (ok && elected) ptx::mma_commit_pair_mc(bar_wfull + 8 * window, 0x3);
                 if (++window == C::WINDOWS) {
                   window = 0;

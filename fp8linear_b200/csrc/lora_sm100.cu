@@ -259,8 +259,9 @@ __device__ __forceinline__ void finish_rows(const Params &p, const float *part, 
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float w = v[i + j] * inv;
+            // cut off: up to fp32's largest value a bf16 stays finite
             hi[j] =
-                f16 ? __half2float(__float2half_rn(w)) : __bfloat162float(__float2bfloat16_rn(w));
+                f16 ? __half2float(__float2half_rz(w)) : __bfloat162float(__float2bfloat16_rz(w));
             lo[j] = fabsf(hi[j]) <= (f16 ? 65504.0f : 3.402823466e38f)
                         ? (w - hi[j]) * (1 << kLoraLowShift)
                         : 0.0f;

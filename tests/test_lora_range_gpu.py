@@ -110,3 +110,15 @@ def test_fp16_rows_far_below_one(M, rows, R, h):
     out = adapters_alone(*args)
     check(out, *ref(*args))
     assert torch.count_nonzero(out[::5]) == 0
+
+
+@pytest.mark.parametrize("M,rows", ROWS)
+def test_bf16_largest_values(M, rows):
+    """h between bf16's largest value and fp32's."""
+    x = torch.ones(M, 16, device="cuda").bfloat16()
+    a = torch.ones(3, 8, 16, device="cuda").bfloat16()
+    a[:, 1:] = 0
+    b = torch.full((3, N, 8), 2.0**-120, device="cuda").bfloat16()
+    sc = torch.full((3,), 3.4e38 / 16, device="cuda")
+    args = x, a, b, make_ids(M, rows), sc
+    check(adapters_alone(*args), *ref(*args))

@@ -195,6 +195,28 @@ __device__ __forceinline__ int adapters_at_most(const Params &p, int m0, int lan
   return n;
 }
 
+// w as a high part, cut off to the type (up to fp32's largest value a bf16 stays finite), and
+// 2^kLoraLowShift times the rest. Both have w's sign, and where the high part is not zero or not
+// finite, nor is the low part: against an infinite B, hi * B + lo * B is what w * B is, and not
+// the NaN of 0 * inf or inf - inf. (A w too small for the high part counts as zero there.)
+__device__ __forceinline__ void split_16(bool f16, float w, uint32_t &hi, uint32_t &lo) {
+  if (f16) {
+    const __half h = __float2half_rz(w);
+    const float rest = (w - __half2float(h)) * (1 << kLoraLowShift);
+    hi = __half_as_ushort(h);
+    lo = __half_as_ushort(__float2half_rn(rest));
+  } else {
+    const __nv_bfloat16 h = __float2bfloat16_rz(w);
+    const float rest = (w - __bfloat162float(h)) * (1 << kLoraLowShift);
+    hi = __bfloat16_as_ushort(h);
+    lo = __bfloat16_as_ushort(__float2bfloat16_rn(rest));
+  }
+  if (fabsf(w) == __uint_as_float(0x7F800000u))
+    lo = hi;
+  else if ((lo & 0x7FFFu) == 0 && (hi & 0x7FFFu) != 0)
+    lo = (hi & 0x8000u) | 1u;
+}
+
 // An item's sums, row by row: the K-splits' parts added in rank order, scaled, and split into
 // the two 16-bit parts. CTA `rank` of the S of a cluster has rows rank, rank + S, ..; a warp
 // has two rows at a time, a lane values 4 lane .. 4 lane + 3, one 16-byte load from each part
@@ -254,20 +276,11 @@ __device__ __forceinline__ void finish_rows(const Params &p, const float *part, 
         uint32_t hi2[2], lo2[2];
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          // an infinity or NaN is the high part's alone
-          float hi[2], lo[2];
+          uint32_t hi[2], lo[2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float w = v[i + j] * inv;
-            // cut off: up to fp32's largest value a bf16 stays finite
-            hi[j] =
-                f16 ? __half2float(__float2half_rz(w)) : __bfloat162float(__float2bfloat16_rz(w));
-            lo[j] = fabsf(hi[j]) <= (f16 ? 65504.0f : 3.402823466e38f)
-                        ? (w - hi[j]) * (1 << kLoraLowShift)
-                        : 0.0f;
-          }
-          hi2[i / 2] = f16 ? ptx::pack_f16x2(hi[0], hi[1]) : ptx::pack_bf16x2(hi[0], hi[1]);
-          lo2[i / 2] = f16 ? ptx::pack_f16x2(lo[0], lo[1]) : ptx::pack_bf16x2(lo[0], lo[1]);
+          for (int j = 0; j < 2; ++j) split_16(f16, v[i + j] * inv, hi[j], lo[j]);
+          hi2[i / 2] = hi[0] | hi[1] << 16;
+          lo2[i / 2] = lo[0] | lo[1] << 16;
         }
         uint32_t *dst = reinterpret_cast<uint32_t *>(p.hl) +
                         static_cast<int64_t>(m0 + row[h]) * p.rank_pad + 2 * lane;

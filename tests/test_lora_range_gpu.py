@@ -122,3 +122,56 @@ def test_bf16_largest_values(M, rows):
     sc = torch.full((3,), 3.4e38 / 16, device="cuda")
     args = x, a, b, make_ids(M, rows), sc
     check(adapters_alone(*args), *ref(*args))
+
+
+def check_with_infinities(got, value, err):
+    for of in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(of(got), of(value)), of.__name__
+    ok = value.isfinite()
+    check(got.where(ok, 0.0), value.where(ok, 0.0), err.where(ok, 0.0))
+
+
+def with_infinities_in_b(M, rows, K, R, exact, dtype):
+    g = torch.Generator(device="cuda").manual_seed(M + R + K)
+
+    def values(*shape):
+        v = torch.randn(*shape, generator=g, device="cuda")
+        return (v * (0.3 if K > 96 else 0.7)).round() if exact else v / 2
+
+    x, a = values(M, K), values(3, R, K)
+    b = torch.randn(3, N, R, generator=g, device="cuda")
+    b[:, 1:60:3, 3] = float("inf")
+    b[:, 60:100:3, R - 1] = -float("inf")
+    b[:, 100:130, 3] = float("inf")
+    b[:, 100:130:2, 5] = float("inf")
+    return x.to(dtype), a.to(dtype), b.to(dtype), make_ids(M, rows), torch.ones(3, device="cuda")
+
+
+@pytest.mark.parametrize("M,rows,K", [(*r, 96) for r in ROWS] + [(*r, 4096) for r in ROWS[1:]])
+@pytest.mark.parametrize("R", [8, 40, 128])
+@pytest.mark.parametrize("exact", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinities_in_b(M, rows, K, R, exact, dtype):
+    """The formula's infinities, by sign, and its NaN (an infinity times a zero h, two of
+    opposite signs), whether h has a rest beside its high part or not (exact: whole numbers
+    below 128, zeros among them)."""
+    args = with_infinities_in_b(M, rows, K, R, exact, dtype)
+    check_with_infinities(adapters_alone(*args), *ref(*args))
+
+
+@pytest.mark.parametrize("M,rows", ROWS)
+@pytest.mark.parametrize("R", [8, 72])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinities_in_h(M, rows, R, dtype):
+    """An infinity in A: infinite h, against finite, zero and infinite values of B."""
+    g = torch.Generator(device="cuda").manual_seed(M + R)
+    K = 96
+    x = torch.randn(M, K, generator=g, device="cuda").to(dtype)
+    a = (torch.randn(3, R, K, generator=g, device="cuda") / 4).to(dtype)
+    b = torch.randn(3, N, R, generator=g, device="cuda").to(dtype)
+    a[1, 2, 7] = float("inf")
+    x[:, 7] = torch.where(torch.arange(M, device="cuda") % 2 == 0, 1.0, -2.0).to(dtype)
+    b[1, ::4, 2] = 0
+    b[1, 1::4, 2] = float("inf")
+    args = x, a, b, make_ids(M, rows), torch.ones(3, device="cuda")
+    check_with_infinities(adapters_alone(*args), *ref(*args))

@@ -195,26 +195,29 @@ __device__ __forceinline__ int adapters_at_most(const Params &p, int m0, int lan
   return n;
 }
 
-// w as a high part, cut off to the type (up to fp32's largest value a bf16 stays finite), and
-// 2^kLoraLowShift times the rest. Both have w's sign, and where the high part is not zero or not
-// finite, nor is the low part: against an infinite B, hi * B + lo * B is what w * B is, and not
-// the NaN of 0 * inf or inf - inf. (A w too small for the high part counts as zero there.)
-__device__ __forceinline__ void split_16(bool f16, float w, uint32_t &hi, uint32_t &lo) {
+// Two values each as a high part, cut off to the type (up to fp32's largest value a bf16 stays
+// finite), and 2^kLoraLowShift times the rest. Both have the value's sign, and where the high part is
+// not zero or not finite, nor is the low part: against an infinite B, hi * B + lo * B is what
+// the value times B is, and not the NaN of 0 * inf or inf - inf. (A value too small for the
+// high part counts as zero there.)
+__device__ __forceinline__ void split_16x2(bool f16, float2 w, uint32_t &hi, uint32_t &lo) {
+  constexpr float kLow = 1 << kLoraLowShift;
   if (f16) {
-    const __half h = __float2half_rz(w);
-    const float rest = (w - __half2float(h)) * (1 << kLoraLowShift);
-    hi = __half_as_ushort(h);
-    lo = __half_as_ushort(__float2half_rn(rest));
+    hi = ptx::pack_f16x2_rz(w.x, w.y);
+    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    lo = ptx::pack_f16x2((w.x - h.x) * kLow, (w.y - h.y) * kLow);
   } else {
-    const __nv_bfloat16 h = __float2bfloat16_rz(w);
-    const float rest = (w - __bfloat162float(h)) * (1 << kLoraLowShift);
-    hi = __bfloat16_as_ushort(h);
-    lo = __bfloat16_as_ushort(__float2bfloat16_rn(rest));
+    hi = ptx::pack_bf16x2_rz(w.x, w.y);
+    lo = ptx::pack_bf16x2((w.x - __uint_as_float(hi << 16)) * kLow,
+                          (w.y - __uint_as_float(hi & 0xFFFF0000u)) * kLow);
   }
-  if (fabsf(w) == __uint_as_float(0x7F800000u))
-    lo = hi;
-  else if ((lo & 0x7FFFu) == 0 && (hi & 0x7FFFu) != 0)
-    lo = (hi & 0x8000u) | 1u;
+  // the halves that are not zero (as bits 15 and 31), and an infinity's bits
+  const uint32_t h = hi & 0x7FFF7FFFu, l = lo & 0x7FFF7FFFu;
+  const uint32_t gone = (h + 0x7FFF7FFFu) & ~(l + 0x7FFF7FFFu) & 0x80008000u;
+  lo |= gone >> 15 | (gone & hi);
+  const uint32_t inf = f16 ? 0x7C00u : 0x7F80u;
+  if ((h & 0xFFFFu) == inf) lo = (lo & 0xFFFF0000u) | (hi & 0xFFFFu);
+  if (h >> 16 == inf) lo = (lo & 0xFFFFu) | (hi & 0xFFFF0000u);
 }
 
 // An item's sums, row by row: the K-splits' parts added in rank order, scaled, and split into
@@ -275,13 +278,8 @@ __device__ __forceinline__ void finish_rows(const Params &p, const float *part, 
       if (col < p.rank_pad) {
         uint32_t hi2[2], lo2[2];
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          uint32_t hi[2], lo[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) split_16(f16, v[i + j] * inv, hi[j], lo[j]);
-          hi2[i / 2] = hi[0] | hi[1] << 16;
-          lo2[i / 2] = lo[0] | lo[1] << 16;
-        }
+        for (int i = 0; i < 2; ++i)
+          split_16x2(f16, make_float2(v[2 * i] * inv, v[2 * i + 1] * inv), hi2[i], lo2[i]);
         uint32_t *dst = reinterpret_cast<uint32_t *>(p.hl) +
                         static_cast<int64_t>(m0 + row[h]) * p.rank_pad + 2 * lane;
         *reinterpret_cast<uint2 *>(dst) = make_uint2(hi2[0], hi2[1]);

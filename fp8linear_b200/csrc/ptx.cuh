@@ -693,6 +693,19 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 
+// The same cut off instead of rounded.
+__device__ __forceinline__ uint32_t pack_bf16x2_rz(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2_rz(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // ---------------------------------------------------------------- warp-level MMA
 
 // Four 8 x 16-byte matrices from shared memory: lane 8j + i gives the address of row i of

@@ -86,6 +86,25 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
   }
 }
 
+// The same for a barrier that hands over what other CTAs of the cluster have written.
+__device__ __forceinline__ bool mbar_wait_bounded_cluster(uint32_t bar, uint32_t parity,
+                                                          const volatile int *abort,
+                                                          uint64_t limit_ns) {
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t n = 1;; ++n) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok != 0) return true;
+    if ((n & 255u) == 0u && (*abort || globaltimer_ns() - t0 > limit_ns)) return false;
+  }
+}
+
 // Wait with only a time limit (used to drain in-flight copies on the way out).
 __device__ __forceinline__ bool mbar_wait_timeout(uint32_t bar, uint32_t parity,
                                                   uint64_t limit_ns) {

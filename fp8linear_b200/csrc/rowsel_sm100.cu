@@ -15,7 +15,7 @@
 //   persist_kernel<CG, LORA>  persistent CTAs (CG = 2: pairs, 256 weight rows x up to 256
 //       tokens; CG = 1: 128 x up to 128, for groups of few rows), TMA ring, two TMEM
 //       accumulators, epilogue of one tile under the main loop of the next.
-//   split_kernel<LORA>  when all tiles together do not fill the GPU: a cluster of CTAs per
+//   split_kernel<LORA, OWN>  when all tiles together do not fill the GPU: a cluster of CTAs per
 //       tile splits K; each CTA adds up a share of the tile's rows, of which the others push
 //       their partial sums into its shared memory, in rank order (the result does not depend
 //       on timing).
@@ -87,8 +87,7 @@ struct Params {
   int plan_mixed;    // .. of several adapters: from this entry on
   const void *hl;
   const float *hscale;
-  // few tokens: the down projection is the GEMM's own (split_kernel)
-  int own_down;
+  // few tokens, whose down projection is the GEMM's own (split_kernel)
   const void *x;       // [M][K] of lora_dtype
   const void *lora_a;  // [L][R][K]
   const float *scaling;
@@ -623,30 +622,42 @@ __device__ __forceinline__ void unpack8(const uint4 &v, bool f16, float (&f)[8])
   }
 }
 
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
 // A few tokens' adapters without a down projection of their own (a launch, and a wait for it,
-// longer than all of this): a CTA of the K-split multiplies its K range of x with that of A
-// and the result with B; the partial results add up with the partial tiles, since both
-// products are linear. CUDA cores, fp32 throughout. Nothing here depends on the quantizer, so
-// it comes before the dependency wait. out[m][row] for the CTA's 128 rows; `h`: M x R floats
-// of shared memory.
+// longer than all of this): the CTAs of the K-split multiply their K ranges of x with those of
+// A and push the parts of h to the first of them, which adds them up in rank order and multiplies
+// with B. (Not each its own part: where B is infinite, parts of different signs would make a NaN of
+// what is an infinity.) CUDA cores, fp32 throughout. Nothing here depends on the quantizer, so it
+// comes before the dependency wait. out[m][row] for the tile's 128 rows, in the first CTA; `h`:
+// OWN_WORK floats of shared memory, and behind them as many for each CTA.
 // Down to here a CTA's values of h times its K-blocks are done before the K-blocks have
-// arrived: 4096 -> 4096 (8 K-blocks a CTA), one token, rank 16: 10.2 us against 16.0 with a down
-// projection of its own; two tokens 12.2 against 16.7; one token, rank 64: 15.7 against 16.5,
-// rank 128: 22.5 against 17.3.
+// arrived: 4096 -> 4096 (8 K-blocks a CTA), one token, rank 16: 10.3 us against 16.2 with a down
+// projection of its own; two tokens 12.4 against 16.8; one token, rank 64: 15.6 against 16.3,
+// rank 128: 22.3 against 16.9.
 constexpr int OWN_WORK = 384;
 __device__ __forceinline__ void own_adapter_sums(const Params &p, int k0, int k1, int n, float *h,
-                                                 float *out, int et, int row) {
+                                                 float *out, int et, int row, int rank,
+                                                 uint32_t bar, volatile int *abort) {
   const bool f16 = p.lora_dtype == kF16;
   const int warp = et >> 5, lane = et & 31;
   const int chunks = p.K / 8;  // 16-byte chunks of a row of x or A; K % 16 == 0
   const int c1 = min(k1, p.K) / 8;
   const uint4 *x4 = reinterpret_cast<const uint4 *>(p.x);
   const uint4 *a4 = reinterpret_cast<const uint4 *>(p.lora_a);
+  const int n_h = p.M * p.R;
+  float *parts = h + OWN_WORK;  // [CTA][n_h]
+  const uint32_t to = ptx::map_shared_rank(ptx::smem_u32(parts + rank * n_h), 0);
+  // lane m has token m's
+  static_assert(kLoraOwnTokens <= 32);
+  const int lane_id = token_id(p, lane, p.M);
+  const float lane_scaling = lane_id >= 0 ? __ldg(p.scaling + lane_id) : 0.0f;
+  bool started = false;  // the first CTA is known to have
   // four values of h at a time (R % 8 == 0: of one token), so that their loads run side by side
 #pragma unroll 1
-  for (int v = 4 * warp; v < p.M * p.R; v += 4 * EPI_WARPS) {
+  for (int v = 4 * warp; v < n_h; v += 4 * EPI_WARPS) {
     const int m = v / p.R, r = v - m * p.R;
-    const int id = token_id(p, m, p.M);
+    const int id = __shfl_sync(0xFFFFFFFFu, lane_id, m);
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (id >= 0) {
 #pragma unroll 2
@@ -669,17 +680,33 @@ __device__ __forceinline__ void own_adapter_sums(const Params &p, int k0, int k1
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) s[i] += __shfl_xor_sync(0xFFFFFFFFu, s[i], d);
-      const float sc = __ldg(p.scaling + id);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] *= sc;
     }
-    if (lane == 0) *reinterpret_cast<float4 *>(h + v) = make_float4(s[0], s[1], s[2], s[3]);
+    if (!started) ptx::cluster_wait_acquire();
+    started = true;
+    const float mine = lane == 0 ? s[0] : lane == 1 ? s[1] : lane == 2 ? s[2] : s[3];
+    if (lane < 4) ptx::st_shared_cluster_f32(to + static_cast<uint32_t>(v + lane) * 4u, mine);
+    __syncwarp();
   }
-  asm volatile("bar.sync 1, 128;" ::: "memory");
+  if (!started) ptx::cluster_wait_acquire();
+  if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_shared_rank(bar, 0));
+  if (rank != 0) return;
+  if (!ptx::mbar_wait_bounded_cluster(bar, 0, abort, kWaitLimitNs) && lane == 0)
+    record_timeout(abort);
+  __syncwarp();
+  for (int m = 0; m < p.M; ++m) {
+    const float sc = __shfl_sync(0xFFFFFFFFu, lane_scaling, m);
+    if (et < p.R) {  // (R <= 128)
+      float s = 0.0f;
+      for (int c = 0; c < p.split; ++c) s += parts[c * n_h + m * p.R + et];
+      h[m * p.R + et] = s * sc;
+    }
+    __syncwarp();
+  }
+  epilogue_sync();
   const uint16_t *lb = reinterpret_cast<const uint16_t *>(p.lora_b);
 #pragma unroll 1
   for (int m = 0; m < p.M; ++m) {
-    const int id = token_id(p, m, p.M);
+    const int id = __shfl_sync(0xFFFFFFFFu, lane_id, m);
     float s = 0.0f;
     if (id >= 0) {
       const uint4 *b4 = reinterpret_cast<const uint4 *>(
@@ -695,8 +722,6 @@ __device__ __forceinline__ void own_adapter_sums(const Params &p, int k0, int k1
     out[m * WROWS + row] = s;
   }
 }
-
-__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // ---------------------------------------------------------------- persistent kernel
 
@@ -1270,21 +1295,29 @@ constexpr int SPLIT_COST = 12;
 constexpr uint32_t SPLIT_EPI = (2 * SPLIT_TOK + 2 * WROWS) * 4;  // xs, ws, bias, hscale
 constexpr uint32_t SPLIT_SMEM = 232448;
 
-template <bool LORA>
-__global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
+// OWN: the adapters by own_adapter_sums. Otherwise a further warp fills the ring of B boxes.
+template <bool LORA, bool OWN>
+constexpr int split_threads() {
+  static_assert(LORA || !OWN);
+  return NUM_THREADS + (LORA && !OWN ? 32 : 0);
+}
+
+template <bool LORA, bool OWN>
+__global__ void __launch_bounds__(split_threads<LORA, OWN>(), 1)
     split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = ptx::smem_u32(smem);
-  __shared__ alignas(8) uint64_t s_bar[2 * SPLIT_STAGES + 2 + SUM_BARS];
+  __shared__ alignas(8) uint64_t s_bar[2 * SPLIT_STAGES + 3 + SUM_BARS];
   __shared__ uint32_t s_slot;
   __shared__ int s_abort;
   const uint32_t bar_full = ptx::smem_u32(s_bar);
   const uint32_t bar_empty = bar_full + 8 * SPLIT_STAGES;
   const uint32_t bar_acc = bar_empty + 8 * SPLIT_STAGES;
   const uint32_t bar_drain = bar_acc + 8;
-  const uint32_t bar_sum = bar_drain + 8;
+  const uint32_t bar_own = bar_drain + 8;
+  const uint32_t bar_sum = bar_own + 8;
   volatile uint32_t *tmem_slot = &s_slot;
   volatile int *abort = &s_abort;
   // partial sums of the rows reduced here: [CTA they come from][token][R rows]
@@ -1313,6 +1346,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     }
     ptx::mbar_init(bar_acc, 1);
     ptx::mbar_init(bar_drain, 1);
+    if (OWN) ptx::mbar_init(bar_own, static_cast<uint32_t>(p.split) * EPI_WARPS);
     for (int i = 0; i < SUM_SLOTS_MAX; ++i) {
       ptx::mbar_init(bar_sum + 8 * i, 1);
       ptx::mbar_init(bar_sum + 8 * (SUM_SLOTS_MAX + i), EPI_WARPS);
@@ -1359,19 +1393,21 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = static_cast<uint32_t>(ptx::uniform(static_cast<int>(*tmem_slot)));
-  ptx::cluster_arrive_release();  // (waited for before the first push: all CTAs have started)
-  if (LORA && p.own_down && warp >= 2 && warp < 2 + EPI_WARPS) {
+  // (waited for before the first push: all CTAs have started)
+  ptx::cluster_arrive_release();
+  if (OWN && warp >= 2) {
     const int row = (warp & 3) * 32 + lane;
     own_adapter_sums(p, kb0 * BK, (kb0 + nkb) * BK, q.wb * WROWS + row,
-                     reinterpret_cast<float *>(smem + p.off_ring), lora, threadIdx.x - 64, row);
+                     reinterpret_cast<float *>(smem + p.off_ring), lora, threadIdx.x - 64, row,
+                     rank, bar_own, abort);
   }
-  // Adapters: the cluster's CTAs share out the tokens, eight at a time (own_down: all tokens,
-  // but only this CTA's K range of them).
-  const bool own = LORA && p.own_down;
+  // Adapters: the cluster's CTAs share out the tokens, eight at a time (OWN: all of them are the
+  // first CTA's).
   const int per_cta = LORA ? ((cnt + 7) / 8 + p.split - 1) / p.split * 8 : 0;
-  const int a0 = own ? 0 : min(cnt, rank * per_cta), a1 = own ? cnt : min(cnt, a0 + per_cta);
+  const int a0 = OWN ? 0 : min(cnt, rank * per_cta);
+  const int a1 = OWN ? (rank == 0 ? cnt : 0) : min(cnt, a0 + per_cta);
   // (B and ids are the call's own inputs: their boxes need no wait for the kernel before)
-  if (LORA && !own && warp == 2 + EPI_WARPS) {
+  if (LORA && !OWN && warp == 2 + EPI_WARPS) {
     SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
     feed_sums(p, &maps.lb, ring, q.t0 + a0, q.t0 + a1, q.wb * WROWS);
     drain_sums(ring);
@@ -1448,8 +1484,8 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     const int et = threadIdx.x - 64;
     for (int i = et; i < q.nn; i += 128) {
       e_xs[i] = i < cnt ? __ldg(p.xs + q.t0 + i) : 0.0f;
-      if constexpr (LORA)
-        e_hs[i] = !own && token_id(p, q.t0 + i, q.t1) >= 0 ? __ldg(p.hscale + q.t0 + i) : 0.0f;
+      if constexpr (LORA && !OWN)
+        e_hs[i] = token_id(p, q.t0 + i, q.t1) >= 0 ? __ldg(p.hscale + q.t0 + i) : 0.0f;
     }
     for (int i = et; i < r1 - r0; i += 128) {
       const int n = n0 + r0 + i;
@@ -1462,7 +1498,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     const int n = n0 + row;
     const float w = LORA && n < p.N ? __ldg(p.ws + n) : 1.0f;
     epilogue_sync();  // xs and hscale are in shared memory
-    if (LORA && !own) {
+    if constexpr (LORA && !OWN) {
       // (a warp writes and reads back its own rows only; after a wait that ran out, whatever)
       SumRing ring(p, sbase + p.off_ring, bar_sum, abort);
       token_sums(p, ring, q.t0 + a0, q.t0 + a1, quarter, [&](int i, float2(&s)[4]) {
@@ -1482,7 +1518,7 @@ __global__ void __launch_bounds__(NUM_THREADS + (LORA ? 32 : 0), 1)
     const bool ok = ptx::mbar_wait_bounded(bar_acc, 0, abort, kWaitLimitNs);
     if (!ok && lane == 0) record_timeout(abort);
     ptx::tc_fence_after();
-    ptx::cluster_wait_acquire();
+    if (!OWN) ptx::cluster_wait_acquire();  // (own_adapter_sums has)
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t dst = ptx::map_shared_rank(
         ptx::smem_u32(part) +
@@ -1673,7 +1709,7 @@ struct SplitInfo {
   int clusters[SPLIT_MAX + 1] = {};
 };
 
-template <bool LORA>
+template <bool LORA, bool OWN = false>
 SplitInfo &split_info(const DeviceInfo &dev) {
   static SplitInfo info[64];
   static std::mutex mu;
@@ -1682,13 +1718,13 @@ SplitInfo &split_info(const DeviceInfo &dev) {
   if (!si.ready) {
     si.ready = true;
     // (the static barriers take a little of the 227 KB)
-    si.err = cudaFuncSetAttribute(split_kernel<LORA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  SPLIT_SMEM - 1024);
+    si.err = cudaFuncSetAttribute(split_kernel<LORA, OWN>,
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize, SPLIT_SMEM - 1024);
     si.clusters[1] = dev.sm_count;
     for (int s = 2; s <= SPLIT_MAX && si.err == cudaSuccess; ++s) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(static_cast<unsigned>(dev.sm_count / s * s));
-      cfg.blockDim = dim3(NUM_THREADS + (LORA ? 32 : 0));
+      cfg.blockDim = dim3(split_threads<LORA, OWN>());
       cfg.dynamicSmemBytes = SPLIT_SMEM - 1024;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1697,7 +1733,7 @@ SplitInfo &split_info(const DeviceInfo &dev) {
       attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      si.err = cudaOccupancyMaxActiveClusters(&si.clusters[s], split_kernel<LORA>, &cfg);
+      si.err = cudaOccupancyMaxActiveClusters(&si.clusters[s], split_kernel<LORA, OWN>, &cfg);
     }
   }
   return si;
@@ -1720,10 +1756,10 @@ int best_split(const SplitInfo &si, int64_t tiles, int k_blocks) {
   return best;
 }
 
-template <bool LORA>
+template <bool LORA, bool OWN = false>
 int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const DeviceInfo &dev,
                  cudaStream_t stream, bool pdl) {
-  SplitInfo &si = split_info<LORA>(dev);
+  SplitInfo &si = split_info<LORA, OWN>(dev);
   if (si.err != cudaSuccess) return launch_failed(op, si.err);
   const int best = best_split(si, tiles, p.k_blocks);
   p.kps = (p.k_blocks + best - 1) / best;
@@ -1731,13 +1767,10 @@ int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const D
   const uint32_t stage = W_STAGE + static_cast<uint32_t>(p.tok_cap) * BK;
   const uint32_t rows = static_cast<uint32_t>(((WROWS + p.split - 1) / p.split + 3) & ~3);
   const uint32_t part = static_cast<uint32_t>(p.split * p.tok_cap) * rows * 4;
-  const uint32_t lora =
-      LORA ? static_cast<uint32_t>(std::max((p.tok_cap / 8 + p.split - 1) / p.split * 8,
-                                            p.own_down ? kLoraOwnTokens : 0)) *
-                 WROWS * 4
-           : 0;
+  const int lora_tok = OWN ? kLoraOwnTokens : (p.tok_cap / 8 + p.split - 1) / p.split * 8;
+  const uint32_t lora = LORA ? static_cast<uint32_t>(lora_tok) * WROWS * 4 : 0;
   const uint32_t tab = static_cast<uint32_t>(p.E + 1) * 8 + 16 + SPLIT_EPI;
-  const uint32_t ring = LORA ? SUM_RING : 0u;
+  const uint32_t ring = OWN ? (1 + SPLIT_MAX) * OWN_WORK * 4u : LORA ? SUM_RING : 0u;
   const uint32_t room = SPLIT_SMEM - 2048 - ring - part - lora - tab;
   p.stages = std::max(1, std::min({static_cast<int>(room / stage), SPLIT_STAGES, p.kps}));
   p.off_ring = static_cast<uint32_t>(p.stages) * stage;
@@ -1745,9 +1778,9 @@ int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const D
   p.off_lora = p.off_part + part;
   p.off_tab = p.off_lora + lora;
   const size_t smem = p.off_tab + tab + 1024;
-  const cudaError_t e = launch(reinterpret_cast<const void *>(&split_kernel<LORA>), maps, p,
-                               tiles * p.split, NUM_THREADS + (LORA ? 32 : 0), p.split, smem,
-                               stream, pdl);
+  const cudaError_t e = launch(reinterpret_cast<const void *>(&split_kernel<LORA, OWN>), maps, p,
+                               tiles * p.split, split_threads<LORA, OWN>(), p.split, smem, stream,
+                               pdl);
   return e == cudaSuccess ? 0 : launch_failed(op, e);
 }
 
@@ -1830,7 +1863,7 @@ bool lora_own_down(int64_t M, int64_t N, int64_t K, int64_t R) {
   using namespace rowsel;
   DeviceInfo dev;
   if (M > kLoraOwnTokens || !current_device_info(&dev)) return false;
-  const SplitInfo &si = split_info<true>(dev);
+  const SplitInfo &si = split_info<true, true>(dev);
   if (si.err != cudaSuccess) return false;
   const int k_blocks = static_cast<int>((K + BK - 1) / BK);
   const int split = best_split(si, (N + WROWS - 1) / WROWS, k_blocks);
@@ -1864,7 +1897,6 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   p.L = static_cast<int>(a.L);
   p.R = static_cast<int>(a.R);
   p.rank_pad = static_cast<int>(rp);
-  p.own_down = lora_own_down(a.M, a.N, a.K, a.R) ? 1 : 0;
   p.x = a.x;
   p.lora_a = a.lora_a;
   p.scaling = a.scaling;
@@ -1904,6 +1936,8 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
     set_error(std::string(op) + ": " + err);
     return 4;
   }
+  if (lora_own_down(a.M, a.N, a.K, a.R))
+    return launch_split<true, true>(op, maps, p, static_cast<int>(tiles), dev, stream, pdl);
   if (few) return launch_split<true>(op, maps, p, static_cast<int>(tiles), dev, stream, pdl);
   return launch_persist<2, true>(op, maps, p, tiles, dev, stream, pdl);
 }

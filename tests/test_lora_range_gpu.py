@@ -175,3 +175,14 @@ def test_infinities_in_h(M, rows, R, dtype):
     b[1, 1::4, 2] = float("inf")
     args = x, a, b, make_ids(M, rows), torch.ones(3, device="cuda")
     check_with_infinities(adapters_alone(*args), *ref(*args))
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 8])
+@pytest.mark.parametrize("K", [528, 4096])
+@pytest.mark.parametrize("R", [8, 16, 40])
+@pytest.mark.parametrize("exact", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinities_in_b_of_few_tokens(M, K, R, exact, dtype):
+    """The same where the CTAs of a tile have parts of K each, whose sums may differ in sign."""
+    args = with_infinities_in_b(M, "runs" if M == 1 else "any", K, R, exact, dtype)
+    check_with_infinities(adapters_alone(*args), *ref(*args))

@@ -494,6 +494,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                   make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
                               __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
           }
+          __syncwarp();  // (the next load is the whole warp's)
         }
       }
       ptx::tc_fence_before();
@@ -519,6 +520,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
 
     // (peers may still be reading this CTA's partial sums, its own warps the lists)
+    __syncwarp();
     ptx::cluster_sync();
   }
 

@@ -715,7 +715,7 @@ int fp8lin_fp8_grouped_gemm(const void *xq, const float *x_scale, const void *wq
   if (rc != FP8LIN_OK || M == 0 || N == 0) return rc;
   GroupedArgs a{static_cast<const uint8_t *>(xq), x_scale, static_cast<const uint8_t *>(wq),
                 w_scale, bias, bias ? bias_dtype : kNone, out, out_dtype, offsets, M, N, K, E};
-  return launch_grouped(a, static_cast<cudaStream_t>(stream), true);
+  return launch_grouped(a, static_cast<cudaStream_t>(stream));
 }
 
 int fp8lin_fp8_grouped_linear(const void *x, int x_dtype, const void *wq, const float *w_scale,
@@ -748,7 +748,7 @@ int fp8lin_fp8_grouped_linear(const void *x, int x_dtype, const void *wq, const 
   GroupedArgs a{xq, xs, static_cast<const uint8_t *>(wq), w_scale, bias,
                 bias ? bias_dtype : kNone, out, out_dtype, offsets, M, N, K, E};
   a.weights_before_wait = true;  // the previous kernel is this call's quantizer
-  return launch_grouped(a, s, true);
+  return launch_grouped(a, s);
 }
 
 size_t fp8lin_fp8_linear_lora_workspace_size(int64_t M, int64_t K, int64_t R) {
@@ -827,13 +827,11 @@ int fp8lin_fp8_linear_lora(const void *x, int x_dtype, const void *wq, const flo
   a.N = N;
   a.K = K;
   a.workspace = xq + fp8lin_linear_workspace_size(M, K);
-  // the kernels before are this call's quantizer and, if any, down projection
-  a.weights_before_wait = true;
   if (!lora_own_down(M, N, K, R)) {
     rc = launch_lora_down(a, s);
     if (rc != FP8LIN_OK) return rc;
   }
-  return launch_lora_gemm(a, s, true);
+  return launch_lora_gemm(a, s);
 }
 
 static_assert(sizeof(cudaIpcMemHandle_t) == FP8LIN_PEER_HANDLE_BYTES,

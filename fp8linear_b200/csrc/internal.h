@@ -156,7 +156,8 @@ struct GroupedArgs {
   // As GemmArgs::weights_before_wait; covers the offsets too.
   bool weights_before_wait = false;
 };
-int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl);
+// Launched as a programmatic dependent, like launch_lora_gemm.
+int launch_grouped(const GroupedArgs &a, cudaStream_t stream);
 
 // One shared projection plus the low-rank adapter of each row (ids[i], none outside [0, L)):
 // out = acc * xs * ws + bias + sum_r h[i, r] * lora_b[ids[i], n, r], h from launch_lora_down.
@@ -182,14 +183,15 @@ struct LoraArgs {
   void *out;
   int out_dtype;
   int64_t M, N, K;
-  void *workspace;       // lora_workspace_bytes(M, R), 256-byte aligned
-  bool weights_before_wait = false;
+  void *workspace;       // lora_workspace(nullptr, M, R).bytes, 256-byte aligned
 };
 // A call of few tokens and ranks has no down projection of its own: the GEMM's CTAs multiply
 // their K ranges of x and A, each weight tile's anew. The K-split's CTAs decide.
 constexpr int kLoraOwnTokens = 8;
 bool lora_own_down(int64_t M, int64_t N, int64_t K, int64_t R);
-int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl);
+// The kernels before it are this call's quantizer and, if any, down projection: it reads weights,
+// adapters and ids before its dependency wait.
+int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream);
 cudaError_t read_rowsel_status(unsigned int *bits, bool clear);
 
 // ---- lora_sm100.cu

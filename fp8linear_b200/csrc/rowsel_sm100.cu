@@ -70,7 +70,7 @@ struct Params {
   int M, N, E;
   int k_blocks;
   int n_wb;        // blocks of weight rows
-  int pdl, pre_w;  // pre_w: weights and offsets may be read before the dependency wait
+  int pre_w;       // weights and offsets may be read before the dependency wait (adapters: always)
   // split_kernel
   int split, kps, stages;
   int tok_cap;        // tokens per tile at most
@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       __syncwarp();
     }
   }
-  if (p.pdl) ptx::grid_dependency_wait();
+  ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   if (!LORA && !p.pre_w) build_groups(p, C::TOK_MAX, g_row, g_tile);
 
@@ -1353,11 +1353,12 @@ __global__ void __launch_bounds__(split_threads<LORA, OWN>(), 1)
     s_abort = 0;
     ptx::fence_mbar_init();
   }
-  if (!p.pre_w && p.pdl) ptx::grid_dependency_wait();
+  const bool pre_w = LORA || p.pre_w;
+  if (!pre_w) ptx::grid_dependency_wait();
   build_groups(p, p.tok_cap, g_row, g_tile);
   const int t = blockIdx.x / p.split;
   if (t >= g_tile[p.E]) {  // the whole cluster: fewer tiles than clusters
-    if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
+    if (pre_w) ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
     zero_rows(p, g_row, 0, blockDim.x);
     return;
@@ -1411,7 +1412,7 @@ __global__ void __launch_bounds__(split_threads<LORA, OWN>(), 1)
     feed_sums(p, &maps.lb, ring, q.t0 + a0, q.t0 + a1, q.wb * WROWS);
     drain_sums(ring);
   }
-  if (p.pre_w && p.pdl) ptx::grid_dependency_wait();
+  if (pre_w) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
   // rows of the tile that this CTA reduces
@@ -1666,7 +1667,7 @@ int launch_failed(const char *op, cudaError_t e) {
 }
 
 cudaError_t launch(const void *kernel, const Maps &maps, const Params &p, int ctas, int threads,
-                   int cluster, size_t smem, cudaStream_t stream, bool pdl) {
+                   int cluster, size_t smem, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -1681,11 +1682,9 @@ cudaError_t launch(const void *kernel, const Maps &maps, const Params &p, int ct
     attr[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (pdl) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
+  attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[n].val.programmaticStreamSerializationAllowed = 1;
+  ++n;
   cfg.attrs = attr;
   cfg.numAttrs = static_cast<unsigned>(n);
   void *args[] = {const_cast<Maps *>(&maps), const_cast<Params *>(&p)};
@@ -1694,13 +1693,13 @@ cudaError_t launch(const void *kernel, const Maps &maps, const Params &p, int ct
 
 template <int CG, bool LORA>
 int launch_persist(const char *op, const Maps &maps, Params &p, int64_t tiles,
-                   const DeviceInfo &dev, cudaStream_t stream, bool pdl) {
+                   const DeviceInfo &dev, cudaStream_t stream) {
   LaunchInfo &li = persist_info<CG, LORA>(dev);
   if (li.err != cudaSuccess) return launch_failed(op, li.err);
   const int groups = static_cast<int>(std::min<int64_t>(tiles, li.max_groups));
   const cudaError_t e =
       launch(reinterpret_cast<const void *>(&persist_kernel<CG, LORA>), maps, p, groups * CG,
-             NUM_THREADS, CG == 2 ? 2 : 0, Cfg<CG, LORA>::SMEM_BYTES, stream, pdl);
+             NUM_THREADS, CG == 2 ? 2 : 0, Cfg<CG, LORA>::SMEM_BYTES, stream);
   return e == cudaSuccess ? 0 : launch_failed(op, e);
 }
 
@@ -1761,7 +1760,7 @@ int best_split(const SplitInfo &si, int64_t tiles, int k_blocks) {
 
 template <bool LORA, bool OWN = false>
 int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const DeviceInfo &dev,
-                 cudaStream_t stream, bool pdl) {
+                 cudaStream_t stream) {
   SplitInfo &si = split_info<LORA, OWN>(dev);
   if (si.err != cudaSuccess) return launch_failed(op, si.err);
   const int best = best_split(si, tiles, p.k_blocks);
@@ -1782,8 +1781,7 @@ int launch_split(const char *op, const Maps &maps, Params &p, int tiles, const D
   p.off_tab = p.off_lora + lora;
   const size_t smem = p.off_tab + tab + 1024;
   const cudaError_t e = launch(reinterpret_cast<const void *>(&split_kernel<LORA, OWN>), maps, p,
-                               tiles * p.split, split_threads<LORA, OWN>(), p.split, smem, stream,
-                               pdl);
+                               tiles * p.split, split_threads<LORA, OWN>(), p.split, smem, stream);
   return e == cudaSuccess ? 0 : launch_failed(op, e);
 }
 
@@ -1812,7 +1810,7 @@ bool check_device(const char *op, DeviceInfo *dev) {
 
 }  // namespace
 
-int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl) {
+int launch_grouped(const GroupedArgs &a, cudaStream_t stream) {
   using namespace rowsel;
   const char *op = "fp8_grouped_gemm";
   DeviceInfo dev;
@@ -1829,7 +1827,6 @@ int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl) {
   p.N = static_cast<int>(a.N);
   p.E = static_cast<int>(a.E);
   p.k_blocks = static_cast<int>((a.K + BK - 1) / BK);
-  p.pdl = pdl ? 1 : 0;
   p.pre_w = a.weights_before_wait ? 1 : 0;
   // Tiles at most, whatever the offsets: every group with rows starts a token block of its own.
   const int64_t live = std::min(a.E, a.M);
@@ -1855,11 +1852,11 @@ int launch_grouped(const GroupedArgs &a, cudaStream_t stream, bool pdl) {
     return 4;
   }
   p.n_wb = static_cast<int>(wb1);
-  if (split) return launch_split<false>(op, maps, p, static_cast<int>(ub1), dev, stream, pdl);
-  if (!pairs) return launch_persist<1, false>(op, maps, p, ub1, dev, stream, pdl);
+  if (split) return launch_split<false>(op, maps, p, static_cast<int>(ub1), dev, stream);
+  if (!pairs) return launch_persist<1, false>(op, maps, p, ub1, dev, stream);
   const int64_t wb2 = (a.N + 2 * WROWS - 1) / (2 * WROWS);
   p.n_wb = static_cast<int>(wb2);
-  return launch_persist<2, false>(op, maps, p, wb2 * (live + a.M / 256), dev, stream, pdl);
+  return launch_persist<2, false>(op, maps, p, wb2 * (live + a.M / 256), dev, stream);
 }
 
 bool lora_own_down(int64_t M, int64_t N, int64_t K, int64_t R) {
@@ -1873,7 +1870,7 @@ bool lora_own_down(int64_t M, int64_t N, int64_t K, int64_t R) {
   return M * R * ((k_blocks + split - 1) / split) <= OWN_WORK;
 }
 
-int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
+int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream) {
   using namespace rowsel;
   const char *op = "fp8_linear_lora";
   DeviceInfo dev;
@@ -1892,8 +1889,6 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
   p.N = static_cast<int>(a.N);
   p.E = 1;
   p.k_blocks = static_cast<int>((a.K + BK - 1) / BK);
-  p.pdl = pdl ? 1 : 0;
-  p.pre_w = a.weights_before_wait ? 1 : 0;
   p.ids = a.ids;
   p.lora_b = a.lora_b;
   p.lora_dtype = a.dtype;
@@ -1940,9 +1935,9 @@ int launch_lora_gemm(const LoraArgs &a, cudaStream_t stream, bool pdl) {
     return 4;
   }
   if (lora_own_down(a.M, a.N, a.K, a.R))
-    return launch_split<true, true>(op, maps, p, static_cast<int>(tiles), dev, stream, pdl);
-  if (few) return launch_split<true>(op, maps, p, static_cast<int>(tiles), dev, stream, pdl);
-  return launch_persist<2, true>(op, maps, p, tiles, dev, stream, pdl);
+    return launch_split<true, true>(op, maps, p, static_cast<int>(tiles), dev, stream);
+  if (few) return launch_split<true>(op, maps, p, static_cast<int>(tiles), dev, stream);
+  return launch_persist<2, true>(op, maps, p, tiles, dev, stream);
 }
 
 cudaError_t read_rowsel_status(unsigned int *bits, bool clear) {

@@ -524,8 +524,9 @@ ExpertArgs prep_experts(const at::Tensor &x, const at::Tensor &wq, const at::Ten
   a.E = wq.size(0);
   a.N = wq.size(1);
   TORCH_CHECK(a.E >= 1 && a.E <= 1024, op, ": 1 to 1024 experts, got ", a.E);
-  TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.numel() == a.E * a.N, op,
-              ": w_scale must be fp32 [E, N]");
+  TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.numel() == a.E * a.N &&
+                  (w_scale.dim() <= 1 || (w_scale.size(0) == a.E && w_scale.size(1) == a.N)),
+              op, ": w_scale must be fp32 [E, N]");
   TORCH_CHECK(offsets.scalar_type() == at::kInt && offsets.dim() == 1 &&
                   offsets.size(0) == a.E + 1,
               op, ": offsets must be int32 [E + 1]");

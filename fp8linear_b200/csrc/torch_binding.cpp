@@ -615,8 +615,18 @@ at::Tensor fp8_linear_lora(at::Tensor x, at::Tensor wq, at::Tensor w_scale, at::
   TORCH_CHECK(L == 0 || (R > 0 && R % 8 == 0 && R <= 128), op,
               ": the rank must be a multiple of 8 from 8 to 128 (pad with zeros), got ", R);
   const int64_t M = x.numel() / K;
-  TORCH_CHECK(adapters.scalar_type() == at::kInt && adapters.numel() == M, op,
-              ": adapters must be int32 with one entry per row of x");
+  // (one dimension, or x's rows' own; sizes of 1 aside)
+  auto sizes_above_one = [](at::IntArrayRef sizes) {
+    std::vector<int64_t> v;
+    for (const int64_t n : sizes)
+      if (n != 1) v.push_back(n);
+    return v;
+  };
+  TORCH_CHECK(adapters.scalar_type() == at::kInt && adapters.numel() == M &&
+                  (adapters.dim() <= 1 || sizes_above_one(adapters.sizes()).size() <= 1 ||
+                   sizes_above_one(adapters.sizes()) ==
+                       sizes_above_one(x.sizes().slice(0, x.dim() - 1))),
+              op, ": adapters must be int32 with one entry per row of x");
   TORCH_CHECK(scaling.scalar_type() == at::kFloat && scaling.numel() == L, op,
               ": scaling must be fp32 [L]");
   check_on(wq, x, op, "wq");

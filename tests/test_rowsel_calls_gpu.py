@@ -58,3 +58,23 @@ def test_scales_of_another_layout_are_refused():
             f.fp8_grouped_linear(x, wq, bad, offsets)
         with pytest.raises(RuntimeError, match="w_scale"):
             f.fp8_grouped_gemm(xq, xs, wq, bad, offsets)
+
+
+def test_adapters_of_another_layout_are_refused():
+    """As many entries as rows, but not in the rows' order."""
+    K, N = 32, 8
+    wq = torch.zeros(N, K, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    ws = torch.ones(N, device="cuda")
+    x = torch.randn(2, 5, K, device="cuda").half()
+    a = torch.randn(3, 8, K, device="cuda").half()
+    b = torch.randn(3, N, 8, device="cuda").half()
+    ids = (torch.arange(10, device="cuda") % 4 - 1).int()
+    sc = torch.ones(3, device="cuda")
+    ref = f.fp8_linear_lora(x, wq, ws, a, b, ids, sc)
+    for same in (ids.view(2, 5), ids.view(2, 5, 1), ids.view(10, 1), ids.view(1, 2, 5)):
+        assert torch.equal(f.fp8_linear_lora(x, wq, ws, a, b, same, sc), ref)
+    assert torch.equal(f.fp8_linear_lora(x.view(10, K), wq, ws, a, b, ids.view(1, 10), sc),
+                       ref.view(10, N))
+    for bad in (ids.view(5, 2), ids.view(2, 5).t()):
+        with pytest.raises(RuntimeError, match="adapters"):
+            f.fp8_linear_lora(x, wq, ws, a, b, bad, sc)

@@ -4,8 +4,8 @@
 // GEMM (rowsel_sm100.cu), which adds h . B^T before its one rounding.
 //
 // tcgen05 (kind::f16) on tiles of 128 rows. All of a tile's adapters stand side by side on the
-// MMA's N side (rank_pad columns each, 256 columns a pass), and each row keeps the columns of
-// its own; rows never mix, so an adapter's infinities and NaN stay with its rows. When the
+// MMA's N side (rank_pad columns each; a pass takes up to 256 columns, four adapters where the
+// tiles are few), and each row keeps the columns of its own; rows never mix, so an adapter's infinities and NaN stay with its rows. When the
 // tiles are few, a cluster splits K.
 //
 // The GEMM's tensor cores take h in x's 16-bit type. h is a sum, and B may bring up what is small
@@ -69,7 +69,7 @@ constexpr int NUM_THREADS = 256;  // producer, MMA, 4 x TMEM, plan, and one more
 constexpr int MAX_SPLIT = 8;
 // dynamic: the ring, cut anew for each item into stages of x_rows + columns rows of 128 bytes,
 // then fp32 [ROWS][rank_pad + 4]
-constexpr uint32_t SMEM_MAX = 232448 - 4096;  // (the static part is below 3 KB)
+constexpr uint32_t SMEM_MAX = 232448 - 4096;  // (the static part is below 4 KB)
 
 __device__ __forceinline__ void record_timeout(volatile int *abort) {
   if (!*abort) {

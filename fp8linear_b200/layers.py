@@ -226,8 +226,11 @@ def fp8_linear_lora(x, wq, w_scale, lora_a, lora_b, adapters, scaling, bias=None
     with ``a = adapters[i]`` (int32, one per row of ``x [..., K]``, on the device); a row whose
     entry lies outside ``[0, L)`` (-1, say) has no adapter. ``lora_a [L, R, K]`` and
     ``lora_b [L, N, R]`` in x's dtype, ``scaling`` fp32 ``[L]``, R a multiple of 8 up to 128
-    (smaller adapters are padded with zeros). x goes into the adapters unquantized. Rows of one
-    request next to each other are fastest; any order is right. No reference counterpart."""
+    (smaller adapters are padded with zeros). x goes into the adapters unquantized; their
+    intermediate ``h = scaling[a] * x[i] @ lora_a[a].T`` is an fp32 sum and is kept to 2^-16 of
+    each value in bf16, and in fp16 to the larger of 2^-22 of each value and 2^-45 of the largest
+    one of its row. Rows of one request next to each other are fastest; any order is right. No
+    reference counterpart."""
     return ops.fp8_linear_lora(x, wq, w_scale, lora_a, lora_b, adapters, scaling, bias)
 
 

@@ -400,6 +400,11 @@ FP8LIN_API int fp8lin_fp8_grouped_linear(const void *x, int x_dtype, const void 
  *   out[i,n] = fp8_linear(x)[i,n] + sum_r h[i,r] * lora_b[a,n,r],  a = adapters[i]
  *   h[i,r]   = scaling[a] * sum_k x[i,k] * lora_a[a,r,k]    (x unquantized, fp32 sums)
  * rounded once to out_dtype; rows whose adapters entry is outside [0, L) have no adapter.
+ * h enters the second sum to the larger of 2^-16 of its value and 2^-140 (BF16), or of 2^-22 of its
+ * value and 2^-45 of the largest finite one of its row (F16); up to 8 tokens it may be kept in
+ * fp32. Infinities and NaN are the formula's, for finite h and for infinite;
+ * against an infinite lora_b, h below BF16's least value 2^-133, or 2^-38 of its row's largest (F16),
+ * may count as zero. They reach no row of another adapter.
  *   lora_a [L,R,K], lora_b [L,N,R] of x_dtype, scaling [L] fp32, adapters [M] int32, all in
  *   device memory; the others as fp8lin_fp8_linear
  *   workspace fp8lin_fp8_linear_lora_workspace_size(M, K, R) bytes, 256-byte aligned
